@@ -4,9 +4,9 @@ management of its pages.
 `run` computes a case with the package's entry points (`own`) or in plain torch, in 32 bits, with the same results.
 
 Records of the cache are 416 bytes a token, two halves of 208: the codes of 256 latent values (128 bytes), the 16 scales of
-their groups of 16 (one byte each), 32 rope values in bf16.  A scale is the upper eight bits behind the sign of an fp16, a code
-a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6.  A 32-bit word holds eight values, the even ones in its low half; `SIGN` and `MAG`
-say where the four of a half have their bits.
+their groups of 16 (one byte each), 32 rope values in bf16.  A scale byte is five bits of exponent e and three of mantissa m,
+(8 + m) 2^(e - 18), 255 = NaN; a code is a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6.  A 32-bit word holds eight values, the
+even ones in its low half; `SIGN` and `MAG` say where the four of a half have their bits.
 
 Kinds
   attn      sparse attention of `tokens` query tokens for each of `batch` sequences over the latents that an indexer selected
@@ -94,12 +94,12 @@ def _quantise(x):
     g = x.view(-1, LATENT // GROUP, GROUP)
     amax = g.abs().amax(-1)
     bad = ~torch.isfinite(amax)
-    want = (torch.where(bad, torch.zeros_like(amax), amax) / torch.full_like(amax, 6.0)).clamp_max(10240.0)
-    step = torch.exp2(torch.frexp(want)[1].clamp_min(-13).float() - 4)       # of three mantissa bits, from 2^-17 on
-    scale = torch.round(want / step) * step
-    byte = (scale.to(torch.float16).view(torch.int16).int() >> 7).masked_fill(bad, 255)
-    y = (g / scale.unsqueeze(-1)).abs().nan_to_num(0.0, posinf=0.0)          # 0 / 0 and x / 0 (x below half the least scale): 0
-    y = y.masked_fill(((scale == 0) | bad).unsqueeze(-1), 0.0)
+    want = (torch.where(bad, torch.zeros_like(amax), amax) / torch.full_like(amax, 6.0)).clamp(2.0 ** -15, 61440.0)
+    e = torch.frexp(want)[1] - 1
+    scale = torch.round(torch.ldexp(want, 3 - e)) * torch.exp2((e - 3).float())          # four significant bits, ties to even
+    e = torch.frexp(scale)[1] - 1
+    byte = ((e + 15) * 8 + torch.ldexp(scale, 3 - e).int() - 8).masked_fill(bad, 255)
+    y = (g / scale.unsqueeze(-1)).abs().masked_fill(bad.unsqueeze(-1), 0.0)
     # halfway cases go to the even level number: up from 0.75, 1.75 and 3.5
     n = ((y > 0.25).int() + (y >= 0.75).int() + (y > 1.25).int() + (y >= 1.75).int() + (y > 2.5).int() + (y >= 3.5).int() + (y > 5.0).int())
     return n.view(-1, LATENT), (torch.signbit(x)).int(), byte
@@ -132,7 +132,8 @@ def _values(rec):
         for at in MAG[k]:
             n = n * 2 + ((w >> at) & 1)
         out[:, :, k] = levels[n] * (1 - 2 * ((w >> SIGN[k]) & 1))
-    scale = (h[..., 128:144].to(torch.int16) << 7).contiguous().view(torch.float16).float()
+    b = h[..., 128:144].int()
+    scale = ((8 + b % 8) * torch.exp2((b // 8 - 18).float())).masked_fill(b == 255, math.nan)
     lat = out.view(-1, LATENT // GROUP, GROUP) * scale.reshape(-1, LATENT // GROUP, 1)
     rope = h[..., 144:].contiguous().view(torch.bfloat16).float()
     return torch.cat((lat.view(-1, LATENT), rope.reshape(-1, ROPE)), -1).view(*lead, LATENT + ROPE)
@@ -429,8 +430,7 @@ def _decode_bits(rec):
         bits = np.unpackbits(part[:, :128], axis=1, bitorder="little").reshape(-1, 64, 16).astype(np.int64)   # 16-bit halves of the words
         scale = part[:, 128:144].astype(np.int64)
         e, m = scale >> 3, scale & 7
-        s = np.where(e == 0, m * 2.0 ** -17, (8 + m) * 2.0 ** (e - 18.0))
-        s = np.where(e == 31, np.nan, s)
+        s = np.where(scale == 255, np.nan, (8 + m) * 2.0 ** (e - 18.0))
         for k in range(4):
             n = bits[:, :, MAG[k][0]] * 4 + bits[:, :, MAG[k][1]] * 2 + bits[:, :, MAG[k][2]]
             v = np.asarray(LEVELS, dtype=np.float64)[n] * np.where(bits[:, :, SIGN[k]] == 1, -1.0, 1.0)
@@ -447,10 +447,8 @@ def exact(case, seed):
     if kind == "cache":
         st = prepare(case, seed)
         x = st["kv"][:, :512].double().view(-1, 32, 16)
-        want = x.abs().amax(-1) / 6
-        grid = torch.tensor([(m / 8 if e == 0 else 1 + m / 8) * 2.0 ** (max(e, 1) - 15) for e in range(31) for m in range(8)],
-                            dtype=torch.float64, device=DEV)
-        grid = grid[grid <= 10240]
+        grid = torch.tensor([(8 + m) * 2.0 ** (e - 18) for e in range(31) for m in range(8)], dtype=torch.float64, device=DEV)
+        want = (x.abs().amax(-1) / 6).clamp(grid[0], grid[-1])
         up = torch.bucketize(want, grid).clamp_max(grid.numel() - 1)
         dn = (up - 1).clamp_min(0)
         a, b = want - grid[dn], grid[up] - want
