@@ -17,7 +17,7 @@
  *   - `status` (may be NULL) is one int32 in device memory, zeroed by the caller.
  *     Kernels write a non-zero code there instead of faulting: 1 = an internal
  *     bounded wait expired, 2 = an index or page id was out of range (the access
- *     was skipped).  Read it after synchronising when you want to check.
+ *     was skipped), 3 = too few free pages (the call changed nothing).  Read it after synchronising when you want to check.
  */
 #ifndef DSA_B200_H_
 #define DSA_B200_H_
@@ -182,6 +182,99 @@ int dsa_decode_step(const void* q_fp8, const void* w, int w_dtype, const void* k
                     int B, int idx_heads, int idx_dim, int max_ctx, int k, int32_t* idx, const void* q_bf16, const void* latent,
                     int latent_pages, void* out_bf16, int H, float scale, void* workspace, size_t workspace_bytes,
                     int32_t* status, void* stream);
+
+/* ---- the paged latent cache in 4 bits -------------------------------------------
+ * No counterpart in the reference (it has no cache, sparse_attn/DSA.py:475-477).
+ * A record is 416 bytes a token, two halves of 208.  Half c holds latent values
+ * 256c .. 256c+255 and rope values 32c .. 32c+31:
+ *   128 bytes  codes, eight values to a little-endian 32-bit word
+ *    16 bytes  scales of the sixteen groups of 16 values
+ *    64 bytes  rope values, bf16
+ * A scale byte (e << 3) + m, e = 0..30, stands for (8 + m) * 2^(e - 18); 255 is a NaN.
+ * A code is a sign and the number of one of 0, .5, 1, 1.5, 2, 3, 4, 6.  Of a word's
+ * values the even ones are in the low 16 bits, the odd ones in the high 16; value k
+ * of a half has its sign and the bits of its number, highest first, at
+ *   k=0: 15, 8 7 6    k=1: 12, 5 4 3    k=2: 9, 2 1 0    k=3: 14, 11 10 13.
+ * value = code * scale (exact in bf16).  Quantising: scale = (largest magnitude of
+ * the group) / 6, held to [2^-15, 61440] and rounded to nearest even; code = value /
+ * scale to nearest, ties to the even number, saturating.  A group with an infinity
+ * or a NaN gets the scale 255 and reads as NaN. */
+
+/* Write side: rows kv [n_tokens, 576] (as for dsa_pack_latent_cache) -> records at the
+ * rows slots[i] of cache [cache_rows, 416] (slots may be NULL: row i).  A negative
+ * slot is skipped, one >= cache_rows is skipped and sets status 2; the slots of a
+ * call must differ.  With k_fp8 (NULL: none) the tokens' indexer keys go to the same
+ * rows of the paged key cache: k_fp8 [n_tokens, 128] e4m3 -> kcache [cache_rows, 128],
+ * k_scale [n_tokens] -> kscale [cache_rows]. */
+int dsa_pack_latent4(const void* kv, int kv_dtype, int64_t row_stride, int64_t n_tokens, void* cache, int64_t cache_rows,
+                     const int32_t* slots, const void* k_fp8, const float* k_scale, void* kcache, float* kscale,
+                     int32_t* status, void* stream);
+/* Read side: positions 0 .. n_tokens-1 of one sequence -> rows out_bf16 [n_tokens, 576], row_stride values apart (a
+ * multiple of 8).  Position p is the record block_table[p/64]*64 + p%64 (block_table may be NULL: record p); a page that
+ * is out of range gives rows of zeros and sets status 2. */
+int dsa_unpack_latent4(const void* cache, int64_t cache_rows, const int32_t* block_table, int64_t n_tokens, void* out_bf16,
+                       int64_t row_stride, int32_t* status, void* stream);
+
+/* dsa_sparse_mla_decode_paged over records of record_bytes = 656 (FP8) or 416 (4 bits), for tokens_per_seq query rows of
+ * each sequence: rows r = b*tokens_per_seq .. of q [T, H, 576], idx [T, K] and out [T, H, 512] go by row b of block_table.
+ * The workspace is that of T sequences.  (4 bits: |q| of the latent part must stay below 2^113.) */
+int dsa_sparse_mla_decode_records(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table,
+                                  int64_t table_stride, int tokens_per_seq, const int32_t* idx, void* out_bf16, int T, int H,
+                                  int K, int num_pages, int max_ctx, float scale, void* workspace, size_t workspace_bytes,
+                                  int32_t* status, void* stream);
+/* dsa_decode_step with such records. */
+int dsa_decode_step_records(const void* q_fp8, const void* w, int w_dtype, const void* kcache, const float* kscale, int k_pages,
+                            const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len, float* logits,
+                            int64_t ld_logits, int B, int idx_heads, int idx_dim, int max_ctx, int k, int32_t* idx,
+                            const void* q_bf16, const void* latent, int record_bytes, int latent_pages, void* out_bf16, int H,
+                            float scale, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
+/* ---- pages of the paged caches ----------------------------------------------------
+ * No counterpart in the reference.  The state is the caller's, in device memory:
+ *   refs [num_pages] int32       how many sequences hold the page, 0 = free
+ *   block_table [B, table_stride] int32, P entries used: the pages of a sequence in
+ *                                order, -1 behind the last one
+ *   ctx_len [B] int32            its tokens (64 to a page); 0 = an empty row
+ * Pages are taken lowest free id first, in the order of the call's list: the ids
+ * depend on the state alone.  A call that takes pages is all or nothing: with a bad
+ * argument (status 2) or too few free pages (status 3) it changes nothing.
+ * B <= 262144.  `workspace` (4-byte aligned): dsa_pages_workspace_bytes(num_pages, n). */
+
+/* A cache whose pages are copied (host struct): `layers` times [num_pages*64, token_bytes] bytes, layer_stride bytes
+ * apart; every layer 16-byte aligned, token_bytes a multiple of 4. */
+typedef struct {
+  void* base;
+  int64_t layer_stride;
+  int32_t layers;
+  int32_t token_bytes;
+} dsa_page_cache;
+
+size_t dsa_pages_workspace_bytes(int num_pages, int n);
+/* Page src[i] -> page dst[i], i < n, in every layer of every cache (`caches`: host array); with tokens [n], the first
+ * tokens[i] of its 64 tokens (held to 0..64).  Entries with a negative id are skipped, ids >= num_pages are skipped and set
+ * status 2.  No page may be written twice, nor be written and read. */
+int dsa_copy_pages(const dsa_page_cache* caches, int n_caches, int num_pages, const int32_t* src, const int32_t* dst,
+                   const int32_t* tokens, int n, int32_t* status, void* stream);
+/* Room for n_new[i] more tokens (0..max_new) in row rows[i], rows all different: pages are taken, ctx_len grows, and
+ * slots [n, max_new] gets the cache rows of the new tokens, -1 behind them (refused: -1 everywhere). */
+int dsa_extend_pages(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages,
+                     const int32_t* rows, const int32_t* n_new, int n, int max_new, int32_t* slots, void* workspace,
+                     size_t workspace_bytes, int32_t* status, void* stream);
+/* Row children[i] (empty, all different, no parent of the call) becomes a copy of row parents[i]: its full pages are
+ * shared, a partly filled last one is copied to a page of the child's own, in every layer of every cache. */
+int dsa_fork_pages(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages,
+                   const int32_t* parents, const int32_t* children, int n, const dsa_page_cache* caches, int n_caches,
+                   void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* Rows rows[i] become empty and give their pages back (one that is named twice does so once; one that is out of range
+ * is skipped and sets status 2, and so does a page that was free already). */
+int dsa_free_pages(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages,
+                   const int32_t* rows, int n, int32_t* status, void* stream);
+/* The L pages in use move to ids 0 .. L-1: the i-th lowest free page below L takes the contents of the i-th highest page
+ * in use, in every layer of every cache.  new_table [B, new_stride] and new_refs are the tables that go with it (they may be
+ * block_table and refs).  The pages moved from are not written: the old table reads right until one of them is taken. */
+int dsa_compact_pages(const int32_t* block_table, int64_t table_stride, int32_t* new_table, int64_t new_stride, int P, int B,
+                      const int32_t* refs, int32_t* new_refs, int num_pages, const dsa_page_cache* caches, int n_caches,
+                      void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* dsa_indexer_topk without a caller-supplied workspace.  No counterpart in the
  * reference: it exists for hosts that cannot allocate device memory at the call

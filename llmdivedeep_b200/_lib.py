@@ -45,6 +45,23 @@ SIGNATURES = {
     "dsa_decode_step": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                                 c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_float,
                                 c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dsa_pack_latent4": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_void_p, c_void_p]),
+    "dsa_unpack_latent4": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "dsa_sparse_mla_decode_records": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int,
+                                              c_int, c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dsa_decode_step_records": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                                        c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                        c_void_p, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dsa_pages_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "dsa_copy_pages": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "dsa_extend_pages": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
+                                 c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dsa_fork_pages": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                               c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dsa_free_pages": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]),
+    "dsa_compact_pages": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                  c_void_p, c_size_t, c_void_p, c_void_p]),
     "dsa_test_indexer_logits_general": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                                 c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p,
                                                 c_void_p]),

@@ -52,8 +52,8 @@ int bounded_wait_probe_launch(uint32_t poll_limit, int32_t* status, cudaStream_t
 
 int sparse_mla_prefill_launch(const void* q, const void* kv, const int32_t* idx, void* out, int T, int H, int S_kv,
                               int K, float scale, int32_t* status, cudaStream_t stream);
-int sparse_mla_decode_launch(const void* q, const void* cache, const int32_t* block_table, int64_t table_stride,
-                             const int32_t* idx, void* out, int B, int H, int K, int num_pages, int max_ctx,
+int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,
+                             int tokens_per_seq, const int32_t* idx, void* out, int B, int H, int K, int num_pages, int max_ctx,
                              float scale, void* workspace, size_t workspace_bytes, int32_t* status, int overlapped,
                              cudaStream_t stream);
 size_t mla_decode_workspace_bytes(int B, int H, int K);
@@ -63,6 +63,21 @@ int block_sparse_mha_launch(const void* q, const void* k, const void* v, const i
 
 int fp8_quant_launch(const void* x, int x_is_bf16, int64_t n_blocks, int block, void* q, float* scale,
                      cudaStream_t stream);
+int pack_latent4_launch(const void* kv, int kv_is_bf16, int64_t row_stride, int64_t n, void* cache, const int32_t* slots, int64_t cache_rows, const void* k8,
+                        const float* k_scale, void* kcache, float* kscale, int32_t* status, cudaStream_t stream);
+int unpack_latent4_launch(const void* cache, int64_t cache_rows, const int32_t* table, int64_t n, void* out, int64_t out_stride, int32_t* status,
+                          cudaStream_t stream);
+int copy_pages_launch(const dsa_page_cache* caches, int n_caches, int num_pages, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n,
+                      int32_t* status, cudaStream_t stream);
+int extend_pages_launch(int32_t* table, int64_t stride, int P, int B, int32_t* ctx, int32_t* refs, int num_pages, const int32_t* rows, const int32_t* n_new, int n,
+                        int max_new, int32_t* slots, int32_t* workspace, int32_t* status, cudaStream_t stream);
+int fork_pages_launch(int32_t* table, int64_t stride, int P, int B, int32_t* ctx, int32_t* refs, int num_pages, const int32_t* parents, const int32_t* children,
+                      int n, const dsa_page_cache* caches, int n_caches, int32_t* workspace, int32_t* status, cudaStream_t stream);
+int free_pages_launch(int32_t* table, int64_t stride, int P, int B, int32_t* ctx, int32_t* refs, int num_pages, const int32_t* rows, int n, int32_t* status,
+                      cudaStream_t stream);
+int compact_pages_launch(const int32_t* table, int64_t stride, int32_t* new_table, int64_t new_stride, int P, int B, const int32_t* refs, int32_t* new_refs,
+                         int num_pages, const dsa_page_cache* caches, int n_caches, int32_t* workspace, int32_t* status, cudaStream_t stream);
+size_t pages_workspace_bytes(int num_pages, int n);
 int pack_latent_launch(const void* kv, int kv_is_bf16, int64_t row_stride, int64_t n, void* rec, cudaStream_t stream);
 int rope_fp8_quant_launch(const void* x, int64_t n_rows, int head_dim, int rope_dim, int interleave, int rows_per_pos,
                           const float* cos_t, const float* sin_t, void* q, float* scale, const void* gate, float mul0,
@@ -206,13 +221,16 @@ int dsa_block_sparse_mha(const void* q_bf16, const void* k_bf16, const void* v_b
                                  static_cast<cudaStream_t>(stream));
 }
 
-static int sparse_mla_decode_checked(const void* q_bf16, const void* cache, const int32_t* block_table,
-                                int64_t table_stride, const int32_t* idx, void* out_bf16, int B, int H, int K,
+static int sparse_mla_decode_checked(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table,
+                                int64_t table_stride, int tokens_per_seq, const int32_t* idx, void* out_bf16, int B, int H, int K,
                                 int num_pages, int max_ctx, float scale, void* workspace, size_t workspace_bytes,
                                 int32_t* status, int overlapped, void* stream) {
   g_err[0] = 0;
   if (B < 0 || H < 0 || K < 0 || num_pages < 0 || max_ctx < 0)
     return set_error(DSA_ERR_SHAPE, "sparse_mla_decode_paged: negative size");
+  if (record_bytes != 656 && record_bytes != 416)
+    return set_error(DSA_ERR_SHAPE, "sparse_mla_decode_paged: records of %d bytes, only 656 (FP8) and 416 (4 bits) are built", record_bytes);
+  if (tokens_per_seq < 1) return set_error(DSA_ERR_SHAPE, "sparse_mla_decode_paged: tokens_per_seq (%d) must be at least 1", tokens_per_seq);
   if (B == 0 || H == 0) return DSA_OK;
   if (!q_bf16 || !out_bf16 || (K > 0 && (!idx || !cache || !block_table)))
     return set_error(DSA_ERR_ARG, "sparse_mla_decode_paged: NULL pointer argument");
@@ -226,7 +244,7 @@ static int sparse_mla_decode_checked(const void* q_bf16, const void* cache, cons
     return set_error(DSA_ERR_SHAPE, "sparse_mla_decode_paged: problem too large");
   if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15))
     return set_error(DSA_ERR_WORKSPACE, "sparse_mla_decode_paged: workspace must be 16-byte aligned");
-  return sparse_mla_decode_launch(q_bf16, cache, block_table, table_stride, idx, out_bf16, B, H, K, num_pages,
+  return sparse_mla_decode_launch(q_bf16, cache, record_bytes, block_table, table_stride, tokens_per_seq, idx, out_bf16, B, H, K, num_pages,
                                   max_ctx, scale, workspace, workspace_bytes, status, overlapped,
                                   static_cast<cudaStream_t>(stream));
 }
@@ -235,14 +253,21 @@ int dsa_sparse_mla_decode_paged(const void* q_bf16, const void* cache, const int
                                 int64_t table_stride, const int32_t* idx, void* out_bf16, int B, int H, int K,
                                 int num_pages, int max_ctx, float scale, void* workspace, size_t workspace_bytes,
                                 int32_t* status, void* stream) {
-  return sparse_mla_decode_checked(q_bf16, cache, block_table, table_stride, idx, out_bf16, B, H, K, num_pages, max_ctx, scale, workspace,
-                                   workspace_bytes, status, /*overlapped=*/0, stream);
+  return sparse_mla_decode_checked(q_bf16, cache, /*record_bytes=*/656, block_table, table_stride, /*tokens_per_seq=*/1, idx, out_bf16, B, H, K,
+                                   num_pages, max_ctx, scale, workspace, workspace_bytes, status, /*overlapped=*/0, stream);
 }
 
-int dsa_decode_step(const void* q_fp8, const void* w, int w_dtype, const void* kcache, const float* kscale, int k_pages,
+int dsa_sparse_mla_decode_records(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,
+                                  int tokens_per_seq, const int32_t* idx, void* out_bf16, int T, int H, int K, int num_pages, int max_ctx, float scale,
+                                  void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  return sparse_mla_decode_checked(q_bf16, cache, record_bytes, block_table, table_stride, tokens_per_seq, idx, out_bf16, T, H, K, num_pages, max_ctx,
+                                   scale, workspace, workspace_bytes, status, /*overlapped=*/0, stream);
+}
+
+int dsa_decode_step_records(const void* q_fp8, const void* w, int w_dtype, const void* kcache, const float* kscale, int k_pages,
                     const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len, float* logits, int64_t ld_logits,
                     int B, int idx_heads, int idx_dim, int max_ctx, int k, int32_t* idx, const void* q_bf16, const void* latent,
-                    int latent_pages, void* out_bf16, int H, float scale, void* workspace, size_t workspace_bytes,
+                    int record_bytes, int latent_pages, void* out_bf16, int H, float scale, void* workspace, size_t workspace_bytes,
                     int32_t* status, void* stream) {
   int rc = dsa_indexer_logits_paged(q_fp8, w, w_dtype, kcache, kscale, block_table, table_stride, ctx_len, logits, ld_logits, B,
                                     idx_heads, idx_dim, k_pages, max_ctx, status, stream);
@@ -254,9 +279,19 @@ int dsa_decode_step(const void* q_fp8, const void* w, int w_dtype, const void* k
   // free, and the rest waits.
   const int overlapped = B <= 24;
   if (!rc) rc = topk_select_checked(logits, ld_logits, nullptr, ctx_len, B, max_ctx, k, idx, /*sample=*/1, overlapped, stream);
-  if (!rc) rc = sparse_mla_decode_checked(q_bf16, latent, block_table, table_stride, idx, out_bf16, B, H, k, latent_pages, max_ctx,
+  if (!rc) rc = sparse_mla_decode_checked(q_bf16, latent, record_bytes, block_table, table_stride, /*tokens_per_seq=*/1, idx, out_bf16, B, H, k, latent_pages, max_ctx,
                                           scale, workspace, workspace_bytes, status, overlapped, stream);
   return rc;
+}
+
+int dsa_decode_step(const void* q_fp8, const void* w, int w_dtype, const void* kcache, const float* kscale, int k_pages,
+                    const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len, float* logits, int64_t ld_logits,
+                    int B, int idx_heads, int idx_dim, int max_ctx, int k, int32_t* idx, const void* q_bf16, const void* latent,
+                    int latent_pages, void* out_bf16, int H, float scale, void* workspace, size_t workspace_bytes,
+                    int32_t* status, void* stream) {
+  return dsa_decode_step_records(q_fp8, w, w_dtype, kcache, kscale, k_pages, block_table, table_stride, ctx_len, logits, ld_logits, B, idx_heads,
+                                 idx_dim, max_ctx, k, idx, q_bf16, latent, /*record_bytes=*/656, latent_pages, out_bf16, H, scale, workspace,
+                                 workspace_bytes, status, stream);
 }
 
 size_t dsa_sparse_mla_decode_workspace_bytes(int B, int H, int K) {
@@ -287,6 +322,131 @@ int dsa_pack_latent_cache(const void* kv, int kv_dtype, int64_t row_stride, int6
   if (!aligned16(kv) || !aligned16(records) || (n_tokens > 1 && (row_stride * elt) % 16))
     return set_error(DSA_ERR_ALIGN, "pack_latent_cache: every row and the records must be 16-byte aligned");
   return pack_latent_launch(kv, kv_dtype == DSA_X_BF16, row_stride, n_tokens, records, static_cast<cudaStream_t>(stream));
+}
+
+int dsa_pack_latent4(const void* kv, int kv_dtype, int64_t row_stride, int64_t n_tokens, void* cache, int64_t cache_rows, const int32_t* slots,
+                     const void* k_fp8, const float* k_scale, void* kcache, float* kscale, int32_t* status, void* stream) {
+  g_err[0] = 0;
+  if (n_tokens < 0 || cache_rows < 0) return set_error(DSA_ERR_SHAPE, "pack_latent4: negative size");
+  if (n_tokens == 0) return DSA_OK;
+  if (!kv || !cache) return set_error(DSA_ERR_ARG, "pack_latent4: NULL pointer argument");
+  if (kv_dtype != DSA_X_F32 && kv_dtype != DSA_X_BF16) return set_error(DSA_ERR_ARG, "pack_latent4: bad kv_dtype");
+  if (!slots && cache_rows < n_tokens)
+    return set_error(DSA_ERR_SHAPE, "pack_latent4: %lld tokens in order need as many records, the cache has %lld", (long long)n_tokens, (long long)cache_rows);
+  const int64_t elt = kv_dtype == DSA_X_BF16 ? 2 : 4;
+  if (n_tokens > 1 && row_stride < 576) return set_error(DSA_ERR_SHAPE, "pack_latent4: row_stride below 576");
+  if (!aligned16(kv) || !aligned16(cache) || (n_tokens > 1 && (row_stride * elt) % 16))
+    return set_error(DSA_ERR_ALIGN, "pack_latent4: every row and the cache must be 16-byte aligned");
+  if (k_fp8 && (!k_scale || !kcache || !kscale)) return set_error(DSA_ERR_ARG, "pack_latent4: NULL pointer argument");
+  if (k_fp8 && (!aligned16(k_fp8) || !aligned16(kcache))) return set_error(DSA_ERR_ALIGN, "pack_latent4: keys and their cache must be 16-byte aligned");
+  return pack_latent4_launch(kv, kv_dtype == DSA_X_BF16, row_stride, n_tokens, cache, slots, cache_rows, k_fp8, k_scale, kcache, kscale, status,
+                             static_cast<cudaStream_t>(stream));
+}
+
+int dsa_unpack_latent4(const void* cache, int64_t cache_rows, const int32_t* block_table, int64_t n_tokens, void* out_bf16, int64_t row_stride,
+                       int32_t* status, void* stream) {
+  g_err[0] = 0;
+  if (n_tokens < 0 || cache_rows < 0) return set_error(DSA_ERR_SHAPE, "unpack_latent4: negative size");
+  if (n_tokens == 0) return DSA_OK;
+  if (!cache || !out_bf16) return set_error(DSA_ERR_ARG, "unpack_latent4: NULL pointer argument");
+  if (!block_table && cache_rows < n_tokens)
+    return set_error(DSA_ERR_SHAPE, "unpack_latent4: %lld tokens in order, the cache has %lld", (long long)n_tokens, (long long)cache_rows);
+  if (n_tokens > 1 && row_stride < 576) return set_error(DSA_ERR_SHAPE, "unpack_latent4: row_stride below 576");
+  if (!aligned16(cache) || !aligned16(out_bf16) || (n_tokens > 1 && row_stride % 8))
+    return set_error(DSA_ERR_ALIGN, "unpack_latent4: the cache and every row must be 16-byte aligned");
+  return unpack_latent4_launch(cache, cache_rows, block_table, n_tokens, out_bf16, row_stride, status, static_cast<cudaStream_t>(stream));
+}
+
+// The caches that a call copies pages of: 0, or an error.
+static int check_page_caches(const char* who, const dsa_page_cache* caches, int n_caches) {
+  if (n_caches < 0) return set_error(DSA_ERR_SHAPE, "%s: negative number of caches", who);
+  if (n_caches > 0 && !caches) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
+  int64_t layers = 0;
+  for (int c = 0; c < n_caches; ++c) {
+    const dsa_page_cache& h = caches[c];
+    if (h.layers < 0 || h.token_bytes <= 0 || h.token_bytes > (1 << 20) || h.token_bytes % 4)
+      return set_error(DSA_ERR_SHAPE, "%s: cache %d: a token's bytes (%d) must be a multiple of 4, up to 1 MiB", who, c, h.token_bytes);
+    if (h.layers > 0 && !h.base) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
+    if (!aligned16(h.base) || (h.layers > 1 && h.layer_stride % 16))
+      return set_error(DSA_ERR_ALIGN, "%s: cache %d: every layer must be 16-byte aligned", who, c);
+    layers += (int64_t)h.layers * ((h.token_bytes * 64 >> 14) + 1);
+  }
+  if (layers > (1 << 24)) return set_error(DSA_ERR_SHAPE, "%s: too many layers", who);
+  return DSA_OK;
+}
+// Sizes of the page tables: 0, or an error.
+static int check_pool(const char* who, const void* table, int64_t stride, int P, int B, const void* refs, int num_pages, int n) {
+  if (P < 0 || B < 0 || num_pages < 0 || n < 0) return set_error(DSA_ERR_SHAPE, "%s: negative size", who);
+  if ((int64_t)num_pages * 64 > 0x7fffffffLL || (int64_t)P * 64 > 0x7fffffffLL) return set_error(DSA_ERR_SHAPE, "%s: too many pages", who);
+  if (B > (1 << 18)) return set_error(DSA_ERR_SHAPE, "%s: %d table rows, 262144 are the most", who, B);
+  if (B > 1 && stride < P) return set_error(DSA_ERR_SHAPE, "%s: table rows overlap", who);
+  if ((B > 0 && P > 0 && !table) || (num_pages > 0 && !refs)) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
+  return DSA_OK;
+}
+static int check_pages_workspace(const char* who, const void* workspace, size_t bytes, int num_pages, int n) {
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || bytes < pages_workspace_bytes(num_pages, n))
+    return set_error(DSA_ERR_WORKSPACE, "%s: workspace missing, unaligned or smaller than %zu B", who, pages_workspace_bytes(num_pages, n));
+  return DSA_OK;
+}
+
+size_t dsa_pages_workspace_bytes(int num_pages, int n) { return num_pages < 0 || n < 0 ? 0 : pages_workspace_bytes(num_pages, n); }
+
+int dsa_copy_pages(const dsa_page_cache* caches, int n_caches, int num_pages, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n,
+                   int32_t* status, void* stream) {
+  g_err[0] = 0;
+  int rc = check_page_caches("copy_pages", caches, n_caches);
+  if (rc) return rc;
+  if (n < 0 || num_pages < 0) return set_error(DSA_ERR_SHAPE, "copy_pages: negative size");
+  if (n == 0 || n_caches == 0) return DSA_OK;
+  if (!src || !dst) return set_error(DSA_ERR_ARG, "copy_pages: NULL pointer argument");
+  return copy_pages_launch(caches, n_caches, num_pages, src, dst, tokens, n, status, static_cast<cudaStream_t>(stream));
+}
+
+int dsa_extend_pages(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages, const int32_t* rows,
+                     const int32_t* n_new, int n, int max_new, int32_t* slots, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  g_err[0] = 0;
+  int rc = check_pool("extend_pages", block_table, table_stride, P, B, refs, num_pages, n);
+  if (rc || n == 0) return rc;
+  if (max_new < 0 || max_new > (1 << 30)) return set_error(DSA_ERR_SHAPE, "extend_pages: bad max_new (%d)", max_new);
+  if (!ctx_len || !rows || !n_new || (max_new > 0 && !slots)) return set_error(DSA_ERR_ARG, "extend_pages: NULL pointer argument");
+  if ((rc = check_pages_workspace("extend_pages", workspace, workspace_bytes, num_pages, n))) return rc;
+  return extend_pages_launch(block_table, table_stride, P, B, ctx_len, refs, num_pages, rows, n_new, n, max_new, slots, static_cast<int32_t*>(workspace),
+                             status, static_cast<cudaStream_t>(stream));
+}
+
+int dsa_fork_pages(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages, const int32_t* parents,
+                   const int32_t* children, int n, const dsa_page_cache* caches, int n_caches, void* workspace, size_t workspace_bytes,
+                   int32_t* status, void* stream) {
+  g_err[0] = 0;
+  int rc = check_pool("fork_pages", block_table, table_stride, P, B, refs, num_pages, n);
+  if (!rc) rc = check_page_caches("fork_pages", caches, n_caches);
+  if (rc || n == 0) return rc;
+  if (!ctx_len || !parents || !children) return set_error(DSA_ERR_ARG, "fork_pages: NULL pointer argument");
+  if ((rc = check_pages_workspace("fork_pages", workspace, workspace_bytes, num_pages, n))) return rc;
+  return fork_pages_launch(block_table, table_stride, P, B, ctx_len, refs, num_pages, parents, children, n, caches, n_caches,
+                           static_cast<int32_t*>(workspace), status, static_cast<cudaStream_t>(stream));
+}
+
+int dsa_free_pages(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages, const int32_t* rows, int n,
+                   int32_t* status, void* stream) {
+  g_err[0] = 0;
+  const int rc = check_pool("free_pages", block_table, table_stride, P, B, refs, num_pages, n);
+  if (rc || n == 0) return rc;
+  if (!ctx_len || !rows) return set_error(DSA_ERR_ARG, "free_pages: NULL pointer argument");
+  return free_pages_launch(block_table, table_stride, P, B, ctx_len, refs, num_pages, rows, n, status, static_cast<cudaStream_t>(stream));
+}
+
+int dsa_compact_pages(const int32_t* block_table, int64_t table_stride, int32_t* new_table, int64_t new_stride, int P, int B, const int32_t* refs,
+                      int32_t* new_refs, int num_pages, const dsa_page_cache* caches, int n_caches, void* workspace, size_t workspace_bytes,
+                      int32_t* status, void* stream) {
+  g_err[0] = 0;
+  int rc = check_pool("compact_pages", block_table, table_stride, P, B, refs, num_pages, 0);
+  if (!rc) rc = check_pool("compact_pages", new_table, new_stride, P, B, new_refs, num_pages, 0);
+  if (!rc) rc = check_page_caches("compact_pages", caches, n_caches);
+  if (rc) return rc;
+  if ((rc = check_pages_workspace("compact_pages", workspace, workspace_bytes, num_pages, 0))) return rc;
+  return compact_pages_launch(block_table, table_stride, new_table, new_stride, P, B, refs, new_refs, num_pages, caches, n_caches,
+                              static_cast<int32_t*>(workspace), status, static_cast<cudaStream_t>(stream));
 }
 
 int dsa_rope_fp8_quant_gated(const void* x_bf16, int64_t n_rows, int head_dim, int rope_dim, int interleave, int rows_per_pos,

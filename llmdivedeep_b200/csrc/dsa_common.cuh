@@ -17,6 +17,7 @@ enum : int {
   kStatusOk = 0,
   kStatusWaitTimeout = 1,     // a bounded mbarrier wait expired
   kStatusBadIndex = 2,        // a gathered index / page id was out of range (access skipped)
+  kStatusNoPages = 3,         // too few free pages: the call changed nothing
 };
 
 // By how much (log2 units) the scores of a row may exceed the softmax reference before it is raised.  Raising it rescales the

@@ -67,6 +67,7 @@
 
 #include "dsa_common.cuh"
 #include "dsa_host.h"
+#include "latent4.cuh"
 
 namespace dsa {
 
@@ -85,9 +86,11 @@ constexpr int kMlaXWarp = kMlaXBytes / 8;          // ... a warp's part of it
 constexpr int kMlaValidRing = 8;                   // validity bytes (64 per block) for the softmax: >= blocks in flight
 // The registers of the launch (896 threads x 72) are dealt out again: setmaxnreg moves what the issuing and gathering
 // warps do not need to the softmax.
-template <bool FP8_PAGED>
+// Where the rows come from: bf16 rows (prefill), records of the paged FP8 latent cache, records of the paged 4-bit one (latent4.cuh).
+enum MlaSrc : int { kSrcRows = 0, kSrcFp8 = 1, kSrc4 = 2 };
+template <bool PAGED>
 struct MlaRegs {                                   // decode's gather converts in registers
-  static constexpr int kSoftmax = FP8_PAGED ? 88 : 96, kOther = FP8_PAGED ? 48 : 40;
+  static constexpr int kSoftmax = PAGED ? 88 : 96, kOther = PAGED ? 48 : 40;
   static_assert(512 * kSoftmax + 384 * kOther <= 896 * 72, "more registers than the launch has");
 };
 constexpr int kMlaMaxParts = 8;                    // parts of a split list
@@ -116,12 +119,13 @@ static_assert(kColQ + kMlaPanels * 32 <= kMlaTmemCols, "tensor memory budget");
 
 struct MlaArgs {
   const uint8_t* kv;              // prefill: [S_kv, 576] bf16 rows
-  const uint8_t* cache;           // decode: [num_pages*64, 656] bytes
-  const int32_t* block_table;     // decode: [B, table_stride]
+  const uint8_t* cache;           // decode: [num_pages*64] records of 656 or 416 bytes
+  const int32_t* block_table;     // decode: [T / tokens_per_seq, table_stride]
   const int32_t* idx;             // [T, K] selected key positions (negative = empty)
   __nv_bfloat16* out;             // [T, H, 512]
   int64_t table_stride;
   int T, H, K;
+  int tokens_per_seq;             // decode: query rows of a sequence, one after the other
   int S_kv;                       // prefill: rows of kv; decode: logical positions per sequence
   int num_phys_rows;              // decode: rows of the cache
   float scale_log2e;              // softmax scale * log2(e)
@@ -215,11 +219,16 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// A gather warp's raw rows of one block: per row this CTA's 256 e4m3 values, the four scales, this CTA's 64 rope bytes.
-constexpr int kRawRow = 256 + 16 + 64, kRawRows = (kMlaBlk + kMlaGatherWarps - 1) / kMlaGatherWarps, kRawBytes = kRawRows * kRawRow;
-constexpr int kRawInBuf = kMlaKBytes / kRawBytes;                     // of the 2 x 11 pieces, those in the fifth KV buffer
-constexpr int kMlaSmemDecode = kMlaSmemBytes + (2 * kMlaGatherWarps - kRawInBuf) * kRawBytes;
-static_assert(kRawRows % 2 == 0 && kMlaSmemBytes % 16 == 0 && kMlaSmemDecode <= 232448, "raw rows of decode");
+// A gather warp's raw rows of one block: per row this CTA's 256 e4m3 values, the four scales, this CTA's 64 rope bytes; of a 4-bit
+// record this CTA's half as it is.
+constexpr int kRawRows = (kMlaBlk + kMlaGatherWarps - 1) / kMlaGatherWarps;
+template <int SRC>
+struct MlaRaw {
+  static constexpr int kRow = SRC == kSrc4 ? kLatent4Half : 256 + 16 + 64, kBytes = kRawRows * kRow, kPieces = 2 * kMlaGatherWarps;
+  static constexpr int kInBuf = kMlaKBytes / kBytes < kPieces ? kMlaKBytes / kBytes : kPieces;      // pieces in the fifth KV buffer
+  static constexpr int kSmem = kMlaSmemBytes + (SRC == kSrcRows ? 0 : (kPieces - kInBuf) * kBytes);
+  static_assert(kRawRows % 2 == 0 && kMlaSmemBytes % 16 == 0 && kSmem <= 232448, "raw rows of decode");
+};
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -243,11 +252,12 @@ __device__ __forceinline__ uint4 e4m3x8_to_bf16(uint2 raw, float sc) {
 
 // OVERLAPPED: a launch that may start under the end of the top-k's (decode of few sequences; in the others its loads and their
 // place cost 2 %: batch 148 122.3 -> 124.9 us).
-template <bool FP8_PAGED, bool OVERLAPPED>
+template <int SRC, bool OVERLAPPED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMlaThreads, 1)
 sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
                   const __grid_constant__ CUtensorMap tmap_o, const MlaArgs a) {
-  constexpr int NB = FP8_PAGED ? kMlaBufs - 1 : kMlaBufs;      // KV buffers in use (decode: the fifth one's space holds raw rows)
+  constexpr bool PAGED = SRC != kSrcRows;
+  constexpr int NB = PAGED ? kMlaBufs - 1 : kMlaBufs;      // KV buffers in use (decode: the fifth one's space holds raw rows)
   extern __shared__ __align__(1024) uint8_t smem[];            // the swizzled panels need 1024-byte alignment
   uint8_t* kv_s = smem;                                        // five buffers: four panels [64 keys x 128 B] and 64 x 64 B
   uint8_t* send_s = kv_s + kMlaBufs * kMlaKBytes;              // this CTA's partial score tile on its way out
@@ -274,7 +284,7 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
 
   const int cta = blockIdx.x & 1, peer = cta ^ 1;              // rank in the cluster = V half = contraction part
   const int unit = blockIdx.x >> 1;
-  const int part = FP8_PAGED ? unit - a.n_full : -1;           // >= 0: a part of a split slot list (prefill's are never cut)
+  const int part = PAGED ? unit - a.n_full : -1;           // >= 0: a part of a split slot list (prefill's are never cut)
   const int n_split = part < 0 ? 1 : a.n_split, t = part < 0 ? unit : a.n_full + part / n_split, split = part < 0 ? 0 : part % n_split;
   const int hg = blockIdx.z;
   const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -316,7 +326,7 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
       const uint32_t count = i == 1 ? 16u                                            // q_moved: lane 0 of the softmax warps
                              : (i == 3 || i == 4) ? 2u * n_quad                      // s_free, p_full: lane 0 of a set's warps
                              : (i >= 9 && i <= 16) ? 2u                              // pm_full: the two warps of a quadrant
-                             : (i >= 49 && i <= 53) ? (FP8_PAGED ? uint32_t(kMlaGatherWarps) : kMlaGatherWarps * 33u)
+                             : (i >= 49 && i <= 53) ? (PAGED ? uint32_t(kMlaGatherWarps) : kMlaGatherWarps * 33u)
                                                     : 1u;                            // the others
       mbar_init(bars + i, count);
     }
@@ -386,8 +396,8 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
   cluster_arrive();
   bool left = false;                                           // this warp has arrived at the barrier that the pair leaves through
 
-  if (warp >= kMlaSoftmaxWarps) regs_dec<MlaRegs<FP8_PAGED>::kOther>();
-  else regs_inc<MlaRegs<FP8_PAGED>::kSoftmax>();
+  if (warp >= kMlaSoftmaxWarps) regs_dec<MlaRegs<PAGED>::kOther>();
+  else regs_inc<MlaRegs<PAGED>::kSoftmax>();
   if (warp == kMlaMmaWarp) {
     // ------------------------------- MMA issuer -------------------------------
     // The partial scores of a block travel to the peer and through the softmax while the next blocks are scored: P.V of a
@@ -456,7 +466,7 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
     constexpr int kG = kMlaGatherWarps;
     // Five of a warp's six slots are always within the block: said so, prefill of 128 heads takes 2160 us instead of 2202 (4096 x 2048
     // keys), of 64 heads 1988 instead of 2044.  (Decode gains nothing.)
-    if constexpr (!FP8_PAGED) __builtin_assume(w4 < kG);
+    if constexpr (!PAGED) __builtin_assume(w4 < kG);
     bool ok = true;
     // A warp fetches every kG-th slot of a block, six at most: lane j < 6 keeps the id of slot w4 + 11 j.
     auto load_pos = [&](int blk) -> int {
@@ -466,7 +476,7 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
     auto mark = [&](int blk, bool used) {
       if (slot < kMlaBlk) valid_s[(blk % kMlaValidRing) * kMlaBlk + slot] = used;
     };
-    if constexpr (!FP8_PAGED) {
+    if constexpr (!PAGED) {
       // Row ids are requested one block ahead.  512 latent bytes are one 16-byte cp.async per lane, this CTA's 64 rope bytes
       // of all six rows another one.  Nobody waits for the copies here: they arrive on the block's barrier by themselves,
       // and the MMA warp orders them before the tensor core's reads (a proxy fence anywhere on the path between the two
@@ -527,10 +537,9 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
       // cp.async two blocks ahead (a cache row is a DRAM and often a TLB miss away, ~3000 cycles), then 8 e4m3 values per
       // lane and row through registers into the KV buffer.  The warps never wait for one another.  Positions travel four
       // blocks ahead, page-table entries three.
-      constexpr int kRows = kRawRows;
-      auto table_entry = [&](int pos) -> int {
-        return (pos >= 0 && pos < a.S_kv) ? __ldg(a.block_table + (int64_t)t * a.table_stride + pos / kLatentPage) : -1;
-      };
+      constexpr int kRows = kRawRows, kRawRow = MlaRaw<SRC>::kRow, kRawBytes = MlaRaw<SRC>::kBytes, kRawInBuf = MlaRaw<SRC>::kInBuf;
+      const int32_t* table = a.block_table + (int64_t)(a.tokens_per_seq > 1 ? t / a.tokens_per_seq : t) * a.table_stride;
+      auto table_entry = [&](int pos) -> int { return (pos >= 0 && pos < a.S_kv) ? __ldg(table + pos / kLatentPage) : -1; };
       auto cache_row = [&](int pos, int phys) -> int {   // -1 = empty slot; bad positions and page ids are flagged and skipped
         if (pos < 0) return -1;
         if (pos < a.S_kv && phys >= 0 && (int64_t)(phys + 1) * kLatentPage <= a.num_phys_rows)
@@ -547,6 +556,16 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
       // request the warp's rows of a block; an empty slot is zero-filled, values and scales
       auto fetch = [&](int blk, int id) {
         uint8_t* st = stage_of(blk);
+        if constexpr (SRC == kSrc4) {                  // thirteen 16-byte pieces a row, the rows one after the other
+#pragma unroll
+          for (int u = 0; u < (kRows * 13 + 31) / 32; ++u) {
+            const int c = u * 32 + lane, j = c / 13, rid = __shfl_sync(0xffffffffu, id, j);
+            if (c < kRows * 13)
+              cp_async_16(st + c * 16, a.cache + (int64_t)max(rid, 0) * kLatent4Bytes + cta * kLatent4Half + (c - j * 13) * 16, rid >= 0 ? 16 : 0);
+          }
+          cp_async_commit();
+          return;
+        }
 #pragma unroll
         for (int u = 0; u < kRows / 2; ++u) {          // two rows of 256 values per instruction
           const int j = 2 * u + (lane >> 4), rid = __shfl_sync(0xffffffffu, id, j);
@@ -592,16 +611,24 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
           const int r = w4 + j * kG;
-          const uint2 raw = *reinterpret_cast<const uint2*>(st + j * kRawRow + lane * 8);
-          const float sc = *reinterpret_cast<const float*>(st + j * kRawRow + 256 + cta * 8 + (lane >> 4) * 4);
-          const uint4 v = e4m3x8_to_bf16(raw, sc);
+          uint4 v;
+          if constexpr (SRC == kSrc4) {
+            uint32_t p[4];
+            latent4_codes(*reinterpret_cast<const uint32_t*>(st + j * kRawRow + lane * 4), p);
+            const uint32_t sc = latent4_scale(st[j * kRawRow + kLatent4Scales + (lane >> 1)]);
+            v = make_uint4(mul_bf16x2(p[0], sc), mul_bf16x2(p[1], sc), mul_bf16x2(p[2], sc), mul_bf16x2(p[3], sc));
+          } else {
+            const uint2 raw = *reinterpret_cast<const uint2*>(st + j * kRawRow + lane * 8);
+            const float sc = *reinterpret_cast<const float*>(st + j * kRawRow + 256 + cta * 8 + (lane >> 4) * 4);
+            v = e4m3x8_to_bf16(raw, sc);
+          }
           if (r < kMlaBlk) *reinterpret_cast<uint4*>(dst_lat + r * 128 + (((lane ^ r) & 7) << 4)) = v;
         }
         {
           const int r = w4 + (lane >> 2) * kG;
           if (lane < 4 * kRows && r < kMlaBlk)
             *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane ^ (r >> 1)) & 3) << 4)) =
-                *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16);
+                *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + (SRC == kSrc4 ? kLatent4Rope : 272) + (lane & 3) * 16);
         }
         __syncwarp();                                  // (the MMA warp makes the writes visible to the tensor core's reads)
         if (lane == 0) mbar_arrive(&kv_full[kvb]);
@@ -629,6 +656,12 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
         for (int c = 0; c < 4; ++c) {
           const uint4 w = *reinterpret_cast<const uint4*>(src + ((((hp & 1) * 4 + c) ^ (row & 7)) << 4));
           qv[4 * c + 0] = w.x; qv[4 * c + 1] = w.y; qv[4 * c + 2] = w.z; qv[4 * c + 3] = w.w;
+        }
+        if constexpr (SRC == kSrc4) {                  // the latents come 2^-14 times what they are (latent4.cuh)
+          if (hp < 8) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) qv[i] = mul_bf16x2(qv[i], kLatent4GainPair);
+          }
         }
         tmem_st16(t_row + kColQ + hp * 16, qv);
       }
@@ -783,7 +816,7 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
         const float2 ml = sum_s[u * 128 + row];
         if (ml.x != -CUDART_INF_F) l += ml.y * fast_exp2(ml.x - mt);
       }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l > 0.f ? (SRC == kSrc4 ? kLatent4Gain : 1.f) / l : 0.f;
       __nv_bfloat16* orow = a.out + ((int64_t)t * a.H + hg * 128 + row) * kMlaDv + cta * kMlaDvHalf;
       const int64_t prow = (int64_t)part * a.H + hg * 128 + row;
       if (part >= 0 && quarter == 0 && row < heads_here)         // what this CTA's half of the columns is weighted with
@@ -892,7 +925,7 @@ __global__ void __launch_bounds__(128) sparse_mla_combine_kernel(const MlaArgs a
 int make_tmap_2d_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t inner_bytes, uint64_t row_pitch,
                        uint32_t box_bytes, uint32_t box_rows);
 
-template <bool FP8_PAGED, bool OVERLAPPED>
+template <int SRC, bool OVERLAPPED>
 static int launch_mla(const void* q, const void* kv, const MlaArgs& args, cudaStream_t stream) {
   if (args.T == 0 || args.H == 0) return DSA_OK;
   if (args.K > kMlaMaxK) return set_error(DSA_ERR_SHAPE, "sparse_mla: K (%d) exceeds %d", args.K, kMlaMaxK);
@@ -908,8 +941,8 @@ static int launch_mla(const void* q, const void* kv, const MlaArgs& args, cudaSt
     if ((rc = make_tmap_2d_bytes(&to, a.out, (uint64_t)a.T * a.H, kMlaDv * 2, kMlaDv * 2, 128, 128))) return rc;
     a.tma_out = 1;
   }
-  auto kern = sparse_mla_kernel<FP8_PAGED, OVERLAPPED>;
-  constexpr int smem_bytes = FP8_PAGED ? kMlaSmemDecode : kMlaSmemBytes;
+  auto kern = sparse_mla_kernel<SRC, OVERLAPPED>;
+  constexpr int smem_bytes = MlaRaw<SRC>::kSmem;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess)
     return set_error(DSA_ERR_CUDA, "sparse_mla: cannot raise dynamic shared memory to %d", smem_bytes);
   const int n_parts = a.T - a.n_full;
@@ -934,7 +967,7 @@ int sparse_mla_prefill_launch(const void* q, const void* kv, const int32_t* idx,
   a.status = status;
   a.n_full = T;
   a.n_split = 1;
-  return launch_mla<false, false>(q, kv, a, stream);
+  return launch_mla<kSrcRows, false>(q, kv, a, stream);
 }
 
 // A CTA pair per query fills the GPU in rounds of (SMs / 2 / head groups) queries; the last, partly filled round would
@@ -957,8 +990,8 @@ size_t mla_decode_workspace_bytes(int B, int H, int K) {
   return parts * mla_part_bytes(H);
 }
 
-int sparse_mla_decode_launch(const void* q, const void* cache, const int32_t* block_table, int64_t table_stride,
-                             const int32_t* idx, void* out, int B, int H, int K, int num_pages, int max_ctx,
+int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,
+                             int tokens_per_seq, const int32_t* idx, void* out, int B, int H, int K, int num_pages, int max_ctx,
                              float scale, void* workspace, size_t workspace_bytes, int32_t* status, int overlapped,
                              cudaStream_t stream) {
   MlaArgs a{};
@@ -982,10 +1015,12 @@ int sparse_mla_decode_launch(const void* q, const void* cache, const int32_t* bl
   a.idx = idx;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.T = B; a.H = H; a.K = K; a.S_kv = max_ctx;
+  a.tokens_per_seq = tokens_per_seq;
   a.num_phys_rows = num_pages * kLatentPage;
   a.scale_log2e = scale * 1.4426950408889634f;
   a.status = status;
-  return overlapped ? launch_mla<true, true>(q, nullptr, a, stream) : launch_mla<true, false>(q, nullptr, a, stream);
+  if (record_bytes == kLatent4Bytes) return overlapped ? launch_mla<kSrc4, true>(q, nullptr, a, stream) : launch_mla<kSrc4, false>(q, nullptr, a, stream);
+  return overlapped ? launch_mla<kSrcFp8, true>(q, nullptr, a, stream) : launch_mla<kSrcFp8, false>(q, nullptr, a, stream);
 }
 
 }  // namespace dsa

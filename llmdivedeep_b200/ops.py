@@ -7,6 +7,7 @@ Nothing here computes on the CPU.
 from __future__ import annotations
 
 import contextlib
+import struct
 from typing import Optional
 
 import torch
@@ -81,7 +82,8 @@ def check_status(device) -> None:
     v = int(w.item())
     if v:
         w.zero_()
-        what = {1: "a bounded wait inside a kernel expired", 2: "an index or page id was out of range"}.get(v, "?")
+        what = {1: "a bounded wait inside a kernel expired", 2: "an index or page id was out of range",
+                3: "too few free pages"}.get(v, "?")
         raise DsaError(f"device status {v}: {what}")
 
 
@@ -307,29 +309,40 @@ def block_sparse_attn(q, k, v, lut, num, sm_scale: float, out: Optional[torch.Te
     return out
 
 
+RECORD_BYTES = (656, 416)         # a token's record in the paged latent cache: FP8, 4 bits
+
+
 def sparse_mla_decode_paged(q, cache, block_table, idx, scale: float, max_ctx: Optional[int] = None,
-                            out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Decode step over the paged FP8 latent cache.  q [B,H,576] bf16, cache uint8
-    [num_pages*64, 656], block_table [B,P] int32, idx [B,K] int32 logical positions."""
+                            out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                            tokens_per_seq: int = 1) -> torch.Tensor:
+    """Decode step over the paged latent cache.  q [T,H,576] bf16, cache uint8 [num_pages*64, 656] (FP8 records,
+    pack_latent_cache) or [num_pages*64, 416] (4-bit records, pack_latent4), block_table [B,P] int32, idx [T,K] int32
+    logical positions.  T = B * tokens_per_seq: a sequence's query rows one after the other.  Returns bf16 [T,H,512]."""
     dev = _need_cuda(q, cache, block_table, idx, out, workspace)
     if q.dtype != torch.bfloat16 or cache.dtype != torch.uint8 or idx.dtype != torch.int32 or block_table.dtype != torch.int32:
         raise DsaError("sparse_mla_decode_paged takes bf16 q, uint8 cache, int32 block_table/idx")
-    if cache.dim() != 2 or cache.shape[1] != 656 or cache.shape[0] % 64:
-        raise DsaError("cache must be uint8 [num_pages*64, 656]")
+    if cache.dim() != 2 or cache.shape[1] not in RECORD_BYTES or cache.shape[0] % 64:
+        raise DsaError("cache must be uint8 [num_pages*64, 656] or [num_pages*64, 416]")
     q, cache, block_table, idx = q.contiguous(), cache.contiguous(), block_table.contiguous(), idx.contiguous()
-    B, H, _ = q.shape
+    T, H, dq = q.shape
     if max_ctx is None:
         max_ctx = block_table.shape[1] * 64
-    out = _check_attn_out(out, (B, H, 512), q.device)
+    plain = cache.shape[1] == 656 and tokens_per_seq == 1
+    if not plain and (tokens_per_seq < 1 or dq != 576 or idx.dim() != 2 or idx.shape[0] != T or block_table.dim() != 2
+                      or block_table.shape[0] * tokens_per_seq < T):
+        raise DsaError(f"bad shapes q {tuple(q.shape)} idx {tuple(idx.shape)} block_table {tuple(block_table.shape)}, {tokens_per_seq} tokens a sequence")
+    out = _check_attn_out(out, (T, H, 512), q.device)
     lib = _lib.load()
     if workspace is None:
-        need = lib.dsa_sparse_mla_decode_workspace_bytes(B, H, idx.shape[1])
+        need = lib.dsa_sparse_mla_decode_workspace_bytes(T, H, idx.shape[1])
         workspace = _workspace(q.device, need) if need else None
+    rest = (_ptr(idx), _ptr(out), T, H, idx.shape[1], cache.shape[0] // 64, max_ctx, float(scale), _ptr(workspace),
+            workspace.numel() if workspace is not None else 0, _ptr(status_word(dev)), _stream(dev))
     with _on(dev):
-        check(lib.dsa_sparse_mla_decode_paged(_ptr(q), _ptr(cache), _ptr(block_table), block_table.stride(0), _ptr(idx),
-                                              _ptr(out), B, H, idx.shape[1], cache.shape[0] // 64, max_ctx, float(scale),
-                                              _ptr(workspace), workspace.numel() if workspace is not None else 0,
-                                              _ptr(status_word(dev)), _stream(dev)))
+        if plain:
+            check(lib.dsa_sparse_mla_decode_paged(_ptr(q), _ptr(cache), _ptr(block_table), block_table.stride(0), *rest))
+        else:
+            check(lib.dsa_sparse_mla_decode_records(_ptr(q), _ptr(cache), cache.shape[1], _ptr(block_table), block_table.stride(0), tokens_per_seq, *rest))
     return out
 
 
@@ -351,7 +364,7 @@ def decode_step(q_fp8, weights, kcache, kscale, block_table, ctx_len, q, cache, 
     Bi, Hi, D = q_fp8.shape
     if (B == 0 or Bi != B or dq != 576 or tuple(weights.shape) != (B, Hi) or kcache.dim() != 2 or kcache.shape[1] != D or kcache.shape[0] % 64
             or kscale.dim() != 1 or kscale.shape[0] != kcache.shape[0] or block_table.shape[0] != B or ctx_len.numel() != B
-            or cache.dim() != 2 or cache.shape[1] != 656 or cache.shape[0] % 64 or idx.shape[0] != B or tuple(out.shape) != (B, H, 512)
+            or cache.dim() != 2 or cache.shape[1] not in RECORD_BYTES or cache.shape[0] % 64 or idx.shape[0] != B or tuple(out.shape) != (B, H, 512)
             or logits.get_device() != i or logits.dim() != 2 or logits.shape[0] < B or logits.shape[1] < max_ctx or logits.stride(1) != 1
             or logits.stride(0) < max_ctx):
         return False
@@ -360,12 +373,16 @@ def decode_step(q_fp8, weights, kcache, kscale, block_table, ctx_len, q, cache, 
             or out.dtype != torch.bfloat16 or logits.dtype != torch.float32 or workspace.dtype != torch.uint8
             or weights.dtype not in (torch.float32, torch.bfloat16)):
         return False
-    with _on(dev):
-        check(_lib.load().dsa_decode_step(
-            q_fp8.data_ptr(), weights.data_ptr(), _w_dtype(weights), kcache.data_ptr(), kscale.data_ptr(), kcache.shape[0] // 64,
+    lib = _lib.load()
+    head = (q_fp8.data_ptr(), weights.data_ptr(), _w_dtype(weights), kcache.data_ptr(), kscale.data_ptr(), kcache.shape[0] // 64,
             block_table.data_ptr(), block_table.stride(0), ctx_len.data_ptr(), logits.data_ptr(), logits.stride(0), B, Hi, D,
-            max_ctx, idx.shape[1], idx.data_ptr(), q.data_ptr(), cache.data_ptr(), cache.shape[0] // 64, out.data_ptr(), H, float(scale),
-            workspace.data_ptr(), workspace.numel(), status_word(dev).data_ptr(), _stream(dev)))
+            max_ctx, idx.shape[1], idx.data_ptr(), q.data_ptr(), cache.data_ptr())
+    rest = (cache.shape[0] // 64, out.data_ptr(), H, float(scale), workspace.data_ptr(), workspace.numel(), status_word(dev).data_ptr())
+    with _on(dev):
+        if cache.shape[1] == 656:
+            check(lib.dsa_decode_step(*head, *rest, _stream(dev)))
+        else:
+            check(lib.dsa_decode_step_records(*head, cache.shape[1], *rest, _stream(dev)))
     return True
 
 
@@ -569,3 +586,185 @@ def rope_fp8_quant(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rope_d
                                            cos.shape[0], _ptr(q), _ptr(scale), _ptr(gate), float(gate_mul[0]), float(gate_mul[1]),
                                            _ptr(w), _stream(dev)))
     return (q, scale) if w is None else (q, scale, w)
+
+
+# ---- the paged latent cache in 4 bits ---------------------------------------------------------------------------------
+def _check_records4(cache: torch.Tensor) -> None:
+    if cache.dtype != torch.uint8 or cache.dim() != 2 or cache.shape[1] != 416 or not cache.is_contiguous():
+        raise DsaError(f"4-bit latent cache must be contiguous uint8 [rows, 416], got {cache.dtype} {tuple(cache.shape)}")
+
+
+def pack_latent4(kv: torch.Tensor, cache: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                 keys: Optional[tuple] = None) -> torch.Tensor:
+    """Latent rows [N, 576] (bf16 or fp32) -> 416-byte records (include/dsa_b200.h) at the rows ``slots`` (int32 [N], negative =
+    skip; None: row i) of ``cache`` (None: a new uint8 [N, 416]), one kernel.  Returns the cache.  ``keys`` = (k_fp8 [N,128] e4m3,
+    k_scale [N] fp32, kcache [rows,128] e4m3, kscale [rows] fp32) sends the tokens' indexer keys to the same rows of the paged key
+    cache along with them."""
+    dev = _need_cuda(kv, cache, slots, *(keys or ()))
+    if kv.dtype not in (torch.bfloat16, torch.float32) or kv.dim() != 2 or kv.shape[1] != 576:
+        raise DsaError(f"pack_latent4 takes bf16 or fp32 rows [N, 576], got {kv.dtype} {tuple(kv.shape)}")
+    N = kv.shape[0]
+    rs, cs = kv.stride()
+    if N and (cs != 1 or (N > 1 and (rs < 576 or rs * kv.element_size() % 16)) or kv.data_ptr() % 16):
+        kv = kv.clone(memory_format=torch.contiguous_format)
+    if cache is None:
+        cache = torch.empty(N, 416, dtype=torch.uint8, device=dev)
+    _check_records4(cache)
+    slots = _as_i32(slots, N, "slots")
+    k8 = ksc = kcache = kscale = None
+    if keys is not None:
+        k8, ksc, kcache, kscale = keys
+        rows = cache.shape[0]
+        if (k8.dtype != FP8 or kcache.dtype != FP8 or ksc.dtype != torch.float32 or kscale.dtype != torch.float32 or tuple(k8.shape) != (N, 128)
+                or tuple(kcache.shape) != (rows, 128) or ksc.numel() != N or tuple(kscale.shape) != (rows,)):
+            raise DsaError("keys must be e4m3 [N,128], fp32 [N], and the caches e4m3 [rows,128], fp32 [rows] of the latent cache's rows")
+        if not (kcache.is_contiguous() and kscale.is_contiguous()):
+            raise DsaError("the key cache and its scales must be contiguous")
+        k8, ksc = k8.contiguous(), ksc.contiguous()
+    with _on(dev):
+        check(_lib.load().dsa_pack_latent4(kv.data_ptr(), 1 if kv.dtype == torch.bfloat16 else 0, kv.stride(0) if N > 1 else 576, N, cache.data_ptr(),
+                                           cache.shape[0], _ptr(slots), _ptr(k8), _ptr(ksc), _ptr(kcache), _ptr(kscale),
+                                           _ptr(status_word(dev)), _stream(dev)))
+    return cache
+
+
+def unpack_latent4(cache: torch.Tensor, n: Optional[int] = None, block_table: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Positions 0..n-1 of one sequence as bf16 rows [n, 576], from its 4-bit records: position p is record
+    block_table[p // 64] * 64 + p % 64 (block_table int32 [P], a row of the batch's; None: record p).  What a chunked prefill
+    hands to sparse_mla_prefill.  ``out`` may have rows further apart than 576 values."""
+    dev = _need_cuda(cache, block_table, out)
+    _check_records4(cache)
+    if block_table is not None:
+        if block_table.dtype != torch.int32 or block_table.dim() != 1:
+            raise DsaError("block_table must be one sequence's int32 [pages]")
+        block_table = block_table.contiguous()
+    most = cache.shape[0] if block_table is None else block_table.shape[0] * 64
+    n = most if n is None else int(n)
+    if n < 0 or n > most:
+        raise DsaError(f"{n} positions of a sequence that has room for {most}")
+    if out is None:
+        out = torch.empty(n, 576, dtype=torch.bfloat16, device=dev)
+    elif (out.dtype != torch.bfloat16 or tuple(out.shape) != (n, 576) or (n and out.stride(1) != 1) or (n > 1 and out.stride(0) % 8)
+          or (n > 1 and out.stride(0) < 576)):
+        raise DsaError(f"out must be bf16 [{n}, 576], rows a multiple of 8 values apart, got {out.dtype} {tuple(out.shape)} strides {tuple(out.stride())}")
+    with _on(dev):
+        check(_lib.load().dsa_unpack_latent4(cache.data_ptr(), cache.shape[0], _ptr(block_table), n, out.data_ptr(), out.stride(0) if n > 1 else 576,
+                                             _ptr(status_word(dev)), _stream(dev)))
+    return out
+
+
+# ---- pages of the paged caches ------------------------------------------------------------------------------------------
+def _page_caches(caches, num_pages: int):
+    """The caches as an array of dsa_page_cache.  A cache is [num_pages*64, ...] or, for several layers, [layers, num_pages*64, ...]."""
+    rows, packed = num_pages * 64, []
+    for t in caches:
+        shape = t.shape
+        one, many = len(shape) >= 1 and shape[0] == rows, len(shape) >= 2 and shape[1] == rows
+        if one == many:
+            raise DsaError(f"a cache must be [{rows}, ...] or [layers, {rows}, ...], got {tuple(shape)}")
+        layers = 1 if one else shape[0]
+        if not t.is_contiguous() and not (many and t[0].is_contiguous()):
+            raise DsaError("the pages of a cache must be contiguous")
+        layer_bytes = (t.stride(0) if many else 0) * t.element_size()
+        packed.append(struct.pack("=Qqii", t.data_ptr(), layer_bytes, layers, t.element_size() * (t.numel() // max(1, layers * rows))))
+    return b"".join(packed), len(packed)
+
+
+def _check_pool(table, ctx_len, refs) -> tuple:
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.numel() and table.stride(1) != 1):
+        raise DsaError("block_table must be int32 [B, pages] with unit column stride")
+    B, P = table.shape
+    if ctx_len is not None:
+        _as_i32(ctx_len, B, "ctx_len")
+    if refs.dtype != torch.int32 or refs.dim() != 1 or not refs.is_contiguous():
+        raise DsaError("refs must be a contiguous int32 [num_pages] tensor")
+    return B, P, refs.shape[0]
+
+
+def _list_i32(t, name: str):
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise DsaError(f"{name} must be a contiguous one-dimensional int32 tensor")
+    return t
+
+
+def copy_pages(caches, src, dst, tokens=None, num_pages: Optional[int] = None) -> None:
+    """Page src[i] -> page dst[i] (int32 [n], negative = skip) in every cache of the list and every layer of it, one launch; with
+    ``tokens`` (int32 [n]) only the first tokens[i] of a page's 64.  No page may be written twice, nor be written and read.
+    ``num_pages`` is needed only where the caches' shapes leave it open."""
+    caches = list(caches)
+    dev = _need_cuda(*caches, src, dst, tokens)
+    n = _list_i32(src, "src").shape[0]
+    dst, tokens = _as_i32(dst, n, "dst"), _as_i32(tokens, n, "tokens")
+    if num_pages is None:
+        rows = set.intersection(*({s for s in t.shape[:2] if s and s % 64 == 0} for t in caches)) if caches else {0}
+        if len(rows) != 1:
+            raise DsaError("the caches' shapes leave the number of pages open: give num_pages")
+        num_pages = rows.pop() // 64
+    packed, count = _page_caches(caches, num_pages)
+    with _on(dev):
+        check(_lib.load().dsa_copy_pages(packed, count, num_pages, src.data_ptr(), dst.data_ptr(), _ptr(tokens), n, _ptr(status_word(dev)), _stream(dev)))
+
+
+def extend_pages(block_table, ctx_len, refs, rows, n_new, max_new: int) -> torch.Tensor:
+    """Room for n_new[i] (int32, 0..max_new) more tokens in row rows[i] (int32, all different): takes the lowest free pages, in order,
+    and writes block_table, ctx_len and refs.  Returns the new tokens' cache rows, int32 [n, max_new], -1 behind them.  All or
+    nothing: with too few free pages (status 3) or a bad argument (status 2) nothing changes and every slot is -1."""
+    dev = _need_cuda(block_table, ctx_len, refs, rows, n_new)
+    B, P, num_pages = _check_pool(block_table, ctx_len, refs)
+    n = _list_i32(rows, "rows").shape[0]
+    n_new = _as_i32(n_new, n, "n_new")
+    max_new = int(max_new)
+    lib = _lib.load()
+    slots = torch.empty(n, max(max_new, 0), dtype=torch.int32, device=dev)
+    ws = _workspace(dev, lib.dsa_pages_workspace_bytes(num_pages, n))
+    with _on(dev):
+        check(lib.dsa_extend_pages(block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages, rows.data_ptr(),
+                                   n_new.data_ptr(), n, max_new, slots.data_ptr(), ws.data_ptr(), ws.numel(), _ptr(status_word(dev)), _stream(dev)))
+    return slots
+
+
+def fork_pages(block_table, ctx_len, refs, parents, children, caches=()) -> None:
+    """Row children[i] (empty, all different) becomes a copy of row parents[i] (int32 lists): full pages are shared, a partly filled
+    last one is copied to a page of the child's own in every cache.  Writes block_table, ctx_len and refs; all or nothing, as
+    extend_pages."""
+    caches = list(caches)
+    dev = _need_cuda(block_table, ctx_len, refs, parents, children, *caches)
+    B, P, num_pages = _check_pool(block_table, ctx_len, refs)
+    n = _list_i32(parents, "parents").shape[0]
+    children = _as_i32(children, n, "children")
+    packed, count = _page_caches(caches, num_pages)
+    lib = _lib.load()
+    ws = _workspace(dev, lib.dsa_pages_workspace_bytes(num_pages, n))
+    with _on(dev):
+        check(lib.dsa_fork_pages(block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages, parents.data_ptr(),
+                                 children.data_ptr(), n, packed, count, ws.data_ptr(), ws.numel(), _ptr(status_word(dev)), _stream(dev)))
+
+
+def free_pages(block_table, ctx_len, refs, rows) -> None:
+    """Rows ``rows`` (int32) become empty and give their pages back: refs - 1, -1 in block_table, 0 in ctx_len."""
+    dev = _need_cuda(block_table, ctx_len, refs, rows)
+    B, P, num_pages = _check_pool(block_table, ctx_len, refs)
+    n = _list_i32(rows, "rows").shape[0]
+    with _on(dev):
+        check(_lib.load().dsa_free_pages(block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages,
+                                         rows.data_ptr(), n, _ptr(status_word(dev)), _stream(dev)))
+
+
+def compact_pages(block_table, refs, caches, out: Optional[tuple] = None) -> tuple:
+    """Moves the pages in use to the lowest ids, the highest ones into the lowest gaps, in every cache.  Returns (block_table, refs)
+    as they are afterwards: new tensors, or ``out`` (which may be the given ones).  The pages moved from stay as they are, so work in
+    flight on the old table reads right until one of them is taken."""
+    caches = list(caches)
+    dev = _need_cuda(block_table, refs, *caches, *(out or ()))
+    B, P, num_pages = _check_pool(block_table, None, refs)
+    new_table, new_refs = out if out is not None else (torch.empty_like(block_table, memory_format=torch.contiguous_format), torch.empty_like(refs))
+    if _check_pool(new_table, None, new_refs) != (B, P, num_pages):
+        raise DsaError("out must be a block table and refs of the same sizes")
+    packed, count = _page_caches(caches, num_pages)
+    lib = _lib.load()
+    ws = _workspace(dev, lib.dsa_pages_workspace_bytes(num_pages, 0))
+    with _on(dev):
+        check(lib.dsa_compact_pages(block_table.data_ptr(), block_table.stride(0), new_table.data_ptr(), new_table.stride(0), P, B, refs.data_ptr(),
+                                    new_refs.data_ptr(), num_pages, packed, count, ws.data_ptr(), ws.numel(), _ptr(status_word(dev)), _stream(dev)))
+    return new_table, new_refs
