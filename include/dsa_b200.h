@@ -217,7 +217,10 @@ int dsa_unpack_latent4(const void* cache, int64_t cache_rows, const int32_t* blo
 
 /* dsa_sparse_mla_decode_paged over records of record_bytes = 656 (FP8) or 416 (4 bits), for tokens_per_seq query rows of
  * each sequence: rows r = b*tokens_per_seq .. of q [T, H, 576], idx [T, K] and out [T, H, 512] go by row b of block_table.
- * The workspace is that of T sequences.  (4 bits: |q| of the latent part must stay below 2^113.) */
+ * (4 bits: |q| of the latent part must stay below 2^113.)  Lists may be cut into parts that different SMs take and a second
+ * kernel merges in fp32; the parts' `workspace` (16-byte aligned) of dsa_sparse_mla_decode_records_workspace_bytes bytes is
+ * enough for every call of up to T rows.  With a smaller one, or NULL, the call works with fewer parts or none. */
+size_t dsa_sparse_mla_decode_records_workspace_bytes(int record_bytes, int T, int H, int K);
 int dsa_sparse_mla_decode_records(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table,
                                   int64_t table_stride, int tokens_per_seq, const int32_t* idx, void* out_bf16, int T, int H,
                                   int K, int num_pages, int max_ctx, float scale, void* workspace, size_t workspace_bytes,

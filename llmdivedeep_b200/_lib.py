@@ -48,6 +48,7 @@ SIGNATURES = {
     "dsa_pack_latent4": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                  c_void_p, c_void_p, c_void_p]),
     "dsa_unpack_latent4": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "dsa_sparse_mla_decode_records_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "dsa_sparse_mla_decode_records": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int,
                                               c_int, c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
     "dsa_decode_step_records": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,

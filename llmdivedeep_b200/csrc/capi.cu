@@ -57,6 +57,7 @@ int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes,
                              float scale, void* workspace, size_t workspace_bytes, int32_t* status, int overlapped,
                              cudaStream_t stream);
 size_t mla_decode_workspace_bytes(int B, int H, int K);
+size_t mla_decode_records_workspace_bytes(int record_bytes, int T, int H, int K);
 int block_sparse_mha_launch(const void* q, const void* k, const void* v, const int32_t* lut, const int32_t* num,
                             void* out, int B, int S, int H, int topk, float scale, int32_t* status,
                             cudaStream_t stream);
@@ -297,6 +298,11 @@ int dsa_decode_step(const void* q_fp8, const void* w, int w_dtype, const void* k
 size_t dsa_sparse_mla_decode_workspace_bytes(int B, int H, int K) {
   if (B <= 0 || H <= 0 || K <= 0) return 0;
   return mla_decode_workspace_bytes(B, H, K);
+}
+
+size_t dsa_sparse_mla_decode_records_workspace_bytes(int record_bytes, int T, int H, int K) {
+  if (T <= 0 || H <= 0 || K <= 0) return 0;
+  return mla_decode_records_workspace_bytes(record_bytes, T, H, K);
 }
 
 int dsa_fp8_quant_per_block(const void* x, int x_dtype, int64_t n_blocks, int block_size, void* q_fp8, float* scale,

@@ -93,6 +93,7 @@ struct MlaRegs {                                   // decode's gather converts i
   static constexpr int kSoftmax = PAGED ? 88 : 96, kOther = PAGED ? 48 : 40;
   static_assert(512 * kSoftmax + 384 * kOther <= 896 * 72, "more registers than the launch has");
 };
+constexpr int kMlaFewHeads = 32;                   // up to here calls go to the kernels for few heads (sparse_mla_few.cu, sparse_mla_few4.cu)
 constexpr int kMlaMaxParts = 8;                    // parts of a split list
 constexpr int kMlaMaxK = 2048;                     // slots of a list
 constexpr int kMlaThreads = 896, kMlaSoftmaxWarps = 16, kMlaMmaWarp = 16, kMlaGatherWarp0 = 17, kMlaGatherWarps = 11;
@@ -957,7 +958,7 @@ int sparse_mla_few_launch(const void* q, const void* kv, const int32_t* idx, voi
 
 int sparse_mla_prefill_launch(const void* q, const void* kv, const int32_t* idx, void* out, int T, int H, int S_kv,
                               int K, float scale, int32_t* status, cudaStream_t stream) {
-  if (H <= 32) return sparse_mla_few_launch(q, kv, idx, out, T, H, S_kv, K, scale, status, stream);
+  if (H <= kMlaFewHeads) return sparse_mla_few_launch(q, kv, idx, out, T, H, S_kv, K, scale, status, stream);
   MlaArgs a{};
   a.kv = static_cast<const uint8_t*>(kv);
   a.idx = idx;
@@ -990,10 +991,22 @@ size_t mla_decode_workspace_bytes(int B, int H, int K) {
   return parts * mla_part_bytes(H);
 }
 
+int sparse_mla_few4_launch(const void* q, const void* cache, const int32_t* block_table, int64_t table_stride, int tokens_per_seq, const int32_t* idx,
+                           void* out, int T, int H, int K, int num_pages, int max_ctx, float scale, void* workspace, size_t workspace_bytes,
+                           int32_t* status, int overlapped, cudaStream_t stream);
+size_t few4_workspace_bytes(int T, int H, int K);
+
+size_t mla_decode_records_workspace_bytes(int record_bytes, int T, int H, int K) {
+  return record_bytes == kLatent4Bytes && H <= kMlaFewHeads ? few4_workspace_bytes(T, H, K) : mla_decode_workspace_bytes(T, H, K);
+}
+
 int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,
                              int tokens_per_seq, const int32_t* idx, void* out, int B, int H, int K, int num_pages, int max_ctx,
                              float scale, void* workspace, size_t workspace_bytes, int32_t* status, int overlapped,
                              cudaStream_t stream) {
+  if (record_bytes == kLatent4Bytes && H <= kMlaFewHeads)
+    return sparse_mla_few4_launch(q, cache, block_table, table_stride, tokens_per_seq, idx, out, B, H, K, num_pages, max_ctx, scale, workspace,
+                                  workspace_bytes, status, overlapped, stream);
   MlaArgs a{};
   const int pairs = mla_pairs(H), rest = B % pairs;
   int ns = mla_parts_per_query(rest, pairs, K);

@@ -406,7 +406,7 @@ class DecodeWorkspace:
         self.k = min(topk, max_ctx)                    # selected keys per sequence (the kernels write rows at this stride)
         self.idx = torch.empty(batch, self.k, dtype=torch.int32, device=device)
         self.out = torch.empty(batch, heads, 512, dtype=torch.bfloat16, device=device)
-        need = _lib.load().dsa_sparse_mla_decode_workspace_bytes(batch, heads, min(topk, max_ctx))
+        need = max(_lib.load().dsa_sparse_mla_decode_records_workspace_bytes(width, batch, heads, min(topk, max_ctx)) for width in ops.RECORD_BYTES)
         self.mla_ws = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
         self.max_ctx, self.topk = max_ctx, topk
 

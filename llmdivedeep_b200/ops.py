@@ -334,7 +334,8 @@ def sparse_mla_decode_paged(q, cache, block_table, idx, scale: float, max_ctx: O
     out = _check_attn_out(out, (T, H, 512), q.device)
     lib = _lib.load()
     if workspace is None:
-        need = lib.dsa_sparse_mla_decode_workspace_bytes(T, H, idx.shape[1])
+        need = (lib.dsa_sparse_mla_decode_workspace_bytes(T, H, idx.shape[1]) if plain else
+                lib.dsa_sparse_mla_decode_records_workspace_bytes(cache.shape[1], T, H, idx.shape[1]))
         workspace = _workspace(q.device, need) if need else None
     rest = (_ptr(idx), _ptr(out), T, H, idx.shape[1], cache.shape[0] // 64, max_ctx, float(scale), _ptr(workspace),
             workspace.numel() if workspace is not None else 0, _ptr(status_word(dev)), _stream(dev))

@@ -281,7 +281,7 @@ def test_streams_and_graphs(H):
         got = ops.sparse_mla_decode_paged(*bufs, 0.07)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want[0])
-    ws = torch.empty(ops._lib.load().dsa_sparse_mla_decode_workspace_bytes(2, H, 2048), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(ops._lib.load().dsa_sparse_mla_decode_records_workspace_bytes(416, 2, H, 2048), dtype=torch.uint8, device="cuda")
     out = torch.empty_like(got)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
