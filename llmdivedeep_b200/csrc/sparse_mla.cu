@@ -223,6 +223,8 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 // A gather warp's raw rows of one block: per row this CTA's 256 e4m3 values, the four scales, this CTA's 64 rope bytes; of a 4-bit
 // record this CTA's half as it is.
 constexpr int kRawRows = (kMlaBlk + kMlaGatherWarps - 1) / kMlaGatherWarps;
+constexpr int kGroup4 = 5;                             // blocks whose positions a gather warp has at a time (4 bits)
+static_assert(kGroup4 * kRawRows <= 32, "a lane per slot");
 template <int SRC>
 struct MlaRaw {
   static constexpr int kRow = SRC == kSrc4 ? kLatent4Half : 256 + 16 + 64, kBytes = kRawRows * kRow, kPieces = 2 * kMlaGatherWarps;
@@ -308,11 +310,15 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
   int look[kMlaLooks];
   const int tail_j = k_cnt - 32 + lane;
   const int slot = warp >= kMlaGatherWarp0 && lane < kRawRows ? warp - kMlaGatherWarp0 + lane * kMlaGatherWarps : kMlaBlk;
+  // 4 bits: a warp's slots of five blocks at a time, lane 6 b + j has slot w + 11 j of block b (a lane without a slot: none)
+  const int slot4 = warp - kMlaGatherWarp0 + lane % kRawRows * kMlaGatherWarps;
+  const int first4 = SRC == kSrc4 && warp >= kMlaGatherWarp0 && lane < kGroup4 * kRawRows && slot4 < kMlaBlk ? lane / kRawRows * kMlaBlk + slot4 : kMlaMaxK;
   auto list_at = [&](int j) { return OVERLAPPED ? idx_row[j] : __ldg(idx_row + j); };
   auto request_list = [&]() {
     if constexpr (OVERLAPPED) idx_row = grid_wait(idx_row);
     tail = tail_j >= 0 ? list_at(tail_j) : -1;
-    slot_pos = slot < kMlaBlk && slot < k_cnt ? list_at(slot) : -1;
+    if constexpr (SRC == kSrc4) slot_pos = first4 < k_cnt ? list_at(first4) : -1;
+    else slot_pos = slot < kMlaBlk && slot < k_cnt ? list_at(slot) : -1;
 #pragma unroll
     for (int u = 0; u < kMlaLooks; ++u) {
       const int j = threadIdx.x + u * kMlaThreads;
@@ -552,21 +558,85 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
         const int c = (blk & 1) * kG + w4;
         return c < kRawInBuf ? kv_s + NB * kMlaKBytes + c * kRawBytes : smem + kMlaSmemBytes + (c - kRawInBuf) * kRawBytes;
       };
+      if constexpr (SRC == kSrc4) {
+        // Rows of 208 bytes, thirteen 16-byte pieces; positions and page-table entries by groups of five blocks, one and two groups ahead:
+        // with one block's at a time the warps waited for them, 600 of the 2450 cycles that a block took them.
+        auto positions = [&](int group) -> int {
+          const int j = group * kGroup4 * kMlaBlk + first4;
+          return first4 < kMlaMaxK && j < k_cnt && j < nblk * kMlaBlk ? list_at(j) : -1;
+        };
+        int ids = cache_row(slot_pos, table_entry(slot_pos)), group = 0, in = 0;      // of the block to fetch next: in-th of its group
+        int p1 = positions(1), e1 = table_entry(p1), p2 = positions(2);
+        uint32_t used0, used1, used2;                  // which of the warp's slots of blocks i, i + 1 and the last one fetched are used
+        auto fetch = [&](int blk) {                    // an empty slot is zero-filled, codes and scales
+          if (in == kGroup4) {
+            in = 0;
+            ++group;
+            ids = cache_row(p1, e1);
+            p1 = p2;
+            e1 = table_entry(p1);
+            p2 = positions(group + 2);
+          }
+          uint8_t* st = stage_of(blk);
+#pragma unroll
+          for (int u = 0; u < (kRows * 13 + 31) / 32; ++u) {
+            const int c = u * 32 + lane, j = c / 13, rid = __shfl_sync(0xffffffffu, ids, in * kRows + min(j, kRows - 1));
+            if (c < kRows * 13)
+              cp_async_16(st + c * 16, a.cache + (int64_t)max(rid, 0) * kLatent4Bytes + cta * kLatent4Half + (c - j * 13) * 16, rid >= 0 ? 16 : 0);
+          }
+          cp_async_commit();
+          used2 = __ballot_sync(0xffffffffu, ids >= 0) >> (in * kRows);
+          ++in;
+        };
+        fetch(0);
+        used0 = used2;
+        fetch(1);
+        used1 = used2;
+        // Two rows at a time, sixteen lanes a row: 16 neighbouring dims, two words and their scale.  Every second four lanes store their
+        // words the other way round, so that the eight lanes of a phase hit all banks.
+        const int l16 = lane & 15, turn = (l16 >> 2) & 1;
+        for (int i = 0, kvb = 0; i < nblk; ++i) {
+          if (i == kQBuf0) ok = mla_wait(q_moved, 0, abort_flag, a.status);   // from here on the buffers held Q
+          if (i >= NB) ok = mla_wait(&kv_free[kvb], ((i / NB) - 1) & 1, abort_flag, a.status);
+          if (!ok) break;
+          mark(i, used0 >> lane & 1u);
+          cp_async_wait<1>();                          // this lane's copies of block i have landed (block i+1 may be in flight) ...
+          __syncwarp();                                // ... and the other lanes'
+          const uint8_t* st = stage_of(i);
+          uint8_t* dst = kv_s + kvb * kMlaKBytes;
+#pragma unroll
+          for (int u = 0; u < kRows / 2; ++u) {
+            const int j = 2 * u + (lane >> 4), r = w4 + j * kG;
+            const uint2 w = *reinterpret_cast<const uint2*>(st + j * kRawRow + l16 * 8);
+            const uint32_t sc = latent4_scale(st[j * kRawRow + kLatent4Scales + l16]);
+            uint8_t* row = dst + (l16 >> 2) * kMlaKPanelBytes + r * 128;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              uint32_t p[4];
+              latent4_codes(x == turn ? w.x : w.y, p);
+              const uint4 v = make_uint4(mul_bf16x2(p[0], sc), mul_bf16x2(p[1], sc), mul_bf16x2(p[2], sc), mul_bf16x2(p[3], sc));
+              if (r < kMlaBlk) *reinterpret_cast<uint4*>(row + ((((2 * l16 + (x ^ turn)) ^ r) & 7) << 4)) = v;
+            }
+          }
+          {
+            const int r = w4 + (lane >> 2) * kG;
+            if (lane < 4 * kRows && r < kMlaBlk)
+              *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane ^ (r >> 1)) & 3) << 4)) =
+                  *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + kLatent4Rope + (lane & 3) * 16);
+          }
+          __syncwarp();                                // (the MMA warp makes the writes visible to the tensor core's reads)
+          if (lane == 0) mbar_arrive(&kv_full[kvb]);
+          fetch(i + 2);                                // into the stage just read: what was loaded from it has been stored
+          used0 = used1;
+          used1 = used2;
+          if (++kvb == NB) kvb = 0;
+        }
+      } else {
       const uint8_t* src_lat = a.cache + cta * kMlaDvHalf + (lane & 15) * 16;
       const uint8_t* src_rope = a.cache + kMlaDv + 16 + cta * 64 + (lane & 3) * 16;
       // request the warp's rows of a block; an empty slot is zero-filled, values and scales
       auto fetch = [&](int blk, int id) {
         uint8_t* st = stage_of(blk);
-        if constexpr (SRC == kSrc4) {                  // thirteen 16-byte pieces a row, the rows one after the other
-#pragma unroll
-          for (int u = 0; u < (kRows * 13 + 31) / 32; ++u) {
-            const int c = u * 32 + lane, j = c / 13, rid = __shfl_sync(0xffffffffu, id, j);
-            if (c < kRows * 13)
-              cp_async_16(st + c * 16, a.cache + (int64_t)max(rid, 0) * kLatent4Bytes + cta * kLatent4Half + (c - j * 13) * 16, rid >= 0 ? 16 : 0);
-          }
-          cp_async_commit();
-          return;
-        }
 #pragma unroll
         for (int u = 0; u < kRows / 2; ++u) {          // two rows of 256 values per instruction
           const int j = 2 * u + (lane >> 4), rid = __shfl_sync(0xffffffffu, id, j);
@@ -612,28 +682,21 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
           const int r = w4 + j * kG;
-          uint4 v;
-          if constexpr (SRC == kSrc4) {
-            uint32_t p[4];
-            latent4_codes(*reinterpret_cast<const uint32_t*>(st + j * kRawRow + lane * 4), p);
-            const uint32_t sc = latent4_scale(st[j * kRawRow + kLatent4Scales + (lane >> 1)]);
-            v = make_uint4(mul_bf16x2(p[0], sc), mul_bf16x2(p[1], sc), mul_bf16x2(p[2], sc), mul_bf16x2(p[3], sc));
-          } else {
-            const uint2 raw = *reinterpret_cast<const uint2*>(st + j * kRawRow + lane * 8);
-            const float sc = *reinterpret_cast<const float*>(st + j * kRawRow + 256 + cta * 8 + (lane >> 4) * 4);
-            v = e4m3x8_to_bf16(raw, sc);
-          }
+          const uint2 raw = *reinterpret_cast<const uint2*>(st + j * kRawRow + lane * 8);
+          const float sc = *reinterpret_cast<const float*>(st + j * kRawRow + 256 + cta * 8 + (lane >> 4) * 4);
+          const uint4 v = e4m3x8_to_bf16(raw, sc);
           if (r < kMlaBlk) *reinterpret_cast<uint4*>(dst_lat + r * 128 + (((lane ^ r) & 7) << 4)) = v;
         }
         {
           const int r = w4 + (lane >> 2) * kG;
           if (lane < 4 * kRows && r < kMlaBlk)
             *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane ^ (r >> 1)) & 3) << 4)) =
-                *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + (SRC == kSrc4 ? kLatent4Rope : 272) + (lane & 3) * 16);
+                *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16);
         }
         __syncwarp();                                  // (the MMA warp makes the writes visible to the tensor core's reads)
         if (lane == 0) mbar_arrive(&kv_full[kvb]);
         fetch(i + 2, id2);                             // into the stage just read: what was loaded from it has been stored
+      }
       }
       cp_async_wait_all();                             // nothing of this thread's is in flight when it leaves
     }
