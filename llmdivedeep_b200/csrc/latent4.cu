@@ -8,27 +8,32 @@
 
 namespace dsa {
 
-// A row's 16 values from 16-byte loads (fp32: four, bf16: two).
+// Eight neighbouring values, from 16-byte loads (fp32: two, bf16: one): their magnitudes, and their signs two by two at bits 15 and 31.
+struct Eight {
+  float v[8];
+  uint32_t sign[4];
+};
 template <typename T>
-__device__ __forceinline__ void load16(const T* __restrict__ src, float (&v)[16]) {
+__device__ __forceinline__ Eight load8(const T* __restrict__ src) {
+  Eight x;
   if constexpr (sizeof(T) == 2) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src));
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + h);
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {                    // bf16 -> fp32: the value is the upper half of the word
-        v[8 * h + 2 * i] = __uint_as_float(w[i] << 16);
-        v[8 * h + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
+    for (int i = 0; i < 4; ++i) {                      // bf16 -> fp32: the value is the upper half of the word
+      x.v[2 * i] = __uint_as_float((w[i] << 16) & 0x7fffffffu);
+      x.v[2 * i + 1] = __uint_as_float(w[i] & 0x7fff0000u);
+      x.sign[i] = w[i] & 0x80008000u;
     }
   } else {
+    const uint4 lo = __ldg(reinterpret_cast<const uint4*>(src)), hi = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const float4 raw = __ldg(reinterpret_cast<const float4*>(src) + h);
-      v[4 * h] = raw.x; v[4 * h + 1] = raw.y; v[4 * h + 2] = raw.z; v[4 * h + 3] = raw.w;
-    }
+    for (int i = 0; i < 8; ++i) x.v[i] = __uint_as_float(w[i] & 0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.sign[i] = ((w[2 * i] >> 16) & 0x8000u) | (w[2 * i + 1] & 0x80000000u);
   }
+  return x;
 }
 
 // Scale byte of a group from its largest magnitude: a / 6 (IEEE) held to the scales' range, to four significant bits, ties to even.
@@ -38,15 +43,27 @@ __device__ __forceinline__ uint32_t latent4_scale_of(float amax) {
   return r - (112u << 3);
 }
 
-// Eight values -> a word of codes.  The conversion rounds to nearest, ties to even, and saturates.
-__device__ __forceinline__ uint32_t latent4_word(const float* v, float scale) {
+// Eight values -> a word of codes.  The conversion rounds to nearest, ties to even, and saturates; for that it needs value / scale on the
+// right side of the halves t between two levels (.25 .75 1.25 1.75 2.5 3.5 5), or on t where it is.  fp32 values are divided (IEEE).  A bf16
+// value has eight significant bits, a scale four: their quotient is t or at least 2^-10 from it (all cases counted), so the value times
+// the rounded reciprocal, 2^-20 off at most, is put on the nearest multiple of 2^-12 (by adding 3 * 2^10, where that is the last place, and
+// taking it away): the same codes.
+template <bool FEW_BITS>
+__device__ __forceinline__ uint32_t latent4_word(const Eight& x, float scale) {
+  const float inv = FEW_BITS ? __frcp_rn(scale) : 0.f;
+  auto level = [&](float v) {
+    if constexpr (FEW_BITS) return __fsub_rn(__fmaf_rn(v, inv, 0x1.8p11f), 0x1.8p11f);
+    else return __fdiv_rn(v, scale);
+  };
+  constexpr int kSign[4] = {0, 3, 6, 1};
   uint32_t w = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const uint32_t b = __nv_cvt_float2_to_fp4x2(make_float2(__fdiv_rn(v[2 * k], scale), __fdiv_rn(v[2 * k + 1], scale)), __NV_E2M1, cudaRoundNearest);
-    const uint32_t n = (b & 15u) | ((b & 0xf0u) << 12);            // sign and number of the even value, of the odd one
-    if (k < 3) w |= ((n & 0x00080008u) << (12 - 3 * k)) | ((n & 0x00070007u) << (6 - 3 * k));
-    else w |= ((n & 0x00080008u) << 11) | ((n & 0x00060006u) << 9) | ((n & 0x00010001u) << 13);
+    const uint32_t b = __nv_cvt_float2_to_fp4x2(make_float2(level(x.v[2 * k]), level(x.v[2 * k + 1])), __NV_E2M1, cudaRoundNearest);
+    const uint32_t n = b | (b << 12);                  // number of the even value at bit 0, of the odd one at bit 16
+    w |= x.sign[k] >> kSign[k];
+    if (k < 3) w |= (n & 0x00070007u) << (6 - 3 * k);
+    else w |= ((n & 0x00060006u) << 9) | ((n & 0x00010001u) << 13);
   }
   return w;
 }
@@ -59,7 +76,7 @@ struct KeyRows {
   float* cache_scale;                                  // [cache_rows]
 };
 
-// Latent rows -> records at the cache rows `slots` (null: row i -> record i).  A warp per token: a lane has one group.
+// Latent rows -> records at the cache rows `slots` (null: row i -> record i).  A warp per token.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_latent4_kernel(const T* __restrict__ kv, int64_t row_stride, int64_t n, uint8_t* __restrict__ cache,
                                                            const int32_t* __restrict__ slots, int64_t cache_rows, const KeyRows keys, int* status) {
@@ -73,24 +90,31 @@ __global__ void __launch_bounds__(256) pack_latent4_kernel(const T* __restrict__
     }
     const T* src = kv + t * row_stride;
     uint8_t* dst = cache + slot * kLatent4Bytes;
-    float v[16];
-    load16(src + lane * 16, v);
-    float amax = 0.f, odd = 0.f;                       // odd: 0 x value, NaN where a value is no number
+    // a lane has dims 8 lane .. of either half: two lanes a group, whole lines to every load and store
+    Eight x[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      amax = fmaxf(amax, fabsf(v[i]));
-      odd = fmaf(v[i], 0.f, odd);
-    }
-    uint32_t byte = latent4_scale_of(amax);
-    if (odd != 0.f) {
-      byte = kLatent4Nan;
+    for (int hf = 0; hf < 2; ++hf) x[hf] = load8(src + hf * 256 + lane * 8);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    for (int hf = 0; hf < 2; ++hf) {
+      float amax = 0.f, odd = 0.f;                     // odd: 0 x value, NaN where a value is no number
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        amax = fmaxf(amax, x[hf].v[i]);
+        odd = fmaf(x[hf].v[i], 0.f, odd);
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+      uint32_t byte = latent4_scale_of(amax);
+      const float scale = __uint_as_float((byte + (112u << 3)) << 20);
+      uint32_t word = latent4_word<sizeof(T) == 2>(x[hf], scale);
+      if (odd != 0.f) {
+        byte = kLatent4Nan;
+        word = 0;
+      }
+      uint8_t* half = dst + hf * kLatent4Half;
+      *reinterpret_cast<uint32_t*>(half + lane * 4) = word;
+      if (!(lane & 1)) half[kLatent4Scales + (lane >> 1)] = (uint8_t)byte;
     }
-    const float scale = __uint_as_float((byte + (112u << 3)) << 20);
-    uint8_t* half = dst + (lane >> 4) * kLatent4Half;
-    *reinterpret_cast<uint2*>(half + (lane & 15) * 8) = make_uint2(latent4_word(v, scale), latent4_word(v + 8, scale));
-    half[kLatent4Scales + (lane & 15)] = (uint8_t)byte;
     if (lane < 8) {                                    // eight rope values each
       uint4 rope;
       if constexpr (sizeof(T) == 2) {
@@ -122,28 +146,28 @@ __global__ void __launch_bounds__(256) unpack_latent4_kernel(const uint8_t* __re
     }
     const bool there = row >= 0 && row < cache_rows;
     if (!there && lane == 0 && status) atomicCAS(status, kStatusOk, kStatusBadIndex);
-    const uint8_t* half = cache + (there ? row : 0) * kLatent4Bytes + (lane >> 4) * kLatent4Half;
-    uint2 w = make_uint2(0, 0);
-    uint32_t byte = 0;
+    const uint8_t* rec = cache + (there ? row : 0) * kLatent4Bytes;
+    // a lane has dims 8 lane .. of either half: whole lines to every load and store
+    uint32_t w[2] = {0, 0}, byte[2] = {0, 0};
     uint4 rope = make_uint4(0, 0, 0, 0);
     if (there) {
-      w = __ldg(reinterpret_cast<const uint2*>(half + (lane & 15) * 8));
-      byte = __ldg(half + kLatent4Scales + (lane & 15));
-      if (lane < 8)
-        rope = __ldg(reinterpret_cast<const uint4*>(cache + row * kLatent4Bytes + (lane >> 2) * kLatent4Half + kLatent4Rope + (lane & 3) * 16));
-    }
-    const uint32_t sc = latent4_scale(byte);
-    uint32_t a[4], b[4];
-    latent4_codes(w.x, a);
-    latent4_codes(w.y, b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = mul_bf16x2(mul_bf16x2(a[i], sc), kLatent4GainPair);
-      b[i] = mul_bf16x2(mul_bf16x2(b[i], sc), kLatent4GainPair);
+      for (int hf = 0; hf < 2; ++hf) {
+        w[hf] = __ldg(reinterpret_cast<const uint32_t*>(rec + hf * kLatent4Half) + lane);
+        byte[hf] = __ldg(rec + hf * kLatent4Half + kLatent4Scales + (lane >> 1));
+      }
+      if (lane < 8) rope = __ldg(reinterpret_cast<const uint4*>(rec + (lane >> 2) * kLatent4Half + kLatent4Rope + (lane & 3) * 16));
     }
     __nv_bfloat16* dst = out + t * out_stride;
-    reinterpret_cast<uint4*>(dst + lane * 16)[0] = make_uint4(a[0], a[1], a[2], a[3]);
-    reinterpret_cast<uint4*>(dst + lane * 16)[1] = make_uint4(b[0], b[1], b[2], b[3]);
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint32_t sc = latent4_scale(byte[hf]);
+      uint32_t c[4];
+      latent4_codes(w[hf], c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = mul_bf16x2(mul_bf16x2(c[i], sc), kLatent4GainPair);
+      reinterpret_cast<uint4*>(dst + hf * 256)[lane] = make_uint4(c[0], c[1], c[2], c[3]);
+    }
     if (lane < 8) reinterpret_cast<uint4*>(dst + 512)[lane] = rope;
   }
 }
