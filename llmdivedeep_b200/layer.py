@@ -17,8 +17,8 @@ class SparseMLA(nn.Module):
     """MQA over the shared latent KV restricted to the selected positions.
 
     forward(q [T,H,576] bf16, kv, topk_idx [T,K] int (negative = empty), block_table=None)
-      kv = [S,576] bf16 (prefill) or the paged FP8 latent cache uint8 [num_pages*64, 656]
-      together with block_table [T, P] (decode, one query token per sequence).
+      kv = [S,576] bf16 (prefill) or the paged latent cache, uint8 [num_pages*64, 656] (FP8) or
+      [num_pages*64, 416] (4 bits), together with block_table [T, P] (decode, one query token per sequence).
     Returns bf16 [T,H,512]."""
 
     def __init__(self, softmax_scale: float):
@@ -30,7 +30,7 @@ class SparseMLA(nn.Module):
         idx = topk_idx if topk_idx.dtype == torch.int32 else topk_idx.to(torch.int32)
         if kv.dtype == torch.uint8:
             if block_table is None:
-                raise ops.DsaError("the paged FP8 latent cache needs a block_table")
+                raise ops.DsaError("the paged latent cache needs a block_table")
             return ops.sparse_mla_decode_paged(q, kv, block_table, idx, self.softmax_scale)
         return ops.sparse_mla_prefill(q, kv, idx, self.softmax_scale)
 
@@ -370,6 +370,7 @@ class HostPrefillPipeline:
 
 
 LATENT_TOKEN_BYTES = 656          # 512 e4m3 latent values, 4 fp32 group scales, 64 bf16 rope values
+LATENT4_TOKEN_BYTES = 416         # 512 4-bit codes, 32 one-byte group scales, 64 bf16 rope values (ops.pack_latent4)
 
 
 def pack_latent_cache(kv: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -415,7 +416,7 @@ class DecodeWorkspace:
 def dsa_decode_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, latent_cache, softmax_scale: float,
                     ws: DecodeWorkspace):
     """One decode step for a batch of sequences: paged indexer scan, top-k over each sequence's
-    context, sparse MLA over the paged FP8 latent cache.  Returns (idx, out) views of ``ws``."""
+    context, sparse MLA over the paged latent cache (FP8 or 4-bit records).  Returns (idx, out) views of ``ws``."""
     B = q.shape[0]
     idx, out = ws.idx[:B], ws.out[:B]
     if ops.decode_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, latent_cache, softmax_scale, ws.max_ctx, ws.logits, idx, out,
@@ -425,3 +426,66 @@ def dsa_decode_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, laten
     ops.topk_select(logits, ws.k, None, ctx_len, out=idx)
     ops.sparse_mla_decode_paged(q, latent_cache, block_table, idx, softmax_scale, ws.max_ctx, out=out, workspace=ws.mla_ws)
     return idx, out
+
+
+class PagedCache:
+    """The decode caches of ``layers`` DSA layers, latents in 4 bits, in one pool of 64-token pages, and the tables that say
+    which sequence has which page: 416 + 132 bytes a token and layer.
+
+        cache = PagedCache(layers, num_pages, batch, max_ctx, "cuda")
+        slots = cache.extend([row], [n], n)                    # room for n tokens in a row of the batch
+        cache.write(layer, slots, kv, k8, k_scale)             # their latents and indexer keys, layer by layer
+        idx, out = cache.decode(layer, q8, w, q, scale, ws)    # one step for all rows; ws = DecodeWorkspace(batch, heads, ...)
+        cache.fork([row], [other])                             # a beam, a shared prompt: full pages are not copied
+        cache.free([row])
+        cache.compact()                                        # pages in use to the lowest ids, contents and tables
+        kv = cache.read(layer, row, n)                         # bf16 rows for a chunked prefill (ops.sparse_mla_prefill)
+
+    Rows are given as int32 tensors on the GPU or as lists, which are copied there.  Nothing else waits; what the kernels find wrong
+    (a pool without free pages, a bad row) leaves the tables as they are and is in ops.check_status.  The tables are tensors of
+    fixed addresses (``table``, ``ctx``, ``refs``), so that steps can be captured in a graph."""
+
+    def __init__(self, layers: int, num_pages: int, batch: int, max_ctx: int, device, index_dim: int = 128):
+        rows, dev = num_pages * 64, torch.device(device)
+        self.k8 = torch.zeros(layers, rows, index_dim, dtype=torch.uint8, device=dev).view(ops.FP8)
+        self.k_scale = torch.zeros(layers, rows, dtype=torch.float32, device=dev)
+        self.latent = torch.zeros(layers, rows, LATENT4_TOKEN_BYTES, dtype=torch.uint8, device=dev)
+        self.table = torch.full((batch, -(-max_ctx // 64)), -1, dtype=torch.int32, device=dev)
+        self.ctx = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.refs = torch.zeros(num_pages, dtype=torch.int32, device=dev)
+        self.device = self.table.device
+
+    def _rows(self, rows) -> torch.Tensor:
+        return rows if isinstance(rows, torch.Tensor) else torch.tensor(rows, dtype=torch.int32, device=self.device)
+
+    @property
+    def caches(self) -> tuple:
+        return self.k8, self.k_scale, self.latent
+
+    def extend(self, rows, n_new, max_new: int) -> torch.Tensor:
+        """Cache rows of n_new[i] <= max_new new tokens of row rows[i]: int32 [n, max_new], -1 behind them."""
+        return ops.extend_pages(self.table, self.ctx, self.refs, self._rows(rows), self._rows(n_new), max_new)
+
+    def write(self, layer: int, slots: torch.Tensor, kv: torch.Tensor, k8: torch.Tensor, k_scale: torch.Tensor) -> None:
+        """Tokens' latents [..., 576] (bf16 or fp32) and indexer keys (e4m3 [..., 128], fp32 scales [...]) of one layer, to the rows
+        that extend gave (a slot of -1 is skipped)."""
+        ops.pack_latent4(kv.reshape(-1, 576), self.latent[layer], slots.reshape(-1),
+                         keys=(k8.reshape(-1, k8.shape[-1]), k_scale.reshape(-1), self.k8[layer], self.k_scale[layer]))
+
+    def read(self, layer: int, row: int, n: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The first n tokens of a row, as bf16 rows [n, 576]."""
+        return ops.unpack_latent4(self.latent[layer], n, self.table[row], out=out)
+
+    def decode(self, layer: int, q8, w, q, softmax_scale: float, ws: DecodeWorkspace):
+        """dsa_decode_step of the first q.shape[0] rows over this layer's caches; empty rows give zeros."""
+        B = q.shape[0]
+        return dsa_decode_step(q8, w, self.k8[layer], self.k_scale[layer], self.table[:B], self.ctx[:B], q, self.latent[layer], softmax_scale, ws)
+
+    def fork(self, parents, children) -> None:
+        ops.fork_pages(self.table, self.ctx, self.refs, self._rows(parents), self._rows(children), self.caches)
+
+    def free(self, rows) -> None:
+        ops.free_pages(self.table, self.ctx, self.refs, self._rows(rows))
+
+    def compact(self) -> None:
+        ops.compact_pages(self.table, self.refs, self.caches, out=(self.table, self.refs))
