@@ -35,7 +35,8 @@ struct Few4Args {
   int list_blocks;                // blocks of 64 slots of a list
   int ctas;
   int rounds;                     // CTA c has lists c, c + ctas, ... of so many rounds, ...
-  int rest, rest_ctas;            // ... and if c < rest_ctas, of the rest blocks of the lists behind them those from c rest / rest_ctas on
+  int rest, rest_ctas;            // ... and if c < rest_ctas, a stretch of the rest blocks of the lists behind them:
+  int per_list;                   // one of so many equal parts of a list, or (0) of all blocks
   float scale_log2e;
   float* part_o;                  // [2 ctas][H][512]: of a CTA's first piece of a list and of its last one
   float* part_lse;                // [2 ctas][H], log2 units, -inf = empty
@@ -97,7 +98,10 @@ __device__ __forceinline__ uint32_t f4_test(uint64_t* bar, uint32_t parity) {
 struct F4Piece {
   int done, all, start;                                // its blocks behind it, and all of them; first block of the stretch
   int t, b0, b1;                                       // the list and its blocks [b0, b1) in this piece
-  static __device__ __forceinline__ int start_of(const Few4Args& a, int c) { return a.rest ? (int)((int64_t)c * a.rest / a.rest_ctas) : 0; }
+  static __device__ __forceinline__ int start_of(const Few4Args& a, int c) {
+    if (a.per_list) return c / a.per_list * a.list_blocks + c % a.per_list * a.list_blocks / a.per_list;
+    return a.rest ? (int)((int64_t)c * a.rest / a.rest_ctas) : 0;
+  }
   __device__ __forceinline__ F4Piece(const Few4Args& a) {
     const int c = blockIdx.x;
     start = start_of(a, c);
@@ -122,6 +126,37 @@ struct F4Piece {
   }
   // The part that this piece leaves if it is not a whole list: of the stretch's first list, or of its last.
   __device__ __forceinline__ int part(const Few4Args& a) const { return 2 * blockIdx.x + (done - (b1 - b0) == a.rounds * a.list_blocks ? 0 : 1); }
+};
+
+// What one of `of` threads sees of the slots [lo, hi) of a list: the last used one, and the largest position.
+struct F4Scan {
+  int last, top;
+  __device__ __forceinline__ void see(int id, int j, int max_ctx) {
+    if (id >= 0 && id < max_ctx) last = j;
+    top = max(top, id);
+  }
+  __device__ __forceinline__ F4Scan(const Few4Args& a, const int32_t* row, int lo, int hi, int me, int of) {
+    last = top = -1;
+    if (((reinterpret_cast<uintptr_t>(row + lo) | (hi - lo) * 4) & 15) == 0) {      // a few loads are requested before the first is looked at
+#pragma unroll 1
+      for (int j0 = lo + me * 4; j0 < hi; j0 += of * 4 * kF4Look) {
+        int4 id[kF4Look];
+#pragma unroll
+        for (int i = 0; i < kF4Look; ++i)
+          id[i] = j0 + i * of * 4 < hi ? *reinterpret_cast<const int4*>(row + j0 + i * of * 4) : make_int4(-1, -1, -1, -1);
+#pragma unroll
+        for (int i = 0; i < kF4Look; ++i) {
+          const int j = j0 + i * of * 4;
+          see(id[i].x, j, a.max_ctx); see(id[i].y, j + 1, a.max_ctx); see(id[i].z, j + 2, a.max_ctx); see(id[i].w, j + 3, a.max_ctx);
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int j = lo + me; j < hi; j += of) see(row[j], j, a.max_ctx);
+    }
+    if (top >= a.max_ctx && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+    last = __reduce_max_sync(0xffffffffu, last);
+  }
 };
 
 template <int N>
@@ -150,9 +185,10 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* valid_s = reinterpret_cast<uint8_t*>(bars) + C::BAR_BYTES;
   volatile uint8_t* len_s = valid_s + kF4Valid * kF4Blk;            // [kF4Pieces] used blocks of the CTA's pieces
+  int* last_s = reinterpret_cast<int*>(bars + kBars + 1);           // [warps] what each has seen of the first list
   float* max_s = reinterpret_cast<float*>(valid_s + kF4Valid * kF4Blk + kF4Pieces);      // [2][4 warps][N] block maxima by block parity
   float* wgt_s = max_s + 2 * kF4SoftmaxWarps * N;      // [4 warps][N]
-  static_assert(kBars * 8 + 8 <= C::BAR_BYTES, "barriers");
+  static_assert((kBars + 1) * 8 + kF4Threads / 32 * 4 <= C::BAR_BYTES, "barriers");
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   launch_dependents();
@@ -169,13 +205,25 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
   }
   for (int i = threadIdx.x; i < kF4Pieces / 4; i += kF4Threads) reinterpret_cast<volatile uint32_t*>(len_s)[i] = 0x01010101u * kF4Unknown;
   const int32_t* idx = grid_wait(a.idx);               // a launch under the top-k's end reads its lists after the wait
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  // The first piece's end is found by all threads together, so that it is known when the roles begin.
+  int blocks0;
+  {
+    F4Piece p0(a);
+    const bool there = p0.next(a);
+    const int lo = p0.b0 * kF4Blk, hi = there ? min(a.K, p0.b1 * kF4Blk) : lo;
+    const F4Scan scan(a, idx + (int64_t)p0.t * a.K, lo, hi, threadIdx.x, kF4Threads);
+    if (lane == 0) last_s[warp] = scan.last;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const int last0 = __reduce_max_sync(0xffffffffu, lane < kF4Threads / 32 ? last_s[lane] : -1);
+    blocks0 = last0 < 0 ? 0 : (last0 - lo) / kF4Blk + 1;
+  }
   const uint32_t tmem = *tmem_slot;
 
   // Used blocks of the CTA's nu-th piece, once the warp that reads the lists has come to it (it waits for nobody).
   auto piece_blocks = [&](uint32_t nu, bool& ok) -> int {
+    if (nu == 0) return blocks0;
     for (uint32_t i = 0; i < kSpinLimit; ++i) {
       const int nb = len_s[nu];
       if (__all_sync(0xffffffffu, nb != kF4Unknown)) return nb;
@@ -196,8 +244,8 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
     // ------------- the last used slot of every piece (it decides the number of blocks), and Q -------------
     // Whichever can go on; Q, which the tensor core waits for, first.
     F4Piece qc(a);
-    uint32_t nu = 0, nq = 0, idle = 0;
-    bool lists = true, queries = true;
+    uint32_t nu = 1, nq = 0, idle = 0;
+    bool lists = pc.next(a), queries = true;           // (the first list's end is known)
     while (lists || queries) {
       if (queries && __all_sync(0xffffffffu, f4_test(q_free, (nq & 1) ^ 1))) {
         queries = qc.next(a);
@@ -211,31 +259,8 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
       } else if (lists) {
         lists = pc.next(a);
         if (!lists) continue;
-        const int32_t* row = idx + (int64_t)pc.t * a.K;
-        const int lo = pc.b0 * kF4Blk, hi = min(a.K, pc.b1 * kF4Blk);
-        int last = -1, top = -1;
-        auto see = [&](int id, int j) {
-          if (id >= 0 && id < a.max_ctx) last = j;
-          top = max(top, id);
-        };
-        if (((reinterpret_cast<uintptr_t>(row + lo) | (hi - lo) * 4) & 15) == 0) {      // all of a lane's loads are requested before the first is looked at
-#pragma unroll 1
-          for (int j0 = lo + lane * 4; j0 < hi; j0 += 128 * kF4Look) {
-            int4 id[kF4Look];
-#pragma unroll
-            for (int i = 0; i < kF4Look; ++i) id[i] = j0 + i * 128 < hi ? *reinterpret_cast<const int4*>(row + j0 + i * 128) : make_int4(-1, -1, -1, -1);
-#pragma unroll
-            for (int i = 0; i < kF4Look; ++i) {
-              const int j = j0 + i * 128;
-              see(id[i].x, j); see(id[i].y, j + 1); see(id[i].z, j + 2); see(id[i].w, j + 3);
-            }
-          }
-        } else {
-#pragma unroll 8
-          for (int j = lo + lane; j < hi; j += 32) see(row[j], j);
-        }
-        last = __reduce_max_sync(0xffffffffu, last);
-        if (top >= a.max_ctx && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+        const int lo = pc.b0 * kF4Blk;
+        const int last = F4Scan(a, idx + (int64_t)pc.t * a.K, lo, min(a.K, pc.b1 * kF4Blk), lane, 32).last;
         if (lane == 0) len_s[nu] = (uint8_t)(last < 0 ? 0 : (last - lo) / kF4Blk + 1);
         ++nu;
       } else if (++idle > kFastSpins) {
@@ -662,7 +687,8 @@ __global__ void __launch_bounds__(128) sparse_mla_few4_merge_kernel(const Few4Ar
   const int t = a.rounds * a.ctas + blockIdx.x, h = blockIdx.y, d = threadIdx.x * 4, lane = threadIdx.x & 31;
   // the CTAs whose stretches have the list's first and last block
   auto cta_of = [&](int x) { return (int)(((int64_t)(x + 1) * a.rest_ctas - 1) / a.rest); };
-  const int blk0 = blockIdx.x * a.list_blocks, c0 = cta_of(blk0), parts = cta_of(blk0 + a.list_blocks - 1) - c0 + 1;
+  const int blk0 = blockIdx.x * a.list_blocks, c0 = a.per_list ? blockIdx.x * a.per_list : cta_of(blk0);
+  const int parts = a.per_list ? a.per_list : cta_of(blk0 + a.list_blocks - 1) - c0 + 1;
   if (parts == 1) return;                              // whole
   const int first = 2 * c0 + (F4Piece::start_of(a, c0) >= blk0 ? 0 : 1);      // the others' stretches begin in this list
   auto slot_of = [&](int p) { return p == 0 ? first : 2 * (c0 + p); };
@@ -703,6 +729,7 @@ int make_tmap_2d_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t
                        uint32_t box_bytes, uint32_t box_rows);
 
 constexpr int kF4LeastBlocks = 2;                      // of a CTA, in calls that have few
+constexpr int kF4PieceBlocks = 2;                      // what a further piece costs a CTA, in blocks
 
 static int f4_list_blocks(int K) { return max(1, (K + kF4Blk - 1) / kF4Blk); }
 static int f4_ctas(int T, int list_blocks) {
@@ -721,7 +748,7 @@ static int launch_few4(const void* q, const Few4Args& a, int overlapped, cudaStr
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return set_error(DSA_ERR_CUDA, "sparse_mla: cannot raise dynamic shared memory to %d", C::SMEM);
   launch_after(overlapped, kern, dim3(a.ctas), kF4Threads, C::SMEM, stream, tq, a);
-  if (a.rest && (a.rest % a.rest_ctas || a.rest / a.rest_ctas % a.list_blocks))      // some list may be cut
+  if (a.per_list > 1 || (!a.per_list && a.rest && (a.rest % a.rest_ctas || a.rest / a.rest_ctas % a.list_blocks)))      // some list may be cut
     launch_after(1, sparse_mla_few4_merge_kernel, dim3(a.T - a.rounds * a.ctas, a.H), 128, 0, stream, a);
   return check_launch("sparse_mla");
 }
@@ -756,6 +783,17 @@ int sparse_mla_few4_launch(const void* q, const void* cache, const int32_t* bloc
     }
     a.rest = max(0, a.T - a.rounds * a.ctas) * a.list_blocks;
     a.rest_ctas = min(a.ctas, max(1, a.rest / kF4LeastBlocks));
+    // Equal parts of each list while they keep the GPU as busy: a CTA whose stretch lies in two lists pays for the second's Q, output and
+    // start what two blocks take.  2048 keys, us with stretches of all blocks and so: 16 heads 12 rows 19.1, 17.0; 24 rows 21.4, 19.1; 64 rows
+    // 34.6, 32.5; 32 heads 64 rows 44.9, 42.3.
+    a.per_list = 0;
+    if (a.rest) {
+      const int lists = a.rest / a.list_blocks, p = min(a.ctas / lists, max(1, a.list_blocks / kF4LeastBlocks));
+      if ((a.list_blocks + p - 1) / p <= (a.rest + a.rest_ctas - 1) / a.rest_ctas + kF4PieceBlocks) {
+        a.per_list = p;
+        a.rest_ctas = lists * p;
+      }
+    }
     const void* qt = static_cast<const uint8_t*>(q) + (size_t)t0 * H * kF4QBytes;
     const int rc = H <= 16 ? launch_few4<16>(qt, a, overlapped, stream) : launch_few4<32>(qt, a, overlapped, stream);
     if (rc) return rc;
