@@ -592,9 +592,9 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
         used0 = used2;
         fetch(1);
         used1 = used2;
-        // Two rows at a time, sixteen lanes a row: 16 neighbouring dims, two words and their scale.  Every second four lanes store their
-        // words the other way round, so that the eight lanes of a phase hit all banks.
-        const int l16 = lane & 15, turn = (l16 >> 2) & 1;
+        // Two rows at a time, sixteen lanes a row: 16 neighbouring dims, two words and their scale.  The eight lanes of a phase have four
+        // such pieces of both rows, which lie 11 apart: the swizzle puts the words of one on even chunks, of the other on odd ones.
+        const int l16 = (lane & 3) | ((lane >> 3) << 2);
         for (int i = 0, kvb = 0; i < nblk; ++i) {
           if (i == kQBuf0) ok = mla_wait(q_moved, 0, abort_flag, a.status);   // from here on the buffers held Q
           if (i >= NB) ok = mla_wait(&kv_free[kvb], ((i / NB) - 1) & 1, abort_flag, a.status);
@@ -606,16 +606,16 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
           uint8_t* dst = kv_s + kvb * kMlaKBytes;
 #pragma unroll
           for (int u = 0; u < kRows / 2; ++u) {
-            const int j = 2 * u + (lane >> 4), r = w4 + j * kG;
+            const int j = 2 * u + ((lane >> 2) & 1), r = w4 + j * kG;
             const uint2 w = *reinterpret_cast<const uint2*>(st + j * kRawRow + l16 * 8);
             const uint32_t sc = latent4_scale(st[j * kRawRow + kLatent4Scales + l16]);
             uint8_t* row = dst + (l16 >> 2) * kMlaKPanelBytes + r * 128;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               uint32_t p[4];
-              latent4_codes(x == turn ? w.x : w.y, p);
+              latent4_codes(x == 0 ? w.x : w.y, p);
               const uint4 v = make_uint4(mul_bf16x2(p[0], sc), mul_bf16x2(p[1], sc), mul_bf16x2(p[2], sc), mul_bf16x2(p[3], sc));
-              if (r < kMlaBlk) *reinterpret_cast<uint4*>(row + ((((2 * l16 + (x ^ turn)) ^ r) & 7) << 4)) = v;
+              if (r < kMlaBlk) *reinterpret_cast<uint4*>(row + ((((2 * l16 + x) ^ r) & 7) << 4)) = v;
             }
           }
           {
