@@ -318,32 +318,60 @@ def sparse_mla_decode_paged(q, cache, block_table, idx, scale: float, max_ctx: O
     """Decode step over the paged latent cache.  q [T,H,576] bf16, cache uint8 [num_pages*64, 656] (FP8 records,
     pack_latent_cache) or [num_pages*64, 416] (4-bit records, pack_latent4), block_table [B,P] int32, idx [T,K] int32
     logical positions.  T = B * tokens_per_seq: a sequence's query rows one after the other.  Returns bf16 [T,H,512]."""
+    if tokens_per_seq == 1 and cache.dim() == 2 and cache.shape[1] == 656:
+        return _sparse_mla_decode_fp8(q, cache, block_table, idx, scale, max_ctx, out, workspace)
+    # A decode step of few rows waits for the host: each tensor is looked at once.
+    dev = q.device
+    i = dev.index
+    if dev.type != "cuda" or cache.get_device() != i or block_table.get_device() != i or idx.get_device() != i:
+        dev = _need_cuda(q, cache, block_table, idx)
+    if (q.dtype is not torch.bfloat16 or cache.dtype is not torch.uint8 or idx.dtype is not torch.int32 or block_table.dtype is not torch.int32):
+        raise DsaError("sparse_mla_decode_paged takes bf16 q, uint8 cache, int32 block_table/idx")
+    if q.dim() != 3 or cache.dim() != 2 or idx.dim() != 2 or block_table.dim() != 2:
+        raise DsaError("sparse_mla_decode_paged takes q [T,H,576], cache [num_pages*64, record], block_table [B,P], idx [T,K]")
+    q, cache, block_table, idx = q.contiguous(), cache.contiguous(), block_table.contiguous(), idx.contiguous()
+    (T, H, dq), (rows, width), (B, P), (Ti, K) = q.shape, cache.shape, block_table.shape, idx.shape
+    if width not in RECORD_BYTES or rows % 64:
+        raise DsaError("cache must be uint8 [num_pages*64, 656] or [num_pages*64, 416]")
+    if tokens_per_seq < 1 or dq != 576 or Ti != T or B * tokens_per_seq < T:
+        raise DsaError(f"bad shapes q {tuple(q.shape)} idx {tuple(idx.shape)} block_table {tuple(block_table.shape)}, {tokens_per_seq} tokens a sequence")
+    if out is None:
+        out = q.new_empty((T, H, 512))
+    else:
+        _need_cuda(q, out)
+        _check_attn_out(out, (T, H, 512), dev)
+    lib = _lib.load()
+    if workspace is None:
+        workspace = cache.new_empty(lib.dsa_sparse_mla_decode_records_workspace_bytes(width, T, H, K))      # as _workspace
+    else:
+        _need_cuda(q, workspace)
+    with _on(dev):
+        check(lib.dsa_sparse_mla_decode_records(q.data_ptr(), cache.data_ptr(), width, block_table.data_ptr(), P, tokens_per_seq, idx.data_ptr(),
+                                                out.data_ptr(), T, H, K, rows // 64, P * 64 if max_ctx is None else max_ctx, float(scale),
+                                                workspace.data_ptr(), workspace.numel(), status_word(dev).data_ptr(), _stream(dev)))
+    return out
+
+
+def _sparse_mla_decode_fp8(q, cache, block_table, idx, scale, max_ctx, out, workspace) -> torch.Tensor:
     dev = _need_cuda(q, cache, block_table, idx, out, workspace)
     if q.dtype != torch.bfloat16 or cache.dtype != torch.uint8 or idx.dtype != torch.int32 or block_table.dtype != torch.int32:
         raise DsaError("sparse_mla_decode_paged takes bf16 q, uint8 cache, int32 block_table/idx")
-    if cache.dim() != 2 or cache.shape[1] not in RECORD_BYTES or cache.shape[0] % 64:
-        raise DsaError("cache must be uint8 [num_pages*64, 656] or [num_pages*64, 416]")
+    if cache.dim() != 2 or cache.shape[1] != 656 or cache.shape[0] % 64:
+        raise DsaError("cache must be uint8 [num_pages*64, 656]")
     q, cache, block_table, idx = q.contiguous(), cache.contiguous(), block_table.contiguous(), idx.contiguous()
-    T, H, dq = q.shape
+    B, H, _ = q.shape
     if max_ctx is None:
         max_ctx = block_table.shape[1] * 64
-    plain = cache.shape[1] == 656 and tokens_per_seq == 1
-    if not plain and (tokens_per_seq < 1 or dq != 576 or idx.dim() != 2 or idx.shape[0] != T or block_table.dim() != 2
-                      or block_table.shape[0] * tokens_per_seq < T):
-        raise DsaError(f"bad shapes q {tuple(q.shape)} idx {tuple(idx.shape)} block_table {tuple(block_table.shape)}, {tokens_per_seq} tokens a sequence")
-    out = _check_attn_out(out, (T, H, 512), q.device)
+    out = _check_attn_out(out, (B, H, 512), q.device)
     lib = _lib.load()
     if workspace is None:
-        need = (lib.dsa_sparse_mla_decode_workspace_bytes(T, H, idx.shape[1]) if plain else
-                lib.dsa_sparse_mla_decode_records_workspace_bytes(cache.shape[1], T, H, idx.shape[1]))
+        need = lib.dsa_sparse_mla_decode_workspace_bytes(B, H, idx.shape[1])
         workspace = _workspace(q.device, need) if need else None
-    rest = (_ptr(idx), _ptr(out), T, H, idx.shape[1], cache.shape[0] // 64, max_ctx, float(scale), _ptr(workspace),
-            workspace.numel() if workspace is not None else 0, _ptr(status_word(dev)), _stream(dev))
     with _on(dev):
-        if plain:
-            check(lib.dsa_sparse_mla_decode_paged(_ptr(q), _ptr(cache), _ptr(block_table), block_table.stride(0), *rest))
-        else:
-            check(lib.dsa_sparse_mla_decode_records(_ptr(q), _ptr(cache), cache.shape[1], _ptr(block_table), block_table.stride(0), tokens_per_seq, *rest))
+        check(lib.dsa_sparse_mla_decode_paged(_ptr(q), _ptr(cache), _ptr(block_table), block_table.stride(0), _ptr(idx),
+                                              _ptr(out), B, H, idx.shape[1], cache.shape[0] // 64, max_ctx, float(scale),
+                                              _ptr(workspace), workspace.numel() if workspace is not None else 0,
+                                              _ptr(status_word(dev)), _stream(dev)))
     return out
 
 
