@@ -9,8 +9,8 @@
 // pair owns latent panels 4c..4c+3 -- its half of V -- and half of the rope panel's contraction:
 //   * it gathers only those 576 bytes of every selected row (36 KB per 64-key block, five blocks in
 //     flight), swizzled by the writing threads: cp.async straight out of the bf16 KV, or -- for the
-//     paged FP8 latent cache of decode -- cp.async of the raw rows two blocks ahead and a conversion
-//     e4m3 x group scale -> bf16 into one of four buffers;
+//     paged latent caches of decode -- cp.async of the raw rows two blocks ahead and a conversion
+//     to bf16 into one of four buffers: e4m3 x group scale, or 4-bit code x group scale (latent4.cuh);
 //   * its five Q panels live in tensor memory as the A operand, so Q.K^T reads no shared memory for
 //     Q, and it computes a PARTIAL score tile S_c = Q_c K_c^T (18 tcgen05.mma kind::f16 of N = 64);
 //   * the two partial tiles ([128 heads x 64 keys], rounded to fp16 for the way: 16 KB) are exchanged
@@ -632,71 +632,71 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
           if (++kvb == NB) kvb = 0;
         }
       } else {
-      const uint8_t* src_lat = a.cache + cta * kMlaDvHalf + (lane & 15) * 16;
-      const uint8_t* src_rope = a.cache + kMlaDv + 16 + cta * 64 + (lane & 3) * 16;
-      // request the warp's rows of a block; an empty slot is zero-filled, values and scales
-      auto fetch = [&](int blk, int id) {
-        uint8_t* st = stage_of(blk);
-#pragma unroll
-        for (int u = 0; u < kRows / 2; ++u) {          // two rows of 256 values per instruction
-          const int j = 2 * u + (lane >> 4), rid = __shfl_sync(0xffffffffu, id, j);
-          cp_async_16(st + j * kRawRow + (lane & 15) * 16, src_lat + (int64_t)max(rid, 0) * kLatentTokenBytes, rid >= 0 ? 16 : 0);
-        }
-        const int rid = __shfl_sync(0xffffffffu, id, lane >> 2);
-        if (lane < kRows)                              // a row's four scales
-          cp_async_16(st + lane * kRawRow + 256, a.cache + kMlaDv + (int64_t)max(id, 0) * kLatentTokenBytes, id >= 0 ? 16 : 0);
-        if (lane < 4 * kRows)                          // this CTA's two K-steps of the rope panel: 64 bytes per row
-          cp_async_16(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16, src_rope + (int64_t)max(rid, 0) * kLatentTokenBytes, rid >= 0 ? 16 : 0);
-        cp_async_commit();
-      };
-      // row ids of blocks i and i+1 (which of them are used), page-table entry and position of i+2, position of i+3
-      int id_cur, id_nxt, pa, ta, pb;
-      {
-        const int p0 = slot_pos, p1 = load_pos(1);
-        pa = load_pos(2);
-        pb = load_pos(3);
-        const int t0 = table_entry(p0), t1 = table_entry(p1);
-        ta = table_entry(pa);
-        id_cur = cache_row(p0, t0);
-        fetch(0, id_cur);
-        id_nxt = cache_row(p1, t1);
-        fetch(1, id_nxt);
-      }
-      for (int i = 0; i < nblk; ++i) {
-        const int kvb = i % NB;
-        const int id2 = cache_row(pa, ta);             // block i+2
-        pa = pb;
-        ta = table_entry(pa);
-        pb = load_pos(i + 4);
-        if (i == kQBuf0) ok = mla_wait(q_moved, 0, abort_flag, a.status);   // from here on the buffers held Q
-        if (i >= NB) ok = mla_wait(&kv_free[kvb], ((i / NB) - 1) & 1, abort_flag, a.status);
-        if (!ok) break;
-        mark(i, id_cur >= 0);
-        id_cur = id_nxt;
-        id_nxt = id2;
-        cp_async_wait<1>();                            // this lane's copies of block i have landed (block i+1 may be in flight) ...
-        __syncwarp();                                  // ... and the other lanes'
-        const uint8_t* st = stage_of(i);
-        uint8_t* dst = kv_s + kvb * kMlaKBytes;
-        uint8_t* dst_lat = dst + (lane >> 3) * kMlaKPanelBytes;
-#pragma unroll
-        for (int j = 0; j < kRows; ++j) {
-          const int r = w4 + j * kG;
-          const uint2 raw = *reinterpret_cast<const uint2*>(st + j * kRawRow + lane * 8);
-          const float sc = *reinterpret_cast<const float*>(st + j * kRawRow + 256 + cta * 8 + (lane >> 4) * 4);
-          const uint4 v = e4m3x8_to_bf16(raw, sc);
-          if (r < kMlaBlk) *reinterpret_cast<uint4*>(dst_lat + r * 128 + (((lane ^ r) & 7) << 4)) = v;
-        }
+        const uint8_t* src_lat = a.cache + cta * kMlaDvHalf + (lane & 15) * 16;
+        const uint8_t* src_rope = a.cache + kMlaDv + 16 + cta * 64 + (lane & 3) * 16;
+        // request the warp's rows of a block; an empty slot is zero-filled, values and scales
+        auto fetch = [&](int blk, int id) {
+          uint8_t* st = stage_of(blk);
+  #pragma unroll
+          for (int u = 0; u < kRows / 2; ++u) {          // two rows of 256 values per instruction
+            const int j = 2 * u + (lane >> 4), rid = __shfl_sync(0xffffffffu, id, j);
+            cp_async_16(st + j * kRawRow + (lane & 15) * 16, src_lat + (int64_t)max(rid, 0) * kLatentTokenBytes, rid >= 0 ? 16 : 0);
+          }
+          const int rid = __shfl_sync(0xffffffffu, id, lane >> 2);
+          if (lane < kRows)                              // a row's four scales
+            cp_async_16(st + lane * kRawRow + 256, a.cache + kMlaDv + (int64_t)max(id, 0) * kLatentTokenBytes, id >= 0 ? 16 : 0);
+          if (lane < 4 * kRows)                          // this CTA's two K-steps of the rope panel: 64 bytes per row
+            cp_async_16(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16, src_rope + (int64_t)max(rid, 0) * kLatentTokenBytes, rid >= 0 ? 16 : 0);
+          cp_async_commit();
+        };
+        // row ids of blocks i and i+1 (which of them are used), page-table entry and position of i+2, position of i+3
+        int id_cur, id_nxt, pa, ta, pb;
         {
-          const int r = w4 + (lane >> 2) * kG;
-          if (lane < 4 * kRows && r < kMlaBlk)
-            *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane ^ (r >> 1)) & 3) << 4)) =
-                *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16);
+          const int p0 = slot_pos, p1 = load_pos(1);
+          pa = load_pos(2);
+          pb = load_pos(3);
+          const int t0 = table_entry(p0), t1 = table_entry(p1);
+          ta = table_entry(pa);
+          id_cur = cache_row(p0, t0);
+          fetch(0, id_cur);
+          id_nxt = cache_row(p1, t1);
+          fetch(1, id_nxt);
         }
-        __syncwarp();                                  // (the MMA warp makes the writes visible to the tensor core's reads)
-        if (lane == 0) mbar_arrive(&kv_full[kvb]);
-        fetch(i + 2, id2);                             // into the stage just read: what was loaded from it has been stored
-      }
+        for (int i = 0; i < nblk; ++i) {
+          const int kvb = i % NB;
+          const int id2 = cache_row(pa, ta);             // block i+2
+          pa = pb;
+          ta = table_entry(pa);
+          pb = load_pos(i + 4);
+          if (i == kQBuf0) ok = mla_wait(q_moved, 0, abort_flag, a.status);   // from here on the buffers held Q
+          if (i >= NB) ok = mla_wait(&kv_free[kvb], ((i / NB) - 1) & 1, abort_flag, a.status);
+          if (!ok) break;
+          mark(i, id_cur >= 0);
+          id_cur = id_nxt;
+          id_nxt = id2;
+          cp_async_wait<1>();                            // this lane's copies of block i have landed (block i+1 may be in flight) ...
+          __syncwarp();                                  // ... and the other lanes'
+          const uint8_t* st = stage_of(i);
+          uint8_t* dst = kv_s + kvb * kMlaKBytes;
+          uint8_t* dst_lat = dst + (lane >> 3) * kMlaKPanelBytes;
+  #pragma unroll
+          for (int j = 0; j < kRows; ++j) {
+            const int r = w4 + j * kG;
+            const uint2 raw = *reinterpret_cast<const uint2*>(st + j * kRawRow + lane * 8);
+            const float sc = *reinterpret_cast<const float*>(st + j * kRawRow + 256 + cta * 8 + (lane >> 4) * 4);
+            const uint4 v = e4m3x8_to_bf16(raw, sc);
+            if (r < kMlaBlk) *reinterpret_cast<uint4*>(dst_lat + r * 128 + (((lane ^ r) & 7) << 4)) = v;
+          }
+          {
+            const int r = w4 + (lane >> 2) * kG;
+            if (lane < 4 * kRows && r < kMlaBlk)
+              *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane ^ (r >> 1)) & 3) << 4)) =
+                  *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16);
+          }
+          __syncwarp();                                  // (the MMA warp makes the writes visible to the tensor core's reads)
+          if (lane == 0) mbar_arrive(&kv_full[kvb]);
+          fetch(i + 2, id2);                             // into the stage just read: what was loaded from it has been stored
+        }
       }
       cp_async_wait_all();                             // nothing of this thread's is in flight when it leaves
     }
