@@ -94,7 +94,8 @@ struct MlaRegs {                                   // decode's gather converts i
   static_assert(512 * kSoftmax + 384 * kOther <= 896 * 72, "more registers than the launch has");
 };
 constexpr int kMlaFewHeads = 32;                   // up to here calls go to the kernels for few heads (sparse_mla_few.cu, sparse_mla_few4.cu)
-constexpr int kMlaMaxParts = 8;                    // parts of a split list
+constexpr int kMlaMaxParts = 8;                    // parts of a split list ...
+constexpr int kMlaMaxParts4 = 16;                  // ... of 4-bit records
 constexpr int kMlaMaxK = 2048;                     // slots of a list
 constexpr int kMlaThreads = 896, kMlaSoftmaxWarps = 16, kMlaMmaWarp = 16, kMlaGatherWarp0 = 17, kMlaGatherWarps = 11;
 template <int R>
@@ -131,6 +132,7 @@ struct MlaArgs {
   int num_phys_rows;              // decode: rows of the cache
   float scale_log2e;              // softmax scale * log2(e)
   int* status;
+  int group;                      // heads of a unit at most: 128, or 32 or 64 (4-bit records)
   int n_full;                     // the first n_full queries are one unit (CTA pair) each; ...
   int n_split;                    // ... the slot list of every later one is cut into n_split parts, a unit each (decode)
   float* part_o;                  // [(T - n_full) * n_split, H, 512] fp32 normalised partial outputs
@@ -254,8 +256,9 @@ __device__ __forceinline__ uint4 e4m3x8_to_bf16(uint2 raw, float sc) {
 }
 
 // OVERLAPPED: a launch that may start under the end of the top-k's (decode of few sequences; in the others its loads and their
-// place cost 2 %: batch 148 122.3 -> 124.9 us).
-template <int SRC, bool OVERLAPPED>
+// place cost 2 %: batch 148 122.3 -> 124.9 us).  GROUPS: units of a.group heads, not 128 (the argument in place of the constant costs
+// 3 %: 64 rows of 4-bit records 43.7 -> 45.0 us).
+template <int SRC, bool OVERLAPPED, bool GROUPS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMlaThreads, 1)
 sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
                   const __grid_constant__ CUtensorMap tmap_o, const MlaArgs a) {
@@ -289,12 +292,12 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
   const int unit = blockIdx.x >> 1;
   const int part = PAGED ? unit - a.n_full : -1;           // >= 0: a part of a split slot list (prefill's are never cut)
   const int n_split = part < 0 ? 1 : a.n_split, t = part < 0 ? unit : a.n_full + part / n_split, split = part < 0 ? 0 : part % n_split;
-  const int hg = blockIdx.z;
+  const int h0 = blockIdx.z * (GROUPS ? a.group : 128);      // the first of its heads
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int k_per = ((a.K + n_split - 1) / n_split + kMlaBlk - 1) / kMlaBlk * kMlaBlk;   // slots per part
   const int k_lo = min(a.K, split * k_per), k_cnt = min(a.K, k_lo + k_per) - k_lo;
   const int32_t* idx_row = a.idx + (int64_t)t * a.K + k_lo;
-  const int heads_here = min(128, a.H - hg * 128);
+  const int heads_here = min(GROUPS ? a.group : 128, a.H - h0);
   const int n_quad = (heads_here + 31) / 32;                   // quadrants of tensor memory with heads in them: the others' warps stand by
   // the five Q panels wait at the end of the KV buffers (from buffer kQBuf0 on) for their move into tensor memory
   constexpr int kQStage = NB * kMlaKBytes - kMlaPanels * kMlaQPanelBytes, kQBuf0 = kQStage / kMlaKBytes;
@@ -347,7 +350,7 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
     __syncwarp();
     // Q is on its way before anything else happens: into this CTA's own shared memory, counted on its own barrier
     if (lane < kMlaPanels)                             // x in 4-byte units: 32 per panel
-      tma_load_2d(q_stage(lane), &tmap_q, (lane < 4 ? cta * 4 + lane : 8) * 32, t * a.H + hg * 128, q_full);
+      tma_load_2d(q_stage(lane), &tmap_q, (lane < 4 ? cta * 4 + lane : 8) * 32, t * a.H + h0, q_full);
     if (lane == kMlaPanels && a.tma_out) tma_prefetch_desc(&tmap_o);
   } else if (warp == kMlaMmaWarp) {
     tmem_alloc(tmem_slot, kMlaTmemCols);
@@ -380,13 +383,13 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
   if (nblk == 0) {   // nothing selected: the output row is zero (a part: weight zero in the combine); no cluster traffic yet
     if (threadIdx.x < 128 && threadIdx.x < heads_here) {
       if (part < 0) {
-        uint4* o = reinterpret_cast<uint4*>(a.out + ((int64_t)t * a.H + hg * 128 + threadIdx.x) * kMlaDv + cta * kMlaDvHalf);
+        uint4* o = reinterpret_cast<uint4*>(a.out + ((int64_t)t * a.H + h0 + threadIdx.x) * kMlaDv + cta * kMlaDvHalf);
         for (int c = 0; c < kMlaDvHalf * 2 / 16; ++c) o[c] = make_uint4(0, 0, 0, 0);
       } else {
-        const int64_t prow = (int64_t)part * a.H + hg * 128 + threadIdx.x;
+        const int64_t prow = (int64_t)part * a.H + h0 + threadIdx.x;
         float4* o = reinterpret_cast<float4*>(a.part_o + prow * kMlaDv + cta * kMlaDvHalf);
         for (int c = 0; c < kMlaDvHalf / 4; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        a.part_lse[((int64_t)part * 2 + cta) * a.H + hg * 128 + threadIdx.x] = -CUDART_INF_F;
+        a.part_lse[((int64_t)part * 2 + cta) * a.H + h0 + threadIdx.x] = -CUDART_INF_F;
       }
     }
     // an index that is out of range is still reported
@@ -881,10 +884,10 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
         if (ml.x != -CUDART_INF_F) l += ml.y * fast_exp2(ml.x - mt);
       }
       const float inv = l > 0.f ? (SRC == kSrc4 ? kLatent4Gain : 1.f) / l : 0.f;
-      __nv_bfloat16* orow = a.out + ((int64_t)t * a.H + hg * 128 + row) * kMlaDv + cta * kMlaDvHalf;
-      const int64_t prow = (int64_t)part * a.H + hg * 128 + row;
+      __nv_bfloat16* orow = a.out + ((int64_t)t * a.H + h0 + row) * kMlaDv + cta * kMlaDvHalf;
+      const int64_t prow = (int64_t)part * a.H + h0 + row;
       if (part >= 0 && quarter == 0 && row < heads_here)         // what this CTA's half of the columns is weighted with
-        a.part_lse[((int64_t)part * 2 + cta) * a.H + hg * 128 + row] = l > 0.f ? mt + log2f(l) : -CUDART_INF_F;
+        a.part_lse[((int64_t)part * 2 + cta) * a.H + h0 + row] = l > 0.f ? mt + log2f(l) : -CUDART_INF_F;
 #pragma unroll 1
       for (int c = quarter * (kMlaDvHalf / 4); c < (quarter + 1) * (kMlaDvHalf / 4); c += 32) {
         uint32_t ov[32];
@@ -926,7 +929,7 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
       fence_async_smem();                              // the store below reads the panel through the async proxy
       named_bar_sync(7 + quarter, 128);
       if ((warp & 3) == 0 && elect_one() && !*abort_flag) {         // x in 4-byte units: 32 per 64-column panel
-        tma_store_2d(&tmap_o, kv_s + quarter * kMlaQPanelBytes, (cta * 4 + quarter) * 32, t * a.H + hg * 128);
+        tma_store_2d(&tmap_o, kv_s + quarter * kMlaQPanelBytes, (cta * 4 + quarter) * 32, t * a.H + h0);
         bulk_commit_and_wait_read();                   // the panel has been read: the CTA may go
       }
     }
@@ -953,31 +956,32 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
 // out[t,h,:] = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M): merges the parts of a split slot list, each half of the columns
 // by the sums of the CTA that computed it.
 // A query in eight parts: 4.8 us with loads behind the weights' loop, 3.6 so.
+template <int PARTS>
 __global__ void __launch_bounds__(128) sparse_mla_combine_kernel(const MlaArgs a) {
   const float *lse = grid_wait(a.part_lse), *part = grid_wait(a.part_o);      // the second returns at once
   const int u = blockIdx.x, t = a.n_full + u, h = blockIdx.y;
   const int d = threadIdx.x * 4, cta = d / kMlaDvHalf;
   // every load is requested before any is used: a part's weight and values do not wait for one another
-  float wgt[kMlaMaxParts];
-  float4 v[kMlaMaxParts];
+  float wgt[PARTS];
+  float4 v[PARTS];
 #pragma unroll
-  for (int sp = 0; sp < kMlaMaxParts; ++sp) {
+  for (int sp = 0; sp < PARTS; ++sp) {
     const int64_t p = (int64_t)u * a.n_split + sp;
     wgt[sp] = sp < a.n_split ? lse[(p * 2 + cta) * a.H + h] : -CUDART_INF_F;
     v[sp] = sp < a.n_split ? *reinterpret_cast<const float4*>(part + (p * a.H + h) * kMlaDv + d) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   float mx = -CUDART_INF_F, den = 0.f;
 #pragma unroll
-  for (int sp = 0; sp < kMlaMaxParts; ++sp) mx = fmaxf(mx, wgt[sp]);
+  for (int sp = 0; sp < PARTS; ++sp) mx = fmaxf(mx, wgt[sp]);
 #pragma unroll
-  for (int sp = 0; sp < kMlaMaxParts; ++sp) {
+  for (int sp = 0; sp < PARTS; ++sp) {
     wgt[sp] = (mx == -CUDART_INF_F) ? 0.f : exp2f(wgt[sp] - mx);
     den += wgt[sp];
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int sp = 0; sp < kMlaMaxParts; ++sp) {
+  for (int sp = 0; sp < PARTS; ++sp) {
     acc.x += wgt[sp] * v[sp].x; acc.y += wgt[sp] * v[sp].y; acc.z += wgt[sp] * v[sp].z; acc.w += wgt[sp] * v[sp].w;
   }
   uint2 o;
@@ -989,7 +993,7 @@ __global__ void __launch_bounds__(128) sparse_mla_combine_kernel(const MlaArgs a
 int make_tmap_2d_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t inner_bytes, uint64_t row_pitch,
                        uint32_t box_bytes, uint32_t box_rows);
 
-template <int SRC, bool OVERLAPPED>
+template <int SRC, bool OVERLAPPED, bool GROUPS = false>
 static int launch_mla(const void* q, const void* kv, const MlaArgs& args, cudaStream_t stream) {
   if (args.T == 0 || args.H == 0) return DSA_OK;
   if (args.K > kMlaMaxK) return set_error(DSA_ERR_SHAPE, "sparse_mla: K (%d) exceeds %d", args.K, kMlaMaxK);
@@ -1005,14 +1009,16 @@ static int launch_mla(const void* q, const void* kv, const MlaArgs& args, cudaSt
     if ((rc = make_tmap_2d_bytes(&to, a.out, (uint64_t)a.T * a.H, kMlaDv * 2, kMlaDv * 2, 128, 128))) return rc;
     a.tma_out = 1;
   }
-  auto kern = sparse_mla_kernel<SRC, OVERLAPPED>;
+  auto kern = sparse_mla_kernel<SRC, OVERLAPPED, GROUPS>;
   constexpr int smem_bytes = MlaRaw<SRC>::kSmem;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess)
     return set_error(DSA_ERR_CUDA, "sparse_mla: cannot raise dynamic shared memory to %d", smem_bytes);
   const int n_parts = a.T - a.n_full;
-  const dim3 grid(2 * (a.n_full + n_parts * a.n_split), 1, (a.H + 127) / 128);
+  const dim3 grid(2 * (a.n_full + n_parts * a.n_split), 1, (a.H + a.group - 1) / a.group);
   launch_after(OVERLAPPED, kern, grid, kMlaThreads, smem_bytes, stream, tq, to, a);
-  if (n_parts > 0) launch_after(OVERLAPPED, sparse_mla_combine_kernel, dim3(n_parts, a.H), 128, 0, stream, a);
+  if (n_parts > 0)
+    launch_after(OVERLAPPED, a.n_split > kMlaMaxParts ? sparse_mla_combine_kernel<kMlaMaxParts4> : sparse_mla_combine_kernel<kMlaMaxParts>,
+                 dim3(n_parts, a.H), 128, 0, stream, a);
   return check_launch("sparse_mla");
 }
 
@@ -1029,6 +1035,7 @@ int sparse_mla_prefill_launch(const void* q, const void* kv, const int32_t* idx,
   a.T = T; a.H = H; a.K = K; a.S_kv = S_kv;
   a.scale_log2e = scale * 1.4426950408889634f;
   a.status = status;
+  a.group = 128;
   a.n_full = T;
   a.n_split = 1;
   return launch_mla<kSrcRows, false>(q, kv, a, stream);
@@ -1039,20 +1046,38 @@ int sparse_mla_prefill_launch(const void* q, const void* kv, const int32_t* idx,
 // eight, of at least 256 slots.  More parts than that lose: every part pays the set-up again and writes an fp32 partial
 // output that the combine kernel reads back.  Batch 160 (two rounds and twelve queries in six parts each): 174 -> 156 us.
 static int mla_pairs(int H) { return max(1, sm_count() / (2 * ((H + 127) / 128))); }
-static int mla_parts_per_query(int rest, int pairs, int K) { return rest == 0 ? 1 : max(1, min(min(kMlaMaxParts, K / 256), pairs / rest)); }
+struct MlaPlan {
+  int group, parts;                                    // heads of a unit; parts of a list of the last round
+};
+// 4-bit records, calls without a full round: fewer heads to a unit where pairs stand idle, 32 or 64, since a block's exchange and softmax
+// take less time the fewer heads there are, and up to sixteen parts of at least 128 slots.  2048 slots, 128 heads, groups of 128 / 64 / 32,
+// each with its best number of parts: 1 row 18.2 / 14.1 / 13.5 us, 2 rows 19.1 / 15.2 / 14.8, 4 rows 20.6 / 17.0 / 18.8, 8 rows
+// 22.6 / 21.4 / 26, 12 rows 25.1 / 25.1 / 30.
+static MlaPlan mla_plan(int record_bytes, bool full_round, int rest, int H, int K) {
+  if (rest == 0) return {128, 1};
+  const auto room = [&](int group) { return sm_count() / 2 / (rest * ((H + group - 1) / group)); };      // parts that run at once
+  if (record_bytes == kLatent4Bytes && !full_round) {
+    const int group = room(32) >= 8 ? 32 : room(64) >= 4 ? 64 : 128;
+    if (group < 128) return {group, max(1, min(min(kMlaMaxParts4, K / 128), room(group)))};
+  }
+  return {128, max(1, min(min(kMlaMaxParts, K / 256), mla_pairs(H) / rest))};
+}
 static size_t mla_part_bytes(int H) { return (size_t)H * (kMlaDv + 2) * sizeof(float); }
 // Enough for every batch of up to B queries.  The need of a batch goes up and down with the queries of its last round (128
 // heads, 2048 slots, 148 SMs: 64 parts for 8 queries, 74 for 37, none for 38 or for 74), and a serving loop runs smaller
 // batches in the buffer that it made for its largest.
-size_t mla_decode_workspace_bytes(int B, int H, int K) {
+static size_t mla_workspace_bytes(int record_bytes, int B, int H, int K) {
   const int pairs = mla_pairs(H);
   int parts = 0;
   for (int rest = 1; rest < pairs && rest <= B; ++rest) {
-    const int ns = mla_parts_per_query(rest, pairs, K);
-    if (ns > 1) parts = max(parts, rest * ns);
+    for (const bool full_round : {false, true}) {
+      const int ns = mla_plan(record_bytes, full_round, rest, H, K).parts;
+      if (ns > 1) parts = max(parts, rest * ns);
+    }
   }
   return parts * mla_part_bytes(H);
 }
+size_t mla_decode_workspace_bytes(int B, int H, int K) { return mla_workspace_bytes(kLatentTokenBytes, B, H, K); }
 
 int sparse_mla_few4_launch(const void* q, const void* cache, const int32_t* block_table, int64_t table_stride, int tokens_per_seq, const int32_t* idx,
                            void* out, int T, int H, int K, int num_pages, int max_ctx, float scale, void* workspace, size_t workspace_bytes,
@@ -1060,7 +1085,7 @@ int sparse_mla_few4_launch(const void* q, const void* cache, const int32_t* bloc
 size_t few4_workspace_bytes(int T, int H, int K);
 
 size_t mla_decode_records_workspace_bytes(int record_bytes, int T, int H, int K) {
-  return record_bytes == kLatent4Bytes && H <= kMlaFewHeads ? few4_workspace_bytes(T, H, K) : mla_decode_workspace_bytes(T, H, K);
+  return record_bytes == kLatent4Bytes && H <= kMlaFewHeads ? few4_workspace_bytes(T, H, K) : mla_workspace_bytes(record_bytes, T, H, K);
 }
 
 int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,
@@ -1072,11 +1097,13 @@ int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes,
                                   workspace_bytes, status, overlapped, stream);
   MlaArgs a{};
   const int pairs = mla_pairs(H), rest = B % pairs;
-  int ns = mla_parts_per_query(rest, pairs, K);
+  const MlaPlan plan = mla_plan(record_bytes, B >= pairs, rest, H, K);
+  int ns = plan.parts;
   if (ns > 1) {                                        // a smaller workspace: as many parts as it holds
     const size_t fit = workspace ? workspace_bytes / mla_part_bytes(H) / rest : 0;
     if (fit < (size_t)ns) ns = fit > 1 ? (int)fit : 1;
   }
+  a.group = plan.group;
   a.n_full = B;
   a.n_split = 1;
   if (ns > 1) {
@@ -1095,7 +1122,10 @@ int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes,
   a.num_phys_rows = num_pages * kLatentPage;
   a.scale_log2e = scale * 1.4426950408889634f;
   a.status = status;
-  if (record_bytes == kLatent4Bytes) return overlapped ? launch_mla<kSrc4, true>(q, nullptr, a, stream) : launch_mla<kSrc4, false>(q, nullptr, a, stream);
+  if (record_bytes == kLatent4Bytes) {
+    if (a.group < 128) return overlapped ? launch_mla<kSrc4, true, true>(q, nullptr, a, stream) : launch_mla<kSrc4, false, true>(q, nullptr, a, stream);
+    return overlapped ? launch_mla<kSrc4, true>(q, nullptr, a, stream) : launch_mla<kSrc4, false>(q, nullptr, a, stream);
+  }
   return overlapped ? launch_mla<kSrcFp8, true>(q, nullptr, a, stream) : launch_mla<kSrcFp8, false>(q, nullptr, a, stream);
 }
 

@@ -170,6 +170,19 @@ def test_attention_against_64_bits(B, tokens, H, P, K):
     check_attention(out, q, rec, table, idx, 192 ** -0.5, tokens)
 
 
+@pytest.mark.parametrize("B", [1, 2, 3, 4, 9, 10])
+@pytest.mark.parametrize("H", [40, 64, 100, 128, 200])
+@pytest.mark.parametrize("room", [0, 2, None])
+def test_few_rows_by_groups_of_heads_and_parts(B, H, room):
+    """The units of small calls are groups of heads and parts of lists; a workspace holds some of the parts, or none."""
+    K = 1100
+    q, rec, table, idx = attention_case(B, 1, H, 20, K, seed=B + H, lens=[K, 1, 700, 0, 64, 129, K, 500, 1000, 64][:B])
+    need = None if room is None else torch.empty(room * B * H * 514 * 4, dtype=torch.uint8, device="cuda")
+    out = ops.sparse_mla_decode_paged(q.cuda(), rec.cuda(), table.cuda(), idx.cuda(), 192 ** -0.5, workspace=need)
+    ops.check_status("cuda")
+    check_attention(out, q, rec, table, idx, 192 ** -0.5)
+
+
 @pytest.mark.parametrize("H", [8, 16, 32, 64, 128])
 def test_lists_that_are_short_empty_or_full_of_holes(H):
     lens = [0, 1, 2, 63, 64, 65, 128, 300, 0, 511, 512]
