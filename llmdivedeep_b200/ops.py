@@ -76,6 +76,29 @@ def status_word(device) -> torch.Tensor:
     return w
 
 
+# For calls that take less time on the GPU than on the host: each tensor is looked at once, no device object, no context.  On the host
+# a scheduler's step (free, extend, fork) 41.5 -> 37.3 us, compacting 19.0 -> 16.7, copying pages 12.5 -> 9.4.
+def _index_of(first, *ts) -> int:
+    """_need_cuda for calls that need the device's number alone."""
+    i = first.get_device()
+    for t in ts:
+        if t.get_device() != i:
+            i = -1
+    return i if i >= 0 else _need_cuda(first, *ts).index
+
+
+def _run(i: int, fn, *args) -> None:
+    """fn(*args, status word, stream) on device i."""
+    w = _status.get(i)
+    if w is None:
+        w = status_word(torch.device("cuda", i))
+    if torch._C._cuda_getDevice() == i:
+        check(fn(*args, w.data_ptr(), torch._C._cuda_getCurrentRawStream(i)))
+    else:
+        with torch.cuda.device(i):
+            check(fn(*args, w.data_ptr(), torch._C._cuda_getCurrentRawStream(i)))
+
+
 def check_status(device) -> None:
     """Synchronise and raise if a kernel flagged a soft error since the last check."""
     w = status_word(device)
@@ -320,11 +343,7 @@ def sparse_mla_decode_paged(q, cache, block_table, idx, scale: float, max_ctx: O
     logical positions.  T = B * tokens_per_seq: a sequence's query rows one after the other.  Returns bf16 [T,H,512]."""
     if tokens_per_seq == 1 and cache.dim() == 2 and cache.shape[1] == 656:
         return _sparse_mla_decode_fp8(q, cache, block_table, idx, scale, max_ctx, out, workspace)
-    # A decode step of few rows waits for the host: each tensor is looked at once.
-    dev = q.device
-    i = dev.index
-    if dev.type != "cuda" or cache.get_device() != i or block_table.get_device() != i or idx.get_device() != i:
-        dev = _need_cuda(q, cache, block_table, idx)
+    i = _index_of(q, cache, block_table, idx)
     if (q.dtype is not torch.bfloat16 or cache.dtype is not torch.uint8 or idx.dtype is not torch.int32 or block_table.dtype is not torch.int32):
         raise DsaError("sparse_mla_decode_paged takes bf16 q, uint8 cache, int32 block_table/idx")
     if q.dim() != 3 or cache.dim() != 2 or idx.dim() != 2 or block_table.dim() != 2:
@@ -339,16 +358,14 @@ def sparse_mla_decode_paged(q, cache, block_table, idx, scale: float, max_ctx: O
         out = q.new_empty((T, H, 512))
     else:
         _need_cuda(q, out)
-        _check_attn_out(out, (T, H, 512), dev)
+        _check_attn_out(out, (T, H, 512), q.device)
     lib = _lib.load()
     if workspace is None:
         workspace = cache.new_empty(lib.dsa_sparse_mla_decode_records_workspace_bytes(width, T, H, K))      # as _workspace
     else:
         _need_cuda(q, workspace)
-    with _on(dev):
-        check(lib.dsa_sparse_mla_decode_records(q.data_ptr(), cache.data_ptr(), width, block_table.data_ptr(), P, tokens_per_seq, idx.data_ptr(),
-                                                out.data_ptr(), T, H, K, rows // 64, P * 64 if max_ctx is None else max_ctx, float(scale),
-                                                workspace.data_ptr(), workspace.numel(), status_word(dev).data_ptr(), _stream(dev)))
+    _run(i, lib.dsa_sparse_mla_decode_records, q.data_ptr(), cache.data_ptr(), width, block_table.data_ptr(), P, tokens_per_seq, idx.data_ptr(),
+         out.data_ptr(), T, H, K, rows // 64, P * 64 if max_ctx is None else max_ctx, float(scale), workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -629,15 +646,16 @@ def pack_latent4(kv: torch.Tensor, cache: Optional[torch.Tensor] = None, slots: 
     skip; None: row i) of ``cache`` (None: a new uint8 [N, 416]), one kernel.  Returns the cache.  ``keys`` = (k_fp8 [N,128] e4m3,
     k_scale [N] fp32, kcache [rows,128] e4m3, kscale [rows] fp32) sends the tokens' indexer keys to the same rows of the paged key
     cache along with them."""
-    dev = _need_cuda(kv, cache, slots, *(keys or ()))
-    if kv.dtype not in (torch.bfloat16, torch.float32) or kv.dim() != 2 or kv.shape[1] != 576:
-        raise DsaError(f"pack_latent4 takes bf16 or fp32 rows [N, 576], got {kv.dtype} {tuple(kv.shape)}")
-    N = kv.shape[0]
+    i = _index_of(kv, *[t for t in (cache, slots, *(keys or ())) if t is not None])
+    dtype, shape = kv.dtype, kv.shape
+    if dtype not in (torch.bfloat16, torch.float32) or len(shape) != 2 or shape[1] != 576:
+        raise DsaError(f"pack_latent4 takes bf16 or fp32 rows [N, 576], got {dtype} {tuple(shape)}")
+    N = shape[0]
     rs, cs = kv.stride()
     if N and (cs != 1 or (N > 1 and (rs < 576 or rs * kv.element_size() % 16)) or kv.data_ptr() % 16):
-        kv = kv.clone(memory_format=torch.contiguous_format)
+        kv, rs = kv.clone(memory_format=torch.contiguous_format), 576
     if cache is None:
-        cache = torch.empty(N, 416, dtype=torch.uint8, device=dev)
+        cache = torch.empty(N, 416, dtype=torch.uint8, device=kv.device)
     _check_records4(cache)
     slots = _as_i32(slots, N, "slots")
     k8 = ksc = kcache = kscale = None
@@ -650,10 +668,8 @@ def pack_latent4(kv: torch.Tensor, cache: Optional[torch.Tensor] = None, slots: 
         if not (kcache.is_contiguous() and kscale.is_contiguous()):
             raise DsaError("the key cache and its scales must be contiguous")
         k8, ksc = k8.contiguous(), ksc.contiguous()
-    with _on(dev):
-        check(_lib.load().dsa_pack_latent4(kv.data_ptr(), 1 if kv.dtype == torch.bfloat16 else 0, kv.stride(0) if N > 1 else 576, N, cache.data_ptr(),
-                                           cache.shape[0], _ptr(slots), _ptr(k8), _ptr(ksc), _ptr(kcache), _ptr(kscale),
-                                           _ptr(status_word(dev)), _stream(dev)))
+    _run(i, _lib.load().dsa_pack_latent4, kv.data_ptr(), 1 if dtype is torch.bfloat16 else 0, rs if N > 1 else 576, N, cache.data_ptr(),
+         cache.shape[0], _ptr(slots), _ptr(k8), _ptr(ksc), _ptr(kcache), _ptr(kscale))
     return cache
 
 
@@ -662,7 +678,7 @@ def unpack_latent4(cache: torch.Tensor, n: Optional[int] = None, block_table: Op
     """Positions 0..n-1 of one sequence as bf16 rows [n, 576], from its 4-bit records: position p is record
     block_table[p // 64] * 64 + p % 64 (block_table int32 [P], a row of the batch's; None: record p).  What a chunked prefill
     hands to sparse_mla_prefill.  ``out`` may have rows further apart than 576 values."""
-    dev = _need_cuda(cache, block_table, out)
+    i = _index_of(cache, *[t for t in (block_table, out) if t is not None])
     _check_records4(cache)
     if block_table is not None:
         if block_table.dtype != torch.int32 or block_table.dim() != 1:
@@ -673,48 +689,48 @@ def unpack_latent4(cache: torch.Tensor, n: Optional[int] = None, block_table: Op
     if n < 0 or n > most:
         raise DsaError(f"{n} positions of a sequence that has room for {most}")
     if out is None:
-        out = torch.empty(n, 576, dtype=torch.bfloat16, device=dev)
+        out = torch.empty((n, 576), dtype=torch.bfloat16, device=cache.device)
     elif (out.dtype != torch.bfloat16 or tuple(out.shape) != (n, 576) or (n and out.stride(1) != 1) or (n > 1 and out.stride(0) % 8)
           or (n > 1 and out.stride(0) < 576)):
         raise DsaError(f"out must be bf16 [{n}, 576], rows a multiple of 8 values apart, got {out.dtype} {tuple(out.shape)} strides {tuple(out.stride())}")
-    with _on(dev):
-        check(_lib.load().dsa_unpack_latent4(cache.data_ptr(), cache.shape[0], _ptr(block_table), n, out.data_ptr(), out.stride(0) if n > 1 else 576,
-                                             _ptr(status_word(dev)), _stream(dev)))
+    _run(i, _lib.load().dsa_unpack_latent4, cache.data_ptr(), cache.shape[0], _ptr(block_table), n, out.data_ptr(), out.stride(0) if n > 1 else 576)
     return out
 
 
 # ---- pages of the paged caches ------------------------------------------------------------------------------------------
 def _page_caches(caches, num_pages: int):
     """The caches as an array of dsa_page_cache.  A cache is [num_pages*64, ...] or, for several layers, [layers, num_pages*64, ...]."""
-    rows, packed = num_pages * 64, []
+    rows, packed = num_pages * 64, b""
     for t in caches:
         shape = t.shape
-        one, many = len(shape) >= 1 and shape[0] == rows, len(shape) >= 2 and shape[1] == rows
+        dims = len(shape)
+        one, many = dims >= 1 and shape[0] == rows, dims >= 2 and shape[1] == rows
         if one == many:
             raise DsaError(f"a cache must be [{rows}, ...] or [layers, {rows}, ...], got {tuple(shape)}")
-        layers = 1 if one else shape[0]
-        if not t.is_contiguous() and not (many and t[0].is_contiguous()):
+        whole = t.is_contiguous()
+        if not whole and not (many and t[0].is_contiguous()):
             raise DsaError("the pages of a cache must be contiguous")
-        layer_bytes = (t.stride(0) if many else 0) * t.element_size()
-        packed.append(struct.pack("=Qqii", t.data_ptr(), layer_bytes, layers, t.element_size() * (t.numel() // max(1, layers * rows))))
-    return b"".join(packed), len(packed)
+        layers = 1 if one else shape[0]
+        token = t.element_size() * (t.numel() // max(1, layers * rows))
+        packed += struct.pack("=Qqii", t.data_ptr(), 0 if one else rows * token if whole else t.stride(0) * t.element_size(), layers, token)
+    return packed, len(caches)
 
 
 def _check_pool(table, ctx_len, refs) -> tuple:
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.numel() and table.stride(1) != 1):
+    shape = table.shape
+    if table.dtype is not torch.int32 or len(shape) != 2 or (table.stride(1) != 1 and table.numel()):
         raise DsaError("block_table must be int32 [B, pages] with unit column stride")
-    B, P = table.shape
     if ctx_len is not None:
-        _as_i32(ctx_len, B, "ctx_len")
-    if refs.dtype != torch.int32 or refs.dim() != 1 or not refs.is_contiguous():
+        _as_i32(ctx_len, shape[0], "ctx_len")
+    if refs.dtype is not torch.int32 or refs.dim() != 1 or not refs.is_contiguous():
         raise DsaError("refs must be a contiguous int32 [num_pages] tensor")
-    return B, P, refs.shape[0]
+    return shape[0], shape[1], refs.numel()
 
 
-def _list_i32(t, name: str):
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+def _list_i32(t, name: str) -> int:
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise DsaError(f"{name} must be a contiguous one-dimensional int32 tensor")
-    return t
+    return t.numel()
 
 
 def copy_pages(caches, src, dst, tokens=None, num_pages: Optional[int] = None) -> None:
@@ -722,34 +738,39 @@ def copy_pages(caches, src, dst, tokens=None, num_pages: Optional[int] = None) -
     ``tokens`` (int32 [n]) only the first tokens[i] of a page's 64.  No page may be written twice, nor be written and read.
     ``num_pages`` is needed only where the caches' shapes leave it open."""
     caches = list(caches)
-    dev = _need_cuda(*caches, src, dst, tokens)
-    n = _list_i32(src, "src").shape[0]
-    dst, tokens = _as_i32(dst, n, "dst"), _as_i32(tokens, n, "tokens")
+    i = _index_of(src, dst, *caches) if tokens is None else _index_of(src, dst, tokens, *caches)
+    n = _list_i32(src, "src")
+    _as_i32(dst, n, "dst")
+    _as_i32(tokens, n, "tokens")
     if num_pages is None:
-        rows = set.intersection(*({s for s in t.shape[:2] if s and s % 64 == 0} for t in caches)) if caches else {0}
-        if len(rows) != 1:
+        rows = None
+        for t in caches:
+            have = {s for s in t.shape[:2] if s and s % 64 == 0}
+            rows = have if rows is None else rows & have
+            if len(rows) == 1:                         # the other caches are held against it below
+                break
+        if rows is not None and len(rows) != 1:
             raise DsaError("the caches' shapes leave the number of pages open: give num_pages")
-        num_pages = rows.pop() // 64
+        num_pages = rows.pop() // 64 if rows else 0
     packed, count = _page_caches(caches, num_pages)
-    with _on(dev):
-        check(_lib.load().dsa_copy_pages(packed, count, num_pages, src.data_ptr(), dst.data_ptr(), _ptr(tokens), n, _ptr(status_word(dev)), _stream(dev)))
+    _run(i, _lib.load().dsa_copy_pages, packed, count, num_pages, src.data_ptr(), dst.data_ptr(), _ptr(tokens), n)
 
 
 def extend_pages(block_table, ctx_len, refs, rows, n_new, max_new: int) -> torch.Tensor:
     """Room for n_new[i] (int32, 0..max_new) more tokens in row rows[i] (int32, all different): takes the lowest free pages, in order,
     and writes block_table, ctx_len and refs.  Returns the new tokens' cache rows, int32 [n, max_new], -1 behind them.  All or
     nothing: with too few free pages (status 3) or a bad argument (status 2) nothing changes and every slot is -1."""
-    dev = _need_cuda(block_table, ctx_len, refs, rows, n_new)
+    i = _index_of(block_table, ctx_len, refs, rows, n_new)
     B, P, num_pages = _check_pool(block_table, ctx_len, refs)
-    n = _list_i32(rows, "rows").shape[0]
-    n_new = _as_i32(n_new, n, "n_new")
+    n = _list_i32(rows, "rows")
+    _as_i32(n_new, n, "n_new")
     max_new = int(max_new)
     lib = _lib.load()
-    slots = torch.empty(n, max(max_new, 0), dtype=torch.int32, device=dev)
-    ws = _workspace(dev, lib.dsa_pages_workspace_bytes(num_pages, n))
-    with _on(dev):
-        check(lib.dsa_extend_pages(block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages, rows.data_ptr(),
-                                   n_new.data_ptr(), n, max_new, slots.data_ptr(), ws.data_ptr(), ws.numel(), _ptr(status_word(dev)), _stream(dev)))
+    slots = rows.new_empty((n, max(max_new, 0)))
+    nbytes = lib.dsa_pages_workspace_bytes(num_pages, n)
+    ws = _workspace(rows.device, nbytes)
+    _run(i, lib.dsa_extend_pages, block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages, rows.data_ptr(),
+         n_new.data_ptr(), n, max_new, slots.data_ptr(), ws.data_ptr(), nbytes)
     return slots
 
 
@@ -758,26 +779,25 @@ def fork_pages(block_table, ctx_len, refs, parents, children, caches=()) -> None
     last one is copied to a page of the child's own in every cache.  Writes block_table, ctx_len and refs; all or nothing, as
     extend_pages."""
     caches = list(caches)
-    dev = _need_cuda(block_table, ctx_len, refs, parents, children, *caches)
+    i = _index_of(block_table, ctx_len, refs, parents, children, *caches)
     B, P, num_pages = _check_pool(block_table, ctx_len, refs)
-    n = _list_i32(parents, "parents").shape[0]
-    children = _as_i32(children, n, "children")
+    n = _list_i32(parents, "parents")
+    _as_i32(children, n, "children")
     packed, count = _page_caches(caches, num_pages)
     lib = _lib.load()
-    ws = _workspace(dev, lib.dsa_pages_workspace_bytes(num_pages, n))
-    with _on(dev):
-        check(lib.dsa_fork_pages(block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages, parents.data_ptr(),
-                                 children.data_ptr(), n, packed, count, ws.data_ptr(), ws.numel(), _ptr(status_word(dev)), _stream(dev)))
+    nbytes = lib.dsa_pages_workspace_bytes(num_pages, n)
+    ws = _workspace(refs.device, nbytes)
+    _run(i, lib.dsa_fork_pages, block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages, parents.data_ptr(),
+         children.data_ptr(), n, packed, count, ws.data_ptr(), nbytes)
 
 
 def free_pages(block_table, ctx_len, refs, rows) -> None:
     """Rows ``rows`` (int32) become empty and give their pages back: refs - 1, -1 in block_table, 0 in ctx_len."""
-    dev = _need_cuda(block_table, ctx_len, refs, rows)
+    i = _index_of(block_table, ctx_len, refs, rows)
     B, P, num_pages = _check_pool(block_table, ctx_len, refs)
-    n = _list_i32(rows, "rows").shape[0]
-    with _on(dev):
-        check(_lib.load().dsa_free_pages(block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages,
-                                         rows.data_ptr(), n, _ptr(status_word(dev)), _stream(dev)))
+    n = _list_i32(rows, "rows")
+    _run(i, _lib.load().dsa_free_pages, block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages,
+         rows.data_ptr(), n)
 
 
 def compact_pages(block_table, refs, caches, out: Optional[tuple] = None) -> tuple:
@@ -785,15 +805,15 @@ def compact_pages(block_table, refs, caches, out: Optional[tuple] = None) -> tup
     as they are afterwards: new tensors, or ``out`` (which may be the given ones).  The pages moved from stay as they are, so work in
     flight on the old table reads right until one of them is taken."""
     caches = list(caches)
-    dev = _need_cuda(block_table, refs, *caches, *(out or ()))
+    i = _index_of(block_table, refs, *caches, *(out or ()))
     B, P, num_pages = _check_pool(block_table, None, refs)
     new_table, new_refs = out if out is not None else (torch.empty_like(block_table, memory_format=torch.contiguous_format), torch.empty_like(refs))
     if _check_pool(new_table, None, new_refs) != (B, P, num_pages):
         raise DsaError("out must be a block table and refs of the same sizes")
     packed, count = _page_caches(caches, num_pages)
     lib = _lib.load()
-    ws = _workspace(dev, lib.dsa_pages_workspace_bytes(num_pages, 0))
-    with _on(dev):
-        check(lib.dsa_compact_pages(block_table.data_ptr(), block_table.stride(0), new_table.data_ptr(), new_table.stride(0), P, B, refs.data_ptr(),
-                                    new_refs.data_ptr(), num_pages, packed, count, ws.data_ptr(), ws.numel(), _ptr(status_word(dev)), _stream(dev)))
+    nbytes = lib.dsa_pages_workspace_bytes(num_pages, 0)
+    ws = _workspace(refs.device, nbytes)
+    _run(i, lib.dsa_compact_pages, block_table.data_ptr(), block_table.stride(0), new_table.data_ptr(), new_table.stride(0), P, B, refs.data_ptr(),
+         new_refs.data_ptr(), num_pages, packed, count, ws.data_ptr(), nbytes)
     return new_table, new_refs
