@@ -11,8 +11,8 @@
 // row's last bits depend on its place in the call.
 //   * warps 0-3: softmax and output; warp 4 issues the scores' MMAs, warp 6 those of P.V; warp 5: the end of every list, Q.
 //   * warps 7-22: four rows of a block each, eight lanes a row: the records are requested two blocks ahead into registers and, converted,
-//     go into a ring of half blocks (256 dims of 64 keys in four 128-byte swizzled panels; two blocks and a half fit).  Positions and
-//     page-table entries come for eight blocks at a time, one and two such groups ahead.
+//     go into a ring of half blocks (256 dims of 64 keys in four 128-byte swizzled panels, four such).  Positions and page-table entries
+//     come for eight blocks at a time, one and two such groups ahead.
 // Every wait is bounded (dsa_common.cuh).
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -58,7 +58,10 @@ constexpr uint32_t kF4RopeGain = 0x38803880u;          // 2^-14 as a pair of bf1
 
 template <int N>
 struct F4Cfg {
-  static constexpr int HALVES = 5;                     // ring of half blocks
+  // Ring of half blocks.  What is not shared memory is L1, and there the loads of the records under way need about 50 KB: five halves are
+  // slower, of 32 heads most, where they leave it 28 KB (148 rows x 2048 keys: 16 heads 54.8 -> 53.5 us, 32 heads 73.7 -> 62.9); three
+  // make the conversion wait for P.V (68.6, 81.2).
+  static constexpr int HALVES = 4;
   static constexpr int PBUFS = 2;
   static constexpr int Q_BYTES = 9 * N * 128, P_BYTES = N * 128;
   static constexpr int BAR_BYTES = 512;
@@ -71,6 +74,12 @@ __device__ __forceinline__ void f4_ld_s(uint32_t taddr, uint32_t (&r)[8]) {     
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr) : "memory");
+}
+// 16 bytes of a record: read once, so nothing is kept for it in L1 (16 heads, 148 rows 53.5 -> 52.9 us, 160 rows 66.6 -> 64.8).
+__device__ __forceinline__ uint4 f4_ld_once(const uint8_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
 }
 __device__ __forceinline__ uint32_t f4_pack(float lo, float hi) {
   uint32_t r;
@@ -170,17 +179,17 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
   uint8_t* q_s = rope_s + kF4Panel;                    // nine panels [N heads x 128 B]
   uint8_t* p_s = q_s + C::Q_BYTES;                     // P^T as [N heads][64 keys], swizzled
   uint64_t* bars = reinterpret_cast<uint64_t*>(p_s + C::PBUFS * C::P_BYTES);
-  uint64_t* half_full = bars + 0;                      // [5] gather -> MMA; a block's second half: its rope values and validity bytes too
-  uint64_t* half_free = bars + 5;                      // [5] P.V of those 256 dims has read the half
-  uint64_t* rope_free = bars + 10;                     // the block's scores have read the rope panel
-  uint64_t* q_full = bars + 11;
-  uint64_t* q_free = bars + 12;
-  uint64_t* s_full = bars + 13;                        // [2] MMA -> softmax
-  uint64_t* pv_done = bars + 15;                       // [2] P.V of the block complete
-  uint64_t* p_full = bars + 17;                        // [2] softmax -> MMA
-  uint64_t* meet = bars + 19;                          // the four softmax warps
-  uint64_t* s_free = bars + 20;                        // [2] the softmax has read S
-  constexpr int kBars = 22;
+  uint64_t* half_full = bars + 0;                      // [4] gather -> MMA; a block's second half: its rope values and validity bytes too
+  uint64_t* half_free = bars + 4;                      // [4] P.V of those 256 dims has read the half
+  uint64_t* rope_free = bars + 8;                      // the block's scores have read the rope panel
+  uint64_t* q_full = bars + 9;
+  uint64_t* q_free = bars + 10;
+  uint64_t* s_full = bars + 11;                        // [2] MMA -> softmax
+  uint64_t* pv_done = bars + 13;                       // [2] P.V of the block complete
+  uint64_t* p_full = bars + 15;                        // [2] softmax -> MMA
+  uint64_t* meet = bars + 17;                          // the four softmax warps
+  uint64_t* s_free = bars + 18;                        // [2] the softmax has read S
+  constexpr int kBars = 20;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* valid_s = reinterpret_cast<uint8_t*>(bars) + C::BAR_BYTES;
@@ -194,7 +203,7 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
   launch_dependents();
   if (warp == 0) {
     for (int i = lane; i < kBars; i += 32) {
-      const uint32_t count = i < 5 ? uint32_t(kF4GatherWarps) : i >= 17 ? uint32_t(kF4SoftmaxWarps) : 1u;
+      const uint32_t count = i < 4 ? uint32_t(kF4GatherWarps) : i >= 15 ? uint32_t(kF4SoftmaxWarps) : 1u;
       mbar_init(bars + i, count);
     }
     mbar_fence_init();
@@ -411,10 +420,10 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
         const uint8_t* src = a.cache + (int64_t)id * kLatent4Bytes;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          x.word[hf] = __ldg(reinterpret_cast<const uint4*>(src + hf * kLatent4Half + l8 * 16));
+          x.word[hf] = f4_ld_once(src + hf * kLatent4Half + l8 * 16);
           x.scales[hf] = __ldg(reinterpret_cast<const uint16_t*>(src + hf * kLatent4Half + kLatent4Scales + l8 * 2));
         }
-        x.rope = __ldg(reinterpret_cast<const uint4*>(src + (l8 >> 2) * kLatent4Half + kLatent4Rope + (l8 & 3) * 16));
+        x.rope = f4_ld_once(src + (l8 >> 2) * kLatent4Half + kLatent4Rope + (l8 & 3) * 16);
         x.used = true;
       }
       ++fetched;
