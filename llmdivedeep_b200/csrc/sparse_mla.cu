@@ -93,7 +93,7 @@ struct MlaRegs {                                   // decode's gather converts i
   static constexpr int kSoftmax = PAGED ? 88 : 96, kOther = PAGED ? 48 : 40;
   static_assert(512 * kSoftmax + 384 * kOther <= 896 * 72, "more registers than the launch has");
 };
-constexpr int kMlaFewHeads = 32;                   // up to here calls go to the kernels for few heads (sparse_mla_few.cu, sparse_mla_few4.cu)
+constexpr int kMlaFewHeads = 32;                   // up to here calls go to the kernels for few heads (sparse_mla_few.cu; mla_few4 below)
 constexpr int kMlaMaxParts = 8;                    // parts of a split list ...
 constexpr int kMlaMaxParts4 = 16;                  // ... of 4-bit records
 constexpr int kMlaMaxK = 2048;                     // slots of a list
@@ -1084,15 +1084,23 @@ int sparse_mla_few4_launch(const void* q, const void* cache, const int32_t* bloc
                            int32_t* status, int overlapped, cudaStream_t stream);
 size_t few4_workspace_bytes(int T, int H, int K);
 
+// 4-bit records, at most 32 heads: pairs while a list can have this many parts, then sparse_mla_few4.cu.  2048 slots, pairs / that one:
+// 16 heads, 1 row 11.6 / 14.3 us, 8 rows 14.9 / 15.9, 12 rows 16.5 / 17.5; 32 heads, 1 row 12.4 / 15.7, 12 rows 16.7 / 19.0, 18 rows
+// 19.5 / 19.3, 37 rows 28.0 / 25.7, 148 rows twice that one's time and more.
+constexpr int kMlaFewParts = 6;
+static bool mla_few4(int record_bytes, int T, int H) { return record_bytes == kLatent4Bytes && H <= kMlaFewHeads && sm_count() / 2 < T * kMlaFewParts; }
+
 size_t mla_decode_records_workspace_bytes(int record_bytes, int T, int H, int K) {
-  return record_bytes == kLatent4Bytes && H <= kMlaFewHeads ? few4_workspace_bytes(T, H, K) : mla_workspace_bytes(record_bytes, T, H, K);
+  if (record_bytes != kLatent4Bytes || H > kMlaFewHeads) return mla_workspace_bytes(record_bytes, T, H, K);
+  const size_t pairs = mla_workspace_bytes(record_bytes, min(T, sm_count() / 2 / kMlaFewParts), H, K);
+  return mla_few4(record_bytes, T, H) ? max(pairs, few4_workspace_bytes(T, H, K)) : pairs;
 }
 
 int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,
                              int tokens_per_seq, const int32_t* idx, void* out, int B, int H, int K, int num_pages, int max_ctx,
                              float scale, void* workspace, size_t workspace_bytes, int32_t* status, int overlapped,
                              cudaStream_t stream) {
-  if (record_bytes == kLatent4Bytes && H <= kMlaFewHeads)
+  if (mla_few4(record_bytes, B, H))
     return sparse_mla_few4_launch(q, cache, block_table, table_stride, tokens_per_seq, idx, out, B, H, K, num_pages, max_ctx, scale, workspace,
                                   workspace_bytes, status, overlapped, stream);
   MlaArgs a{};

@@ -1,5 +1,6 @@
-// Attention of at most 32 heads over the paged 4-bit latent cache (latent4.cuh): the function of sparse_mla.cu's decode with scores and
-// output TRANSPOSED, as in sparse_mla_few.cu, so that the heads are the N of the tensor-core tiles and not the M:
+// Attention of at most 32 heads over the paged 4-bit latent cache (latent4.cuh) for calls of more than a few rows (sparse_mla.cu takes
+// those): the function of that file's decode with scores and output TRANSPOSED, as in sparse_mla_few.cu, so that the heads are the N of
+// the tensor-core tiles and not the M:
 //   S^T [64 keys x N heads] = K Q^T     (M = 64, 36 K-steps over the 576 dims)
 //   O^T [512 dims x N heads] += V^T P^T (four M = 128 tiles, 4 K-steps over a block's 64 keys)
 // N is 16 or 32.  The latents are converted to bf16 times 2^-14, the rope values too: the scores come out 2^-14 times what they are and
@@ -13,6 +14,14 @@
 //   * warps 7-22: four rows of a block each, eight lanes a row: the records are requested two blocks ahead into registers and, converted,
 //     go into a ring of half blocks (256 dims of 64 keys in four 128-byte swizzled panels, four such).  Positions and page-table entries
 //     come for eight blocks at a time, one and two such groups ahead.
+//
+// What bounds it: 52 MMAs a block, which take about 45 cycles each whatever their N up to 32: 2340 of the ~2450 cycles that a block takes
+// (1200 of them the tensor cores' reads of shared memory, 600 the conversion's writes).  Issued by one warp, scores and P.V take 69.9 us
+// where two take 55.8 (148 rows x 2048 keys x 16 heads, then).  A call adds ~12000 cycles until the first block's scores are complete, a
+// further list two blocks, parts their merge.  2048 keys, 16 heads: 64 rows 33.3 us, 148 rows 53.0 (126 MB of records: 2.4 TB/s, 199 TFLOP/s),
+// 160 rows 64.5, 296 rows 98.5; 32 heads: 64 rows 39.9, 148 rows 62.4 (339 TFLOP/s), 256 rows 116.
+// Tried and dropped: rows by cp.async or bulk copies through a stage of raw records (65 to 84 us where this took 55.8), eight softmax warps
+// (60 to 66), Q of two lists (no gain), a prefetch of the first records into L2 (+4 us).
 // Every wait is bounded (dsa_common.cuh).
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -793,8 +802,8 @@ int sparse_mla_few4_launch(const void* q, const void* cache, const int32_t* bloc
     a.rest = max(0, a.T - a.rounds * a.ctas) * a.list_blocks;
     a.rest_ctas = min(a.ctas, max(1, a.rest / kF4LeastBlocks));
     // Equal parts of each list while they keep the GPU as busy: a CTA whose stretch lies in two lists pays for the second's Q, output and
-    // start what two blocks take.  2048 keys, us with stretches of all blocks and so: 16 heads 12 rows 19.1, 17.0; 24 rows 21.4, 19.1; 64 rows
-    // 34.6, 32.5; 32 heads 64 rows 44.9, 42.3.
+    // start what two blocks take.  2048 keys, us with stretches of all blocks and so: 16 heads 24 rows 21.4, 19.1; 64 rows 34.6, 32.5; 32 heads
+    // 64 rows 44.9, 42.3.
     a.per_list = 0;
     if (a.rest) {
       const int lists = a.rest / a.list_blocks, p = min(a.ctas / lists, max(1, a.list_blocks / kF4LeastBlocks));

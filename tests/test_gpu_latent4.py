@@ -183,6 +183,28 @@ def test_few_rows_by_groups_of_heads_and_parts(B, H, room):
     check_attention(out, q, rec, table, idx, 192 ** -0.5)
 
 
+@pytest.mark.parametrize("B,tokens,H,P,K,lens", [
+    (13, 1, 16, 33, 2048, [2048, 0, 1, 1000, 64, 65, 2048]), (7, 4, 9, 9, 512, [0, 512, 63, 300, 1]), (24, 1, 32, 20, 1100, [1100, 0, 129, 640]),
+    (70, 1, 16, 5, 300, [300, 0, 64, 17]), (149, 1, 16, 3, 130, [130, 0, 1, 64, 65]), (160, 1, 24, 3, 192, [192, 5, 0]), (300, 1, 8, 2, 128, [128, 0, 3]),
+])
+def test_few_heads_of_many_rows(B, tokens, H, P, K, lens):
+    """Short lists, holes and rows without keys, whole lists, stretches and equal parts of lists, NaN in what nobody selected."""
+    q, rec, table, idx = attention_case(B, tokens, H, P, K, seed=B + H, lens=lens)
+    g = torch.Generator().manual_seed(B)
+    idx[::4] = torch.where(torch.rand(idx[::4].shape, generator=g) < 0.3, torch.full_like(idx[::4], -1), idx[::4])
+    q[1::5] *= 4                                                   # references that grow
+    seen = torch.zeros(rec.shape[0], dtype=torch.bool)
+    for r in range(B * tokens):
+        pos = idx[r][idx[r] >= 0].long()
+        seen[table[r // tokens][pos // 64].long() * 64 + pos % 64] = True
+    rec[~seen] = 255
+    out = torch.full((B * tokens, H, 512), 9.0, dtype=torch.bfloat16, device="cuda")
+    for room in (None, torch.empty(0, dtype=torch.uint8, device="cuda")):
+        ops.sparse_mla_decode_paged(q.cuda(), rec.cuda(), table.cuda(), idx.cuda(), 192 ** -0.5, out=out, tokens_per_seq=tokens, workspace=room)
+        ops.check_status("cuda")
+        check_attention(out, q, rec, table, idx, 192 ** -0.5, tokens)
+
+
 @pytest.mark.parametrize("H", [8, 16, 32, 64, 128])
 def test_lists_that_are_short_empty_or_full_of_holes(H):
     lens = [0, 1, 2, 63, 64, 65, 128, 300, 0, 511, 512]
@@ -235,8 +257,8 @@ def test_numbers_that_are_none_stay_where_they_are(H):
 
 
 def test_bad_positions_and_pages_are_flagged_and_skipped():
-    for H in (16, 128):
-        q, rec, table, idx = attention_case(2, 1, H, 4, 100, seed=3)
+    for B, H in ((2, 16), (20, 16), (2, 128)):
+        q, rec, table, idx = attention_case(B, 1, H, 4, 100, seed=3)
         bad, tab = idx.clone(), table.clone()
         bad[0, 3], bad[0, 70] = 256, 1 << 30                       # at max_ctx, far past it
         tab[1, 2] = 9999                                           # a page that is none
