@@ -445,9 +445,9 @@ class PagedCache:
     (a pool without free pages, a bad row) leaves the tables as they are and is in ops.check_status.  The tables are tensors of
     fixed addresses (``table``, ``ctx``, ``refs``), so that steps can be captured in a graph."""
 
-    def __init__(self, layers: int, num_pages: int, batch: int, max_ctx: int, device, index_dim: int = 128):
+    def __init__(self, layers: int, num_pages: int, batch: int, max_ctx: int, device):
         rows, dev = num_pages * 64, torch.device(device)
-        self.k8 = torch.zeros(layers, rows, index_dim, dtype=torch.uint8, device=dev).view(ops.FP8)
+        self.k8 = torch.zeros(layers, rows, 128, dtype=torch.uint8, device=dev).view(ops.FP8)
         self.k_scale = torch.zeros(layers, rows, dtype=torch.float32, device=dev)
         self.latent = torch.zeros(layers, rows, LATENT4_TOKEN_BYTES, dtype=torch.uint8, device=dev)
         self.table = torch.full((batch, -(-max_ctx // 64)), -1, dtype=torch.int32, device=dev)
