@@ -76,8 +76,8 @@ struct KeyRows {
   float* cache_scale;                                  // [cache_rows]
 };
 
-// Latent rows -> records at the cache rows `slots` (null: row i -> record i).  A warp per token: 1152 bytes in (bf16), 416 out.  8192 tokens: 7.8 us,
-// of which the bytes are 2; a launch and one wave of loads, arithmetic and stores one after the other.  (8.6 with a lane to every group of 16,
+// Latent rows -> records at the cache rows `slots` (null: row i -> record i).  A warp per token: 1152 bytes in (bf16), 416 out.  8192 tokens: 7.8 us
+// from memory (5.0 out of L2), of which the bytes are 2; a launch and one wave of loads, arithmetic and stores one after the other.  (8.6 with a lane to every group of 16,
 // whose loads and stores are pieces of lines, and an IEEE division for every value.)
 template <typename T>
 __global__ void __launch_bounds__(256) pack_latent4_kernel(const T* __restrict__ kv, int64_t row_stride, int64_t n, uint8_t* __restrict__ cache,
@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(256) pack_latent4_kernel(const T* __restrict__
 
 // Records of positions 0 .. n-1 -> bf16 rows.  Position p is the record table[p / 64] * 64 + p % 64 (no table: record p); a page that does not
 // exist gives a row of zeros.  A warp per token: 416 bytes in, 1152 out.  131072 tokens: 36.1 us = 5.7 TB/s, HBM (38.4 with a lane to every
-// group of 16).
+// group of 16).  Two or four tokens of a warp requested together 37.6, 43.1; a page to a CTA 38.7; one wave of CTAs 37.8; a CTA to every eight
+// tokens 36.9.
 __global__ void __launch_bounds__(256) unpack_latent4_kernel(const uint8_t* __restrict__ cache, int64_t cache_rows, const int32_t* __restrict__ table, int64_t n,
                                                              __nv_bfloat16* __restrict__ out, int64_t out_stride, int* status) {
   const int lane = threadIdx.x & 31;
