@@ -15,9 +15,10 @@
 //     go into a ring of half blocks (256 dims of 64 keys in four 128-byte swizzled panels, four such).  Positions and page-table entries
 //     come for eight blocks at a time, one and two such groups ahead.
 //
-// What bounds it: 52 MMAs a block, which take about 45 cycles each whatever their N up to 32: 2340 of the ~2450 cycles that a block takes
-// (1200 of them the tensor cores' reads of shared memory, 600 the conversion's writes).  Issued by one warp, scores and P.V take 69.9 us
-// where two take 55.8 (148 rows x 2048 keys x 16 heads, then).  A call adds ~12000 cycles until the first block's scores are complete, a
+// What bounds it: shared memory.  Of the ~2450 cycles that a block takes the tensor cores read it for 1300 (K and V once each, Q and P
+// with every instruction) and the warps use it for 860, the conversion's 73 KB most of it.  The number of MMAs does not: 34 a block in place of 52,
+// with score tiles of 128 rows -- two panels at a time, their sums exchanged between softmax warps -- take 55.1 us where this takes
+// 53.0 (148 rows, 16 heads).  Issued by one warp, though, scores and P.V took 69.9 us where two took 55.8.  A call adds ~12000 cycles until the first block's scores are complete, a
 // further list two blocks, parts their merge.  2048 keys, 16 heads: 64 rows 33.3 us, 148 rows 53.0 (126 MB of records: 2.4 TB/s, 199 TFLOP/s),
 // 160 rows 64.5, 296 rows 98.5; 32 heads: 64 rows 39.9, 148 rows 62.4 (339 TFLOP/s), 256 rows 116.
 // Tried and dropped: rows by cp.async or bulk copies through a stage of raw records (65 to 84 us where this took 55.8), eight softmax warps
