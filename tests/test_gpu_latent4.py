@@ -345,3 +345,18 @@ def test_decode_step_and_module_over_4_bits(B):
     check_attention(out, q, rec.cpu(), table, idx.cpu(), 0.06)
     again = layer.SparseMLA(0.06)(q.cuda(), rec, idx, table.cuda())
     assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("H", [16, 128])
+@pytest.mark.parametrize("tokens", [2, 5])
+def test_several_tokens_over_fp8_records(H, tokens):
+    """FP8 records with several query rows a sequence: bit for bit what the rows get as sequences of their own."""
+    B, P, K = 3, 9, 300
+    q, _, table, idx = attention_case(B, tokens, H, P, K, seed=tokens, lens=[300, 0, 65, 17])
+    g = torch.Generator().manual_seed(1)
+    cache = layer.pack_latent_cache(torch.randn((B * P + 2) * 64, 576, generator=g).bfloat16().cuda())
+    q, table, idx = q.cuda(), table.cuda(), idx.cuda()
+    got = ops.sparse_mla_decode_paged(q, cache, table, idx, 0.07, tokens_per_seq=tokens)
+    want = ops.sparse_mla_decode_paged(q, cache, table.repeat_interleave(tokens, 0), idx, 0.07)
+    ops.check_status("cuda")
+    assert torch.equal(got, want) and bool((got[1] == 0).all()) and bool(got[0].any())
