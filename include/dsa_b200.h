@@ -316,7 +316,12 @@ int dsa_indexer_topk_static(const void* q_fp8, const void* k_fp8, const float* k
  *   falls back to this path when the sample misleads it); same sets, same order.
  * dsa_test_bounded_wait: launches one thread that waits, with the wait helper all
  *   pipeline roles use, on a barrier nobody arrives at; after poll_limit
- *   (1..65536) polls it must give up and write status 1 to *status. */
+ *   (1..65536) polls it must give up and write status 1 to *status.
+ * dsa_test_few_heads_plan: how the 4-bit attention of few heads divides T lists of K
+ *   slots among `sms` CTAs (parts != 0: lists may be cut), on the host, launch by
+ *   launch: adds to seen[T][blocks of a list] (host bytes; a block is 64 slots, a list
+ *   has at least one) how often a CTA has the block, and returns the most pieces of
+ *   lists that a CTA has in a launch (at most 1024), or a negative error. */
 int dsa_test_indexer_logits_general(const void* q_fp8, const void* k_fp8, const float* k_scale, const void* w,
                                     int w_dtype, const int32_t* ks, const int32_t* ke, float* logits,
                                     int64_t ld_logits, int T, int S, int H, int D, int clean, int32_t* status,
@@ -324,6 +329,7 @@ int dsa_test_indexer_logits_general(const void* q_fp8, const void* k_fp8, const 
 int dsa_test_topk_select_two_pass(const float* logits, int64_t ld_logits, const int32_t* ks, const int32_t* ke, int T,
                                   int S, int k, int32_t* out_idx, void* stream);
 int dsa_test_bounded_wait(int poll_limit, int32_t* status, void* stream);
+int dsa_test_few_heads_plan(int T, int K, int sms, int parts, uint8_t* seen);
 
 #ifdef __cplusplus
 }

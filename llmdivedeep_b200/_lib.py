@@ -69,6 +69,7 @@ SIGNATURES = {
     "dsa_test_topk_select_two_pass": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
                                               c_void_p]),
     "dsa_test_bounded_wait": (c_int, [c_int, c_void_p, c_void_p]),
+    "dsa_test_few_heads_plan": (c_int, [c_int, c_int, c_int, c_int, c_void_p]),
     "dsa_indexer_topk_static_max_bytes": (c_size_t, []),
     "dsa_indexer_topk_static": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                                         c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),

@@ -58,6 +58,7 @@ int sparse_mla_decode_launch(const void* q, const void* cache, int record_bytes,
                              cudaStream_t stream);
 size_t mla_decode_workspace_bytes(int B, int H, int K);
 size_t mla_decode_records_workspace_bytes(int record_bytes, int T, int H, int K);
+int few4_plan_probe(int T, int K, int sms, int parts, uint8_t* seen);
 int block_sparse_mha_launch(const void* q, const void* k, const void* v, const int32_t* lut, const int32_t* num,
                             void* out, int B, int S, int H, int topk, float scale, int32_t* status,
                             cudaStream_t stream);
@@ -148,6 +149,13 @@ int dsa_test_indexer_logits_general(const void* q_fp8, const void* k_fp8, const 
 int dsa_test_topk_select_two_pass(const float* logits, int64_t ld_logits, const int32_t* ks, const int32_t* ke, int T,
                                   int S, int k, int32_t* out_idx, void* stream) {
   return topk_select_checked(logits, ld_logits, ks, ke, T, S, k, out_idx, /*sample=*/0, /*overlapped=*/0, stream);
+}
+
+int dsa_test_few_heads_plan(int T, int K, int sms, int parts, uint8_t* seen) {
+  g_err[0] = 0;
+  if (T < 0 || K < 0 || K > 2048 || sms < 1) return set_error(DSA_ERR_SHAPE, "test_few_heads_plan: bad sizes");
+  if (T > 0 && !seen) return set_error(DSA_ERR_ARG, "test_few_heads_plan: NULL pointer argument");
+  return few4_plan_probe(T, K, sms, parts, seen);
 }
 
 int dsa_test_bounded_wait(int poll_limit, int32_t* status, void* stream) {

@@ -36,11 +36,12 @@ namespace dsa {
 
 struct Few4Args {
   const uint8_t* cache;           // [num_rows, 416]
-  const int32_t* block_table;     // [T / tokens_per_seq, table_stride]
+  const int32_t* block_table;     // [sequences, table_stride]: list t is of sequence (row0 + t) / tokens_per_seq
   const int32_t* idx;             // [T, K] positions (negative = empty)
   __nv_bfloat16* out;             // [T, H, 512]
   int64_t table_stride;
   int T, H, K, max_ctx, tokens_per_seq;
+  int row0;                       // the call's row that this launch begins with
   int num_rows;
   int list_blocks;                // blocks of 64 slots of a list
   int ctas;
@@ -61,7 +62,7 @@ constexpr int kF4Panel = kF4Blk * 128;                 // 64 keys x 64 dims, 128
 constexpr int kF4Half = 4 * kF4Panel;                  // 256 dims of a block
 constexpr int kF4Dv = 512, kF4QBytes = 1152;
 constexpr int kF4Valid = 8;                            // ring of validity bytes, by block
-constexpr int kF4Pieces = 1024;                        // pieces of a CTA at most (the launcher cuts longer calls)
+constexpr int kF4Pieces = 1024;                        // pieces of a CTA at most: the launcher cuts longer calls, inside a sequence too
 constexpr uint8_t kF4Unknown = 255;                    // a piece's length before the list's end is known
 constexpr int kF4Look = 8;                             // 16-byte pieces of a list that a lane looks at together
 constexpr uint32_t kF4RopeGain = 0x38803880u;          // 2^-14 as a pair of bf16
@@ -115,23 +116,23 @@ __device__ __forceinline__ uint32_t f4_test(uint64_t* bar, uint32_t parity) {
 }
 // What a CTA has to do, list by list: the whole lists of its rounds, then its stretch.
 struct F4Piece {
+  int cta;
   int done, all, start;                                // its blocks behind it, and all of them; first block of the stretch
   int t, b0, b1;                                       // the list and its blocks [b0, b1) in this piece
-  static __device__ __forceinline__ int start_of(const Few4Args& a, int c) {
+  static __host__ __device__ __forceinline__ int start_of(const Few4Args& a, int c) {
     if (a.per_list) return c / a.per_list * a.list_blocks + c % a.per_list * a.list_blocks / a.per_list;
     return a.rest ? (int)((int64_t)c * a.rest / a.rest_ctas) : 0;
   }
-  __device__ __forceinline__ F4Piece(const Few4Args& a) {
-    const int c = blockIdx.x;
+  __host__ __device__ __forceinline__ F4Piece(const Few4Args& a, int c) : cta(c) {
     start = start_of(a, c);
     done = t = b0 = b1 = 0;
     all = min(a.rounds, (a.T - c + a.ctas - 1) / a.ctas) * a.list_blocks + (c < a.rest_ctas ? start_of(a, c + 1) - start : 0);
   }
-  __device__ __forceinline__ bool next(const Few4Args& a) {
+  __host__ __device__ __forceinline__ bool next(const Few4Args& a) {
     if (done >= all) return false;
     const int x = done - a.rounds * a.list_blocks;
     if (x < 0) {
-      t = done / a.list_blocks * a.ctas + blockIdx.x;
+      t = done / a.list_blocks * a.ctas + cta;
       b0 = 0;
       b1 = a.list_blocks;
     } else {
@@ -144,7 +145,7 @@ struct F4Piece {
     return true;
   }
   // The part that this piece leaves if it is not a whole list: of the stretch's first list, or of its last.
-  __device__ __forceinline__ int part(const Few4Args& a) const { return 2 * blockIdx.x + (done - (b1 - b0) == a.rounds * a.list_blocks ? 0 : 1); }
+  __device__ __forceinline__ int part(const Few4Args& a) const { return 2 * cta + (done - (b1 - b0) == a.rounds * a.list_blocks ? 0 : 1); }
 };
 
 // What one of `of` threads sees of the slots [lo, hi) of a list: the last used one, and the largest position.
@@ -227,7 +228,7 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
   // The first piece's end is found by all threads together, so that it is known when the roles begin.
   int blocks0;
   {
-    F4Piece p0(a);
+    F4Piece p0(a, blockIdx.x);
     const bool there = p0.next(a);
     const int lo = p0.b0 * kF4Blk, hi = there ? min(a.K, p0.b1 * kF4Blk) : lo;
     const F4Scan scan(a, idx + (int64_t)p0.t * a.K, lo, hi, threadIdx.x, kF4Threads);
@@ -256,13 +257,13 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
     ok = false;
     return 0;
   };
-  F4Piece pc(a);
+  F4Piece pc(a, blockIdx.x);
   constexpr uint64_t kHalf = kF4Half >> 4, kOne = kF4Panel >> 4, kQPanel = (N * 128) >> 4;      // descriptor steps
 
   if (warp == kF4StageWarp) {
     // ------------- the last used slot of every piece (it decides the number of blocks), and Q -------------
     // Whichever can go on; Q, which the tensor core waits for, first.
-    F4Piece qc(a);
+    F4Piece qc(a, blockIdx.x);
     uint32_t nu = 1, nq = 0, idle = 0;
     bool lists = pc.next(a), queries = true;           // (the first list's end is known)
     while (lists || queries) {
@@ -396,7 +397,7 @@ sparse_mla_few4_kernel(const __grid_constant__ CUtensorMap tmap_q, const Few4Arg
       return h;
     };
     auto table_entry = [&](const Group& h) -> int {
-      return h.pos >= 0 && h.pos < a.max_ctx ? __ldg(a.block_table + (int64_t)(h.list / a.tokens_per_seq) * a.table_stride + h.pos / 64) : -1;
+      return h.pos >= 0 && h.pos < a.max_ctx ? __ldg(a.block_table + (int64_t)((a.row0 + h.list) / a.tokens_per_seq) * a.table_stride + h.pos / 64) : -1;
     };
     auto cache_row = [&](const Group& h, int page) -> int {        // -1 = empty; bad positions are flagged by the warp that reads the list
       if (h.pos < 0 || h.pos >= a.max_ctx) return -1;
@@ -751,11 +752,54 @@ constexpr int kF4LeastBlocks = 2;                      // of a CTA, in calls tha
 constexpr int kF4PieceBlocks = 2;                      // what a further piece costs a CTA, in blocks
 
 static int f4_list_blocks(int K) { return max(1, (K + kF4Blk - 1) / kF4Blk); }
-static int f4_ctas(int T, int list_blocks) {
-  return (int)min((int64_t)sm_count(), max((int64_t)T, (int64_t)T * list_blocks / kF4LeastBlocks));
+static int f4_ctas(int T, int list_blocks, int sms) {
+  return (int)min((int64_t)sms, max((int64_t)T, (int64_t)T * list_blocks / kF4LeastBlocks));
 }
 static size_t f4_parts_bytes(int ctas, int H) { return (size_t)2 * ctas * H * (kF4Dv + 1) * sizeof(float); }
-size_t few4_workspace_bytes(int T, int H, int K) { return f4_parts_bytes(f4_ctas(T, f4_list_blocks(K)), H); }
+size_t few4_workspace_bytes(int T, int H, int K) { return f4_parts_bytes(f4_ctas(T, f4_list_blocks(K), sm_count()), H); }
+
+// The lists from row t0 of the call's T that one launch takes, and which CTA has what of them; without parts, every list in one piece.  A CTA's
+// pieces fit its table: it has a list of each round, and its stretch lies in three others at most.
+static void f4_plan(Few4Args& a, int t0, int T, int sms, bool parts) {
+  a.row0 = t0;
+  a.T = min(T - t0, kF4Pieces / 2 * sms);
+  a.list_blocks = f4_list_blocks(a.K);
+  a.ctas = parts ? f4_ctas(a.T, a.list_blocks, sms) : min(a.T, sms);
+  a.rounds = parts ? a.T / a.ctas : (a.T + a.ctas - 1) / a.ctas;
+  a.rest = max(0, a.T - a.rounds * a.ctas) * a.list_blocks;
+  a.rest_ctas = min(a.ctas, max(1, a.rest / kF4LeastBlocks));
+  // Equal parts of each list while they keep the GPU as busy: a CTA whose stretch lies in two lists pays for the second's Q, output and
+  // start what two blocks take.  2048 keys, us with stretches of all blocks and so: 16 heads 24 rows 21.4, 19.1; 64 rows 34.6, 32.5; 32 heads
+  // 64 rows 44.9, 42.3.
+  a.per_list = 0;
+  if (a.rest) {
+    const int lists = a.rest / a.list_blocks, p = min(a.ctas / lists, max(1, a.list_blocks / kF4LeastBlocks));
+    if ((a.list_blocks + p - 1) / p <= (a.rest + a.rest_ctas - 1) / a.rest_ctas + kF4PieceBlocks) {
+      a.per_list = p;
+      a.rest_ctas = lists * p;
+    }
+  }
+}
+
+// Walks the plans of a call of T rows on the host: for every block of every list how often a CTA has it (`seen`, [T, blocks of a list]), and the most pieces
+// that a CTA has in a launch, or -1 where a piece lies outside its lists.
+int few4_plan_probe(int T, int K, int sms, int parts, uint8_t* seen) {
+  Few4Args a{};
+  a.K = K;
+  int most = 0;
+  for (int t0 = 0; t0 < T; t0 += a.T) {
+    f4_plan(a, t0, T, sms, parts != 0);
+    for (int c = 0; c < a.ctas; ++c) {
+      int n = 0;
+      for (F4Piece pc(a, c); pc.next(a); ++n) {
+        if (pc.t < 0 || pc.t >= a.T || pc.b0 < 0 || pc.b1 <= pc.b0 || pc.b1 > a.list_blocks) return -1;
+        for (int b = pc.b0; b < pc.b1; ++b) ++seen[(int64_t)(t0 + pc.t) * a.list_blocks + b];
+      }
+      most = max(most, n);
+    }
+  }
+  return most;
+}
 
 template <int N>
 static int launch_few4(const void* q, const Few4Args& a, int overlapped, cudaStream_t stream) {
@@ -777,42 +821,23 @@ int sparse_mla_few4_launch(const void* q, const void* cache, const int32_t* bloc
                            int32_t* status, int overlapped, cudaStream_t stream) {
   Few4Args a{};
   a.cache = static_cast<const uint8_t*>(cache);
+  a.block_table = block_table;
   a.table_stride = table_stride;
   a.tokens_per_seq = tokens_per_seq;
   a.H = H; a.K = K; a.max_ctx = max_ctx;
   a.num_rows = num_pages * 64;
-  a.list_blocks = f4_list_blocks(K);
   a.scale_log2e = scale * 1.4426950408889634f * kLatent4Gain;
   a.status = status;
-  // a CTA's pieces fit its table: whole sequences, so that a call's rows keep their table rows
-  const int most = max(1, kF4Pieces * sm_count() / 2 / tokens_per_seq) * tokens_per_seq;
-  for (int t0 = 0; t0 < T; t0 += most) {
-    a.T = min(most, T - t0);
-    a.block_table = block_table + (int64_t)(t0 / tokens_per_seq) * table_stride;
-    a.idx = idx + (int64_t)t0 * K;
-    a.out = static_cast<__nv_bfloat16*>(out) + (int64_t)t0 * H * kF4Dv;
-    a.ctas = f4_ctas(a.T, a.list_blocks);
+  for (int t0 = 0; t0 < T; t0 += a.T) {
+    f4_plan(a, t0, T, sm_count(), /*parts=*/true);
     if (workspace && workspace_bytes >= f4_parts_bytes(a.ctas, H)) {
       a.part_o = static_cast<float*>(workspace);
       a.part_lse = a.part_o + (size_t)2 * a.ctas * H * kF4Dv;
-      a.rounds = a.T / a.ctas;
-    } else {                                           // no room for parts: every list in one piece
-      a.ctas = min(a.T, sm_count());
-      a.rounds = (a.T + a.ctas - 1) / a.ctas;
+    } else {
+      f4_plan(a, t0, T, sm_count(), /*parts=*/false);
     }
-    a.rest = max(0, a.T - a.rounds * a.ctas) * a.list_blocks;
-    a.rest_ctas = min(a.ctas, max(1, a.rest / kF4LeastBlocks));
-    // Equal parts of each list while they keep the GPU as busy: a CTA whose stretch lies in two lists pays for the second's Q, output and
-    // start what two blocks take.  2048 keys, us with stretches of all blocks and so: 16 heads 24 rows 21.4, 19.1; 64 rows 34.6, 32.5; 32 heads
-    // 64 rows 44.9, 42.3.
-    a.per_list = 0;
-    if (a.rest) {
-      const int lists = a.rest / a.list_blocks, p = min(a.ctas / lists, max(1, a.list_blocks / kF4LeastBlocks));
-      if ((a.list_blocks + p - 1) / p <= (a.rest + a.rest_ctas - 1) / a.rest_ctas + kF4PieceBlocks) {
-        a.per_list = p;
-        a.rest_ctas = lists * p;
-      }
-    }
+    a.idx = idx + (int64_t)t0 * K;
+    a.out = static_cast<__nv_bfloat16*>(out) + (int64_t)t0 * H * kF4Dv;
     const void* qt = static_cast<const uint8_t*>(q) + (size_t)t0 * H * kF4QBytes;
     const int rc = H <= 16 ? launch_few4<16>(qt, a, overlapped, stream) : launch_few4<32>(qt, a, overlapped, stream);
     if (rc) return rc;
