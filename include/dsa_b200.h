@@ -259,7 +259,7 @@ size_t dsa_pages_workspace_bytes(int num_pages, int n);
 int dsa_copy_pages(const dsa_page_cache* caches, int n_caches, int num_pages, const int32_t* src, const int32_t* dst,
                    const int32_t* tokens, int n, int32_t* status, void* stream);
 /* Room for n_new[i] more tokens (0..max_new) in row rows[i], rows all different: pages are taken, ctx_len grows, and
- * slots [n, max_new] gets the cache rows of the new tokens, -1 behind them (refused: -1 everywhere). */
+ * slots [n, max_new] gets the cache rows of the new tokens, -1 behind them (refused: -1 everywhere).  B * P < 2^31. */
 int dsa_extend_pages(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages,
                      const int32_t* rows, const int32_t* n_new, int n, int max_new, int32_t* slots, void* workspace,
                      size_t workspace_bytes, int32_t* status, void* stream);

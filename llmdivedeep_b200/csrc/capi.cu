@@ -421,6 +421,8 @@ int dsa_extend_pages(int32_t* block_table, int64_t table_stride, int P, int B, i
   g_err[0] = 0;
   int rc = check_pool("extend_pages", block_table, table_stride, P, B, refs, num_pages, n);
   if (rc || n == 0) return rc;
+  if ((int64_t)B * P > 0x7fffffffLL)                   // the pages that a call asks for are summed in 32 bits
+    return set_error(DSA_ERR_SHAPE, "extend_pages: more than 2147483647 table entries (%d rows of %d)", B, P);
   if (max_new < 0 || max_new > (1 << 30)) return set_error(DSA_ERR_SHAPE, "extend_pages: bad max_new (%d)", max_new);
   if (!ctx_len || !rows || !n_new || (max_new > 0 && !slots)) return set_error(DSA_ERR_ARG, "extend_pages: NULL pointer argument");
   if ((rc = check_pages_workspace("extend_pages", workspace, workspace_bytes, num_pages, n))) return rc;
