@@ -381,6 +381,11 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
       last = *last_s;
     }
     nblk = (last + kMlaBlk) / kMlaBlk;
+    // Positions out of range: skipped by the gather, and said here of the whole list, the slots behind the last usable one too.
+    bool bad = tail >= a.S_kv;
+#pragma unroll
+    for (int u = 0; u < kMlaLooks; ++u) bad |= look[u] >= a.S_kv;
+    if (bad && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
   }
   if (nblk == 0) {   // nothing selected: the output row is zero (a part: weight zero in the combine); no cluster traffic yet
     if (threadIdx.x < 128 && threadIdx.x < heads_here) {
@@ -394,9 +399,6 @@ sparse_mla_kernel(const __grid_constant__ CUtensorMap tmap_q,
         a.part_lse[((int64_t)part * 2 + cta) * a.H + h0 + threadIdx.x] = -CUDART_INF_F;
       }
     }
-    // an index that is out of range is still reported
-    for (int j = threadIdx.x; j < k_cnt; j += kMlaThreads)
-      if (idx_row[j] >= a.S_kv && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
     if (threadIdx.x == 0) mbar_wait(q_full, 0, abort_flag, a.status);     // the Q copy must have landed before the CTA goes
     if (warp == kMlaMmaWarp) tmem_dealloc(*tmem_slot, kMlaTmemCols);
     return;
