@@ -240,7 +240,9 @@ int dsa_decode_step_records(const void* q_fp8, const void* w, int w_dtype, const
  *   ctx_len [B] int32            its tokens (64 to a page); 0 = an empty row
  * Pages are taken lowest free id first, in the order of the call's list: the ids
  * depend on the state alone.  A call that takes pages is all or nothing: with a bad
- * argument (status 2) or too few free pages (status 3) it changes nothing.
+ * argument, a partly filled last page that it copies or fills and that is no page of the
+ * pool (status 2), or too few free pages (status 3) it changes nothing.  Entries of full
+ * pages are believed: a fork copies one that is no page as it stands and sets status 2.
  * B <= 262144.  `workspace` (4-byte aligned): dsa_pages_workspace_bytes(num_pages, n). */
 
 /* A cache whose pages are copied (host struct): `layers` times [num_pages*64, token_bytes] bytes, layer_stride bytes

@@ -2,8 +2,9 @@
 //
 // State, all of it the caller's: refs[num_pages], how many sequences hold a page (0 = free); table[B, stride], the pages of a sequence in
 // order, -1 behind the last one; ctx_len[B], its tokens.  A page holds 64 tokens.  Pages are taken lowest free id first, in the order
-// of the call's list, so that ids depend on nothing but the state.  The calls that take pages are all or nothing: a bad argument (status
-// 2) or too few free pages (status 3) leaves everything as it was.
+// of the call's list, so that ids depend on nothing but the state.  The calls that take pages are all or nothing: a bad argument, a partly filled
+// last page that they copy or fill and that is no page (status 2), or too few free pages (status 3) leaves everything as it was.  Of full
+// pages the table is believed: a fork copies an entry that is no page as it stands, and says so (status 2).
 //
 // Who gets which page is decided by one cluster of CTAs that scan refs (each a stretch of it, counts exchanged through distributed
 // shared memory).  What is long goes to a second kernel over the whole GPU, which starts under the first one's end: the contents, the rows
@@ -163,6 +164,9 @@ struct PoolArgs {
   int* status;
 };
 
+// Whether entry p of a row names a page of the pool.
+__device__ __forceinline__ bool names_page(const PoolArgs& a, int row, int p) { return (unsigned)a.table[(int64_t)row * a.stride + p] < (unsigned)a.num_pages; }
+
 // ---- room for new tokens ---------------------------------------------------------------------------------------------
 // Pages that an entry's new tokens lie in, at most
 __host__ __device__ __forceinline__ int64_t extend_per(int max_new) { return ((int64_t)max_new + 2 * kPageTokens - 2) / kPageTokens; }
@@ -208,8 +212,12 @@ __global__ void __launch_bounds__(kPoolThreads) extend_kernel(const PoolArgs a) 
     if (i < a.n) {
       const int row = a.a[i], nn = a.b[i];
       if (name_row(seen, row, a.B)) c = a.ctx[row];
-      if (c < 0 || nn < 0 || nn > a.max_new || (int64_t)c + nn > (int64_t)a.P * kPageTokens) bad = true;
-      else need = pages_of(c + nn) - pages_of(c);
+      if (c < 0 || nn < 0 || nn > a.max_new || (int64_t)c + nn > (int64_t)a.P * kPageTokens) {
+        bad = true;
+      } else {
+        need = pages_of(c + nn) - pages_of(c);
+        if (nn > 0 && c % kPageTokens && !names_page(a, row, c / kPageTokens)) bad = true;      // the first new token goes there
+      }
     }
     int total;
     const int at = block_prefix(s, turn, need, total);
@@ -271,7 +279,7 @@ __global__ void __launch_bounds__(kPoolThreads) fork_kernel(const PoolArgs a) {
         bad = true;
       } else {
         const int c = a.ctx[parent];
-        if (c < 0 || (int64_t)c > (int64_t)a.P * kPageTokens) bad = true;
+        if (c < 0 || (int64_t)c > (int64_t)a.P * kPageTokens || (c % kPageTokens && !names_page(a, parent, c / kPageTokens))) bad = true;
         else need = c % kPageTokens;
       }
     }

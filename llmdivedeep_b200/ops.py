@@ -759,7 +759,8 @@ def copy_pages(caches, src, dst, tokens=None, num_pages: Optional[int] = None) -
 def extend_pages(block_table, ctx_len, refs, rows, n_new, max_new: int) -> torch.Tensor:
     """Room for n_new[i] (int32, 0..max_new) more tokens in row rows[i] (int32, all different): takes the lowest free pages, in order,
     and writes block_table, ctx_len and refs.  Returns the new tokens' cache rows, int32 [n, max_new], -1 behind them.  All or
-    nothing: with too few free pages (status 3) or a bad argument (status 2) nothing changes and every slot is -1."""
+    nothing: with too few free pages (status 3), a bad argument or a last page to be filled that is none (status 2) nothing changes and every
+    slot is -1."""
     i = _index_of(block_table, ctx_len, refs, rows, n_new)
     B, P, num_pages = _check_pool(block_table, ctx_len, refs)
     n = _list_i32(rows, "rows")
