@@ -699,14 +699,18 @@ def unpack_latent4(cache: torch.Tensor, n: Optional[int] = None, block_table: Op
 
 # ---- pages of the paged caches ------------------------------------------------------------------------------------------
 def _page_caches(caches, num_pages: int):
-    """The caches as an array of dsa_page_cache.  A cache is [num_pages*64, ...] or, for several layers, [layers, num_pages*64, ...]."""
+    """The caches as an array of dsa_page_cache.  A cache is [num_pages*64, ...] or, for several layers, [layers, num_pages*64, ...].  Where
+    both fit, FP8 keys [num_pages*64, width] are one layer's (a token of one byte is no cache); others are refused: t[None] says
+    that t is one layer."""
     rows, packed = num_pages * 64, b""
     for t in caches:
         shape = t.shape
         dims = len(shape)
         one, many = dims >= 1 and shape[0] == rows, dims >= 2 and shape[1] == rows
+        if one and many and dims == 2 and t.dtype is FP8:
+            many = False
         if one == many:
-            raise DsaError(f"a cache must be [{rows}, ...] or [layers, {rows}, ...], got {tuple(shape)}")
+            raise DsaError(f"a cache must be [{rows}, ...] or [layers, {rows}, ...], got {tuple(shape)}" + (": both fit; t[None] is one layer" if one else ""))
         whole = t.is_contiguous()
         if not whole and not (many and t[0].is_contiguous()):
             raise DsaError("the pages of a cache must be contiguous")
