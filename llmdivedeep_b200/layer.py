@@ -399,7 +399,8 @@ def _pack_by_parts(kv: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tenso
 
 
 class DecodeWorkspace:
-    """Buffers of one decode step, allocated once and reused every step."""
+    """Buffers of one decode step, allocated once and reused every step.  Over 4-bit records the parts of the lists may need more room than
+    over FP8 ones: that is made by the first such step (before a graph is captured, if it is not to be the graph's)."""
 
     def __init__(self, batch: int, heads: int, max_ctx: int, topk: int, device):
         ld = (max_ctx + 3) // 4 * 4
@@ -407,9 +408,18 @@ class DecodeWorkspace:
         self.k = min(topk, max_ctx)                    # selected keys per sequence (the kernels write rows at this stride)
         self.idx = torch.empty(batch, self.k, dtype=torch.int32, device=device)
         self.out = torch.empty(batch, heads, 512, dtype=torch.bfloat16, device=device)
-        need = max(_lib.load().dsa_sparse_mla_decode_records_workspace_bytes(width, batch, heads, min(topk, max_ctx)) for width in ops.RECORD_BYTES)
-        self.mla_ws = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+        need, self._need4 = (max(_lib.load().dsa_sparse_mla_decode_records_workspace_bytes(width, batch, heads, self.k), 16) for width in ops.RECORD_BYTES)
+        self.mla_ws = torch.empty(need, dtype=torch.uint8, device=device)
+        self._ws4 = self.mla_ws if self._need4 <= need else None
         self.max_ctx, self.topk = max_ctx, topk
+
+    def parts(self, record_bytes: int) -> torch.Tensor:
+        """The room for parts of lists over records of this width."""
+        if record_bytes != LATENT4_TOKEN_BYTES:
+            return self.mla_ws
+        if self._ws4 is None:
+            self._ws4 = torch.empty(self._need4, dtype=torch.uint8, device=self.mla_ws.device)
+        return self._ws4
 
 
 @torch.no_grad()
@@ -418,13 +428,12 @@ def dsa_decode_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, laten
     """One decode step for a batch of sequences: paged indexer scan, top-k over each sequence's
     context, sparse MLA over the paged latent cache (FP8 or 4-bit records).  Returns (idx, out) views of ``ws``."""
     B = q.shape[0]
-    idx, out = ws.idx[:B], ws.out[:B]
-    if ops.decode_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, latent_cache, softmax_scale, ws.max_ctx, ws.logits, idx, out,
-                       ws.mla_ws):
+    idx, out, parts = ws.idx[:B], ws.out[:B], ws.parts(latent_cache.shape[-1])
+    if ops.decode_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, latent_cache, softmax_scale, ws.max_ctx, ws.logits, idx, out, parts):
         return idx, out
     logits = ops.fp8_paged_mqa_logits(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, ws.max_ctx, out=ws.logits)
     ops.topk_select(logits, ws.k, None, ctx_len, out=idx)
-    ops.sparse_mla_decode_paged(q, latent_cache, block_table, idx, softmax_scale, ws.max_ctx, out=out, workspace=ws.mla_ws)
+    ops.sparse_mla_decode_paged(q, latent_cache, block_table, idx, softmax_scale, ws.max_ctx, out=out, workspace=parts)
     return idx, out
 
 

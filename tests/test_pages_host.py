@@ -1,10 +1,10 @@
-"""What the page calls refuse before any launch."""
+"""What the page calls refuse before any launch, and the room that a decode step asks for."""
 import struct
 
 import pytest
 import torch
 
-from llmdivedeep_b200 import _lib, build, ops
+from llmdivedeep_b200 import _lib, build, layer, ops
 
 
 @pytest.fixture(scope="module")
@@ -35,3 +35,15 @@ def test_caches_that_can_be_read_in_two_ways():
     assert entry(wide[None]) == (1, 512)
     with pytest.raises(ops.DsaError, match="must be"):
         ops._page_caches([torch.zeros(64, 4)], 2)
+
+
+@pytest.mark.parametrize("heads", [8, 16, 64, 128])
+def test_a_decode_workspace_over_fp8_records_is_no_larger_for_the_4_bit_ones(lib, heads):
+    """Its parts are what FP8 records need; the first step over 4-bit records makes room for theirs, once."""
+    ws = layer.DecodeWorkspace(64, heads, 4096, 2048, "cpu")
+    need = [lib.dsa_sparse_mla_decode_records_workspace_bytes(w, 64, heads, 2048) for w in (656, 416)]
+    assert need[0] == lib.dsa_sparse_mla_decode_workspace_bytes(64, heads, 2048)
+    assert ws.mla_ws.numel() == need[0]
+    assert ws.parts(656) is ws.mla_ws
+    four = ws.parts(416)
+    assert four.numel() >= need[1] and ws.parts(416) is four
