@@ -242,6 +242,12 @@ def _workspace(device, nbytes: int) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+def _check_scratch(workspace: torch.Tensor) -> None:
+    """The kernels write the workspace's numel() bytes from its first one on: of an expanded tensor, or one with gaps, those are not its own."""
+    if not workspace.is_contiguous():
+        raise DsaError(f"workspace must be contiguous, got {tuple(workspace.shape)} strides {tuple(workspace.stride())}")
+
+
 def indexer_topk(q_fp8, k_fp8, k_scale, weights, ks, ke, k: int, workspace: Optional[torch.Tensor] = None,
                  max_workspace_bytes: int = 8 << 30, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Indexer logits + top-k (IndexerSimulator.logits_step, sparse_attn/DSA.py:336-362)
@@ -260,6 +266,8 @@ def indexer_topk(q_fp8, k_fp8, k_scale, weights, ks, ke, k: int, workspace: Opti
         full = lib.dsa_indexer_topk_workspace_bytes(T, S)
         row = full // max(T, 1)
         workspace = _workspace(q_fp8.device, min(full, max(max_workspace_bytes, 256 * row)))
+    else:
+        _check_scratch(workspace)
     with _on(dev):
         check(lib.dsa_indexer_topk(_ptr(q_fp8), _ptr(k_fp8), _ptr(k_scale), _ptr(weights), _w_dtype(weights),
                                    _ptr(ks), _ptr(ke), T, S, H, D, k, _ptr(out), _ptr(workspace), workspace.numel(),
@@ -364,6 +372,7 @@ def sparse_mla_decode_paged(q, cache, block_table, idx, scale: float, max_ctx: O
         workspace = cache.new_empty(lib.dsa_sparse_mla_decode_records_workspace_bytes(width, T, H, K))      # as _workspace
     else:
         _need_cuda(q, workspace)
+        _check_scratch(workspace)
     _run(i, lib.dsa_sparse_mla_decode_records, q.data_ptr(), cache.data_ptr(), width, block_table.data_ptr(), P, tokens_per_seq, idx.data_ptr(),
          out.data_ptr(), T, H, K, rows // 64, P * 64 if max_ctx is None else max_ctx, float(scale), workspace.data_ptr(), workspace.numel())
     return out
@@ -384,6 +393,8 @@ def _sparse_mla_decode_fp8(q, cache, block_table, idx, scale, max_ctx, out, work
     if workspace is None:
         need = lib.dsa_sparse_mla_decode_workspace_bytes(B, H, idx.shape[1])
         workspace = _workspace(q.device, need) if need else None
+    else:
+        _check_scratch(workspace)
     with _on(dev):
         check(lib.dsa_sparse_mla_decode_paged(_ptr(q), _ptr(cache), _ptr(block_table), block_table.stride(0), _ptr(idx),
                                               _ptr(out), B, H, idx.shape[1], cache.shape[0] // 64, max_ctx, float(scale),
