@@ -217,7 +217,10 @@ int dsa_unpack_latent4(const void* cache, int64_t cache_rows, const int32_t* blo
 
 /* dsa_sparse_mla_decode_paged over records of record_bytes = 656 (FP8) or 416 (4 bits), for tokens_per_seq query rows of
  * each sequence: rows r = b*tokens_per_seq .. of q [T, H, 576], idx [T, K] and out [T, H, 512] go by row b of block_table.
- * (4 bits: |q| of the latent part must stay below 2^113.)  Lists may be cut into parts that different SMs take and a second
+ * T and tokens_per_seq may be as large as the tensors.  The kernels that work in pairs of SMs -- FP8 records, more than 32
+ * heads, or calls of few rows -- exchange the two halves of a score q.k (256 latent and 32 rope values each) in fp16: a half
+ * beyond 65504, before the softmax scale, saturates, and the two halves of an output row disagree.  (4-bit values reach 368640.
+ * |q| of the latent part must stay below 2^113 there.)  Lists may be cut into parts that different SMs take and a second
  * kernel merges in fp32; the parts' `workspace` (16-byte aligned) of dsa_sparse_mla_decode_records_workspace_bytes bytes is
  * enough for every call of up to T rows.  With a smaller one, or NULL, the call works with fewer parts or none. */
 size_t dsa_sparse_mla_decode_records_workspace_bytes(int record_bytes, int T, int H, int K);

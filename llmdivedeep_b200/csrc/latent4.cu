@@ -77,7 +77,8 @@ struct KeyRows {
 };
 
 // Latent rows -> records at the cache rows `slots` (null: row i -> record i).  A warp per token: 1152 bytes in (bf16), 416 out.  8192 tokens: 7.8 us
-// from memory (5.0 out of L2), of which the bytes are 2; a launch and one wave of loads, arithmetic and stores one after the other.  (8.6 with a lane to every group of 16,
+// from memory (5.0 out of L2), of which the bytes are 2: a launch, and one wave of warps that, as written, go to memory three times one after the other, for the slot, for
+// the token's latents once the slot has been tested, and for its rope values and key behind the codes' stores.  (8.6 with a lane to every group of 16,
 // whose loads and stores are pieces of lines, and an IEEE division for every value.)
 template <typename T>
 __global__ void __launch_bounds__(256) pack_latent4_kernel(const T* __restrict__ kv, int64_t row_stride, int64_t n, uint8_t* __restrict__ cache,

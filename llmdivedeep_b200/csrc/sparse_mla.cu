@@ -1089,8 +1089,8 @@ int sparse_mla_few4_launch(const void* q, const void* cache, const int32_t* bloc
 size_t few4_workspace_bytes(int T, int H, int K);
 
 // 4-bit records, at most 32 heads: pairs while a list can have this many parts, then sparse_mla_few4.cu.  2048 slots, pairs / that one:
-// 16 heads, 1 row 11.6 / 14.3 us, 8 rows 14.9 / 15.9, 12 rows 16.5 / 17.5; 32 heads, 1 row 12.4 / 15.7, 12 rows 16.7 / 19.0, 18 rows
-// 19.5 / 19.3, 37 rows 28.0 / 25.7, 148 rows twice that one's time and more.
+// 16 heads, 1 row 11.5 / 14.5 us, 8 rows 14.2 to 14.9 / 16.0, 12 rows 16.5 / 17.6, 18 rows 18.6 / 17.4; 32 heads, 1 row 12.5 / 16.0, 8 rows 15.7 / 18.0,
+// 12 rows 17.4 / 19.1, 18 rows 19.5 / 19.5, 37 rows 27.6 / 25.8, 148 rows twice that one's time and more.
 constexpr int kMlaFewParts = 6;
 static bool mla_few4(int record_bytes, int T, int H) { return record_bytes == kLatent4Bytes && H <= kMlaFewHeads && sm_count() / 2 < T * kMlaFewParts; }
 

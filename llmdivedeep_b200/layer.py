@@ -439,7 +439,8 @@ def dsa_decode_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, laten
 
 class PagedCache:
     """The decode caches of ``layers`` DSA layers, latents in 4 bits, in one pool of 64-token pages, and the tables that say
-    which sequence has which page: 416 + 132 bytes a token and layer.
+    which sequence has which page: 416 + 132 bytes a token and layer.  What 4 bits cost: latents drawn from N(0,1) read back 9.5 % off (root
+    mean square; FP8 records of 656 bytes, pack_latent_cache: 2.6 %).
 
         cache = PagedCache(layers, num_pages, batch, max_ctx, "cuda")
         slots = cache.extend([row], [n], n)                    # room for n tokens in a row of the batch
@@ -448,7 +449,7 @@ class PagedCache:
         cache.fork([row], [other])                             # a beam, a shared prompt: full pages are not copied
         cache.free([row])
         cache.compact()                                        # pages in use to the lowest ids, contents and tables
-        kv = cache.read(layer, row, n)                         # bf16 rows for a chunked prefill (ops.sparse_mla_prefill)
+        kv = cache.read(layer, row, n)                         # latents as bf16 rows for a chunked prefill (ops.sparse_mla_prefill)
 
     Rows are given as int32 tensors on the GPU or as lists, which are copied there.  Nothing else waits; what the kernels find wrong
     (a pool without free pages, a bad row) leaves the tables as they are and is in ops.check_status.  The tables are tensors of
