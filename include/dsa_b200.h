@@ -284,6 +284,77 @@ int dsa_compact_pages(const int32_t* block_table, int64_t table_stride, int32_t*
                       const int32_t* refs, int32_t* new_refs, int num_pages, const dsa_page_cache* caches, int n_caches,
                       void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
+/* ---- window layers and drafted tokens ----------------------------------------------
+ * No counterpart in the reference, whose attention is block-sparse or over a selection
+ * and which has no cache (sparse_attn/DSA.py:208-249, 475-477).
+ *
+ * Attention over a sliding window and the first tokens: a query row at position p of its
+ * sequence sees the positions s with s < first or p - window < s <= p:
+ *   out[r,h,:] = sum_s softmax_s(scale * q[r,h,:576] . kv[s,:576]) * kv[s,:512];
+ * a row that sees nothing gives zeros, and what a row does not see -- infinities and NaN
+ * too -- leaves it as it is.  window >= 1 (as large as the sequence: all of it), first >= 0,
+ * any H >= 1.  The two halves of a score are exchanged between two SMs in fp16 (as for
+ * dsa_sparse_mla_decode_records).
+ * Calls that would leave SMs idle cut their rows' keys into parts that a second kernel
+ * merges in fp32: `workspace` (16-byte aligned) of ..._workspace_bytes bytes holds
+ * those; with a smaller one, or NULL, the call works with fewer parts or none. */
+
+/* Prompts: q_bf16 [T, H, 576], kv_bf16 [S, 576], out_bf16 [T, H, 512], contiguous.  Row t
+ * is the position ke[t]-1 of a sequence that begins at ks[t] (windows as for
+ * dsa_indexer_logits; ks NULL = 0, ke NULL = S-T+t+1, held to [0, S]; positions of a row
+ * count from its ks): packed sequences, chunks behind a context, rows in any order.  Rows
+ * of one sequence that follow one another share the reads of their keys. */
+size_t dsa_window_mla_prefill_workspace_bytes(int T, int H, int window, int first);
+int dsa_window_mla_prefill(const void* q_bf16, const void* kv_bf16, const int32_t* ks, const int32_t* ke, void* out_bf16,
+                           int T, int H, int S, int window, int first, float scale, void* workspace, size_t workspace_bytes,
+                           int32_t* status, void* stream);
+
+/* Drafted tokens: of a sequence's ctx_len[b] tokens in the cache the last n_new[b] are drafts
+ * (n_new NULL: min(ctx_len[b], tokens_per_seq); one: the newest token of a plain decode
+ * step), their query rows b*tokens_per_seq + i, i < n_new[b]; the rows behind them belong to no
+ * token.  P = ctx_len[b] - n_new[b] tokens stand before them.  tree [B, tokens_per_seq] (8-byte
+ * aligned; at most 64 tokens a sequence): bit j of tree[b, i], j < i, says that draft i
+ * descends from draft j; a draft sees the P tokens, the drafts that its mask names and itself, and
+ * its position is P plus the number of those drafts.  Bits i and up are not looked at.
+ * tree NULL: chains, draft i sees all before it.  A sequence with ctx_len outside [0,
+ * max_ctx] or n_new outside [0, min(tokens_per_seq, ctx_len)] counts as empty and sets status 2.
+ * A position whose page is none is not seen, and sets status 2. */
+
+/* The window attention over records of record_bytes = 656 or 416 of a paged latent cache: q_bf16
+ * [B*tokens_per_seq, H, 576], out_bf16 [B*tokens_per_seq, H, 512]; rows without a token give
+ * zeros.  Positions are those along a draft's path. */
+size_t dsa_window_mla_decode_workspace_bytes(int record_bytes, int B, int tokens_per_seq, int H, int window, int first, int max_ctx);
+int dsa_window_mla_decode_paged(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table,
+                                int64_t table_stride, const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree,
+                                int tokens_per_seq, void* out_bf16, int B, int H, int window, int first, int num_pages,
+                                int max_ctx, float scale, void* workspace, size_t workspace_bytes, int32_t* status,
+                                void* stream);
+
+/* dsa_indexer_logits_paged for drafts: q_fp8 [B*tokens_per_seq, H, 128], w [B*tokens_per_seq, H], logits
+ * [B*tokens_per_seq, ld_logits]; H in {16, 32, 64}.  Columns of [0, ctx_len[b]) that a row does not see get -inf, and so
+ * do those behind ctx_len[b] up to a multiple of 128 (and max_ctx); beyond are untouched. */
+int dsa_indexer_logits_drafts(const void* q_fp8, const void* w, int w_dtype, const void* kcache, const float* kscale,
+                              const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len, const int32_t* n_new,
+                              const int64_t* tree, int tokens_per_seq, float* logits, int64_t ld_logits, int B, int H, int D,
+                              int num_pages, int max_ctx, int32_t* status, void* stream);
+/* dsa_topk_select of such logits: of every row the k largest of the positions that its draft sees, -1 in the slots
+ * that are left (anywhere in the list); rows without a token: -1. */
+size_t dsa_topk_select_drafts_workspace_bytes(int B, int tokens_per_seq);
+int dsa_topk_select_drafts(const float* logits, int64_t ld_logits, const int32_t* ctx_len, const int32_t* n_new,
+                           const int64_t* tree, int tokens_per_seq, int B, int max_ctx, int k, int32_t* out_idx,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Row rows[i] of the tables above, i < n, keeps n_keep[i] of its last n_new[i] tokens, the drafts path[i, 0 .. n_keep[i])
+ * (numbers 0 .. n_new[i]-1, ascending; path [n, path_stride] int32): their records move to the first places behind the tokens
+ * before them, in every layer of every cache, ctx_len follows, and pages behind it are given back.  A row that
+ * the list has named before, whose numbers make no sense or whose drafts lie in pages that are none stays as it is and sets
+ * status 2; so does one that drops drafts and has kept ones, or the last tokens before them, in a page that another
+ * sequence holds too.  `workspace`: dsa_pages_workspace_bytes(0, n). */
+int dsa_accept_drafts(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages,
+                      const int32_t* rows, const int32_t* n_new, const int32_t* path, int path_stride, const int32_t* n_keep,
+                      int n, const dsa_page_cache* caches, int n_caches, void* workspace, size_t workspace_bytes,
+                      int32_t* status, void* stream);
+
 /* dsa_indexer_topk without a caller-supplied workspace.  No counterpart in the
  * reference: it exists for hosts that cannot allocate device memory at the call
  * site (a runtime that owns the whole device heap and forbids allocation inside

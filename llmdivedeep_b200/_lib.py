@@ -63,6 +63,19 @@ SIGNATURES = {
     "dsa_free_pages": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]),
     "dsa_compact_pages": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dsa_window_mla_prefill_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "dsa_window_mla_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
+                                       c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dsa_window_mla_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "dsa_window_mla_decode_paged": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                            c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dsa_indexer_logits_drafts": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                          c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "dsa_topk_select_drafts_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "dsa_topk_select_drafts": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                       c_size_t, c_void_p]),
+    "dsa_accept_drafts": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                                  c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
     "dsa_test_indexer_logits_general": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                                 c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p,
                                                 c_void_p]),

@@ -80,6 +80,19 @@ int free_pages_launch(int32_t* table, int64_t stride, int P, int B, int32_t* ctx
 int compact_pages_launch(const int32_t* table, int64_t stride, int32_t* new_table, int64_t new_stride, int P, int B, const int32_t* refs, int32_t* new_refs,
                          int num_pages, const dsa_page_cache* caches, int n_caches, int32_t* workspace, int32_t* status, cudaStream_t stream);
 size_t pages_workspace_bytes(int num_pages, int n);
+int accept_drafts_launch(int32_t* table, int64_t stride, int P, int B, int32_t* ctx, int32_t* refs, int num_pages, const int32_t* rows, const int32_t* n_new,
+                         const int32_t* path, int path_stride, const int32_t* n_keep, int n, const dsa_page_cache* caches, int n_caches, int32_t* workspace,
+                         int32_t* status, cudaStream_t stream);
+int indexer_logits_drafts_launch(const void* q, const void* w, int w_is_bf16, const void* kcache, const float* kscale, const int32_t* block_table,
+                                 int64_t table_stride, const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree, int tokens_per_seq, float* logits,
+                                 int64_t ld, int B, int H, int num_pages, int max_ctx, int32_t* status, cudaStream_t stream);
+int topk_select_drafts_launch(const float* logits, int64_t ld, const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree, int tokens_per_seq, int B,
+                              int max_ctx, int k, int32_t* out, int32_t* ends, cudaStream_t stream);
+int window_mla_prefill_launch(const void* q, const void* kv, const int32_t* ks, const int32_t* ke, void* out, int T, int H, int S, int window, int first,
+                              float scale, int32_t* status, cudaStream_t stream);
+int window_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len,
+                             const int32_t* n_new, const int64_t* tree, int tokens_per_seq, void* out, int B, int H, int window, int first, int num_pages,
+                             int max_ctx, float scale, int32_t* status, cudaStream_t stream);
 int pack_latent_launch(const void* kv, int kv_is_bf16, int64_t row_stride, int64_t n, void* rec, cudaStream_t stream);
 int rope_fp8_quant_launch(const void* x, int64_t n_rows, int head_dim, int rope_dim, int interleave, int rows_per_pos,
                           const float* cos_t, const float* sin_t, void* q, float* scale, const void* gate, float mul0,
@@ -462,6 +475,118 @@ int dsa_compact_pages(const int32_t* block_table, int64_t table_stride, int32_t*
   if (rc) return rc;
   if ((rc = check_pages_workspace("compact_pages", workspace, workspace_bytes, num_pages, 0))) return rc;
   return compact_pages_launch(block_table, table_stride, new_table, new_stride, P, B, refs, new_refs, num_pages, caches, n_caches,
+                              static_cast<int32_t*>(workspace), status, static_cast<cudaStream_t>(stream));
+}
+
+// ---- window layers and drafted tokens ------------------------------------------------------------------------------------
+static int check_drafts(const char* who, int B, int tokens_per_seq, const void* tree, int max_ctx) {
+  if (B < 0 || max_ctx < 0) return set_error(DSA_ERR_SHAPE, "%s: negative size", who);
+  if (tokens_per_seq < 1) return set_error(DSA_ERR_SHAPE, "%s: tokens_per_seq (%d) must be at least 1", who, tokens_per_seq);
+  if (tree && tokens_per_seq > 64) return set_error(DSA_ERR_SHAPE, "%s: a tree has at most 64 drafts, not %d", who, tokens_per_seq);
+  if ((int64_t)B * tokens_per_seq > 0x7fffffffLL) return set_error(DSA_ERR_SHAPE, "%s: more than 2147483647 query rows", who);
+  if (reinterpret_cast<uintptr_t>(tree) & 7) return set_error(DSA_ERR_ALIGN, "%s: tree must be 8-byte aligned", who);
+  return DSA_OK;
+}
+static int check_window(const char* who, int H, int window, int first, float scale) {
+  if (H < 0) return set_error(DSA_ERR_SHAPE, "%s: negative size", who);
+  if (window < 1 || first < 0) return set_error(DSA_ERR_SHAPE, "%s: window (%d) must be at least 1 and first (%d) at least 0", who, window, first);
+  if (!(scale > 0.f)) return set_error(DSA_ERR_ARG, "%s: the softmax scale must be positive", who);
+  return DSA_OK;
+}
+
+size_t dsa_window_mla_prefill_workspace_bytes(int T, int H, int window, int first) { return 0; }
+
+int dsa_window_mla_prefill(const void* q_bf16, const void* kv_bf16, const int32_t* ks, const int32_t* ke, void* out_bf16, int T, int H, int S, int window,
+                           int first, float scale, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  g_err[0] = 0;
+  if (T < 0 || S < 0) return set_error(DSA_ERR_SHAPE, "window_mla_prefill: negative size");
+  const int rc = check_window("window_mla_prefill", H, window, first, scale);
+  if (rc || T == 0 || H == 0) return rc;
+  if (!q_bf16 || !out_bf16 || (S > 0 && !kv_bf16)) return set_error(DSA_ERR_ARG, "window_mla_prefill: NULL pointer argument");
+  if (!aligned16(q_bf16) || !aligned16(kv_bf16) || !aligned16(out_bf16))
+    return set_error(DSA_ERR_ALIGN, "window_mla_prefill: q, kv and out must be 16-byte aligned");
+  if ((int64_t)T * H > 0x7fffffffLL) return set_error(DSA_ERR_SHAPE, "window_mla_prefill: T*H exceeds 2^31");
+  if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return set_error(DSA_ERR_WORKSPACE, "window_mla_prefill: workspace must be 16-byte aligned");
+  return window_mla_prefill_launch(q_bf16, kv_bf16, ks, ke, out_bf16, T, H, S, window, first, scale, status, static_cast<cudaStream_t>(stream));
+}
+
+size_t dsa_window_mla_decode_workspace_bytes(int record_bytes, int B, int tokens_per_seq, int H, int window, int first, int max_ctx) { return 0; }
+
+int dsa_window_mla_decode_paged(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,
+                                const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree, int tokens_per_seq, void* out_bf16, int B, int H,
+                                int window, int first, int num_pages, int max_ctx, float scale, void* workspace, size_t workspace_bytes, int32_t* status,
+                                void* stream) {
+  const char* who = "window_mla_decode_paged";
+  g_err[0] = 0;
+  int rc = check_drafts(who, B, tokens_per_seq, tree, max_ctx);
+  if (!rc) rc = check_window(who, H, window, first, scale);
+  if (rc) return rc;
+  if (num_pages < 0) return set_error(DSA_ERR_SHAPE, "%s: negative size", who);
+  if (record_bytes != 656 && record_bytes != 416) return set_error(DSA_ERR_SHAPE, "%s: records of %d bytes, only 656 (FP8) and 416 (4 bits) are built", who, record_bytes);
+  if (B == 0 || H == 0) return DSA_OK;
+  if (!q_bf16 || !out_bf16 || !ctx_len || (max_ctx > 0 && (!cache || !block_table))) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
+  if (!aligned16(q_bf16) || !aligned16(cache) || !aligned16(out_bf16)) return set_error(DSA_ERR_ALIGN, "%s: q, cache and out must be 16-byte aligned", who);
+  if (table_stride * 64 < max_ctx) return set_error(DSA_ERR_SHAPE, "%s: block table row shorter than max_ctx", who);
+  if ((int64_t)num_pages * 64 > 0x7fffffffLL || (int64_t)B * tokens_per_seq * H > 0x7fffffffLL) return set_error(DSA_ERR_SHAPE, "%s: problem too large", who);
+  if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15)) return set_error(DSA_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", who);
+  return window_mla_decode_launch(q_bf16, cache, record_bytes, block_table, table_stride, ctx_len, n_new, tree, tokens_per_seq, out_bf16, B, H, window, first,
+                                  num_pages, max_ctx, scale, status, static_cast<cudaStream_t>(stream));
+}
+
+int dsa_indexer_logits_drafts(const void* q_fp8, const void* w, int w_dtype, const void* kcache, const float* kscale, const int32_t* block_table,
+                              int64_t table_stride, const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree, int tokens_per_seq, float* logits,
+                              int64_t ld_logits, int B, int H, int D, int num_pages, int max_ctx, int32_t* status, void* stream) {
+  const char* who = "indexer_logits_drafts";
+  g_err[0] = 0;
+  const int rc = check_drafts(who, B, tokens_per_seq, tree, max_ctx);
+  if (rc) return rc;
+  if (num_pages < 0) return set_error(DSA_ERR_SHAPE, "%s: negative size", who);
+  if (D != 128 || (H != 64 && H != 32 && H != 16)) return set_error(DSA_ERR_SHAPE, "%s: unsupported (heads=%d, head_dim=%d)", who, H, D);
+  if (B == 0 || max_ctx == 0) return DSA_OK;
+  if (!q_fp8 || !w || !kcache || !kscale || !block_table || !ctx_len || !logits) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
+  if (w_dtype != DSA_W_F32 && w_dtype != DSA_W_BF16) return set_error(DSA_ERR_ARG, "%s: bad w_dtype", who);
+  if (ld_logits < max_ctx) return set_error(DSA_ERR_SHAPE, "%s: ld_logits < max_ctx", who);
+  if (ld_logits * 64 > 0x7fffffffLL) return set_error(DSA_ERR_SHAPE, "%s: ld_logits too large", who);
+  if (table_stride * 64 < max_ctx) return set_error(DSA_ERR_SHAPE, "%s: block table row (%lld pages) shorter than max_ctx %d", who, (long long)table_stride, max_ctx);
+  if (!aligned16(q_fp8) || !aligned16(kcache) || !aligned16(kscale)) return set_error(DSA_ERR_ALIGN, "%s: q_fp8, kcache and kscale must be 16-byte aligned", who);
+  if ((int64_t)num_pages * 64 > 0x7fffffffLL || (int64_t)B * tokens_per_seq * H > 0x7fffffffLL) return set_error(DSA_ERR_SHAPE, "%s: problem too large", who);
+  return indexer_logits_drafts_launch(q_fp8, w, w_dtype == DSA_W_BF16, kcache, kscale, block_table, table_stride, ctx_len, n_new, tree, tokens_per_seq, logits,
+                                      ld_logits, B, H, num_pages, max_ctx, status, static_cast<cudaStream_t>(stream));
+}
+
+size_t dsa_topk_select_drafts_workspace_bytes(int B, int tokens_per_seq) { return B < 0 || tokens_per_seq < 1 ? 0 : (size_t)B * tokens_per_seq * sizeof(int32_t); }
+
+int dsa_topk_select_drafts(const float* logits, int64_t ld_logits, const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree, int tokens_per_seq,
+                           int B, int max_ctx, int k, int32_t* out_idx, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "topk_select_drafts";
+  g_err[0] = 0;
+  const int rc = check_drafts(who, B, tokens_per_seq, tree, max_ctx);
+  if (rc) return rc;
+  if (k < 0) return set_error(DSA_ERR_SHAPE, "%s: negative size", who);
+  if (B == 0 || k == 0) return DSA_OK;
+  if (!logits || !ctx_len || !out_idx) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
+  if (ld_logits < max_ctx) return set_error(DSA_ERR_SHAPE, "%s: ld_logits < max_ctx", who);
+  if (k > 65535) return set_error(DSA_ERR_SHAPE, "%s: k (%d) exceeds 65535", who, k);
+  const size_t need = dsa_topk_select_drafts_workspace_bytes(B, tokens_per_seq);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || workspace_bytes < need)
+    return set_error(DSA_ERR_WORKSPACE, "%s: workspace missing, unaligned or smaller than %zu B", who, need);
+  return topk_select_drafts_launch(logits, ld_logits, ctx_len, n_new, tree, tokens_per_seq, B, max_ctx, k, out_idx, static_cast<int32_t*>(workspace),
+                                   static_cast<cudaStream_t>(stream));
+}
+
+int dsa_accept_drafts(int32_t* block_table, int64_t table_stride, int P, int B, int32_t* ctx_len, int32_t* refs, int num_pages, const int32_t* rows,
+                      const int32_t* n_new, const int32_t* path, int path_stride, const int32_t* n_keep, int n, const dsa_page_cache* caches, int n_caches,
+                      void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  const char* who = "accept_drafts";
+  g_err[0] = 0;
+  int rc = check_pool(who, block_table, table_stride, P, B, refs, num_pages, n);
+  if (!rc) rc = check_page_caches(who, caches, n_caches);
+  if (rc || n == 0) return rc;
+  if (path_stride < 0) return set_error(DSA_ERR_SHAPE, "%s: negative size", who);
+  if (!ctx_len || !rows || !n_new || !n_keep || (path_stride > 0 && !path)) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
+  if ((rc = check_pages_workspace(who, workspace, workspace_bytes, 0, n))) return rc;
+  return accept_drafts_launch(block_table, table_stride, P, B, ctx_len, refs, num_pages, rows, n_new, path, path_stride, n_keep, n, caches, n_caches,
                               static_cast<int32_t*>(workspace), status, static_cast<cudaStream_t>(stream));
 }
 

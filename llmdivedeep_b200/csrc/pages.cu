@@ -552,6 +552,102 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
   }
 }
 
+// ---- acceptance of drafts ----------------------------------------------------------------------------------------------
+// Row rows[i] keeps the drafts path[i, 0 .. n_keep[i]) of its last n_new[i] tokens: draft path[k] moves to place k behind the P tokens before
+// them, in every cache; what lies behind goes.  path[k] >= k, so a place that is written is read by no later move, and a thread that takes
+// the same 16 bytes of every token in order needs no barrier.
+struct AcceptArgs {
+  CacheEntry cache[kCopyCaches];
+  int32_t first[kCopyCaches + 1];                      // columns of one token in the caches before
+  int n_caches;
+  int32_t *table, *ctx, *refs;
+  int64_t stride;
+  int P, B, num_pages, n;
+  const int32_t *rows, *n_new, *path, *n_keep;
+  int path_stride;
+  int32_t* accepted;                                   // workspace [n]: whether row i is
+  int* status;
+};
+// Whether entry i can be done; every thread of the CTA comes here.  A row is refused that the list has named before, whose numbers make no
+// sense, whose drafts lie in pages that are none, or -- where something moves or goes -- whose kept drafts do in pages that others hold too.
+__device__ __forceinline__ bool accept_valid(const AcceptArgs& a, int i) {
+  const int row = a.rows[i], nn = a.n_new[i], keep = a.n_keep[i];
+  bool bad = row < 0 || row >= a.B || nn < 0 || keep < 0 || keep > nn || keep > a.path_stride;
+  const int c = bad ? 0 : a.ctx[row];
+  if (c < nn || (int64_t)c > (int64_t)a.P * kPageTokens) bad = true;
+  for (int j = threadIdx.x; j < i; j += blockDim.x) bad |= a.rows[j] == row;
+  if (!bad) {
+    for (int k = threadIdx.x; k < keep; k += blockDim.x) {
+      const int at = a.path[(int64_t)i * a.path_stride + k], before = k ? a.path[(int64_t)i * a.path_stride + k - 1] : -1;
+      bad |= at <= before || at >= nn;
+    }
+    const int p0 = (c - nn) / kPageTokens, kept = pages_of(c - nn + keep);
+    for (int p = p0 + threadIdx.x; p < pages_of(c); p += blockDim.x) {
+      const int page = a.table[(int64_t)row * a.stride + p];
+      if ((unsigned)page >= (unsigned)a.num_pages) bad = true;
+      else if (keep < nn && p < kept && a.refs[page] != 1) bad = true;
+    }
+  }
+  return !__syncthreads_or(bad);
+}
+template <typename W>
+__device__ __forceinline__ void accept_column(const AcceptArgs& a, const CacheEntry& ce, uint8_t* base, const int32_t* trow, const int32_t* path, int P, int keep) {
+  constexpr int kAhead = 8;                            // loads of as many tokens under way
+  auto at = [&](int pos) { return reinterpret_cast<W*>(base + ((int64_t)trow[pos / kPageTokens] * kPageTokens + pos % kPageTokens) * ce.token_bytes); };
+  for (int k0 = 0; k0 < keep; k0 += kAhead) {
+    W v[kAhead];
+    int from[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      from[j] = k0 + j < keep ? path[k0 + j] : -1;
+      if (from[j] > k0 + j) v[j] = *at(P + from[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (from[j] > k0 + j) *at(P + k0 + j) = v[j];
+  }
+}
+__global__ void __launch_bounds__(kCopyThreads) accept_kernel(const __grid_constant__ AcceptArgs a, int lead) {
+  launch_dependents();
+  const int i = blockIdx.x, cols = a.first[a.n_caches];
+  const bool ok = accept_valid(a, i);
+  if (lead && blockIdx.y == 0 && threadIdx.x == 0) a.accepted[i] = ok;
+  if (!ok) {
+    if (threadIdx.x == 0 && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+    return;
+  }
+  const int row = a.rows[i], P = a.ctx[row] - a.n_new[i], keep = a.n_keep[i];
+  const int32_t *trow = a.table + (int64_t)row * a.stride, *path = a.path + (int64_t)i * a.path_stride;
+  for (int c = blockIdx.y * kCopyThreads + threadIdx.x; c < cols; c += gridDim.y * kCopyThreads) {
+    int e = 0;
+    for (int hi = a.n_caches; hi - e > 1;) {           // the cache that column c belongs to
+      const int mid = (e + hi) / 2;
+      (c >= a.first[mid] ? e : hi) = mid;
+    }
+    const CacheEntry& ce = a.cache[e];
+    const int wide = ce.token_bytes % 16 == 0 ? 16 : 4, per = ce.token_bytes / wide, in = c - a.first[e], layer = in / per;
+    uint8_t* base = ce.base + layer * ce.layer_stride + (in - layer * per) * wide;
+    if (wide == 16) accept_column<uint4>(a, ce, base, trow, path, P, keep);
+    else accept_column<uint32_t>(a, ce, base, trow, path, P, keep);
+  }
+}
+// Lengths and pages, when all contents have moved.
+__global__ void __launch_bounds__(kCopyThreads) accept_pages_kernel(const __grid_constant__ AcceptArgs a) {
+  const int i = blockIdx.x;
+  if (!grid_wait(a.accepted)[i]) return;
+  const int row = a.rows[i], c = a.ctx[row], now = c - a.n_new[i] + a.n_keep[i];
+  __syncthreads();                                     // every thread has read the length
+  if (threadIdx.x == 0) a.ctx[row] = now;
+  for (int p = pages_of(now) + threadIdx.x; p < pages_of(c); p += kCopyThreads) {
+    int32_t* entry = a.table + (int64_t)row * a.stride + p;
+    const int page = *entry;
+    *entry = -1;
+    if (atomicSub(&a.refs[page], 1) > 0) continue;
+    atomicAdd(&a.refs[page], 1);                       // was free already: the state is not what it says
+    if (a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+  }
+}
+
 // ---- launches --------------------------------------------------------------------------------------------------------
 template <typename... Params, typename... Args>
 static void launch_pool(void (*kern)(Params...), int num_pages, size_t smem, cudaStream_t stream, Args... args) {
@@ -683,6 +779,32 @@ int compact_pages_launch(const int32_t* table, int64_t stride, int32_t* new_tabl
   c.status = status;
   const RemapArgs m{table, a.remap, a.count, new_table, stride, new_stride, B, P, num_pages};
   return launch_copies<kCopyCompact>(c, PoolArgs{}, m, caches, n_caches, num_pages / 2, ((int64_t)B * P + 31) / 32, stream);
+}
+
+int accept_drafts_launch(int32_t* table, int64_t stride, int P, int B, int32_t* ctx, int32_t* refs, int num_pages, const int32_t* rows, const int32_t* n_new,
+                         const int32_t* path, int path_stride, const int32_t* n_keep, int n, const dsa_page_cache* caches, int n_caches, int32_t* workspace,
+                         int32_t* status, cudaStream_t stream) {
+  AcceptArgs a{};
+  a.table = table; a.stride = stride; a.P = P; a.B = B;
+  a.ctx = ctx; a.refs = refs; a.num_pages = num_pages; a.n = n;
+  a.rows = rows; a.n_new = n_new; a.path = path; a.path_stride = path_stride; a.n_keep = n_keep;
+  a.accepted = workspace;
+  a.status = status;
+  int c0 = 0;
+  do {
+    a.n_caches = min(n_caches - c0, kCopyCaches);
+    a.first[0] = 0;
+    for (int c = 0; c < a.n_caches; ++c) {
+      const dsa_page_cache& h = caches[c0 + c];
+      a.cache[c] = {static_cast<uint8_t*>(h.base), h.layer_stride, h.layers, h.token_bytes};
+      a.first[c + 1] = a.first[c] + h.layers * (h.token_bytes / (h.token_bytes % 16 == 0 ? 16 : 4));
+    }
+    const int split = min(max(1, (a.first[a.n_caches] + kCopyThreads - 1) / kCopyThreads), 65535);
+    accept_kernel<<<dim3(n, split), kCopyThreads, 0, stream>>>(a, c0 == 0);
+    c0 += kCopyCaches;
+  } while (c0 < n_caches);
+  launch_after(1, accept_pages_kernel, dim3(n), kCopyThreads, 0, stream, a);
+  return check_launch("accept_drafts");
 }
 
 }  // namespace dsa

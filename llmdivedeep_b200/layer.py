@@ -35,6 +35,28 @@ class SparseMLA(nn.Module):
         return ops.sparse_mla_prefill(q, kv, idx, self.softmax_scale)
 
 
+class WindowMLA(nn.Module):
+    """MQA over the shared latent KV restricted to a sliding window and the first tokens: the layers of a hybrid model that stand next to the
+    sparse ones and read the same caches.
+
+    forward(q [T,H,576] bf16, kv [S,576] bf16, ks=None, ke=None) for prompts (ops.window_mla_prefill),
+    forward(q [B*n,H,576] bf16, cache, block_table=..., ctx_len=..., tokens_per_seq=n, n_new=None, tree=None) for decode over the paged latent
+    cache, FP8 or 4 bits (ops.window_mla_decode_paged).  Returns bf16 [.., H, 512]."""
+
+    def __init__(self, softmax_scale: float, window: int, first: int = 0):
+        super().__init__()
+        self.softmax_scale, self.window, self.first = float(softmax_scale), int(window), int(first)
+
+    @torch.no_grad()
+    def forward(self, q, kv, ks=None, ke=None, block_table: Optional[torch.Tensor] = None, ctx_len: Optional[torch.Tensor] = None,
+                tokens_per_seq: int = 1, n_new: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None):
+        if kv.dtype == torch.uint8:
+            if block_table is None or ctx_len is None:
+                raise ops.DsaError("the paged latent cache needs a block_table and ctx_len")
+            return ops.window_mla_decode_paged(q, kv, block_table, ctx_len, self.window, self.first, self.softmax_scale, tokens_per_seq, n_new, tree)
+        return ops.window_mla_prefill(q, kv, ks, ke, self.window, self.first, self.softmax_scale)
+
+
 class DSALayer(nn.Module):
     """One DSA attention layer from hidden states: lightning indexer -> top-k -> sparse MLA.
 
@@ -437,6 +459,22 @@ def dsa_decode_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, laten
     return idx, out
 
 
+@torch.no_grad()
+def dsa_draft_step(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, q, latent_cache, softmax_scale: float, ws: DecodeWorkspace,
+                   tokens_per_seq: int, n_new: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None):
+    """dsa_decode_step for ``tokens_per_seq`` drafted tokens a sequence, a chain or a tree (ops.fp8_paged_mqa_logits): every draft gets the selection
+    and the output that a step of its own would give it.  ``ws`` has room for a row per draft: DecodeWorkspace(batch * tokens_per_seq, ...).
+    Returns (idx, out) views of it; rows without a token have indices of -1 and zeros."""
+    T = q.shape[0]
+    idx, out = ws.idx[:T], ws.out[:T]
+    logits = ops.fp8_paged_mqa_logits(q_idx_fp8, w, kcache, kscale, block_table, ctx_len, ws.max_ctx, out=ws.logits, tokens_per_seq=tokens_per_seq,
+                                      n_new=n_new, tree=tree)
+    ops.topk_select_drafts(logits, ws.k, ctx_len, tokens_per_seq, n_new, tree, out=idx)
+    ops.sparse_mla_decode_paged(q, latent_cache, block_table, idx, softmax_scale, ws.max_ctx, out=out, workspace=ws.parts(latent_cache.shape[-1]),
+                                tokens_per_seq=tokens_per_seq)
+    return idx, out
+
+
 class PagedCache:
     """The decode caches of ``layers`` DSA layers, latents in 4 bits, in one pool of 64-token pages, and the tables that say
     which sequence has which page: 416 + 132 bytes a token and layer.  What 4 bits cost: latents drawn from N(0,1) read back 9.5 % off (root
@@ -446,6 +484,9 @@ class PagedCache:
         slots = cache.extend([row], [n], n)                    # room for n tokens in a row of the batch
         cache.write(layer, slots, kv, k8, k_scale)             # their latents and indexer keys, layer by layer
         idx, out = cache.decode(layer, q8, w, q, scale, ws)    # one step for all rows; ws = DecodeWorkspace(batch, heads, ...)
+        idx, out = cache.decode_drafts(layer, q8, w, q, scale, ws, n, n_new, tree)      # the last n_new[b] tokens of every row are drafts
+        out = cache.window(layer, q, window, first, scale)     # a window layer's attention, of the newest tokens or of drafts
+        cache.accept([row], [n_new], [path], [n_keep])         # the drafts that are kept; the others' tokens and pages go
         cache.fork([row], [other])                             # a beam, a shared prompt: full pages are not copied
         cache.free([row])
         cache.compact()                                        # pages in use to the lowest ids, contents and tables
@@ -490,6 +531,23 @@ class PagedCache:
         """dsa_decode_step of the first q.shape[0] rows over this layer's caches; empty rows give zeros."""
         B = q.shape[0]
         return dsa_decode_step(q8, w, self.k8[layer], self.k_scale[layer], self.table[:B], self.ctx[:B], q, self.latent[layer], softmax_scale, ws)
+
+    def decode_drafts(self, layer: int, q8, w, q, softmax_scale: float, ws: DecodeWorkspace, tokens_per_seq: int, n_new=None, tree=None):
+        """dsa_draft_step of the first q.shape[0] / tokens_per_seq rows: the last n_new[b] tokens of a row (None: tokens_per_seq) are drafts."""
+        B = q.shape[0] // tokens_per_seq
+        return dsa_draft_step(q8, w, self.k8[layer], self.k_scale[layer], self.table[:B], self.ctx[:B], q, self.latent[layer], softmax_scale, ws,
+                              tokens_per_seq, n_new, tree)
+
+    def window(self, layer: int, q, window: int, first: int, softmax_scale: float, tokens_per_seq: int = 1, n_new=None, tree=None,
+               out: Optional[torch.Tensor] = None):
+        """Attention of the newest tokens, or of drafts, over a sliding window and the first tokens of this layer's latents."""
+        B = q.shape[0] // tokens_per_seq
+        return ops.window_mla_decode_paged(q, self.latent[layer], self.table[:B], self.ctx[:B], window, first, softmax_scale, tokens_per_seq, n_new, tree,
+                                           out=out)
+
+    def accept(self, rows, n_new, path, n_keep) -> None:
+        """Of the last n_new[i] tokens of row rows[i] the drafts path[i, :n_keep[i]] stay, moved up; path is int32 [n, most], ascending."""
+        ops.accept_drafts(self.table, self.ctx, self.refs, self._rows(rows), self._rows(n_new), self._rows(path), self._rows(n_keep), self.caches)
 
     def fork(self, parents, children) -> None:
         ops.fork_pages(self.table, self.ctx, self.refs, self._rows(parents), self._rows(children), self.caches)

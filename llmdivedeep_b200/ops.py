@@ -187,11 +187,19 @@ def fp8_mqa_logits(q_fp8, kv, weights, ks, ke, clean_logits: bool = True,
 
 
 def fp8_paged_mqa_logits(q_fp8, weights, kcache, kscale, block_table, ctx_len, max_ctx: int,
-                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                         out: Optional[torch.Tensor] = None, tokens_per_seq: int = 1, n_new: Optional[torch.Tensor] = None,
+                         tree: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Decode indexer over the paged FP8 key cache.  q_fp8 [B,H,128], weights [B,H],
     kcache [num_pages*64,128] e4m3, kscale [num_pages*64] fp32, block_table [B,P] int32,
     ctx_len [B] int32.  Returns fp32 [B, max_ctx]; columns >= ctx_len[b] inside a
-    processed 128-key tile hold -inf, columns beyond are uninitialised."""
+    processed 128-key tile hold -inf, columns beyond are uninitialised.
+
+    With ``tokens_per_seq`` = n rows [B*n, ...] of query tokens, which are the last n_new[b] tokens of their sequences (int32 [B]; None:
+    min(ctx_len[b], n)), row b*n + i draft i: a chain, or with ``tree`` (int64 [B, n], n <= 64) the tree whose bit j < i of tree[b, i] says that
+    draft i descends from draft j.  A draft sees the tokens before the drafts, its ancestors and itself; what it does not see is
+    -inf, and so are rows without a token (n_new[b] <= i), up to ctx_len[b] and the end of that 128-key tile."""
+    if tokens_per_seq != 1 or n_new is not None or tree is not None:
+        return _draft_logits(q_fp8, weights, kcache, kscale, block_table, ctx_len, max_ctx, out, tokens_per_seq, n_new, tree)
     dev = _need_cuda(q_fp8, weights, kcache, kscale, block_table, ctx_len, out)
     B, H, D = q_fp8.shape
     if kcache.dtype != FP8 or q_fp8.dtype != FP8 or kcache.dim() != 2 or kcache.shape[1] != D:
@@ -441,6 +449,137 @@ def decode_step(q_fp8, weights, kcache, kscale, block_table, ctx_len, q, cache, 
         else:
             check(lib.dsa_decode_step_records(*head, cache.shape[1], *rest, _stream(dev)))
     return True
+
+
+# ---- window layers and drafted tokens ------------------------------------------------------------------------------------
+def _check_drafts(T: int, tokens_per_seq: int, ctx_len, n_new, tree) -> tuple:
+    """Sequences of T query rows, and their (ctx_len, n_new, tree) as the library takes them."""
+    if tokens_per_seq < 1 or T % tokens_per_seq:
+        raise DsaError(f"{T} query rows are no {tokens_per_seq} a sequence")
+    B = T // tokens_per_seq
+    if tree is not None:
+        if tree.dtype is not torch.int64 or tuple(tree.shape) != (B, tokens_per_seq):
+            raise DsaError(f"tree must be int64 [{B}, {tokens_per_seq}], got {tree.dtype} {tuple(tree.shape)}")
+        if tokens_per_seq > 64:
+            raise DsaError(f"a tree has at most 64 drafts, not {tokens_per_seq}")
+        tree = tree.contiguous()
+    return B, _as_i32(ctx_len, B, "ctx_len"), _as_i32(n_new, B, "n_new"), tree
+
+
+def _check_table(block_table, B: int, max_ctx: int) -> torch.Tensor:
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise DsaError(f"block_table must be int32 [{B}, pages], got {block_table.dtype} {tuple(block_table.shape)}")
+    if max_ctx > block_table.shape[1] * 64:
+        raise DsaError(f"max_ctx {max_ctx} is more than the {block_table.shape[1]} pages of a table row hold")
+    return block_table.contiguous()
+
+
+def _draft_logits(q_fp8, weights, kcache, kscale, block_table, ctx_len, max_ctx, out, tokens_per_seq, n_new, tree) -> torch.Tensor:
+    i = _index_of(q_fp8, *[t for t in (weights, kcache, kscale, block_table, ctx_len, out, n_new, tree) if t is not None])
+    if q_fp8.dtype is not FP8 or kcache.dtype is not FP8 or q_fp8.dim() != 3 or kcache.dim() != 2 or kcache.shape[1] != q_fp8.shape[2]:
+        raise DsaError(f"q must be e4m3 [T, H, D] and kcache e4m3 [num_pages*64, D], got {q_fp8.dtype} {tuple(q_fp8.shape)}, {kcache.dtype} {tuple(kcache.shape)}")
+    T, H, D = q_fp8.shape
+    if kcache.shape[0] % 64:
+        raise DsaError("kcache rows must be a multiple of the 64-token page")
+    if tuple(weights.shape) != (T, H):
+        raise DsaError(f"weights must be [{T}, {H}], got {tuple(weights.shape)}")
+    B, ctx_len, n_new, tree = _check_drafts(T, tokens_per_seq, ctx_len, n_new, tree)
+    block_table = _check_table(block_table, B, max_ctx)
+    q_fp8, kcache, weights, kscale = q_fp8.contiguous(), kcache.contiguous(), weights.contiguous(), _flat_f32(kscale)
+    if kscale.numel() != kcache.shape[0]:
+        raise DsaError("kscale must have an entry for every row of kcache")
+    if out is None:
+        out = torch.empty(T, (max_ctx + 3) // 4 * 4, dtype=torch.float32, device=q_fp8.device)
+    elif out.dtype is not torch.float32 or out.dim() != 2 or out.shape[0] < T or out.shape[1] < max_ctx or out.stride(1) != 1 or (T > 1 and out.stride(0) < max_ctx):
+        raise DsaError("out must be fp32 [>=T, >=max_ctx] with unit column stride")
+    _run(i, _lib.load().dsa_indexer_logits_drafts, q_fp8.data_ptr(), weights.data_ptr(), _w_dtype(weights), kcache.data_ptr(), kscale.data_ptr(),
+         block_table.data_ptr(), block_table.stride(0), ctx_len.data_ptr(), _ptr(n_new), _ptr(tree), tokens_per_seq, out.data_ptr(),
+         max(out.stride(0), max_ctx), B, H, D, kcache.shape[0] // 64, max_ctx)
+    return out[:T, :max_ctx]
+
+
+def topk_select_drafts(logits, k: int, ctx_len, tokens_per_seq: int = 1, n_new: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """topk_select of what fp8_paged_mqa_logits gives for drafts (arguments as there): of every row the k largest of the positions that its draft
+    sees, int32 [B*tokens_per_seq, k], unsorted, -1 in the slots that are left, wherever they are in the list."""
+    i = _index_of(logits, *[t for t in (ctx_len, n_new, tree, out) if t is not None])
+    if logits.dtype is not torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise DsaError("logits must be fp32 [T, S] with unit column stride")
+    T, S = logits.shape
+    B, ctx_len, n_new, tree = _check_drafts(T, tokens_per_seq, ctx_len, n_new, tree)
+    if T > 1 and logits.stride(0) < S:
+        raise DsaError("rows of logits overlap")
+    out = _check_idx_out(out, T, k, logits.device)
+    lib = _lib.load()
+    nbytes = lib.dsa_topk_select_drafts_workspace_bytes(B, tokens_per_seq)
+    ws = _workspace(logits.device, nbytes)
+    with _on(logits.device):
+        check(lib.dsa_topk_select_drafts(logits.data_ptr(), max(logits.stride(0), S), ctx_len.data_ptr(), _ptr(n_new), _ptr(tree), tokens_per_seq, B, S, k,
+                                         out.data_ptr(), ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(i)))
+    return out
+
+
+def _check_window(window: int, first: int) -> tuple:
+    if window < 1 or first < 0:
+        raise DsaError(f"window must be at least 1 and first at least 0, got {window} and {first}")
+    return min(int(window), 0x7fffffff), min(int(first), 0x7fffffff)
+
+
+def window_mla_prefill(q, kv, ks, ke, window: int, first: int, scale: float, out: Optional[torch.Tensor] = None,
+                       workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """MLA over a sliding window and the first tokens.  q [T,H,576] bf16, kv [S,576] bf16; row t is position ke[t]-1 of a sequence that begins
+    at ks[t] (int32 [T], as the indexer's windows; None: 0, and the last T positions of kv) and sees the sequence's first ``first``
+    positions and the last ``window`` up to its own.  Returns bf16 [T,H,512]; zeros where a row sees nothing."""
+    i = _index_of(q, *[t for t in (kv, ks, ke, out, workspace) if t is not None])
+    if q.dtype is not torch.bfloat16 or kv.dtype is not torch.bfloat16:
+        raise DsaError("window_mla_prefill takes bf16 q and kv")
+    if q.dim() != 3 or q.shape[2] != 576 or kv.dim() != 2 or kv.shape[1] != 576:
+        raise DsaError(f"bad shapes q {tuple(q.shape)} kv {tuple(kv.shape)}")
+    window, first = _check_window(window, first)
+    q, kv = q.contiguous(), kv.contiguous()
+    (T, H, _), S = q.shape, kv.shape[0]
+    if ke is None and T > S:
+        raise DsaError(f"{T} rows are no last positions of {S}: give ke")
+    ks, ke = _as_i32(ks, T, "ks"), _as_i32(ke, T, "ke")
+    out = _check_attn_out(out, (T, H, 512), q.device)
+    lib = _lib.load()
+    if workspace is None:
+        workspace = _workspace(q.device, lib.dsa_window_mla_prefill_workspace_bytes(T, H, window, first))
+    else:
+        _check_scratch(workspace)
+    _run(i, lib.dsa_window_mla_prefill, q.data_ptr(), kv.data_ptr(), _ptr(ks), _ptr(ke), out.data_ptr(), T, H, S, window, first, float(scale),
+         workspace.data_ptr(), workspace.numel())
+    return out
+
+
+def window_mla_decode_paged(q, cache, block_table, ctx_len, window: int, first: int, scale: float, tokens_per_seq: int = 1,
+                            n_new: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None,
+                            out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The same over a paged latent cache: q [B*n,H,576] bf16, n = tokens_per_seq query tokens a sequence, the last of its ctx_len[b] (int32 [B])
+    in cache uint8 [num_pages*64, 656 or 416]; one, a chain, or a tree of drafts (n_new, tree: fp8_paged_mqa_logits).  The window goes along
+    a draft's path.  Returns bf16 [B*n,H,512]; zeros in rows without a token."""
+    i = _index_of(q, *[t for t in (cache, block_table, ctx_len, n_new, tree, out, workspace) if t is not None])
+    if q.dtype is not torch.bfloat16 or cache.dtype is not torch.uint8:
+        raise DsaError("window_mla_decode_paged takes bf16 q and a uint8 cache")
+    if q.dim() != 3 or q.shape[2] != 576 or cache.dim() != 2 or cache.shape[1] not in RECORD_BYTES or cache.shape[0] % 64:
+        raise DsaError(f"window_mla_decode_paged takes q [T,H,576] and a cache [num_pages*64, 656 or 416], got {tuple(q.shape)} and {tuple(cache.shape)}")
+    window, first = _check_window(window, first)
+    T, H, _ = q.shape
+    B, ctx_len, n_new, tree = _check_drafts(T, tokens_per_seq, ctx_len, n_new, tree)
+    if max_ctx is None:
+        max_ctx = block_table.shape[-1] * 64
+    block_table = _check_table(block_table, B, max_ctx)
+    q, cache = q.contiguous(), cache.contiguous()
+    out = _check_attn_out(out, (T, H, 512), q.device)
+    lib, width = _lib.load(), cache.shape[1]
+    if workspace is None:
+        workspace = _workspace(q.device, lib.dsa_window_mla_decode_workspace_bytes(width, B, tokens_per_seq, H, window, first, max_ctx))
+    else:
+        _check_scratch(workspace)
+    _run(i, lib.dsa_window_mla_decode_paged, q.data_ptr(), cache.data_ptr(), width, block_table.data_ptr(), block_table.stride(0), ctx_len.data_ptr(),
+         _ptr(n_new), _ptr(tree), tokens_per_seq, out.data_ptr(), B, H, window, first, cache.shape[0] // 64, max_ctx, float(scale), workspace.data_ptr(),
+         workspace.numel())
+    return out
 
 
 class HostIndexerPipeline:
@@ -833,3 +972,23 @@ def compact_pages(block_table, refs, caches, out: Optional[tuple] = None) -> tup
     _run(i, lib.dsa_compact_pages, block_table.data_ptr(), block_table.stride(0), new_table.data_ptr(), new_table.stride(0), P, B, refs.data_ptr(),
          new_refs.data_ptr(), num_pages, packed, count, ws.data_ptr(), nbytes)
     return new_table, new_refs
+
+
+def accept_drafts(block_table, ctx_len, refs, rows, n_new, path, n_keep, caches) -> None:
+    """Row rows[i] keeps, of its last n_new[i] tokens, the drafts path[i, :n_keep[i]] (int32 [n, most], ascending numbers 0..n_new[i]-1): their records move
+    up behind the tokens before them in every cache, ctx_len and the pages follow.  A row that is named before, makes no sense or would
+    write to a page that another sequence holds stays as it is (status 2)."""
+    caches = list(caches)
+    i = _index_of(block_table, ctx_len, refs, rows, n_new, path, n_keep, *caches)
+    B, P, num_pages = _check_pool(block_table, ctx_len, refs)
+    n = _list_i32(rows, "rows")
+    _as_i32(n_new, n, "n_new")
+    _as_i32(n_keep, n, "n_keep")
+    if path.dtype is not torch.int32 or path.dim() != 2 or path.shape[0] != n or not path.is_contiguous():
+        raise DsaError(f"path must be a contiguous int32 [{n}, drafts] tensor, got {path.dtype} {tuple(path.shape)}")
+    packed, count = _page_caches(caches, num_pages)
+    lib = _lib.load()
+    nbytes = lib.dsa_pages_workspace_bytes(0, n)
+    ws = _workspace(refs.device, nbytes)
+    _run(i, lib.dsa_accept_drafts, block_table.data_ptr(), block_table.stride(0), P, B, ctx_len.data_ptr(), refs.data_ptr(), num_pages, rows.data_ptr(),
+         n_new.data_ptr(), path.data_ptr(), path.shape[1], n_keep.data_ptr(), n, packed, count, ws.data_ptr(), nbytes)
