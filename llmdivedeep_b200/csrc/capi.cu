@@ -89,10 +89,12 @@ int indexer_logits_drafts_launch(const void* q, const void* w, int w_is_bf16, co
 int topk_select_drafts_launch(const float* logits, int64_t ld, const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree, int tokens_per_seq, int B,
                               int max_ctx, int k, int32_t* out, int32_t* ends, cudaStream_t stream);
 int window_mla_prefill_launch(const void* q, const void* kv, const int32_t* ks, const int32_t* ke, void* out, int T, int H, int S, int window, int first,
-                              float scale, int32_t* status, cudaStream_t stream);
+                              float scale, void* workspace, size_t workspace_bytes, int32_t* status, cudaStream_t stream);
+size_t window_mla_prefill_workspace(int T, int H, int window, int first);
+size_t window_mla_decode_workspace(int B, int tokens_per_seq, int H, int window, int first, int max_ctx);
 int window_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len,
                              const int32_t* n_new, const int64_t* tree, int tokens_per_seq, void* out, int B, int H, int window, int first, int num_pages,
-                             int max_ctx, float scale, int32_t* status, cudaStream_t stream);
+                             int max_ctx, float scale, void* workspace, size_t workspace_bytes, int32_t* status, cudaStream_t stream);
 int pack_latent_launch(const void* kv, int kv_is_bf16, int64_t row_stride, int64_t n, void* rec, cudaStream_t stream);
 int rope_fp8_quant_launch(const void* x, int64_t n_rows, int head_dim, int rope_dim, int interleave, int rows_per_pos,
                           const float* cos_t, const float* sin_t, void* q, float* scale, const void* gate, float mul0,
@@ -494,7 +496,9 @@ static int check_window(const char* who, int H, int window, int first, float sca
   return DSA_OK;
 }
 
-size_t dsa_window_mla_prefill_workspace_bytes(int T, int H, int window, int first) { return 0; }
+size_t dsa_window_mla_prefill_workspace_bytes(int T, int H, int window, int first) {
+  return T <= 0 || H <= 0 || window < 1 || first < 0 ? 0 : window_mla_prefill_workspace(T, H, window, first);
+}
 
 int dsa_window_mla_prefill(const void* q_bf16, const void* kv_bf16, const int32_t* ks, const int32_t* ke, void* out_bf16, int T, int H, int S, int window,
                            int first, float scale, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
@@ -508,10 +512,13 @@ int dsa_window_mla_prefill(const void* q_bf16, const void* kv_bf16, const int32_
   if ((int64_t)T * H > 0x7fffffffLL) return set_error(DSA_ERR_SHAPE, "window_mla_prefill: T*H exceeds 2^31");
   if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15))
     return set_error(DSA_ERR_WORKSPACE, "window_mla_prefill: workspace must be 16-byte aligned");
-  return window_mla_prefill_launch(q_bf16, kv_bf16, ks, ke, out_bf16, T, H, S, window, first, scale, status, static_cast<cudaStream_t>(stream));
+  return window_mla_prefill_launch(q_bf16, kv_bf16, ks, ke, out_bf16, T, H, S, window, first, scale, workspace, workspace_bytes, status,
+                                   static_cast<cudaStream_t>(stream));
 }
 
-size_t dsa_window_mla_decode_workspace_bytes(int record_bytes, int B, int tokens_per_seq, int H, int window, int first, int max_ctx) { return 0; }
+size_t dsa_window_mla_decode_workspace_bytes(int record_bytes, int B, int tokens_per_seq, int H, int window, int first, int max_ctx) {
+  return B <= 0 || tokens_per_seq < 1 || H <= 0 || window < 1 || first < 0 || max_ctx <= 0 ? 0 : window_mla_decode_workspace(B, tokens_per_seq, H, window, first, max_ctx);
+}
 
 int dsa_window_mla_decode_paged(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,
                                 const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree, int tokens_per_seq, void* out_bf16, int B, int H,
@@ -531,7 +538,7 @@ int dsa_window_mla_decode_paged(const void* q_bf16, const void* cache, int recor
   if ((int64_t)num_pages * 64 > 0x7fffffffLL || (int64_t)B * tokens_per_seq * H > 0x7fffffffLL) return set_error(DSA_ERR_SHAPE, "%s: problem too large", who);
   if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15)) return set_error(DSA_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", who);
   return window_mla_decode_launch(q_bf16, cache, record_bytes, block_table, table_stride, ctx_len, n_new, tree, tokens_per_seq, out_bf16, B, H, window, first,
-                                  num_pages, max_ctx, scale, status, static_cast<cudaStream_t>(stream));
+                                  num_pages, max_ctx, scale, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
 int dsa_indexer_logits_drafts(const void* q_fp8, const void* w, int w_dtype, const void* kcache, const float* kscale, const int32_t* block_table,
