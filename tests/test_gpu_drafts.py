@@ -93,6 +93,19 @@ def test_logits_of_ragged_drafts(per, w_dtype):
     check_logits(got, c.want(), c.ctx, per)
 
 
+@pytest.mark.parametrize("H", [64, 32, 16])
+@pytest.mark.parametrize("per", [1, 2, 3, 5, 8])
+def test_logits_of_a_draft_are_those_of_a_decode_step(H, per):
+    """Bit for bit: drafts that are checked together and tokens that are made one by one select the same keys."""
+    c = Case(3, per, H, [500, 33, 640], seed=per)
+    got = c.logits(n_new=i32([per] * 3))
+    for i in range(per):
+        ctx = [x - per + i + 1 for x in c.ctx]
+        one = ops.fp8_paged_mqa_logits(c.q8[i::per], c.w[i::per], c.k8, c.ksc, c.table, i32(ctx), c.max_ctx)
+        for b in range(3):
+            assert torch.equal(got[b * per + i, :ctx[b]], one[b, :ctx[b]])
+
+
 def test_logits_bad_lengths_and_pages():
     c = Case(5, 3, 64, [200] * 5, seed=4, n_new=[3, 4, -1, 3, 3])
     ctx = i32([200, 200, 200, 2, 201])
