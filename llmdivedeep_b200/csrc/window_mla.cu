@@ -1,259 +1,61 @@
 // MLA attention over a sliding window and the first tokens (MQA over the shared 576-dim latent KV, 512-dim V): a query row at position p of its
 // sequence sees the positions < first and the last `window` ones, p itself included,
 //   o[r, :] = sum_s softmax_s(scale * q[r, :] . kv[s, :]) * kv[s, :512],   s < first or p - window < s <= p,
-// over bf16 rows (prompts) or the records of the paged latent caches (decode, one or several query tokens a sequence: a chain, or a tree of
-// drafts, drafts.cuh).
+// here over the records of the paged latent caches: decode, one or several query tokens a sequence, a chain or a tree of drafts (drafts.cuh).  Prompts:
+// window_prompt.cu.
 #include <cuda.h>
 #include <cudaTypedefs.h>
-#include <math_constants.h>
 
-#include "dsa_common.cuh"
-#include "dsa_host.h"
-#include "drafts.cuh"
-#include "mla_pair.cuh"
+#include "window_mla.cuh"
 
 namespace dsa {
 
-struct WinArgs {
-  const __nv_bfloat16* q;         // [T, H, 576]
-  const uint8_t* kv;              // prompts: [S, 576] bf16 rows; decode: [num_phys_rows] records
-  const int32_t *ks, *ke;         // prompts: [T] rows' windows; null: 0, and the last T positions of S
-  const int32_t* block_table;     // decode: [B, table_stride]
-  int64_t table_stride;
-  DraftArgs drafts;               // decode
-  __nv_bfloat16* out;             // [T, H, 512]
-  int T, H, S;                    // S: prompts, rows of kv
-  int window, first;
-  int num_phys_rows;
-  float scale_log2e;
-  int* status;
-  int seq_rows, seq_units;        // query rows (token, head) of a sequence, and its units of 128 of them; prompts: all rows are one sequence's
-  int n_full;                     // the first n_full units are a CTA pair each; ...
-  int n_split;                    // ... the keys of every later one are cut into n_split parts, a pair each
-  float* part_o;                  // [parts, 128, 512] fp32 normalised partial outputs
-  float* part_lse;                // [parts, 2, 128] their log2-sum-exp as each CTA of the pair has it (-inf: nothing seen)
-  int tma_out;                    // the output tensor map is valid: full units leave through TMA stores
-};
-
-// What a row sees: two stretches of positions, a1 <= b0, and single ones behind `at`.
-struct Sees {
-  int a0, a1, b0, b1, at;
-  uint64_t bits;
-};
-__device__ __forceinline__ Sees sees_prompt(const WinArgs& a, int t) {
-  const int ks = a.ks ? max(__ldg(a.ks + t), 0) : 0, ke = a.ke ? min(__ldg(a.ke + t), a.S) : a.S - a.T + t + 1;
-  Sees s{};
-  if (ke <= ks) return s;
-  s.a0 = ks;
-  s.a1 = a.first < ke - ks ? ks + a.first : ke;
-  s.b0 = max(s.a1, ke - a.window);
-  s.b1 = ke;
-  return s;
-}
-__device__ __forceinline__ Sees sees_draft(const WinArgs& a, const Drafts& dr, int b, int i) {
-  Sees s{};
-  if (i >= dr.m) return s;
-  const int P = dr.ctx - dr.m;
-  s.at = P;
-  if (!a.drafts.tree) {
-    const int ke = P + i + 1;
-    s.a1 = min(a.first, ke);
-    s.b0 = max(s.a1, ke - a.window);
-    s.b1 = ke;
-    return s;
-  }
-  s.bits = draft_mask(a.drafts, b, i);
-  const int n = __popcll(s.bits);
-  s.a1 = min(a.first, P);
-  s.b0 = max(s.a1, P + n - a.window);                  // its own position is P + n - 1
-  s.b1 = max(s.b0, P);
-  uint64_t left = s.bits;
-  for (int k = 0; k < n - a.window; ++k) {             // drafts of its path that the window has passed
-    const uint64_t lowest = left & (0 - left);
-    left ^= lowest;
-    if (P + k >= a.first) s.bits ^= lowest;
-  }
-  return s;
-}
-
-// A lane's share of a row: values 8 lane .. of either half of the latent, rope values 2 lane ..
-struct RowShare {
-  float x[2][8], r[2];
-};
-template <int SRC>
-__device__ __forceinline__ RowShare load_share(const uint8_t* __restrict__ row, int lane) {
-  RowShare v;
-  uint32_t rope;
-  if constexpr (SRC == kSrcRows) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + h * 512 + lane * 16));
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v.x[h][i] = __uint_as_float(i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
-    }
-    rope = __ldg(reinterpret_cast<const uint32_t*>(row + 1024) + lane);
-  } else if constexpr (SRC == kSrcFp8) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + h * 256 + lane * 8));
-      const uint4 b = e4m3x8_to_bf16(w, __ldg(reinterpret_cast<const float*>(row + 512) + h * 2 + (lane >> 4)));
-      const uint32_t u[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v.x[h][i] = __uint_as_float(i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
-    }
-    rope = __ldg(reinterpret_cast<const uint32_t*>(row + 528) + lane);
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t* half = row + h * kLatent4Half;
-      uint32_t u[4];
-      latent4_codes(__ldg(reinterpret_cast<const uint32_t*>(half) + lane), u);
-      const uint32_t sc = latent4_scale(__ldg(half + kLatent4Scales + (lane >> 1)));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t p = mul_bf16x2(u[i], sc);
-        v.x[h][2 * i] = __uint_as_float(p << 16) * kLatent4Gain;
-        v.x[h][2 * i + 1] = __uint_as_float(p & 0xffff0000u) * kLatent4Gain;
-      }
-    }
-    rope = __ldg(reinterpret_cast<const uint32_t*>(row + (lane >> 4) * kLatent4Half + kLatent4Rope) + (lane & 15));
-  }
-  v.r[0] = __uint_as_float(rope << 16);
-  v.r[1] = __uint_as_float(rope & 0xffff0000u);
-  return v;
-}
-
-// The score of a row and a key, times log2(e): every lane has it.
-__device__ __forceinline__ float row_score(const RowShare& q, const RowShare& k, float scale_log2e) {
-  float d = q.r[0] * k.r[0] + q.r[1] * k.r[1];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) d += q.x[0][i] * k.x[0][i] + q.x[1][i] * k.x[1][i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-  return d * scale_log2e;
-}
-
 // ---- the pair kernel ---------------------------------------------------------------------------------------------------
-constexpr int kWinSegs = 256;                          // stretches of keys of a unit: two for each of at most 128 sequences in it
-constexpr int kWinMaxParts = 16;
-constexpr int kWinTmaWarp = 17, kWinFixWarp = 18;      // prompts: loads, and rows behind the end of a stretch
 template <int SRC>
 struct WinCfg {
-  static constexpr bool kPaged = SRC != kSrcRows;
-  static constexpr int kThreads = kPaged ? kMlaThreads : 640, kLaunchRegs = kPaged ? 72 : 96;
-  static constexpr int kRegsSoftmax = kPaged ? 88 : 104, kRegsOther = kPaged ? 48 : 56;
-  static_assert(512 * kRegsSoftmax + (kThreads - 512) * kRegsOther <= kThreads * kLaunchRegs, "more registers than the launch has");
-  static constexpr int kBufs = kPaged ? kMlaBufs - 1 : kMlaBufs;      // decode: the fifth one's space holds raw rows
+  static constexpr int kBufs = kMlaBufs - 1;           // the fifth one's space holds raw rows
   static constexpr int kOffBars = kMlaBufs * kMlaKBytes + 2 * kMlaXBytes;
   static constexpr int kOffValid = kOffBars + 640;
   static constexpr int kOffPm = kOffValid + kMlaValidRing * kMlaBlk;
   static constexpr int kOffSees = kOffPm + kMlaPairBytes;             // int4 a row
-  static constexpr int kOffMore = kOffSees + 128 * 16;                // 8 bytes a row: the drafts it sees, or its token's number in the unit
-  static constexpr int kOffSegs = kOffMore + 128 * 8;
-  static constexpr int kOffRaw = kOffSegs + (kPaged ? 0 : (kWinSegs + 1) * 16);
-  static constexpr int kSmem = kOffRaw + (kPaged ? (MlaRaw<SRC>::kPieces - MlaRaw<SRC>::kInBuf) * MlaRaw<SRC>::kBytes : 0);
+  static constexpr int kOffMore = kOffSees + 128 * 16;                // 8 bytes a row: the drafts it sees
+  static constexpr int kOffRaw = kOffMore + 128 * 8;
+  static constexpr int kSmem = kOffRaw + (MlaRaw<SRC>::kPieces - MlaRaw<SRC>::kInBuf) * MlaRaw<SRC>::kBytes;
   static_assert(kSmem <= 232448 && kOffRaw % 16 == 0, "shared memory budget of one CTA");
 };
 
-__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u; }
-// which of the 32 keys from k0 on are in [lo, hi)
-__device__ __forceinline__ uint32_t range_bits(int lo, int hi, int k0) { return low_bits(hi - k0) & ~low_bits(lo - k0); }
 // which of the 32 keys from k0 on have their bit set, bit j at `at` + j
 __device__ __forceinline__ uint32_t draft_bits(uint64_t bits, int at, int k0) {
   const int sh = k0 - at;
   return sh >= 64 || sh <= -32 ? 0u : sh >= 0 ? static_cast<uint32_t>(bits >> sh) : static_cast<uint32_t>(bits) << -sh;
 }
 
-// Prompts: the keys of a unit, as stretches of at most one sequence each, written by one warp.  Neighbouring rows of a sequence whose windows
-// touch share two: its first keys and those of their windows.  {first key, end, blocks before, tokens of the unit that it is for}
-struct UnitWords {
-  int segs, blocks;
-  int full0, full1;                                    // keys that every row sees which sees any (one sequence in the unit)
-};
-__device__ __forceinline__ void build_segs(const WinArgs& a, int t0, int n_tok, int4* segs, UnitWords* out) {
-  const int lane = threadIdx.x & 31;
-  int n = 0, blocks = 0, runs = 0;
-  int rk = 0, ra = 0, rlo = 0, rhi = 0, r0 = 0, r1 = -1;             // the run that is open (r1 >= r0)
-  int full0 = 0, full1 = 0x7fffffff, heads = 0x7fffffff;
-  auto put = [&](int lo, int hi) {
-    if (lo >= hi) return;
-    if (lane == 0) segs[n] = make_int4(lo, hi, blocks, r0 | r1 << 16);
-    ++n;
-    blocks += (hi - lo + kMlaBlk - 1) / kMlaBlk;
-  };
-  auto close = [&]() {
-    if (r1 < r0) return;
-    ++runs;
-    if (rlo <= ra) {
-      put(rk, rhi);
-    } else {
-      put(rk, ra);
-      put(rlo, rhi);
-    }
-  };
-  for (int base = 0; base < n_tok; base += 32) {
-    const Sees mine = base + lane < n_tok ? sees_prompt(a, t0 + base + lane) : Sees{};
-    for (int j = 0; j < min(32, n_tok - base); ++j) {
-      const int k = __shfl_sync(0xffffffffu, mine.a0, j), a1 = __shfl_sync(0xffffffffu, mine.a1, j), lo = __shfl_sync(0xffffffffu, mine.b0, j),
-                hi = __shfl_sync(0xffffffffu, mine.b1, j);
-      if (hi <= k) continue;                           // sees nothing
-      full0 = max(full0, lo);
-      full1 = min(full1, hi);
-      heads = min(heads, a1);
-      if (r1 >= r0 && k == rk && lo <= rhi && hi >= rlo) {
-        ra = max(ra, a1);
-        rlo = min(rlo, lo);
-        rhi = max(rhi, hi);
-      } else {
-        close();
-        r0 = base + j;
-        rk = k; ra = a1; rlo = lo; rhi = hi;
-      }
-      r1 = base + j;
-    }
-  }
-  close();
-  if (lane == 0) {
-    segs[n] = make_int4(0, 0, 0x7fffffff, 0);
-    out->segs = n;
-    out->blocks = blocks;
-    out->full0 = runs != 1 ? 0x7fffffff : full0 <= heads ? rk : full0;
-    out->full1 = full1;
-  }
-}
-
 template <int SRC>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WinCfg<SRC>::kThreads, 1)
-window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ CUtensorMap tmap_lat,
-                  const __grid_constant__ CUtensorMap tmap_rope, const WinArgs a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMlaThreads, 1)
+window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o, const WinArgs a) {
   using C = WinCfg<SRC>;
-  constexpr bool PAGED = C::kPaged;
   constexpr int NB = C::kBufs;
   extern __shared__ __align__(1024) uint8_t smem[];            // the swizzled panels need 1024-byte alignment
   uint8_t* kv_s = smem;                                        // five buffers: four panels [64 keys x 128 B] and 64 x 64 B
   uint8_t* send_s = kv_s + kMlaBufs * kMlaKBytes;              // this CTA's partial score tile on its way out
   uint8_t* recv_s = send_s + kMlaXBytes;                       // the peer's
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBars);      // as in sparse_mla.cu, and fix_done
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBars);      // as in sparse_mla.cu
   uint64_t *q_full = bars + 0, *q_moved = bars + 1, *o_final = bars + 2, *s_free = bars + 3, *p_full = bars + 4, *s_full = bars + 5, *pv_done = bars + 7,
            *pm_full = bars + 9, *recv_full = bars + 17, *xchg_free = bars + 33, *kv_full = bars + 49, *kv_free = bars + 54;
-  uint64_t* fix_done = bars + 59;                              // [5] prompts: the rows behind the end of the block's stretch are zeros
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 64);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* odd_s = abort_flag + 1;                        // [4 quadrants] a row must be done key by key
-  UnitWords* words = reinterpret_cast<UnitWords*>(tmem_slot + 8);
   uint8_t* valid_s = smem + C::kOffValid;                      // decode: [kMlaValidRing][64] 1 = the slot of the block has a page
   uint16_t* pm_s = reinterpret_cast<uint16_t*>(smem + C::kOffPm);        // block maxima, rounded up to bf16
   int4* sees_s = reinterpret_cast<int4*>(smem + C::kOffSees);
   uint64_t* more_s = reinterpret_cast<uint64_t*>(smem + C::kOffMore);
-  int4* segs_s = reinterpret_cast<int4*>(smem + C::kOffSegs);
 
   const int cta = blockIdx.x & 1, peer = cta ^ 1;              // rank in the cluster = V half = contraction part
   const int job = blockIdx.x >> 1;
   const int part = job < a.n_full ? -1 : job - a.n_full;       // >= 0: a part of a unit's keys
   const int n_split = part < 0 ? 1 : a.n_split, unit = part < 0 ? job : a.n_full + part / n_split, split = part < 0 ? 0 : part % n_split;
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int seq = PAGED ? unit / a.seq_units : 0;
+  const int seq = unit / a.seq_units;
   const int row0 = (unit - seq * a.seq_units) * 128;           // of the sequence's query rows
   const int rows_here = min(128, a.seq_rows - row0);
   const int64_t g0 = (int64_t)seq * a.seq_rows + row0;
@@ -266,12 +68,12 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 
   // ---- set-up ----------------------------------------------------------------------------------------------------------
   if (warp == 0) {
-    for (int i = lane; i < 64; i += 32) {
+    for (int i = lane; i < 59; i += 32) {
       const uint32_t count = i == 1 ? 16u                                            // q_moved: lane 0 of the softmax warps
                              : (i == 3 || i == 4) ? 2u * n_quad                      // s_free, p_full: lane 0 of a set's warps
                              : (i >= 9 && i <= 16) ? 2u                              // pm_full: the two warps of a quadrant
-                             : (i >= 49 && i <= 53 && PAGED) ? uint32_t(kMlaGatherWarps)
-                                                             : 1u;                   // the others
+                             : (i >= 49 && i <= 53) ? uint32_t(kMlaGatherWarps)
+                                                    : 1u;                   // the others
       mbar_init(bars + i, count);
     }
     mbar_fence_init();
@@ -286,9 +88,9 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     tmem_alloc(tmem_slot, kMlaTmemCols);
     tmem_relinquish();
   }
-  // Decode: keys by slots, the first tokens' [0, head) and behind them the windows' [shift + head, ...): slot j is position j or j + shift.
+  // Keys by slots, the first tokens' [0, head) and behind them the windows' [shift + head, ...): slot j is position j or j + shift.
   int head = 0, shift = 0, n_slots = 0, full0 = 0, full1 = 0;
-  if constexpr (PAGED) {
+  {
     const Drafts dr = drafts_of(a.drafts, seq);
     if (dr.bad && threadIdx.x == 0 && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
     const int P = dr.ctx - dr.m, last = min(tok1, dr.m - 1);
@@ -310,29 +112,15 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       sees_s[r] = make_int4(a1, s.b0 - shift, s.b1 - shift, s.at - shift);
       more_s[r] = s.bits;
     }
-  } else {
-    const int r = threadIdx.x - 32;
-    if (r >= 0 && r < 128) {
-      const int t = r < rows_here ? (row0 + r) / a.H : tok0;
-      const Sees s = r < rows_here ? sees_prompt(a, t) : Sees{};
-      sees_s[r] = make_int4(s.a0, s.a1, s.b0, s.b1);
-      more_s[r] = t - tok0;
-    }
-    if (warp == 5) build_segs(a, tok0, tok1 - tok0 + 1, segs_s, words);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  int blocks = (n_slots + kMlaBlk - 1) / kMlaBlk;
-  if constexpr (!PAGED) {
-    blocks = words->blocks;
-    full0 = words->full0;
-    full1 = words->full1;
-  }
+  const int blocks = (n_slots + kMlaBlk - 1) / kMlaBlk;
   const int per = (blocks + n_split - 1) / n_split, blk_lo = min(blocks, split * per), nblk = min(blocks, blk_lo + per) - blk_lo;
   if (nblk == 0) {   // nothing seen: zeros (a part: weight zero in the combine); no cluster traffic yet
     if (part < 0) {
-      for (int e = threadIdx.x; e < rows_here * 32; e += C::kThreads)
+      for (int e = threadIdx.x; e < rows_here * 32; e += kMlaThreads)
         reinterpret_cast<uint4*>(a.out + (g0 + (e >> 5)) * kMlaDv + cta * kMlaDvHalf)[e & 31] = make_uint4(0, 0, 0, 0);
     } else if (threadIdx.x < 128) {
       a.part_lse[((int64_t)part * 2 + cta) * 128 + threadIdx.x] = -CUDART_INF_F;
@@ -347,16 +135,8 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   cluster_arrive();
   bool left = false;                                           // this warp has arrived at the barrier that the pair leaves through
 
-  // prompts: the stretch of block g, looked for from the one before on
-  int seg_at = 0;
-  auto seg_of = [&](int g) -> int4 {
-    while (g >= segs_s[seg_at + 1].z) ++seg_at;
-    return segs_s[seg_at];
-  };
-  auto rows_of = [&](int4 s, int g) { return min(kMlaBlk, s.y - s.x - (g - s.z) * kMlaBlk); };      // of block g
-
-  if (warp >= kMlaSoftmaxWarps) regs_dec<C::kRegsOther>();
-  else regs_inc<C::kRegsSoftmax>();
+  if (warp >= kMlaSoftmaxWarps) regs_dec<MlaRegs<true>::kOther>();
+  else regs_inc<MlaRegs<true>::kSoftmax>();
   if (warp == kMlaMmaWarp) {
     // ------------------------------- MMA issuer: as in sparse_mla.cu -------------------------------
     constexpr uint32_t idesc_qk = umma_idesc(1, 1, 0, 0, 128, kMlaBlk);
@@ -370,12 +150,9 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (n < nblk) {
         const int buf = n % NB;
         ok = mla_wait(&kv_full[buf], (n / NB) & 1, abort_flag, a.status);
-        if constexpr (!PAGED) {
-          if (ok) ok = mla_wait(&fix_done[buf], (n / NB) & 1, abort_flag, a.status);
-        }
         if (ok && n > 0) ok = mla_wait(s_free, (n - 1) & 1, abort_flag, a.status);
         if (!ok) break;
-        if constexpr (PAGED) fence_async_smem();       // the rows were written by st, the tensor core reads through the async proxy
+        fence_async_smem();       // the rows were written by st, the tensor core reads through the async proxy
         tc_fence_after();
         if (elect_one()) {
           const uint64_t kd0 = kdesc0 + uint64_t(buf) * (kMlaKBytes >> 4);
@@ -409,157 +186,117 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       }
     }
   } else if (warp > kMlaMmaWarp) {
-    if constexpr (!PAGED) {
-      if (warp == kWinTmaWarp) {
-        // ---- prompts: 64 rows of a stretch a block, this CTA's half of the latent and of the rope panel ----
-        bool ok = true;
-        for (int i = 0, buf = 0; i < nblk; ++i) {
-          const int4 s = seg_of(blk_lo + i);
-          const int key0 = s.x + (blk_lo + i - s.z) * kMlaBlk;
-          if (i == kQBuf0) ok = mla_wait(q_moved, 0, abort_flag, a.status);   // from here on the buffers held Q
-          if (i >= NB) ok = mla_wait(&kv_free[buf], ((i / NB) - 1) & 1, abort_flag, a.status);
-          if (!ok) break;
-          uint8_t* dst = kv_s + buf * kMlaKBytes;
-          if (lane == 0) mbar_expect_tx(&kv_full[buf], kMlaKBytes);
-          __syncwarp();
-          if (lane < 4) tma_load_2d(dst + lane * kMlaKPanelBytes, &tmap_lat, (cta * 4 + lane) * 32, key0, &kv_full[buf]);      // x in 4-byte units
-          else if (lane == 4) tma_load_2d(dst + kMlaRopeOff, &tmap_rope, kMlaDv / 2 + cta * 16, key0, &kv_full[buf]);
-          __syncwarp();
-          if (++buf == NB) buf = 0;
+    // ---- decode: the records of 64 slots a block, each warp every eleventh: raw into shared memory two blocks ahead (cp.async), then to bf16 ----
+    constexpr int kG = kMlaGatherWarps, kRows = kRawRows, kRawRow = MlaRaw<SRC>::kRow, kRawBytes = MlaRaw<SRC>::kBytes, kRawInBuf = MlaRaw<SRC>::kInBuf;
+    constexpr int kBytes = SRC == kSrc4 ? kLatent4Bytes : kLatentTokenBytes;
+    const int w4 = warp - kMlaGatherWarp0;
+    const int slot = lane < kRows ? w4 + lane * kG : kMlaBlk;      // lane j < 6 looks after slot w4 + 11 j
+    const int32_t* table = a.block_table + (int64_t)seq * a.table_stride;
+    auto position = [&](int i) -> int {
+      const int j = (blk_lo + i) * kMlaBlk + slot;
+      return slot < kMlaBlk && i < nblk && j < n_slots ? (j < head ? j : j + shift) : -1;
+    };
+    auto table_entry = [&](int pos) -> int { return pos >= 0 ? __ldg(table + pos / kLatentPage) : -1; };
+    auto cache_row = [&](int pos, int page) -> int {   // -1 = no slot, or a page that is none: flagged
+      if (pos < 0) return -1;
+      if (page >= 0 && (int64_t)(page + 1) * kLatentPage <= a.num_phys_rows) return page * kLatentPage + pos % kLatentPage;
+      if (a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+      return -1;
+    };
+    auto mark = [&](int i, bool used) {
+      if (slot < kMlaBlk) valid_s[(i % kMlaValidRing) * kMlaBlk + slot] = used;
+    };
+    auto stage_of = [&](int i) -> uint8_t* {         // the fifth KV buffer, and what does not fit there behind everything else
+      const int c = (i & 1) * kG + w4;
+      return c < kRawInBuf ? kv_s + NB * kMlaKBytes + c * kRawBytes : smem + C::kOffRaw + (c - kRawInBuf) * kRawBytes;
+    };
+    auto fetch = [&](int i, int id) {                // an empty slot is zero-filled, values and scales
+      uint8_t* st = stage_of(i);
+      if constexpr (SRC == kSrc4) {
+#pragma unroll
+        for (int u = 0; u < (kRows * 13 + 31) / 32; ++u) {         // 208 bytes a row: thirteen pieces
+          const int c = u * 32 + lane, j = c / 13, rid = __shfl_sync(0xffffffffu, id, min(j, kRows - 1));
+          if (c < kRows * 13)
+            cp_async_16(st + c * 16, a.kv + (int64_t)max(rid, 0) * kBytes + cta * kLatent4Half + (c - j * 13) * 16, rid >= 0 ? 16 : 0);
         }
-      } else if (warp == kWinFixWarp) {
-        // ---- rows behind the end of a stretch: zeros, whatever they are (P is 0 there, and 0 x NaN is none) ----
-        bool ok = true;
-        for (int i = 0, buf = 0; i < nblk; ++i) {
-          const int n = rows_of(seg_of(blk_lo + i), blk_lo + i);
-          ok = mla_wait(&kv_full[buf], (i / NB) & 1, abort_flag, a.status);
-          if (!ok) break;
-          if (n < kMlaBlk) {
-            uint8_t* dst = kv_s + buf * kMlaKBytes;
-            for (int r = n; r < kMlaBlk; ++r) {
-              *reinterpret_cast<uint4*>(dst + (lane >> 3) * kMlaKPanelBytes + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-              if (lane < 4) *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + lane * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_async_smem();
-            __syncwarp();
-          }
-          if (lane == 0) mbar_arrive(&fix_done[buf]);  // of every block: a warp that skipped some would wait for a parity that may be two phases old
-          if (++buf == NB) buf = 0;
+      } else {
+#pragma unroll
+        for (int u = 0; u < kRows / 2; ++u) {        // two rows of 256 values per instruction
+          const int j = 2 * u + (lane >> 4), rid = __shfl_sync(0xffffffffu, id, j);
+          cp_async_16(st + j * kRawRow + (lane & 15) * 16, a.kv + cta * kMlaDvHalf + (lane & 15) * 16 + (int64_t)max(rid, 0) * kBytes, rid >= 0 ? 16 : 0);
         }
+        const int rid = __shfl_sync(0xffffffffu, id, lane >> 2);
+        if (lane < kRows) cp_async_16(st + lane * kRawRow + 256, a.kv + kMlaDv + (int64_t)max(id, 0) * kBytes, id >= 0 ? 16 : 0);      // a row's four scales
+        if (lane < 4 * kRows)                        // this CTA's two K-steps of the rope panel: 64 bytes per row
+          cp_async_16(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16, a.kv + kMlaDv + 16 + cta * 64 + (lane & 3) * 16 + (int64_t)max(rid, 0) * kBytes, rid >= 0 ? 16 : 0);
       }
-    } else {
-      // ---- decode: the records of 64 slots a block, each warp every eleventh: raw into shared memory two blocks ahead (cp.async), then to bf16 ----
-      constexpr int kG = kMlaGatherWarps, kRows = kRawRows, kRawRow = MlaRaw<SRC>::kRow, kRawBytes = MlaRaw<SRC>::kBytes, kRawInBuf = MlaRaw<SRC>::kInBuf;
-      constexpr int kBytes = SRC == kSrc4 ? kLatent4Bytes : kLatentTokenBytes;
-      const int w4 = warp - kMlaGatherWarp0;
-      const int slot = lane < kRows ? w4 + lane * kG : kMlaBlk;      // lane j < 6 looks after slot w4 + 11 j
-      const int32_t* table = a.block_table + (int64_t)seq * a.table_stride;
-      auto position = [&](int i) -> int {
-        const int j = (blk_lo + i) * kMlaBlk + slot;
-        return slot < kMlaBlk && i < nblk && j < n_slots ? (j < head ? j : j + shift) : -1;
-      };
-      auto table_entry = [&](int pos) -> int { return pos >= 0 ? __ldg(table + pos / kLatentPage) : -1; };
-      auto cache_row = [&](int pos, int page) -> int {   // -1 = no slot, or a page that is none: flagged
-        if (pos < 0) return -1;
-        if (page >= 0 && (int64_t)(page + 1) * kLatentPage <= a.num_phys_rows) return page * kLatentPage + pos % kLatentPage;
-        if (a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
-        return -1;
-      };
-      auto mark = [&](int i, bool used) {
-        if (slot < kMlaBlk) valid_s[(i % kMlaValidRing) * kMlaBlk + slot] = used;
-      };
-      auto stage_of = [&](int i) -> uint8_t* {         // the fifth KV buffer, and what does not fit there behind everything else
-        const int c = (i & 1) * kG + w4;
-        return c < kRawInBuf ? kv_s + NB * kMlaKBytes + c * kRawBytes : smem + C::kOffRaw + (c - kRawInBuf) * kRawBytes;
-      };
-      auto fetch = [&](int i, int id) {                // an empty slot is zero-filled, values and scales
-        uint8_t* st = stage_of(i);
-        if constexpr (SRC == kSrc4) {
-#pragma unroll
-          for (int u = 0; u < (kRows * 13 + 31) / 32; ++u) {         // 208 bytes a row: thirteen pieces
-            const int c = u * 32 + lane, j = c / 13, rid = __shfl_sync(0xffffffffu, id, min(j, kRows - 1));
-            if (c < kRows * 13)
-              cp_async_16(st + c * 16, a.kv + (int64_t)max(rid, 0) * kBytes + cta * kLatent4Half + (c - j * 13) * 16, rid >= 0 ? 16 : 0);
-          }
-        } else {
-#pragma unroll
-          for (int u = 0; u < kRows / 2; ++u) {        // two rows of 256 values per instruction
-            const int j = 2 * u + (lane >> 4), rid = __shfl_sync(0xffffffffu, id, j);
-            cp_async_16(st + j * kRawRow + (lane & 15) * 16, a.kv + cta * kMlaDvHalf + (lane & 15) * 16 + (int64_t)max(rid, 0) * kBytes, rid >= 0 ? 16 : 0);
-          }
-          const int rid = __shfl_sync(0xffffffffu, id, lane >> 2);
-          if (lane < kRows) cp_async_16(st + lane * kRawRow + 256, a.kv + kMlaDv + (int64_t)max(id, 0) * kBytes, id >= 0 ? 16 : 0);      // a row's four scales
-          if (lane < 4 * kRows)                        // this CTA's two K-steps of the rope panel: 64 bytes per row
-            cp_async_16(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16, a.kv + kMlaDv + 16 + cta * 64 + (lane & 3) * 16 + (int64_t)max(rid, 0) * kBytes, rid >= 0 ? 16 : 0);
-        }
-        cp_async_commit();
-      };
-      bool ok = true;
-      int id_cur, id_nxt, pa, ta;                      // row ids of blocks i and i+1, position and page of i+2
-      {
-        const int p0 = position(0), p1 = position(1), t0 = table_entry(p0), t1 = table_entry(p1);
-        pa = position(2);
-        ta = table_entry(pa);
-        id_cur = cache_row(p0, t0);
-        fetch(0, id_cur);
-        id_nxt = cache_row(p1, t1);
-        fetch(1, id_nxt);
-      }
-      const int l16 = (lane & 3) | ((lane >> 3) << 2);         // 4 bits: sixteen lanes a row, two rows at a time (sparse_mla.cu)
-      for (int i = 0, buf = 0; i < nblk; ++i) {
-        const int id2 = cache_row(pa, ta);             // block i+2
-        pa = position(i + 3);
-        ta = table_entry(pa);
-        if (i == kQBuf0) ok = mla_wait(q_moved, 0, abort_flag, a.status);   // from here on the buffers held Q
-        if (i >= NB) ok = mla_wait(&kv_free[buf], ((i / NB) - 1) & 1, abort_flag, a.status);
-        if (!ok) break;
-        mark(i, id_cur >= 0);
-        id_cur = id_nxt;
-        id_nxt = id2;
-        cp_async_wait<1>();                            // this lane's copies of block i have landed (block i+1 may be in flight) ...
-        __syncwarp();                                  // ... and the other lanes'
-        const uint8_t* st = stage_of(i);
-        uint8_t* dst = kv_s + buf * kMlaKBytes;
-        if constexpr (SRC == kSrc4) {
-#pragma unroll
-          for (int u = 0; u < kRows / 2; ++u) {
-            const int j = 2 * u + ((lane >> 2) & 1), r = w4 + j * kG;
-            const uint2 w = *reinterpret_cast<const uint2*>(st + j * kRawRow + l16 * 8);
-            const uint32_t sc = latent4_scale(st[j * kRawRow + kLatent4Scales + l16]);
-            uint8_t* row = dst + (l16 >> 2) * kMlaKPanelBytes + r * 128;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              uint32_t p[4];
-              latent4_codes(x == 0 ? w.x : w.y, p);
-              const uint4 v = make_uint4(mul_bf16x2(p[0], sc), mul_bf16x2(p[1], sc), mul_bf16x2(p[2], sc), mul_bf16x2(p[3], sc));
-              if (r < kMlaBlk) *reinterpret_cast<uint4*>(row + ((((2 * l16 + x) ^ r) & 7) << 4)) = v;
-            }
-          }
-        } else {
-          uint8_t* dst_lat = dst + (lane >> 3) * kMlaKPanelBytes;
-#pragma unroll
-          for (int j = 0; j < kRows; ++j) {
-            const int r = w4 + j * kG;
-            const uint2 raw = *reinterpret_cast<const uint2*>(st + j * kRawRow + lane * 8);
-            const float sc = *reinterpret_cast<const float*>(st + j * kRawRow + 256 + cta * 8 + (lane >> 4) * 4);
-            const uint4 v = e4m3x8_to_bf16(raw, sc);
-            if (r < kMlaBlk) *reinterpret_cast<uint4*>(dst_lat + r * 128 + (((lane ^ r) & 7) << 4)) = v;
-          }
-        }
-        {
-          constexpr int kRope = SRC == kSrc4 ? kLatent4Rope : 272;
-          const int r = w4 + (lane >> 2) * kG;
-          if (lane < 4 * kRows && r < kMlaBlk)
-            *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane ^ (r >> 1)) & 3) << 4)) =
-                *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + kRope + (lane & 3) * 16);
-        }
-        __syncwarp();                                  // (the MMA warp makes the writes visible to the tensor core's reads)
-        if (lane == 0) mbar_arrive(&kv_full[buf]);
-        fetch(i + 2, id2);                             // into the stage just read: what was loaded from it has been stored
-        if (++buf == NB) buf = 0;
-      }
-      cp_async_wait_all();                             // nothing of this thread's is in flight when it leaves
+      cp_async_commit();
+    };
+    bool ok = true;
+    int id_cur, id_nxt, pa, ta;                      // row ids of blocks i and i+1, position and page of i+2
+    {
+      const int p0 = position(0), p1 = position(1), t0 = table_entry(p0), t1 = table_entry(p1);
+      pa = position(2);
+      ta = table_entry(pa);
+      id_cur = cache_row(p0, t0);
+      fetch(0, id_cur);
+      id_nxt = cache_row(p1, t1);
+      fetch(1, id_nxt);
     }
+    const int l16 = (lane & 3) | ((lane >> 3) << 2);         // 4 bits: sixteen lanes a row, two rows at a time (sparse_mla.cu)
+    for (int i = 0, buf = 0; i < nblk; ++i) {
+      const int id2 = cache_row(pa, ta);             // block i+2
+      pa = position(i + 3);
+      ta = table_entry(pa);
+      if (i == kQBuf0) ok = mla_wait(q_moved, 0, abort_flag, a.status);   // from here on the buffers held Q
+      if (i >= NB) ok = mla_wait(&kv_free[buf], ((i / NB) - 1) & 1, abort_flag, a.status);
+      if (!ok) break;
+      mark(i, id_cur >= 0);
+      id_cur = id_nxt;
+      id_nxt = id2;
+      cp_async_wait<1>();                            // this lane's copies of block i have landed (block i+1 may be in flight) ...
+      __syncwarp();                                  // ... and the other lanes'
+      const uint8_t* st = stage_of(i);
+      uint8_t* dst = kv_s + buf * kMlaKBytes;
+      if constexpr (SRC == kSrc4) {
+#pragma unroll
+        for (int u = 0; u < kRows / 2; ++u) {
+          const int j = 2 * u + ((lane >> 2) & 1), r = w4 + j * kG;
+          const uint2 w = *reinterpret_cast<const uint2*>(st + j * kRawRow + l16 * 8);
+          const uint32_t sc = latent4_scale(st[j * kRawRow + kLatent4Scales + l16]);
+          uint8_t* row = dst + (l16 >> 2) * kMlaKPanelBytes + r * 128;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t p[4];
+            latent4_codes(x == 0 ? w.x : w.y, p);
+            const uint4 v = make_uint4(mul_bf16x2(p[0], sc), mul_bf16x2(p[1], sc), mul_bf16x2(p[2], sc), mul_bf16x2(p[3], sc));
+            if (r < kMlaBlk) *reinterpret_cast<uint4*>(row + ((((2 * l16 + x) ^ r) & 7) << 4)) = v;
+          }
+        }
+      } else {
+        uint8_t* dst_lat = dst + (lane >> 3) * kMlaKPanelBytes;
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+          const int r = w4 + j * kG;
+          const uint2 raw = *reinterpret_cast<const uint2*>(st + j * kRawRow + lane * 8);
+          const float sc = *reinterpret_cast<const float*>(st + j * kRawRow + 256 + cta * 8 + (lane >> 4) * 4);
+          const uint4 v = e4m3x8_to_bf16(raw, sc);
+          if (r < kMlaBlk) *reinterpret_cast<uint4*>(dst_lat + r * 128 + (((lane ^ r) & 7) << 4)) = v;
+        }
+      }
+      {
+        constexpr int kRope = SRC == kSrc4 ? kLatent4Rope : 272;
+        const int r = w4 + (lane >> 2) * kG;
+        if (lane < 4 * kRows && r < kMlaBlk)
+          *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane ^ (r >> 1)) & 3) << 4)) =
+              *reinterpret_cast<const uint4*>(st + (lane >> 2) * kRawRow + kRope + (lane & 3) * 16);
+      }
+      __syncwarp();                                  // (the MMA warp makes the writes visible to the tensor core's reads)
+      if (lane == 0) mbar_arrive(&kv_full[buf]);
+      fetch(i + 2, id2);                             // into the stage just read: what was loaded from it has been stored
+      if (++buf == NB) buf = 0;
+    }
+    cp_async_wait_all();                             // nothing of this thread's is in flight when it leaves
   } else {
     // ------------- partial-score exchange, softmax and output: thread = (row, half of a block's keys); as in sparse_mla.cu but for the masks -------------
     const int qd = warp & 3, hf = (warp >> 2) & 1, set = warp >> 3;      // hf: key half; set: takes the blocks of that parity
@@ -606,15 +343,8 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     // which of the 32 keys of this thread's half of block g this row sees
     auto seen_of = [&](int r, int g, int half) -> uint32_t {
       const int4 v = sees_s[r];
-      if constexpr (PAGED) {
-        const int k0 = g * kMlaBlk + 32 * half;
-        return (range_bits(0, v.x, k0) | range_bits(v.y, v.z, k0) | draft_bits(more_s[r], v.w, k0)) & low_bits(n_slots - k0);
-      } else {
-        const int4 s = seg_of(g);
-        const int k0 = s.x + (g - s.z) * kMlaBlk + 32 * half, tok = (int)more_s[r];
-        if (tok < (s.w & 0xffff) || tok > (s.w >> 16)) return 0u;
-        return (range_bits(v.x, v.y, k0) | range_bits(v.z, v.w, k0)) & low_bits(s.y - k0);
-      }
+      const int k0 = g * kMlaBlk + 32 * half;
+      return (range_bits(0, v.x, k0) | range_bits(v.y, v.z, k0) | draft_bits(more_s[r], v.w, k0)) & low_bits(n_slots - k0);
     };
     if (qd < n_quad && set < nblk && lane == 0) mbar_expect_tx(&recv_full[warp], kMlaXWarp);
     for (int n = qd < n_quad ? set : nblk; n < nblk && ok; n += 2) {
@@ -642,15 +372,8 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (elect_one()) bulk_copy_to_peer(peer_recv, send, kMlaXWarp, peer_recv_full);
       __syncwarp();
       uint32_t seen = 0xffffffffu;
-      bool whole;
-      if constexpr (PAGED) {
-        const int k0 = (blk_lo + n) * kMlaBlk;
-        whole = k0 >= full0 && k0 + kMlaBlk <= full1;
-      } else {
-        const int4 s = seg_of(blk_lo + n);
-        const int k0 = s.x + (blk_lo + n - s.z) * kMlaBlk;
-        whole = k0 >= full0 && k0 + kMlaBlk <= full1;
-      }
+      const int k0 = (blk_lo + n) * kMlaBlk;
+      const bool whole = k0 >= full0 && k0 + kMlaBlk <= full1;
       if (!whole) {
         seen = seen_of(row, blk_lo + n, hf);
         float z = 0.f;
@@ -677,7 +400,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         for (int k = 0; k < 4; ++k)
           add_f16x2(tw[k], __uint_as_float(sv[8 * c + 2 * k]), __uint_as_float(sv[8 * c + 2 * k + 1]), s[8 * c + 2 * k], s[8 * c + 2 * k + 1]);
       }
-      if constexpr (PAGED) seen &= __ballot_sync(0xffffffffu, valid_s[(n % kMlaValidRing) * kMlaBlk + 32 * hf + lane]);
+      seen &= __ballot_sync(0xffffffffu, valid_s[(n % kMlaValidRing) * kMlaBlk + 32 * hf + lane]);
       auto largest = [&]() {
         float bm[4] = {s[0], s[1], s[2], s[3]};        // four independent chains
 #pragma unroll
@@ -752,7 +475,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     float2* sum_s = reinterpret_cast<float2*>(kv_s + 2 * kMlaKBytes);
     const int quarter = warp >> 2;                     // which quarter of the row's columns this thread writes
     const int4 mine = sees_s[row];
-    const bool any = PAGED ? mine.x > 0 || mine.z > mine.y || more_s[row] != 0 : mine.y > mine.x || mine.w > mine.z;      // the row sees something
+    const bool any = mine.x > 0 || mine.z > mine.y || more_s[row] != 0;      // the row sees something
     if (ok) sum_s[quarter * 128 + row] = make_float2(m, l);
     if (odd && any && row < rows_here) odd_s[qd] = 1;
     named_bar_sync(3 + qd, 128);
@@ -761,30 +484,23 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     if (ok && odd_s[qd]) {
       // Rare: among the keys of a row's blocks there is one that it does not see and that is no number.  The quadrant's rows, each by a warp, key by
       // key over what they see of this part: this CTA's half of the output from whole scores.
-      constexpr int kBytes = SRC == kSrcRows ? kMlaDqk * 2 : SRC == kSrcFp8 ? kLatentTokenBytes : kLatent4Bytes;
+      constexpr int kBytes = SRC == kSrcFp8 ? kLatentTokenBytes : kLatent4Bytes;
 #pragma unroll 1
       for (int rr = quarter; rr < 32; rr += 4) {
         const int r = qd * 32 + rr;
         if (r >= rows_here) break;
         const RowShare q = load_share<kSrcRows>(reinterpret_cast<const uint8_t*>(a.q + (g0 + r) * kMlaDqk), lane);
         float rm = -CUDART_INF_F, rl = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        seg_at = 0;
 #pragma unroll 1
         for (int n = 0; n < 2 * nblk; ++n) {
           const int g = blk_lo + (n >> 1);
           uint32_t todo = seen_of(r, g, n & 1);
 #pragma unroll 1
           for (; todo; todo &= todo - 1) {
-            int64_t key;
-            if constexpr (PAGED) {
-              const int j = g * kMlaBlk + 32 * (n & 1) + __ffs(todo) - 1, pos = j < head ? j : j + shift;
-              const int page = __ldg(a.block_table + (int64_t)seq * a.table_stride + pos / kLatentPage);
-              if (page < 0 || (int64_t)(page + 1) * kLatentPage > a.num_phys_rows) continue;
-              key = (int64_t)page * kLatentPage + pos % kLatentPage;
-            } else {
-              const int4 s = segs_s[seg_at];
-              key = s.x + (g - s.z) * kMlaBlk + 32 * (n & 1) + __ffs(todo) - 1;
-            }
+            const int j = g * kMlaBlk + 32 * (n & 1) + __ffs(todo) - 1, pos = j < head ? j : j + shift;
+            const int page = __ldg(a.block_table + (int64_t)seq * a.table_stride + pos / kLatentPage);
+            if (page < 0 || (int64_t)(page + 1) * kLatentPage > a.num_phys_rows) continue;
+            const int64_t key = (int64_t)page * kLatentPage + pos % kLatentPage;
             const RowShare k = load_share<SRC>(a.kv + key * kBytes, lane);
             const float s = row_score(q, k, a.scale_log2e), mx = fmaxf(rm, s), at = mx == -CUDART_INF_F ? 0.f : mx;
             const float keep = rm == -CUDART_INF_F ? 0.f : exp2f(rm - at), p = exp2f(s - at);
@@ -885,8 +601,8 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 template <int PARTS>
 __global__ void __launch_bounds__(128) window_combine_kernel(const WinArgs a) {
   const float *lse = grid_wait(a.part_lse), *part = grid_wait(a.part_o);
-  const int unit = a.n_full + blockIdx.x, r = blockIdx.y, seq = unit / a.seq_units, row = (unit - seq * a.seq_units) * 128 + r;
-  if (row >= a.seq_rows) return;
+  const int unit = a.n_full + blockIdx.x, r = blockIdx.y, seq = unit / a.seq_units, row = (unit - seq * a.seq_units) * a.unit_rows + r;
+  if (r >= a.unit_rows || row >= a.seq_rows) return;
   const int d = threadIdx.x * 4, cta = d / kMlaDvHalf;
   float wgt[PARTS];
   float4 v[PARTS];
@@ -919,29 +635,8 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const WinArgs a) {
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------
-int make_tmap_2d_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t inner_bytes, uint64_t row_pitch, uint32_t box_bytes, uint32_t box_rows);
-
-// Units run in rounds of one to a pair of SMs.  The keys of a partly filled last round's units are cut into parts, as many as there are pairs for.
-constexpr int kWinPartBlocks = 2;                      // blocks of a part at least
-constexpr size_t kWinPartBytes = (size_t)128 * (kMlaDv + 2) * sizeof(float);
-static int window_parts(int64_t units, int64_t keys) {
-  const int pairs = max(1, sm_count() / 2), rest = (int)(units % pairs);
-  const int64_t blocks = (keys + kMlaBlk - 1) / kMlaBlk;
-  return rest == 0 ? 1 : (int)max((int64_t)1, min(min((int64_t)kWinMaxParts, blocks / kWinPartBlocks), (int64_t)(pairs / rest)));
-}
-// of every call of up to `units` of them
-static size_t window_workspace(int64_t units, int64_t keys) {
-  const int pairs = max(1, sm_count() / 2);
-  size_t most = 0;
-  for (int64_t u = 1; u < pairs && u <= units; ++u) {
-    const int parts = window_parts(u, keys);
-    if (parts > 1) most = max(most, (size_t)u * parts);
-  }
-  return most * kWinPartBytes;
-}
-// Keys of a unit at most, that parts are worth: first tokens, window, and the tokens of the unit.
-static int64_t window_keys(int H, int64_t window, int64_t first, int64_t tokens, int64_t most) {
-  return min(most, window + first + min(tokens, (int64_t)(127 / H + 2)));
+void window_combine(const WinArgs& a, int64_t units, cudaStream_t stream) {
+  launch_after(0, a.n_split > 8 ? window_combine_kernel<kWinMaxParts> : window_combine_kernel<8>, dim3((unsigned)(units - a.n_full), 128), 128, 0, stream, a);
 }
 
 template <int SRC>
@@ -949,65 +644,27 @@ static int launch_window(WinArgs a, int64_t units, int64_t keys, void* workspace
   using C = WinCfg<SRC>;
   if (a.T == 0 || a.H == 0) return DSA_OK;
   const int64_t rows = (int64_t)a.T * a.H;
-  const int pairs = max(1, sm_count() / 2), rest = (int)(units % pairs);
-  int ns = window_parts(units, keys);
-  if (ns > 1) {                                        // a smaller workspace: as many parts as it holds
-    const size_t fit = workspace ? workspace_bytes / kWinPartBytes / rest : 0;
-    if (fit < (size_t)ns) ns = fit > 1 ? (int)fit : 1;
-  }
-  a.n_full = (int)(ns > 1 ? units - rest : units);
-  a.n_split = ns;
-  if (ns > 1) {
-    a.part_o = static_cast<float*>(workspace);
-    a.part_lse = a.part_o + (size_t)rest * ns * 128 * kMlaDv;
-  }
-  CUtensorMap tq, to, tl, tr;
+  window_plan(a, units, keys, workspace, workspace_bytes);
+  CUtensorMap tq, to;
   int rc = make_tmap_2d_bytes(&tq, a.q, rows, kMlaDqk * 2, kMlaDqk * 2, 128, 128);
   if (rc) return rc;
-  to = tl = tr = tq;
+  to = tq;
   if (a.n_full > 0 && rows >= 128) {
     if ((rc = make_tmap_2d_bytes(&to, a.out, rows, kMlaDv * 2, kMlaDv * 2, 128, 128))) return rc;
     a.tma_out = 1;
   }
-  if constexpr (SRC == kSrcRows) {
-    if (a.S > 0) {
-      if ((rc = make_tmap_2d_bytes(&tl, a.kv, a.S, kMlaDqk * 2, kMlaDqk * 2, 128, kMlaBlk))) return rc;
-      if ((rc = make_tmap_2d_bytes(&tr, a.kv, a.S, kMlaDqk * 2, kMlaDqk * 2, 64, kMlaBlk))) return rc;
-    }
-  }
   auto kern = window_mla_kernel<SRC>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
     return set_error(DSA_ERR_CUDA, "window_mla: cannot raise dynamic shared memory to %d", C::kSmem);
-  const int64_t jobs = a.n_full + (units - a.n_full) * ns;
+  const int64_t jobs = a.n_full + (units - a.n_full) * a.n_split;
   if (2 * jobs > 0x7fffffff) return set_error(DSA_ERR_SHAPE, "window_mla: too many work units");
-  kern<<<(unsigned)(2 * jobs), C::kThreads, C::kSmem, stream>>>(tq, to, tl, tr, a);
-  if (ns > 1)
-    launch_after(0, ns > 8 ? window_combine_kernel<kWinMaxParts> : window_combine_kernel<8>, dim3((unsigned)(units - a.n_full), 128), 128, 0, stream, a);
+  kern<<<(unsigned)(2 * jobs), kMlaThreads, C::kSmem, stream>>>(tq, to, a);
+  if (a.n_split > 1) window_combine(a, units, stream);
   return check_launch("window_mla");
 }
 
-size_t window_mla_prefill_workspace(int T, int H, int window, int first) {
-  return window_workspace(((int64_t)T * H + 127) / 128, window_keys(H, window, first, T, 0x7fffffff));
-}
 size_t window_mla_decode_workspace(int B, int tokens_per_seq, int H, int window, int first, int max_ctx) {
   return window_workspace((int64_t)B * (((int64_t)tokens_per_seq * H + 127) / 128), window_keys(H, window, first, tokens_per_seq, max_ctx));
-}
-
-int window_mla_prefill_launch(const void* q, const void* kv, const int32_t* ks, const int32_t* ke, void* out, int T, int H, int S, int window, int first,
-                              float scale, void* workspace, size_t workspace_bytes, int32_t* status, cudaStream_t stream) {
-  WinArgs a{};
-  a.q = static_cast<const __nv_bfloat16*>(q);
-  a.kv = static_cast<const uint8_t*>(kv);
-  a.ks = ks; a.ke = ke;
-  a.out = static_cast<__nv_bfloat16*>(out);
-  a.T = T; a.H = H; a.S = S;
-  a.window = window; a.first = first;
-  a.scale_log2e = scale * 1.4426950408889634f;
-  a.status = status;
-  a.seq_rows = T * H;
-  const int64_t units = ((int64_t)T * H + 127) / 128;
-  a.seq_units = (int)units;
-  return launch_window<kSrcRows>(a, units, window_keys(H, window, first, T, S), workspace, workspace_bytes, stream);
 }
 
 int window_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len,
@@ -1025,6 +682,7 @@ int window_mla_decode_launch(const void* q, const void* cache, int record_bytes,
   a.num_phys_rows = num_pages * kLatentPage;
   a.scale_log2e = scale * 1.4426950408889634f;
   a.status = status;
+  a.unit_rows = 128;
   a.seq_rows = tokens_per_seq * H;
   a.seq_units = (a.seq_rows - 1) / 128 + 1;
   const int64_t units = (int64_t)B * a.seq_units, keys = window_keys(H, window, first, tokens_per_seq, max_ctx);
