@@ -366,53 +366,67 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (!odd) {
         uint8_t* const stage0 = smem + (e % NB) * kMlaKBytes + qd * 8192 + lane * 128;      // two panels of 32 rows to a warp
         __nv_bfloat16* const orow = a.out + (int64_t)(row0 + row) * kMlaDv + cta * kMlaDvHalf;
-        auto put = [&](int c, uint32_t (&ov)[16]) {
-          if (by_tma && c >= 128 && (c & 63) == 0) {   // the store of two panels before has read its own
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-            __syncwarp();
-          }
+        const uint64_t inv2 = pack_f32x2(inv, inv);
+        const bool blind = __any_sync(0xffffffffu, !any);
+        auto scaled = [&](uint32_t (&ov)[16]) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(any ? __uint_as_float(ov[i]) * inv : 0.f);
-          if (part >= 0) {
-            if (row < rows) {
+          for (int i = 0; i < 16; i += 2) {
+            float x, y;
+            unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(ov[i]), __uint_as_float(ov[i + 1])), inv2), x, y);
+            ov[i] = __float_as_uint(x);
+            ov[i + 1] = __float_as_uint(y);
+          }
+          if (blind) {                                 // a row that sees nothing: zeros, whatever the blocks of the others gave it
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ov[i] = any ? ov[i] : 0u;
+          }
+        };
+        auto eight = [&](const uint32_t (&ov)[16], int i) {
+          return make_uint4(pack_bf16x2(__uint_as_float(ov[i]), __uint_as_float(ov[i + 1])), pack_bf16x2(__uint_as_float(ov[i + 2]), __uint_as_float(ov[i + 3])),
+                            pack_bf16x2(__uint_as_float(ov[i + 4]), __uint_as_float(ov[i + 5])), pack_bf16x2(__uint_as_float(ov[i + 6]), __uint_as_float(ov[i + 7])));
+        };
+        // the next sixteen columns are on their way while these are written; with every address known beforehand
+        uint32_t ov[2][16];
+        tmem_ld16(t_row + kColO, ov[0]);
+        if (by_tma) {
+#pragma unroll
+          for (int c = 0; c < kMlaDvHalf; c += 16) {
+            uint32_t (&now)[16] = ov[(c >> 4) & 1];
+            tmem_wait_ld();
+            if (c + 16 < kMlaDvHalf) tmem_ld16(t_row + kColO + c + 16, ov[((c >> 4) & 1) ^ 1]);
+            if (c >= 128 && (c & 63) == 0) {           // the store of two panels before has read its own
+              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+              __syncwarp();
+            }
+            scaled(now);
+            uint8_t* stage = stage0 + ((c >> 6) & 1) * 4096;
+            *reinterpret_cast<uint4*>(stage + (((((c & 63) >> 3) + 0) ^ (lane & 7)) << 4)) = eight(now, 0);
+            *reinterpret_cast<uint4*>(stage + (((((c & 63) >> 3) + 1) ^ (lane & 7)) << 4)) = eight(now, 8);
+            if ((c & 63) == 48) {
+              fence_async_smem();                      // the store reads the panel through the async proxy
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&tmap_o, stage, (cta * 4 + (c >> 6)) * 32, row0 + qd * 32);      // x in 4-byte units: 32 per 64-column panel
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              }
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < kMlaDvHalf; c += 16) {
+            tmem_ld16(t_row + kColO + c, ov[0]);
+            tmem_wait_ld();
+            scaled(ov[0]);
+            if (row < rows && part >= 0) {
               float4* po = reinterpret_cast<float4*>(a.part_o + ((int64_t)part * 128 + row) * kMlaDv + cta * kMlaDvHalf + c);
 #pragma unroll
               for (int i = 0; i < 16; i += 4)
-                po[i >> 2] = make_float4(__uint_as_float(ov[i]), __uint_as_float(ov[i + 1]), __uint_as_float(ov[i + 2]), __uint_as_float(ov[i + 3]));
-            }
-            return;
-          }
-          uint8_t* stage = stage0 + ((c >> 6) & 1) * 4096;
-#pragma unroll
-          for (int i = 0; i < 16; i += 8) {
-            uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(ov[i + 0]), __uint_as_float(ov[i + 1]));
-            w.y = pack_bf16x2(__uint_as_float(ov[i + 2]), __uint_as_float(ov[i + 3]));
-            w.z = pack_bf16x2(__uint_as_float(ov[i + 4]), __uint_as_float(ov[i + 5]));
-            w.w = pack_bf16x2(__uint_as_float(ov[i + 6]), __uint_as_float(ov[i + 7]));
-            if (by_tma) *reinterpret_cast<uint4*>(stage + (((((c & 63) + i) >> 3) ^ (lane & 7)) << 4)) = w;
-            else if (row < rows) *reinterpret_cast<uint4*>(orow + c + i) = w;
-          }
-          if (by_tma && (c & 63) == 48) {
-            fence_async_smem();                        // the store reads the panel through the async proxy
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&tmap_o, stage - lane * 128, (cta * 4 + (c >> 6)) * 32, row0 + qd * 32);      // x in 4-byte units: 32 per 64-column panel
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                po[i >> 2] = make_float4(__uint_as_float(ov[0][i]), __uint_as_float(ov[0][i + 1]), __uint_as_float(ov[0][i + 2]), __uint_as_float(ov[0][i + 3]));
+            } else if (row < rows) {
+              *reinterpret_cast<uint4*>(orow + c) = eight(ov[0], 0);
+              *reinterpret_cast<uint4*>(orow + c + 8) = eight(ov[0], 8);
             }
           }
-        };
-        // the next sixteen columns are on their way while these are written
-        uint32_t ov[2][16];
-        tmem_ld16(t_row + kColO, ov[0]);
-#pragma unroll 1
-        for (int c = 0; c < kMlaDvHalf; c += 32) {
-          tmem_wait_ld();
-          tmem_ld16(t_row + kColO + c + 16, ov[1]);
-          put(c, ov[0]);
-          tmem_wait_ld();
-          if (c + 32 < kMlaDvHalf) tmem_ld16(t_row + kColO + c + 32, ov[0]);
-          put(c + 16, ov[1]);
         }
       }
       tc_fence_before();
