@@ -38,6 +38,16 @@ int sm_count() {
   return cached[dev];
 }
 
+bool allow_smem(const void* kern, int bytes, uint64_t* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (__atomic_load_n(done, __ATOMIC_RELAXED) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  __atomic_fetch_or(done, bit, __ATOMIC_RELAXED);
+  return true;
+}
+
 // launchers implemented next to their kernels
 int indexer_logits_contiguous(const void* q, const void* k, const float* k_scale, const void* w, int w_dtype,
                               const int32_t* ks, const int32_t* ke, float* logits, int64_t ld, int T, int S,

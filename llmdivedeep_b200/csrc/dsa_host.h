@@ -28,5 +28,7 @@ inline void launch_after(int overlapped, void (*kern)(Params...), dim3 grid, int
 }
 // Multiprocessor count of the current device (cached per device).
 int sm_count();
+// Lets a kernel have `bytes` of dynamic shared memory on the current device.  `done`: the kernel's own word, a bit for each device where it has been said.
+bool allow_smem(const void* kern, int bytes, uint64_t* done);
 
 }  // namespace dsa

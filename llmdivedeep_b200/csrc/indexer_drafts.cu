@@ -380,7 +380,8 @@ static int launch_draft_logits(const DraftLogitsArgs& a, cudaStream_t stream) {
   if (units(chunk) > 0x7fffffff) return set_error(DSA_ERR_SHAPE, "indexer_logits_drafts: too many work units");
   const int n_units = (int)units(chunk);
   auto kern = draft_logits_kernel<H, NT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) != cudaSuccess)
+  static uint64_t allowed = 0;
+  if (!allow_smem(reinterpret_cast<const void*>(kern), C::SMEM_BYTES, &allowed))
     return set_error(DSA_ERR_CUDA, "indexer_logits_drafts: cannot raise dynamic shared memory to %d", C::SMEM_BYTES);
   kern<<<min(n_units, sm_count()), C::THREADS, C::SMEM_BYTES, stream>>>(tq, tk, a, groups, chunk, n_units);
   return check_launch("indexer_logits_drafts");

@@ -556,10 +556,13 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
 // Row rows[i] keeps the drafts path[i, 0 .. n_keep[i]) of its last n_new[i] tokens: draft path[k] moves to place k behind the P tokens before
 // them, in every cache; what lies behind goes.  path[k] >= k, so a place that is written is read by no later move, and a thread that takes
 // the same 16 bytes of every token in order needs no barrier.
-struct AcceptArgs {
-  CacheEntry cache[kCopyCaches];
-  int32_t first[kCopyCaches + 1];                      // columns of one token in the caches before
+template <int N>
+struct AcceptCaches {                                  // of a launch; eight hold most models' in a tenth of the parameters
+  CacheEntry cache[N];
+  int32_t first[N + 1];                                // columns of one token in the caches before
   int n_caches;
+};
+struct AcceptArgs {
   int32_t *table, *ctx, *refs;
   int64_t stride;
   int P, B, num_pages, n;
@@ -607,9 +610,10 @@ __device__ __forceinline__ void accept_column(const AcceptArgs& a, const CacheEn
       if (from[j] > k0 + j) *at(P + k0 + j) = v[j];
   }
 }
-__global__ void __launch_bounds__(kCopyThreads) accept_kernel(const __grid_constant__ AcceptArgs a, int lead) {
+template <int N>
+__global__ void __launch_bounds__(kCopyThreads) accept_kernel(const AcceptArgs a, const __grid_constant__ AcceptCaches<N> cs, int lead) {
   launch_dependents();
-  const int i = blockIdx.x, cols = a.first[a.n_caches];
+  const int i = blockIdx.x, cols = cs.first[cs.n_caches];
   const bool ok = accept_valid(a, i);
   if (lead && blockIdx.y == 0 && threadIdx.x == 0) a.accepted[i] = ok;
   if (!ok) {
@@ -620,19 +624,19 @@ __global__ void __launch_bounds__(kCopyThreads) accept_kernel(const __grid_const
   const int32_t *trow = a.table + (int64_t)row * a.stride, *path = a.path + (int64_t)i * a.path_stride;
   for (int c = blockIdx.y * kCopyThreads + threadIdx.x; c < cols; c += gridDim.y * kCopyThreads) {
     int e = 0;
-    for (int hi = a.n_caches; hi - e > 1;) {           // the cache that column c belongs to
+    for (int hi = cs.n_caches; hi - e > 1;) {          // the cache that column c belongs to
       const int mid = (e + hi) / 2;
-      (c >= a.first[mid] ? e : hi) = mid;
+      (c >= cs.first[mid] ? e : hi) = mid;
     }
-    const CacheEntry& ce = a.cache[e];
-    const int wide = ce.token_bytes % 16 == 0 ? 16 : 4, per = ce.token_bytes / wide, in = c - a.first[e], layer = in / per;
+    const CacheEntry& ce = cs.cache[e];
+    const int wide = ce.token_bytes % 16 == 0 ? 16 : 4, per = ce.token_bytes / wide, in = c - cs.first[e], layer = in / per;
     uint8_t* base = ce.base + layer * ce.layer_stride + (in - layer * per) * wide;
     if (wide == 16) accept_column<uint4>(a, ce, base, trow, path, P, keep);
     else accept_column<uint32_t>(a, ce, base, trow, path, P, keep);
   }
 }
 // Lengths and pages, when all contents have moved.
-__global__ void __launch_bounds__(kCopyThreads) accept_pages_kernel(const __grid_constant__ AcceptArgs a) {
+__global__ void __launch_bounds__(kCopyThreads) accept_pages_kernel(const AcceptArgs a) {
   const int i = blockIdx.x;
   if (!grid_wait(a.accepted)[i]) return;
   const int row = a.rows[i], c = a.ctx[row], now = c - a.n_new[i] + a.n_keep[i];
@@ -781,6 +785,20 @@ int compact_pages_launch(const int32_t* table, int64_t stride, int32_t* new_tabl
   return launch_copies<kCopyCompact>(c, PoolArgs{}, m, caches, n_caches, num_pages / 2, ((int64_t)B * P + 31) / 32, stream);
 }
 
+template <int N>
+static void launch_accept(const AcceptArgs& a, const dsa_page_cache* caches, int n_caches, int lead, cudaStream_t stream) {
+  AcceptCaches<N> cs;
+  cs.n_caches = n_caches;
+  cs.first[0] = 0;
+  for (int c = 0; c < n_caches; ++c) {
+    const dsa_page_cache& h = caches[c];
+    cs.cache[c] = {static_cast<uint8_t*>(h.base), h.layer_stride, h.layers, h.token_bytes};
+    cs.first[c + 1] = cs.first[c] + h.layers * (h.token_bytes / (h.token_bytes % 16 == 0 ? 16 : 4));
+  }
+  const int split = min(max(1, (cs.first[n_caches] + kCopyThreads - 1) / kCopyThreads), 65535);
+  accept_kernel<N><<<dim3(a.n, split), kCopyThreads, 0, stream>>>(a, cs, lead);
+}
+
 int accept_drafts_launch(int32_t* table, int64_t stride, int P, int B, int32_t* ctx, int32_t* refs, int num_pages, const int32_t* rows, const int32_t* n_new,
                          const int32_t* path, int path_stride, const int32_t* n_keep, int n, const dsa_page_cache* caches, int n_caches, int32_t* workspace,
                          int32_t* status, cudaStream_t stream) {
@@ -790,19 +808,11 @@ int accept_drafts_launch(int32_t* table, int64_t stride, int P, int B, int32_t* 
   a.rows = rows; a.n_new = n_new; a.path = path; a.path_stride = path_stride; a.n_keep = n_keep;
   a.accepted = workspace;
   a.status = status;
-  int c0 = 0;
-  do {
-    a.n_caches = min(n_caches - c0, kCopyCaches);
-    a.first[0] = 0;
-    for (int c = 0; c < a.n_caches; ++c) {
-      const dsa_page_cache& h = caches[c0 + c];
-      a.cache[c] = {static_cast<uint8_t*>(h.base), h.layer_stride, h.layers, h.token_bytes};
-      a.first[c + 1] = a.first[c] + h.layers * (h.token_bytes / (h.token_bytes % 16 == 0 ? 16 : 4));
-    }
-    const int split = min(max(1, (a.first[a.n_caches] + kCopyThreads - 1) / kCopyThreads), 65535);
-    accept_kernel<<<dim3(n, split), kCopyThreads, 0, stream>>>(a, c0 == 0);
-    c0 += kCopyCaches;
-  } while (c0 < n_caches);
+  if (n_caches <= 8) {
+    launch_accept<8>(a, caches, n_caches, 1, stream);
+  } else {
+    for (int c0 = 0; c0 < n_caches; c0 += kCopyCaches) launch_accept<kCopyCaches>(a, caches + c0, min(n_caches - c0, kCopyCaches), c0 == 0, stream);
+  }
   launch_after(1, accept_pages_kernel, dim3(n), kCopyThreads, 0, stream, a);
   return check_launch("accept_drafts");
 }

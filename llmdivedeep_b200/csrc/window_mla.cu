@@ -36,6 +36,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   using C = WinCfg<SRC>;
   constexpr int NB = C::kBufs;
   extern __shared__ __align__(1024) uint8_t smem[];            // the swizzled panels need 1024-byte alignment
+  launch_dependents();                                         // (the kernel that merges the parts)
   uint8_t* kv_s = smem;                                        // five buffers: four panels [64 keys x 128 B] and 64 x 64 B
   uint8_t* send_s = kv_s + kMlaBufs * kMlaKBytes;              // this CTA's partial score tile on its way out
   uint8_t* recv_s = send_s + kMlaXBytes;                       // the peer's
@@ -56,8 +57,8 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   const int n_split = part < 0 ? 1 : a.n_split, unit = part < 0 ? job : a.n_full + part / n_split, split = part < 0 ? 0 : part % n_split;
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int seq = unit / a.seq_units;
-  const int row0 = (unit - seq * a.seq_units) * 128;           // of the sequence's query rows
-  const int rows_here = min(128, a.seq_rows - row0);
+  const int row0 = (unit - seq * a.seq_units) * a.unit_rows;   // of the sequence's query rows
+  const int rows_here = min(a.unit_rows, a.seq_rows - row0);
   const int64_t g0 = (int64_t)seq * a.seq_rows + row0;
   const int n_quad = (rows_here + 31) / 32;                    // quadrants of tensor memory with rows in them: the others' warps stand by
   const int tok0 = row0 / a.H, tok1 = (row0 + rows_here - 1) / a.H;
@@ -89,35 +90,80 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     tmem_relinquish();
   }
   // Keys by slots, the first tokens' [0, head) and behind them the windows' [shift + head, ...): slot j is position j or j + shift.
+  const Drafts dr = drafts_of(a.drafts, seq);
   int head = 0, shift = 0, n_slots = 0, full0 = 0, full1 = 0;
-  {
-    const Drafts dr = drafts_of(a.drafts, seq);
-    if (dr.bad && threadIdx.x == 0 && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
-    const int P = dr.ctx - dr.m, last = min(tok1, dr.m - 1);
-    if (tok0 <= last) {
-      const bool tree = a.drafts.tree != nullptr;
-      const int hi = P + last + 1, near = P + 1 + (tree ? 0 : tok0), lo = max(0, near - a.window), least = tree ? P : near;      // positions up to `least` are all seen
-      head = min(a.first, hi);
-      if (lo <= head) head = 0;
-      else shift = lo - head;
-      n_slots = hi - shift;
-      full0 = max(min(a.first, hi), hi - a.window);    // (of a tree: its path may be shorter)
-      full0 = full0 <= min(a.first, least) ? 0 : full0 - shift;
-      full1 = least - shift;
+  if (dr.bad && threadIdx.x == 0 && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+  if (tok0 < dr.m) {
+    const bool tree = a.drafts.tree != nullptr;
+    const int P = dr.ctx - dr.m, hi = P + min(tok1, dr.m - 1) + 1, near = P + 1 + (tree ? 0 : tok0), lo = max(0, near - a.window);
+    const int least = tree ? P : near;                 // positions up to here are seen by every row
+    head = min(a.first, hi);
+    if (lo <= head) head = 0;
+    else shift = lo - head;
+    n_slots = hi - shift;
+    full0 = max(min(a.first, hi), hi - a.window);      // (of a tree: its path may be shorter)
+    full0 = full0 <= min(a.first, least) ? 0 : full0 - shift;
+    full1 = least - shift;
+  }
+  const int blocks = (n_slots + kMlaBlk - 1) / kMlaBlk;
+  const int per = (blocks + n_split - 1) / n_split, blk_lo = min(blocks, split * per), nblk = min(blocks, blk_lo + per) - blk_lo;
+  // The records of 64 slots a block, each gather warp every eleventh: raw into shared memory two blocks ahead (cp.async), then to bf16.  The first two
+  // blocks are sent for before anything of the set-up is waited for: a page's entry and a record are two times the way to memory.
+  constexpr int kG = kMlaGatherWarps, kRows = kRawRows, kRawRow = MlaRaw<SRC>::kRow, kRawBytes = MlaRaw<SRC>::kBytes, kRawInBuf = MlaRaw<SRC>::kInBuf;
+  constexpr int kBytes = SRC == kSrc4 ? kLatent4Bytes : kLatentTokenBytes;
+  const int w4 = warp - kMlaGatherWarp0;
+  const int slot = warp >= kMlaGatherWarp0 && lane < kRows ? w4 + lane * kG : kMlaBlk;      // lane j < 6 looks after slot w4 + 11 j
+  const int32_t* table = a.block_table + (int64_t)seq * a.table_stride;
+  auto position = [&](int i) -> int {
+    const int j = (blk_lo + i) * kMlaBlk + slot;
+    return slot < kMlaBlk && i < nblk && j < n_slots ? (j < head ? j : j + shift) : -1;
+  };
+  auto table_entry = [&](int pos) -> int { return pos >= 0 ? __ldg(table + pos / kLatentPage) : -1; };
+  auto cache_row = [&](int pos, int page) -> int {   // -1 = no slot, or a page that is none: flagged
+    if (pos < 0) return -1;
+    if (page >= 0 && (int64_t)(page + 1) * kLatentPage <= a.num_phys_rows) return page * kLatentPage + pos % kLatentPage;
+    if (a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+    return -1;
+  };
+  auto stage_of = [&](int i) -> uint8_t* {           // the fifth KV buffer, and what does not fit there behind everything else
+    const int c = (i & 1) * kG + w4;
+    return c < kRawInBuf ? kv_s + NB * kMlaKBytes + c * kRawBytes : smem + C::kOffRaw + (c - kRawInBuf) * kRawBytes;
+  };
+  auto fetch = [&](int i, int id) {                  // an empty slot is zero-filled, values and scales
+    uint8_t* st = stage_of(i);
+    if constexpr (SRC == kSrc4) {
+#pragma unroll
+      for (int u = 0; u < (kRows * 13 + 31) / 32; ++u) {         // 208 bytes a row: thirteen pieces
+        const int c = u * 32 + lane, j = c / 13, rid = __shfl_sync(0xffffffffu, id, min(j, kRows - 1));
+        if (c < kRows * 13)
+          cp_async_16(st + c * 16, a.kv + (int64_t)max(rid, 0) * kBytes + cta * kLatent4Half + (c - j * 13) * 16, rid >= 0 ? 16 : 0);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kRows / 2; ++u) {        // two rows of 256 values per instruction
+        const int j = 2 * u + (lane >> 4), rid = __shfl_sync(0xffffffffu, id, j);
+        cp_async_16(st + j * kRawRow + (lane & 15) * 16, a.kv + cta * kMlaDvHalf + (lane & 15) * 16 + (int64_t)max(rid, 0) * kBytes, rid >= 0 ? 16 : 0);
+      }
+      const int rid = __shfl_sync(0xffffffffu, id, lane >> 2);
+      if (lane < kRows) cp_async_16(st + lane * kRawRow + 256, a.kv + kMlaDv + (int64_t)max(id, 0) * kBytes, id >= 0 ? 16 : 0);      // a row's four scales
+      if (lane < 4 * kRows)                        // this CTA's two K-steps of the rope panel: 64 bytes per row
+        cp_async_16(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16, a.kv + kMlaDv + 16 + cta * 64 + (lane & 3) * 16 + (int64_t)max(rid, 0) * kBytes, rid >= 0 ? 16 : 0);
     }
-    const int r = threadIdx.x - 32;
-    if (r >= 0 && r < 128) {
-      const Sees s = r < rows_here ? sees_draft(a, dr, seq, (row0 + r) / a.H) : Sees{};
-      const int a1 = shift ? min(s.a1, head) : s.a1;
-      sees_s[r] = make_int4(a1, s.b0 - shift, s.b1 - shift, s.at - shift);
-      more_s[r] = s.bits;
-    }
+    cp_async_commit();
+  };
+  int id_cur = -1, id_nxt = -1, pa = -1, ta = -1;      // row ids of blocks i and i+1, position and page of i+2
+  if (warp >= kMlaGatherWarp0 && nblk > 0) {
+    const int p0 = position(0), p1 = position(1), t0 = table_entry(p0), t1 = table_entry(p1);
+    pa = position(2);
+    ta = table_entry(pa);
+    id_cur = cache_row(p0, t0);
+    fetch(0, id_cur);
+    id_nxt = cache_row(p1, t1);
+    fetch(1, id_nxt);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const int blocks = (n_slots + kMlaBlk - 1) / kMlaBlk;
-  const int per = (blocks + n_split - 1) / n_split, blk_lo = min(blocks, split * per), nblk = min(blocks, blk_lo + per) - blk_lo;
   if (nblk == 0) {   // nothing seen: zeros (a part: weight zero in the combine); no cluster traffic yet
     if (part < 0) {
       for (int e = threadIdx.x; e < rows_here * 32; e += kMlaThreads)
@@ -186,63 +232,11 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       }
     }
   } else if (warp > kMlaMmaWarp) {
-    // ---- decode: the records of 64 slots a block, each warp every eleventh: raw into shared memory two blocks ahead (cp.async), then to bf16 ----
-    constexpr int kG = kMlaGatherWarps, kRows = kRawRows, kRawRow = MlaRaw<SRC>::kRow, kRawBytes = MlaRaw<SRC>::kBytes, kRawInBuf = MlaRaw<SRC>::kInBuf;
-    constexpr int kBytes = SRC == kSrc4 ? kLatent4Bytes : kLatentTokenBytes;
-    const int w4 = warp - kMlaGatherWarp0;
-    const int slot = lane < kRows ? w4 + lane * kG : kMlaBlk;      // lane j < 6 looks after slot w4 + 11 j
-    const int32_t* table = a.block_table + (int64_t)seq * a.table_stride;
-    auto position = [&](int i) -> int {
-      const int j = (blk_lo + i) * kMlaBlk + slot;
-      return slot < kMlaBlk && i < nblk && j < n_slots ? (j < head ? j : j + shift) : -1;
-    };
-    auto table_entry = [&](int pos) -> int { return pos >= 0 ? __ldg(table + pos / kLatentPage) : -1; };
-    auto cache_row = [&](int pos, int page) -> int {   // -1 = no slot, or a page that is none: flagged
-      if (pos < 0) return -1;
-      if (page >= 0 && (int64_t)(page + 1) * kLatentPage <= a.num_phys_rows) return page * kLatentPage + pos % kLatentPage;
-      if (a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
-      return -1;
-    };
+    // ----------------------------- records to bf16 -----------------------------
+    bool ok = true;
     auto mark = [&](int i, bool used) {
       if (slot < kMlaBlk) valid_s[(i % kMlaValidRing) * kMlaBlk + slot] = used;
     };
-    auto stage_of = [&](int i) -> uint8_t* {         // the fifth KV buffer, and what does not fit there behind everything else
-      const int c = (i & 1) * kG + w4;
-      return c < kRawInBuf ? kv_s + NB * kMlaKBytes + c * kRawBytes : smem + C::kOffRaw + (c - kRawInBuf) * kRawBytes;
-    };
-    auto fetch = [&](int i, int id) {                // an empty slot is zero-filled, values and scales
-      uint8_t* st = stage_of(i);
-      if constexpr (SRC == kSrc4) {
-#pragma unroll
-        for (int u = 0; u < (kRows * 13 + 31) / 32; ++u) {         // 208 bytes a row: thirteen pieces
-          const int c = u * 32 + lane, j = c / 13, rid = __shfl_sync(0xffffffffu, id, min(j, kRows - 1));
-          if (c < kRows * 13)
-            cp_async_16(st + c * 16, a.kv + (int64_t)max(rid, 0) * kBytes + cta * kLatent4Half + (c - j * 13) * 16, rid >= 0 ? 16 : 0);
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < kRows / 2; ++u) {        // two rows of 256 values per instruction
-          const int j = 2 * u + (lane >> 4), rid = __shfl_sync(0xffffffffu, id, j);
-          cp_async_16(st + j * kRawRow + (lane & 15) * 16, a.kv + cta * kMlaDvHalf + (lane & 15) * 16 + (int64_t)max(rid, 0) * kBytes, rid >= 0 ? 16 : 0);
-        }
-        const int rid = __shfl_sync(0xffffffffu, id, lane >> 2);
-        if (lane < kRows) cp_async_16(st + lane * kRawRow + 256, a.kv + kMlaDv + (int64_t)max(id, 0) * kBytes, id >= 0 ? 16 : 0);      // a row's four scales
-        if (lane < 4 * kRows)                        // this CTA's two K-steps of the rope panel: 64 bytes per row
-          cp_async_16(st + (lane >> 2) * kRawRow + 272 + (lane & 3) * 16, a.kv + kMlaDv + 16 + cta * 64 + (lane & 3) * 16 + (int64_t)max(rid, 0) * kBytes, rid >= 0 ? 16 : 0);
-      }
-      cp_async_commit();
-    };
-    bool ok = true;
-    int id_cur, id_nxt, pa, ta;                      // row ids of blocks i and i+1, position and page of i+2
-    {
-      const int p0 = position(0), p1 = position(1), t0 = table_entry(p0), t1 = table_entry(p1);
-      pa = position(2);
-      ta = table_entry(pa);
-      id_cur = cache_row(p0, t0);
-      fetch(0, id_cur);
-      id_nxt = cache_row(p1, t1);
-      fetch(1, id_nxt);
-    }
     const int l16 = (lane & 3) | ((lane >> 3) << 2);         // 4 bits: sixteen lanes a row, two rows at a time (sparse_mla.cu)
     for (int i = 0, buf = 0; i < nblk; ++i) {
       const int id2 = cache_row(pa, ta);             // block i+2
@@ -330,6 +324,12 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(q_moved);             // one arrival per warp
     }
+    if (warp < 4) {                                    // what this quadrant's rows see, in slots
+      const Sees v = row < rows_here ? sees_draft(a, dr, seq, (row0 + row) / a.H) : Sees{};
+      sees_s[row] = make_int4(shift ? min(v.a1, head) : v.a1, v.b0 - shift, v.b1 - shift, v.at - shift);
+      more_s[row] = v.bits;
+    }
+    named_bar_sync(3 + qd, 128);
     cluster_wait();
     const int xw = hf * 4 + qd;                        // this warp's part of the set's partial tile: 32 rows x 32 keys, 2 KB
     uint8_t* send = send_s + xw * kMlaXWarp;
@@ -602,7 +602,7 @@ template <int PARTS>
 __global__ void __launch_bounds__(128) window_combine_kernel(const WinArgs a) {
   const float *lse = grid_wait(a.part_lse), *part = grid_wait(a.part_o);
   const int unit = a.n_full + blockIdx.x, r = blockIdx.y, seq = unit / a.seq_units, row = (unit - seq * a.seq_units) * a.unit_rows + r;
-  if (r >= a.unit_rows || row >= a.seq_rows) return;
+  if (row >= a.seq_rows) return;
   const int d = threadIdx.x * 4, cta = d / kMlaDvHalf;
   float wgt[PARTS];
   float4 v[PARTS];
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(128) window_combine_kernel(const WinArgs a) {
 
 // ---- launches --------------------------------------------------------------------------------------------------------
 void window_combine(const WinArgs& a, int64_t units, cudaStream_t stream) {
-  launch_after(0, a.n_split > 8 ? window_combine_kernel<kWinMaxParts> : window_combine_kernel<8>, dim3((unsigned)(units - a.n_full), 128), 128, 0, stream, a);
+  launch_after(1, a.n_split > 8 ? window_combine_kernel<kWinMaxParts> : window_combine_kernel<8>, dim3((unsigned)(units - a.n_full), a.unit_rows), 128, 0, stream, a);
 }
 
 template <int SRC>
@@ -654,7 +654,8 @@ static int launch_window(WinArgs a, int64_t units, int64_t keys, void* workspace
     a.tma_out = 1;
   }
   auto kern = window_mla_kernel<SRC>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+  static uint64_t allowed = 0;
+  if (!allow_smem(reinterpret_cast<const void*>(kern), C::kSmem, &allowed))
     return set_error(DSA_ERR_CUDA, "window_mla: cannot raise dynamic shared memory to %d", C::kSmem);
   const int64_t jobs = a.n_full + (units - a.n_full) * a.n_split;
   if (2 * jobs > 0x7fffffff) return set_error(DSA_ERR_SHAPE, "window_mla: too many work units");
@@ -663,8 +664,27 @@ static int launch_window(WinArgs a, int64_t units, int64_t keys, void* workspace
   return check_launch("window_mla");
 }
 
+// Rows of a unit.  Calls that leave most pairs idle have fewer: a block's exchange and softmax take less time, and there are more units to share its keys.
+static int decode_unit_rows(int B, int64_t seq_rows) {
+  const int pairs = max(1, sm_count() / 2);
+  for (const int rows : {32, 64})
+    if (seq_rows > rows && pairs / (B * ((seq_rows + rows - 1) / rows)) >= 256 / rows) return rows;
+  return 128;
+}
+static int64_t decode_units(int B, int64_t seq_rows) {
+  const int rows = decode_unit_rows(B, seq_rows);
+  return B * ((seq_rows + rows - 1) / rows);
+}
+// Of every call of up to B sequences.
 size_t window_mla_decode_workspace(int B, int tokens_per_seq, int H, int window, int first, int max_ctx) {
-  return window_workspace((int64_t)B * (((int64_t)tokens_per_seq * H + 127) / 128), window_keys(H, window, first, tokens_per_seq, max_ctx));
+  const int64_t seq_rows = (int64_t)tokens_per_seq * H, keys = window_keys(H, window, first, tokens_per_seq, max_ctx);
+  size_t most = window_workspace(B * ((seq_rows + 127) / 128), keys);
+  for (int b = 1; b <= min(B, 16); ++b) {              // more have units of 128 rows
+    const int64_t units = decode_units(b, seq_rows);
+    const int parts = window_parts(units, keys);
+    if (parts > 1) most = max(most, (size_t)(units % max(1, sm_count() / 2)) * parts * kWinPartBytes);
+  }
+  return most;
 }
 
 int window_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len,
@@ -682,9 +702,9 @@ int window_mla_decode_launch(const void* q, const void* cache, int record_bytes,
   a.num_phys_rows = num_pages * kLatentPage;
   a.scale_log2e = scale * 1.4426950408889634f;
   a.status = status;
-  a.unit_rows = 128;
   a.seq_rows = tokens_per_seq * H;
-  a.seq_units = (a.seq_rows - 1) / 128 + 1;
+  a.unit_rows = decode_unit_rows(B, a.seq_rows);
+  a.seq_units = (a.seq_rows - 1) / a.unit_rows + 1;
   const int64_t units = (int64_t)B * a.seq_units, keys = window_keys(H, window, first, tokens_per_seq, max_ctx);
   return record_bytes == kLatent4Bytes ? launch_window<kSrc4>(a, units, keys, workspace, workspace_bytes, stream)
                                        : launch_window<kSrcFp8>(a, units, keys, workspace, workspace_bytes, stream);

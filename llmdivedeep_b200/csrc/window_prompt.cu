@@ -125,6 +125,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   float2* sums_s = reinterpret_cast<float2*>(smem + kWpOffSums);
   PromptPlan* plans = reinterpret_cast<PromptPlan*>(smem + kWpOffPlans);
 
+  launch_dependents();                                         // (the kernel that merges the parts)
   const int cta = blockIdx.x & 1, peer = cta ^ 1;              // rank in the cluster = V half = contraction part
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -794,7 +795,8 @@ int window_mla_prefill_launch(const void* q, const void* kv, const int32_t* ks, 
     if (!rc) rc = make_tmap_2d_bytes(&tr, kv, S, kMlaDqk * 2, kMlaDqk * 2, 64, kMlaBlk);
     if (rc) return rc;
   }
-  if (cudaFuncSetAttribute(window_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWpSmem) != cudaSuccess)
+  static uint64_t allowed = 0;
+  if (!allow_smem(reinterpret_cast<const void*>(window_prompt_kernel), kWpSmem, &allowed))
     return set_error(DSA_ERR_CUDA, "window_mla: cannot raise dynamic shared memory to %d", kWpSmem);
   const int64_t jobs = a.n_full + (units - a.n_full) * a.n_split;
   if (jobs > 0x7ffffff0) return set_error(DSA_ERR_SHAPE, "window_mla: too many work units");
