@@ -45,7 +45,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
            *pm_full = bars + 9, *recv_full = bars + 17, *xchg_free = bars + 33, *kv_full = bars + 49, *kv_free = bars + 54;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 64);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* odd_s = abort_flag + 1;                        // [4 quadrants] a row must be done key by key
+  uint32_t* odd_s = tmem_slot + 2;                             // [4 quadrants] rows with a key that they do not see and that is no number
   uint8_t* valid_s = smem + C::kOffValid;                      // decode: [kMlaValidRing][64] 1 = the slot of the block has a page
   uint16_t* pm_s = reinterpret_cast<uint16_t*>(smem + C::kOffPm);        // block maxima, rounded up to bf16
   int4* sees_s = reinterpret_cast<int4*>(smem + C::kOffSees);
@@ -422,7 +422,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       ok = mla_wait(&pm_full[set * 4 + qd], ph, abort_flag, a.status);
       if (!ok) break;
       m = raise(m_prev, pair_max(pm_of(n)));
-      if (m != m_own) l = m_own == -CUDART_INF_F ? 0.f : l * fast_exp2(m_own - m);
+      if (m != m_own && m_own != -CUDART_INF_F) l *= fast_exp2(m_own - m);      // (without a reference l is 0, or NaN, and stays so)
       bool waited_pv = n == 0;
       if (__any_sync(0xffffffffu, m != m_prev) && n > 0) {
         // O must be quiescent: P.V of the previous block has to be complete.  This thread scales its half of the columns.
@@ -477,18 +477,65 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const int4 mine = sees_s[row];
     const bool any = mine.x > 0 || mine.z > mine.y || more_s[row] != 0;      // the row sees something
     if (ok) sum_s[quarter * 128 + row] = make_float2(m, l);
-    if (odd && any && row < rows_here) odd_s[qd] = 1;
+    const uint32_t odds = __ballot_sync(0xffffffffu, odd && any && row < rows_here);
+    if (odds && lane == 0) atomicOr(odd_s + qd, odds);
     named_bar_sync(3 + qd, 128);
+    uint32_t again = 0;                                // rows of the quadrant that have to be done again
     __nv_bfloat16* const orow = a.out + (g0 + row) * kMlaDv + cta * kMlaDvHalf;
     const int64_t prow = (int64_t)part * 128 + row;
-    if (ok && odd_s[qd]) {
-      // Rare: among the keys of a row's blocks there is one that it does not see and that is no number.  The quadrant's rows, each by a warp, key by
-      // key over what they see of this part: this CTA's half of the output from whole scores.
+    if (ok) {
+      tc_fence_after();
+      float mt = -CUDART_INF_F;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) mt = fmaxf(mt, sum_s[u * 128 + row].x);
+      l = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float2 ml = sum_s[u * 128 + row];
+        l += ml.x != -CUDART_INF_F ? ml.y * fast_exp2(ml.x - mt) : ml.y;
+      }
+      // A key that a row does not see and that is no number has come in through 0 x NaN, unless the row is none anyway.
+      again = __ballot_sync(0xffffffffu, (odd_s[qd] >> lane & 1u) && l == l);
+      if (!any) l = 0.f;                               // a block that every other row sees is not masked
+      const float inv = l > 0.f ? (SRC == kSrc4 ? kLatent4Gain : 1.f) / l : l;      // (a NaN stays one)
+      if (part >= 0 && quarter == 0)                   // what this CTA's half of the columns is weighted with
+        a.part_lse[((int64_t)part * 2 + cta) * 128 + row] = l > 0.f ? mt + log2f(l) : l == 0.f ? -CUDART_INF_F : l;
+#pragma unroll 1
+      for (int c = quarter * (kMlaDvHalf / 4); c < (quarter + 1) * (kMlaDvHalf / 4); c += 32) {
+        uint32_t ov[32];
+        tmem_ld32(t_row + kColO + c, ov);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(any ? __uint_as_float(ov[i]) * inv : 0.f);
+        if (row < rows_here && part >= 0) {
+          float4* po = reinterpret_cast<float4*>(a.part_o + prow * kMlaDv + cta * kMlaDvHalf + c);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            po[i >> 2] = make_float4(__uint_as_float(ov[i]), __uint_as_float(ov[i + 1]), __uint_as_float(ov[i + 2]), __uint_as_float(ov[i + 3]));
+        } else if (row < rows_here) {
+          uint8_t* prow_s = kv_s + (c >> 6) * kMlaQPanelBytes + row * 128;
+          const int ch0 = (c & 63) >> 3;               // first of this iteration's four 16-byte chunks in the 128-byte row
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 w;
+            w.x = pack_bf16x2(__uint_as_float(ov[i + 0]), __uint_as_float(ov[i + 1]));
+            w.y = pack_bf16x2(__uint_as_float(ov[i + 2]), __uint_as_float(ov[i + 3]));
+            w.z = pack_bf16x2(__uint_as_float(ov[i + 4]), __uint_as_float(ov[i + 5]));
+            w.w = pack_bf16x2(__uint_as_float(ov[i + 6]), __uint_as_float(ov[i + 7]));
+            if (by_tma) *reinterpret_cast<uint4*>(prow_s + (((ch0 + (i >> 3)) ^ (row & 7)) << 4)) = w;
+            else *reinterpret_cast<uint4*>(orow + c + i) = w;
+          }
+        }
+      }
+    }
+    if (again) {
+      // Rare: these rows, each by a warp, key by key over what they see of this part: this CTA's half of the output from whole scores.
+      named_bar_sync(3 + qd, 128);                     // what the four warps have written of them is overwritten
       constexpr int kBytes = SRC == kSrcFp8 ? kLatentTokenBytes : kLatent4Bytes;
 #pragma unroll 1
-      for (int rr = quarter; rr < 32; rr += 4) {
-        const int r = qd * 32 + rr;
-        if (r >= rows_here) break;
+      for (int nth = 0; again; again &= again - 1, ++nth) {
+        if ((nth & 3) != quarter) continue;
+        const int r = qd * 32 + __ffs(again) - 1;
         const RowShare q = load_share<kSrcRows>(reinterpret_cast<const uint8_t*>(a.q + (g0 + r) * kMlaDqk), lane);
         float rm = -CUDART_INF_F, rl = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -526,48 +573,6 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       }
       fence_async_smem();
       named_bar_sync(3 + qd, 128);                     // a panel below has rows of all four warps
-    } else if (ok) {
-      tc_fence_after();
-      float mt = -CUDART_INF_F;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) mt = fmaxf(mt, sum_s[u * 128 + row].x);
-      l = 0.f;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float2 ml = sum_s[u * 128 + row];
-        if (ml.x != -CUDART_INF_F) l += ml.y * fast_exp2(ml.x - mt);
-      }
-      if (!any) l = 0.f;                               // a block that every other row sees is not masked
-      const float inv = l > 0.f ? (SRC == kSrc4 ? kLatent4Gain : 1.f) / l : l;      // (a NaN stays one)
-      if (part >= 0 && quarter == 0)                   // what this CTA's half of the columns is weighted with
-        a.part_lse[((int64_t)part * 2 + cta) * 128 + row] = l > 0.f ? mt + log2f(l) : l == 0.f ? -CUDART_INF_F : l;
-#pragma unroll 1
-      for (int c = quarter * (kMlaDvHalf / 4); c < (quarter + 1) * (kMlaDvHalf / 4); c += 32) {
-        uint32_t ov[32];
-        tmem_ld32(t_row + kColO + c, ov);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(any ? __uint_as_float(ov[i]) * inv : 0.f);
-        if (row < rows_here && part >= 0) {
-          float4* po = reinterpret_cast<float4*>(a.part_o + prow * kMlaDv + cta * kMlaDvHalf + c);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            po[i >> 2] = make_float4(__uint_as_float(ov[i]), __uint_as_float(ov[i + 1]), __uint_as_float(ov[i + 2]), __uint_as_float(ov[i + 3]));
-        } else if (row < rows_here) {
-          uint8_t* prow_s = kv_s + (c >> 6) * kMlaQPanelBytes + row * 128;
-          const int ch0 = (c & 63) >> 3;               // first of this iteration's four 16-byte chunks in the 128-byte row
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(ov[i + 0]), __uint_as_float(ov[i + 1]));
-            w.y = pack_bf16x2(__uint_as_float(ov[i + 2]), __uint_as_float(ov[i + 3]));
-            w.z = pack_bf16x2(__uint_as_float(ov[i + 4]), __uint_as_float(ov[i + 5]));
-            w.w = pack_bf16x2(__uint_as_float(ov[i + 6]), __uint_as_float(ov[i + 7]));
-            if (by_tma) *reinterpret_cast<uint4*>(prow_s + (((ch0 + (i >> 3)) ^ (row & 7)) << 4)) = w;
-            else *reinterpret_cast<uint4*>(orow + c + i) = w;
-          }
-        }
-      }
     }
     if (by_tma) {                                      // every softmax thread comes here, whatever became of its waits
       fence_async_smem();                              // the store below reads the panel through the async proxy

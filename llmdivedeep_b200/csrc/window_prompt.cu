@@ -26,6 +26,7 @@ struct PromptPlan {
   int blocks, blk_lo;                                  // blocks of the job (-1: there are no more jobs), and which is its first
   int full0, full1;                                    // keys that every row sees which sees any (one sequence in the unit)
   int row0, rows, part, tok0;                          // first query row, rows, part (-1: a whole unit), token of the first row
+  int job, pad[3];
   int4 sees[kWpTokens];                                // of the unit's tokens: {a0, a1, b0, b1}
   int4 segs[kWpSegs + 1];                              // {first key, end, blocks before, tokens of the unit that it is for}
 };
@@ -34,7 +35,9 @@ constexpr int kWpOffBars = kMlaBufs * kMlaKBytes + 2 * kMlaXBytes;
 constexpr int kWpOffPm = kWpOffBars + 640;
 constexpr int kWpOffSums = kWpOffPm + kMlaPairBytes;   // [4][128] (m, l)
 constexpr int kWpOffPlans = kWpOffSums + 4 * 128 * 8;
-constexpr int kWpSmem = kWpOffPlans + kWpPlans * (int)sizeof(PromptPlan);
+constexpr int kWpOffRedo = kWpOffPlans + kWpPlans * (int)sizeof(PromptPlan);
+constexpr int kWpRedo = 48;                            // quadrants of jobs that a warp has on its list of rows to be done key by key
+constexpr int kWpSmem = kWpOffRedo + 4 * kWpRedo * 8;
 static_assert(kWpSmem <= 232448 && sizeof(PromptPlan) % 16 == 0, "shared memory budget of one CTA");
 
 __device__ __forceinline__ float dot_bf16x2(uint32_t x, uint32_t y, float d) {
@@ -91,6 +94,20 @@ __device__ __forceinline__ int build_segs(const WinArgs& a, int n_tok, PromptPla
   return blocks;
 }
 
+// A job: a whole unit, or a part of the keys of one.
+struct JobRows {
+  int part, n_split, split, row0, rows;                // part < 0: a whole unit
+};
+__device__ __forceinline__ JobRows job_rows(const WinArgs& a, int job) {
+  JobRows j;
+  j.part = job < a.n_full ? -1 : job - a.n_full;
+  j.n_split = j.part < 0 ? 1 : a.n_split;
+  j.split = j.part < 0 ? 0 : j.part % j.n_split;
+  j.row0 = (j.part < 0 ? job : a.n_full + j.part / j.n_split) * a.unit_rows;
+  j.rows = min(a.unit_rows, a.seq_rows - j.row0);
+  return j;
+}
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWpThreads, 1)
 window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ CUtensorMap tmap_lat,
                      const __grid_constant__ CUtensorMap tmap_rope, const WinArgs a, const int jobs) {
@@ -120,7 +137,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   uint64_t* sums_free = bars + 74;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 75);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* odd_s = abort_flag + 1;              // [4 quadrants]
+  uint32_t* odd_s = tmem_slot + 2;                   // [4 quadrants] rows with a key that they do not see and that is no number
   uint16_t* pm_s = reinterpret_cast<uint16_t*>(smem + kWpOffPm);         // block maxima, rounded up to bf16
   float2* sums_s = reinterpret_cast<float2*>(smem + kWpOffSums);
   PromptPlan* plans = reinterpret_cast<PromptPlan*>(smem + kWpOffPlans);
@@ -275,7 +292,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (lane == 0) mbar_expect_tx(&recv_full[warp], kMlaXWarp);
         if (!(ok = wait(&pm_full[set * 4 + qd], ph))) break;
         m = raise(m_prev, pair_max(pm_of(n)));
-        if (m != m_own) l = m_own == -CUDART_INF_F ? 0.f : l * fast_exp2(m_own - m);
+        if (m != m_own && m_own != -CUDART_INF_F) l *= fast_exp2(m_own - m);      // (without a reference l is 0, or NaN, and stays so)
         bool waited_pv = n == 0;
         if (__any_sync(0xffffffffu, m != m_prev) && begun) {
           // O must be quiescent: P.V of the previous block has to be complete.  This thread scales its half of the columns.
@@ -320,9 +337,10 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       base += blocks;
       if (k > 0 && !(ok = wait(sums_free, k - 1))) break;
       sums_s[(warp >> 2) * 128 + row] = make_float2(m, l);
-      if (odd) odd_s[qd] = 1;
+      const uint32_t odds = __ballot_sync(0xffffffffu, odd);
       __syncwarp();
       if (lane == 0) {
+        if (odds) atomicOr(odd_s + qd, odds);
         mbar_arrive(sums_full);
         mbar_arrive(&plan_free[k % kWpPlans]);
       }
@@ -333,6 +351,8 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const int qd = warp & 3, row = qd * 32 + lane;
     const uint32_t t_row = tmem + (uint32_t(qd * 32) << 16);
     bool ok = true;
+    uint2* redo_s = reinterpret_cast<uint2*>(smem + kWpOffRedo) + qd * kWpRedo;
+    int redos = 0;
     auto give_back = [&](uint32_t e) {                 // the four warps are done with a buffer
       named_bar_sync(1, 128);
       if (warp == kWpOutWarp && lane == 0) mbar_arrive(&ring_free[e % NB]);
@@ -345,14 +365,14 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       ok = wait(sums_full, k) && wait(o_final, k) && wait(&ring_full[e % NB], e / NB);
       if (!ok) return;
       tc_fence_after();
-      const bool odd = odd_s[qd] != 0;
+      const uint32_t odd = odd_s[qd];
       float mt = -CUDART_INF_F, l = 0.f;
 #pragma unroll
       for (int u = 0; u < 4; ++u) mt = fmaxf(mt, sums_s[u * 128 + row].x);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float2 ml = sums_s[u * 128 + row];
-        if (ml.x != -CUDART_INF_F) l += ml.y * fast_exp2(ml.x - mt);
+        l += ml.x != -CUDART_INF_F ? ml.y * fast_exp2(ml.x - mt) : ml.y;
       }
       __syncwarp();
       if (lane == 0) {
@@ -361,10 +381,16 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       }
       if (!any) l = 0.f;                               // a block that every other row sees is not masked
       const float inv = l > 0.f ? 1.f / l : l;         // (a NaN stays one)
-      const bool by_tma = part < 0 && qd * 32 + 32 <= rows && !odd;
-      if (part >= 0 && !odd)                           // what this CTA's half of the columns is weighted with
+      const bool by_tma = part < 0 && qd * 32 + 32 <= rows;
+      // A key that a row does not see and that is no number has come in through 0 x NaN, unless the row is none anyway: done again when all jobs are done.
+      const uint32_t again = __ballot_sync(0xffffffffu, (odd >> lane & 1u) && any && l == l);
+      if (again) {
+        if (lane == 0 && redos < kWpRedo) redo_s[redos] = make_uint2(p.job, again);
+        ++redos;
+      }
+      if (part >= 0)                                   // what this CTA's half of the columns is weighted with
         a.part_lse[((int64_t)part * 2 + cta) * 128 + row] = l > 0.f ? mt + log2f(l) : l == 0.f ? -CUDART_INF_F : l;
-      if (!odd) {
+      {
         uint8_t* const stage0 = smem + (e % NB) * kMlaKBytes + qd * 8192 + lane * 128;      // two panels of 32 rows to a warp
         __nv_bfloat16* const orow = a.out + (int64_t)(row0 + row) * kMlaDv + cta * kMlaDvHalf;
         const uint64_t inv2 = pack_f32x2(inv, inv);
@@ -433,56 +459,6 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
-      if (odd) {
-        // Rare: among the keys of a row's blocks there is one that it does not see and that is no number.  The quadrant's rows key by key over what they
-        // see of this job's blocks: this CTA's half of the output from whole scores.
-#pragma unroll 1
-        for (int r = qd * 32; r < min(rows, qd * 32 + 32); ++r) {
-          const int tok = (row0 + r) / a.H - p.tok0;
-          const int4 sees = p.sees[tok];
-          // a lane has values 8 lane .. of either half of the latent and two rope values
-          const uint4* qp = reinterpret_cast<const uint4*>(a.q + (int64_t)(row0 + r) * kMlaDqk);
-          const uint4 q0 = __ldg(qp + lane), q1 = __ldg(qp + 32 + lane);
-          const uint32_t qr = __ldg(reinterpret_cast<const uint32_t*>(qp + 64) + lane);
-          float rm = -CUDART_INF_F, rl = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          int at = 0;
-#pragma unroll 1
-          for (int n = 0; n < 2 * p.blocks; ++n) {
-            const int blk = p.blk_lo + (n >> 1);
-            const int4 s = seg_of(p, at, blk);
-            const int k0 = s.x + (blk - s.z) * kMlaBlk + 32 * (n & 1);
-            uint32_t todo = (range_bits(sees.x, sees.y, k0) | range_bits(sees.z, sees.w, k0)) & low_bits(s.y - k0);
-            if (tok < (s.w & 0xffff) || tok > (s.w >> 16)) todo = 0;
-#pragma unroll 1
-            for (; todo; todo &= todo - 1) {
-              const uint4* kp = reinterpret_cast<const uint4*>(a.kv + (int64_t)(k0 + __ffs(todo) - 1) * (kMlaDqk * 2));
-              const uint4 v0 = __ldg(kp + lane), v1 = __ldg(kp + 32 + lane);
-              float d = dot_bf16x2(qr, __ldg(reinterpret_cast<const uint32_t*>(kp + 64) + lane), 0.f);
-              d = dot_bf16x2(q0.x, v0.x, d); d = dot_bf16x2(q0.y, v0.y, d); d = dot_bf16x2(q0.z, v0.z, d); d = dot_bf16x2(q0.w, v0.w, d);
-              d = dot_bf16x2(q1.x, v1.x, d); d = dot_bf16x2(q1.y, v1.y, d); d = dot_bf16x2(q1.z, v1.z, d); d = dot_bf16x2(q1.w, v1.w, d);
-#pragma unroll
-              for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-              const float sc = d * a.scale_log2e, mx = fmaxf(rm, sc), ref = mx == -CUDART_INF_F ? 0.f : mx;
-              const float keep = rm == -CUDART_INF_F ? 0.f : exp2f(rm - ref), pr = exp2f(sc - ref);
-              const uint32_t mine[4] = {cta ? v1.x : v0.x, cta ? v1.y : v0.y, cta ? v1.z : v0.z, cta ? v1.w : v0.w};
-              rm = mx;
-              rl = rl * keep + pr;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) o[i] = o[i] * keep + pr * __uint_as_float(i & 1 ? mine[i >> 1] & 0xffff0000u : mine[i >> 1] << 16);
-            }
-          }
-          const float ri = rl > 0.f ? 1.f / rl : rl;
-          if (part >= 0) {
-            float4* po = reinterpret_cast<float4*>(a.part_o + ((int64_t)part * 128 + r) * kMlaDv + cta * kMlaDvHalf + lane * 8);
-            po[0] = make_float4(o[0] * ri, o[1] * ri, o[2] * ri, o[3] * ri);
-            po[1] = make_float4(o[4] * ri, o[5] * ri, o[6] * ri, o[7] * ri);
-            if (lane == 0) a.part_lse[((int64_t)part * 2 + cta) * 128 + r] = rl > 0.f ? rm + log2f(rl) : rl == 0.f ? -CUDART_INF_F : rl;
-          } else {
-            reinterpret_cast<uint4*>(a.out + (int64_t)(row0 + r) * kMlaDv + cta * kMlaDvHalf)[lane] =
-                make_uint4(pack_bf16x2(o[0] * ri, o[1] * ri), pack_bf16x2(o[2] * ri, o[3] * ri), pack_bf16x2(o[4] * ri, o[5] * ri), pack_bf16x2(o[6] * ri, o[7] * ri));
-          }
-        }
-      }
       plan_done(k);
       if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the buffer may be written again
       __syncwarp();
@@ -521,7 +497,71 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       e += n + (k > 0);
     }
     if (ok && k > 0) drain(k - 1, e);
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+    // Rare: rows key by key over what they see of their job's blocks, this CTA's half of the output from whole scores.  Nobody waits for this warp now (but at the
+    // barrier that the pair leaves through, which has no limit).  With more on the list than it holds: every row of the pair's jobs.
+    const int redo_jobs = redos > kWpRedo ? (jobs - pair + n_pairs - 1) / n_pairs : redos;
+#pragma unroll 1
+    for (int x = 0; ok && x < redo_jobs; ++x) {
+      const int job = redos > kWpRedo ? pair + x * n_pairs : (int)redo_s[x].x;
+      uint32_t mask = redos > kWpRedo ? 0xffffffffu : redo_s[x].y;
+      PromptPlan& p = plans[qd];                       // each warp its own; of the jobs' plans nobody needs more than `blocks`
+      const JobRows j = job_rows(a, job);
+      if (j.rows < qd * 32 + 32) mask &= low_bits(j.rows - qd * 32);
+      __syncwarp();
+      if (lane == 0) p.tok0 = j.row0 / a.H;
+      __syncwarp();
+      const int blocks = build_segs(a, (j.row0 + j.rows - 1) / a.H - j.row0 / a.H + 1, p);
+      __syncwarp();
+      const int per = (blocks + j.n_split - 1) / j.n_split, blk_lo = min(blocks, j.split * per), n_blk = min(blocks, blk_lo + per) - blk_lo;
+#pragma unroll 1
+      for (; mask; mask &= mask - 1) {
+        const int r = qd * 32 + __ffs(mask) - 1, tok = (j.row0 + r) / a.H - p.tok0;
+        const int4 sees = p.sees[tok];
+        // a lane has values 8 lane .. of either half of the latent and two rope values
+        const uint4* qp = reinterpret_cast<const uint4*>(a.q + (int64_t)(j.row0 + r) * kMlaDqk);
+        const uint4 q0 = __ldg(qp + lane), q1 = __ldg(qp + 32 + lane);
+        const uint32_t qr = __ldg(reinterpret_cast<const uint32_t*>(qp + 64) + lane);
+        float rm = -CUDART_INF_F, rl = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        int at = 0;
+#pragma unroll 1
+        for (int n = 0; n < 2 * n_blk; ++n) {
+          const int blk = blk_lo + (n >> 1);
+          const int4 s = seg_of(p, at, blk);
+          const int k0 = s.x + (blk - s.z) * kMlaBlk + 32 * (n & 1);
+          uint32_t todo = (range_bits(sees.x, sees.y, k0) | range_bits(sees.z, sees.w, k0)) & low_bits(s.y - k0);
+          if (tok < (s.w & 0xffff) || tok > (s.w >> 16)) todo = 0;
+#pragma unroll 1
+          for (; todo; todo &= todo - 1) {
+            const uint4* kp = reinterpret_cast<const uint4*>(a.kv + (int64_t)(k0 + __ffs(todo) - 1) * (kMlaDqk * 2));
+            const uint4 v0 = __ldg(kp + lane), v1 = __ldg(kp + 32 + lane);
+            float d = dot_bf16x2(qr, __ldg(reinterpret_cast<const uint32_t*>(kp + 64) + lane), 0.f);
+            d = dot_bf16x2(q0.x, v0.x, d); d = dot_bf16x2(q0.y, v0.y, d); d = dot_bf16x2(q0.z, v0.z, d); d = dot_bf16x2(q0.w, v0.w, d);
+            d = dot_bf16x2(q1.x, v1.x, d); d = dot_bf16x2(q1.y, v1.y, d); d = dot_bf16x2(q1.z, v1.z, d); d = dot_bf16x2(q1.w, v1.w, d);
+#pragma unroll
+            for (int y = 16; y > 0; y >>= 1) d += __shfl_xor_sync(0xffffffffu, d, y);
+            const float sc = d * a.scale_log2e, mx = fmaxf(rm, sc), ref = mx == -CUDART_INF_F ? 0.f : mx;
+            const float keep = rm == -CUDART_INF_F ? 0.f : exp2f(rm - ref), pr = exp2f(sc - ref);
+            const uint32_t mine[4] = {cta ? v1.x : v0.x, cta ? v1.y : v0.y, cta ? v1.z : v0.z, cta ? v1.w : v0.w};
+            rm = mx;
+            rl = rl * keep + pr;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = o[i] * keep + pr * __uint_as_float(i & 1 ? mine[i >> 1] & 0xffff0000u : mine[i >> 1] << 16);
+          }
+        }
+        const float ri = rl > 0.f ? 1.f / rl : rl;
+        if (j.part >= 0) {
+          float4* po = reinterpret_cast<float4*>(a.part_o + ((int64_t)j.part * 128 + r) * kMlaDv + cta * kMlaDvHalf + lane * 8);
+          po[0] = make_float4(o[0] * ri, o[1] * ri, o[2] * ri, o[3] * ri);
+          po[1] = make_float4(o[4] * ri, o[5] * ri, o[6] * ri, o[7] * ri);
+          if (lane == 0) a.part_lse[((int64_t)j.part * 2 + cta) * 128 + r] = rl > 0.f ? rm + log2f(rl) : rl == 0.f ? -CUDART_INF_F : rl;
+        } else {
+          reinterpret_cast<uint4*>(a.out + (int64_t)(j.row0 + r) * kMlaDv + cta * kMlaDvHalf)[lane] =
+              make_uint4(pack_bf16x2(o[0] * ri, o[1] * ri), pack_bf16x2(o[2] * ri, o[3] * ri), pack_bf16x2(o[4] * ri, o[5] * ri), pack_bf16x2(o[6] * ri, o[7] * ri));
+        }
+      }
+    }
   } else {
     regs_dec<kWpRegsRoles>();
     if (warp == kWpMmaWarp) {
@@ -714,14 +754,13 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           }
           break;
         }
-        const int part = job < a.n_full ? -1 : job - a.n_full;         // >= 0: a part of a unit's keys
-        const int n_split = part < 0 ? 1 : a.n_split, unit = part < 0 ? job : a.n_full + part / n_split, split = part < 0 ? 0 : part % n_split;
-        const int row0 = unit * a.unit_rows, rows = min(a.unit_rows, a.seq_rows - row0), tok0 = row0 / a.H;
+        const JobRows j = job_rows(a, job);
+        const int row0 = j.row0, rows = j.rows, part = j.part, tok0 = row0 / a.H;
         __syncwarp();
         if (lane == 0) p.tok0 = tok0;
         __syncwarp();
         const int blocks = build_segs(a, (row0 + rows - 1) / a.H - tok0 + 1, p);
-        const int per = (blocks + n_split - 1) / n_split, blk_lo = min(blocks, split * per), n = min(blocks, blk_lo + per) - blk_lo;
+        const int per = (blocks + j.n_split - 1) / j.n_split, blk_lo = min(blocks, j.split * per), n = min(blocks, blk_lo + per) - blk_lo;
         if (n == 0) {                                    // nothing seen: zeros (a part: weight zero when they are merged)
           if (part < 0) {
             for (int r = 0; r < rows; ++r)
@@ -733,7 +772,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         }
         if (lane == 0) {
           p.blocks = n; p.blk_lo = blk_lo;
-          p.row0 = row0; p.rows = rows; p.part = part;
+          p.row0 = row0; p.rows = rows; p.part = part; p.job = job;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&plan_full[k % kWpPlans]);

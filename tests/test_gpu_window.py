@@ -35,6 +35,7 @@ def i32(x):
 @pytest.mark.parametrize("T,S,H,window,first", [
     (1, 1, 128, 1, 0), (1, 1, 1, 5, 3), (40, 40, 128, 128, 4), (130, 300, 128, 64, 0), (7, 500, 128, 200, 70), (200, 200, 16, 50, 4), (77, 400, 16, 130, 64),
     (300, 300, 1, 40, 3), (50, 90, 3, 33, 5), (33, 700, 64, 128, 128), (9, 2100, 8, 2048, 4), (5, 130, 256, 100, 1), (7, 150, 192, 64, 0), (21, 333, 100, 65, 2),
+    (400, 400, 128, 5, 2), (500, 500, 128, 64, 0), (300, 3000, 128, 130, 4), (131, 400, 2, 70, 1),
     (65, 65, 32, 1, 0), (64, 1000, 40, 1000, 0), (3, 200, 128, 1 << 30, 0), (3, 200, 16, 7, 1 << 30), (150, 5000, 128, 4096, 4), (2, 9000, 16, 1 << 31, 0),
 ])
 def test_prompts(T, S, H, window, first):
@@ -114,6 +115,56 @@ def test_what_a_row_does_not_see_leaves_it_as_it_is(H, bad):
         touched = sees[:, at].cuda()
         assert bool((~out[touched].isfinite()).flatten(1).any(1).all())
         check(out[~touched], D.attend(q, kv, sees, SCALE).cuda()[~touched])
+
+
+@pytest.mark.parametrize("H", [16, 40])
+def test_numbers_that_are_none_in_parts(H):
+    """Few rows over many keys: the keys are cut into parts, and a part's rows are done again by themselves."""
+    q, kv = rows(20, H, seed=3), rows(900, seed=4)
+    sees = D.prompt_sees(20, 900, 600, 70)
+    want = D.attend(q, kv, sees, SCALE)
+    for at in (282, 290, 300, 885, 899):
+        dirty = kv.clone()
+        dirty[at, 40], dirty[at, 400] = float("nan"), float("inf")
+        out = ops.window_mla_prefill(q, dirty, None, None, 600, 70, SCALE)
+        ops.check_status("cuda")
+        touched = sees[:, at].cuda()
+        assert bool((~out[touched].isfinite()).flatten(1).any(1).all())
+        check(out[~touched], want[~touched])
+
+
+@pytest.mark.parametrize("T", [600, 7402])
+def test_numbers_that_are_none_in_every_unit(T):
+    """Every second key is none, every row sees itself alone: as many rows to be done again as there are units, more than a list of them holds."""
+    q, kv = rows(T, 64, seed=1), rows(T, seed=2)
+    kv[1::2] = float("nan")
+    out = ops.window_mla_prefill(q, kv, None, None, 1, 0, SCALE)
+    ops.check_status("cuda")
+    assert torch.equal(out[::2], kv[::2, None, :512].expand(-1, 64, -1)) and bool(out[1::2].isnan().all())
+
+
+def test_a_query_that_is_no_number_is_its_rows_own_affair():
+    q, kv = rows(300, 16, seed=1), rows(3000, seed=2)
+    want = ops.window_mla_prefill(q, kv, None, None, 2000, 4, SCALE)
+    dirty = q.clone()
+    dirty[7, 3], dirty[120] = float("nan"), float("inf")
+    out = ops.window_mla_prefill(dirty, kv, None, None, 2000, 4, SCALE)
+    ops.check_status("cuda")
+    keep = torch.ones(300, 16, dtype=torch.bool, device="cuda")
+    keep[7, 3], keep[120] = False, False
+    assert torch.equal(out[keep], want[keep]) and bool((~out[~keep].isfinite()).any(-1).all())
+
+
+def test_keys_past_two_gigabytes():
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("needs 8 GB")
+    S = 2000000
+    far, near, q = torch.empty(S, 576, dtype=torch.bfloat16, device="cuda"), rows(300, seed=5), rows(20, 16, seed=6)
+    far[:10], far[-290:] = near[:10], near[10:]
+    far[10:-290] = float("nan")
+    out = ops.window_mla_prefill(q, far, None, None, 250, 10, SCALE)
+    ops.check_status("cuda")
+    check(out, D.attend(q, near, D.prompt_sees(20, 300, 250, 10), SCALE))
 
 
 def test_other_strides_streams_and_a_graph():
@@ -242,6 +293,36 @@ def test_records_that_are_no_numbers(record, H, per, tree):
         touched[b * per:(b + 1) * per] = sees[b * per:(b + 1) * per, pos]
         assert bool(out[touched.cuda()].isnan().flatten(1).any(1).all())
         check(out[~touched.cuda()], clean[~touched.cuda()])
+
+
+@pytest.mark.parametrize("record", [656, 416])
+@pytest.mark.parametrize("H", [128, 16])
+def test_records_that_are_no_numbers_in_parts(record, H):
+    c = Case(2, 5, H, [1500, 900], record, seed=H, tree=True)
+    sees, clean = c.sees(1 << 20, 0), c.want(1 << 20, 0)
+    for b, pos in ((0, 1496), (0, 1498), (1, 896), (1, 300)):
+        dirty = c.args()
+        dirty["cache"] = c.rec.clone()
+        dirty["cache"][int(c.table[b, pos // 64]) * 64 + pos % 64] = 255
+        out = ops.window_mla_decode_paged(**dirty, window=1 << 20, first=0, scale=SCALE)
+        ops.check_status("cuda")
+        touched = torch.zeros(10, dtype=torch.bool)
+        touched[b * 5:(b + 1) * 5] = sees[b * 5:(b + 1) * 5, pos]
+        assert bool(out[touched.cuda()].isnan().flatten(1).any(1).all())
+        check(out[~touched.cuda()], clean[~touched.cuda()])
+
+
+@pytest.mark.parametrize("record", [656, 416])
+@pytest.mark.parametrize("B", [1, 3, 5, 9, 30])
+@pytest.mark.parametrize("H", [64, 128, 200])
+def test_units_of_fewer_rows_and_parts(record, B, H):
+    """Small calls: units of 32, 64 and 128 rows, up to sixteen parts, room for some of them."""
+    c = Case(B, 1, H, ([1100, 1, 700, 0, 64, 1100, 129, 1000, 500] * 4)[:B], record, seed=B + H)
+    want = c.want(1000, 70)
+    for room in (0, 3000000, None):
+        ws = None if room is None else torch.empty(room, dtype=torch.uint8, device="cuda")
+        check(ops.window_mla_decode_paged(**c.args(), window=1000, first=70, scale=SCALE, workspace=ws), want)
+    ops.check_status("cuda")
 
 
 def test_bad_lengths_and_pages_are_flagged_and_skipped():
