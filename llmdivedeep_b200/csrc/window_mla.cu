@@ -24,12 +24,6 @@ struct WinCfg {
   static_assert(kSmem <= 232448 && kOffRaw % 16 == 0, "shared memory budget of one CTA");
 };
 
-// which of the 32 keys from k0 on have their bit set, bit j at `at` + j
-__device__ __forceinline__ uint32_t draft_bits(uint64_t bits, int at, int k0) {
-  const int sh = k0 - at;
-  return sh >= 64 || sh <= -32 ? 0u : sh >= 0 ? static_cast<uint32_t>(bits >> sh) : static_cast<uint32_t>(bits) << -sh;
-}
-
 template <int SRC>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMlaThreads, 1)
 window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o, const WinArgs a) {
@@ -89,22 +83,10 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     tmem_alloc(tmem_slot, kMlaTmemCols);
     tmem_relinquish();
   }
-  // Keys by slots, the first tokens' [0, head) and behind them the windows' [shift + head, ...): slot j is position j or j + shift.
   const Drafts dr = drafts_of(a.drafts, seq);
-  int head = 0, shift = 0, n_slots = 0, full0 = 0, full1 = 0;
   if (dr.bad && threadIdx.x == 0 && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
-  if (tok0 < dr.m) {
-    const bool tree = a.drafts.tree != nullptr;
-    const int P = dr.ctx - dr.m, hi = P + min(tok1, dr.m - 1) + 1, near = P + 1 + (tree ? 0 : tok0), lo = max(0, near - a.window);
-    const int least = tree ? P : near;                 // positions up to here are seen by every row
-    head = min(a.first, hi);
-    if (lo <= head) head = 0;
-    else shift = lo - head;
-    n_slots = hi - shift;
-    full0 = max(min(a.first, hi), hi - a.window);      // (of a tree: its path may be shorter)
-    full0 = full0 <= min(a.first, least) ? 0 : full0 - shift;
-    full1 = least - shift;
-  }
+  const Slots sl = slots_of(a, dr, tok0, tok1);
+  const int head = sl.head, shift = sl.shift, n_slots = sl.n, full0 = sl.full0, full1 = sl.full1;
   const int blocks = (n_slots + kMlaBlk - 1) / kMlaBlk;
   const int per = (blocks + n_split - 1) / n_split, blk_lo = min(blocks, split * per), nblk = min(blocks, blk_lo + per) - blk_lo;
   // The records of 64 slots a block, each gather warp every eleventh: raw into shared memory two blocks ahead (cp.async), then to bf16.  The first two
@@ -669,6 +651,69 @@ static int launch_window(WinArgs a, int64_t units, int64_t keys, void* workspace
   return check_launch("window_mla");
 }
 
+// ---- drafts of many rows: records to bf16 rows once, for all of a sequence's units -------------------------------------
+// Slots of every sequence (those of all its drafts) -> rows [B * pad, 576], and a bit for each that has a page.  A warp for eight slots.
+constexpr int kRowsSlots = 8;
+template <int SRC>
+__global__ void __launch_bounds__(256) window_rows_kernel(const WinArgs a, const uint8_t* __restrict__ cache, uint4* __restrict__ rows, int B) {
+  constexpr int kBytes = SRC == kSrc4 ? kLatent4Bytes : kLatentTokenBytes;
+  const int lane = threadIdx.x & 31, per = a.pad / kRowsSlots;
+  const int64_t job = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int b = (int)(job / per), j0 = (int)(job - (int64_t)b * per) * kRowsSlots;
+  if (b >= B) return;
+  const Drafts dr = drafts_of(a.drafts, b);
+  if (dr.bad && j0 == 0 && lane == 0 && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+  const Slots sl = slots_of(a, dr, 0, a.drafts.per_seq - 1);
+  if (j0 >= sl.n) return;
+  int id = -1;
+  if (lane < kRowsSlots && j0 + lane < sl.n) {
+    const int pos = j0 + lane < sl.head ? j0 + lane : j0 + lane + sl.shift;
+    const int page = __ldg(a.block_table + (int64_t)b * a.table_stride + pos / kLatentPage);
+    if (page >= 0 && (int64_t)(page + 1) * kLatentPage <= a.num_phys_rows) id = page * kLatentPage + pos % kLatentPage;
+    else if (a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+  }
+  const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
+  if (lane == 0) reinterpret_cast<uint8_t*>(a.valid)[((int64_t)b * a.pad + j0) / 8] = (uint8_t)have;
+  uint4* out = rows + ((int64_t)b * a.pad + j0) * (kMlaDqk / 8);
+#pragma unroll 4
+  for (int j = 0; j < kRowsSlots; ++j) {
+    const int r = __shfl_sync(0xffffffffu, id, j);
+    if (j0 + j >= sl.n) break;
+    uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    uint32_t rope = 0;
+    if (r >= 0) {
+      const uint8_t* rec = cache + (int64_t)r * kBytes;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {                    // a lane has values 8 lane .. of either half
+        if constexpr (SRC == kSrcFp8) {
+          v[h] = e4m3x8_to_bf16(__ldg(reinterpret_cast<const uint2*>(rec + h * 256 + lane * 8)), __ldg(reinterpret_cast<const float*>(rec + 512) + h * 2 + (lane >> 4)));
+        } else {
+          const uint8_t* half = rec + h * kLatent4Half;
+          uint32_t p[4];
+          latent4_codes(__ldg(reinterpret_cast<const uint32_t*>(half) + lane), p);
+          const uint32_t sc = latent4_scale(__ldg(half + kLatent4Scales + (lane >> 1)));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = mul_bf16x2(mul_bf16x2(p[i], sc), kLatent4GainPair);      // both exact
+          v[h] = make_uint4(p[0], p[1], p[2], p[3]);
+        }
+      }
+      rope = SRC == kSrcFp8 ? __ldg(reinterpret_cast<const uint32_t*>(rec + 528) + lane)
+                            : __ldg(reinterpret_cast<const uint32_t*>(rec + (lane >> 4) * kLatent4Half + kLatent4Rope) + (lane & 15));
+    }
+    out[j * (kMlaDqk / 8) + lane] = v[0];
+    out[j * (kMlaDqk / 8) + 32 + lane] = v[1];
+    reinterpret_cast<uint32_t*>(out + j * (kMlaDqk / 8) + 64)[lane] = rope;
+  }
+}
+constexpr int kRowsUnits = 4;                          // units of 128 rows from which on a sequence's records are made rows first
+constexpr int64_t kRowsMost = 512ll << 20;             // bytes of rows at most
+static int rows_pad(int64_t keys) { return (int)((keys + 63) / 64 * 64); }
+// Bytes of the rows, 0: not this way.
+static int64_t rows_bytes(int B, int64_t seq_rows, int64_t keys) {
+  const int64_t bytes = (int64_t)B * rows_pad(keys) * (kMlaDqk * 2);
+  return seq_rows > (kRowsUnits - 1) * 128 && bytes <= kRowsMost ? bytes : 0;
+}
+
 // Rows of a unit.  Calls that leave most pairs idle have fewer: a block's exchange and softmax take less time, and there are more units to share its keys.
 static int decode_unit_rows(int B, int64_t seq_rows) {
   const int pairs = max(1, sm_count() / 2);
@@ -689,6 +734,8 @@ size_t window_mla_decode_workspace(int B, int tokens_per_seq, int H, int window,
     const int parts = window_parts(units, keys);
     if (parts > 1) most = max(most, (size_t)(units % max(1, sm_count() / 2)) * parts * kWinPartBytes);
   }
+  const int64_t slots = min((int64_t)max_ctx, (int64_t)window + first + tokens_per_seq), rows = rows_bytes(B, seq_rows, slots);
+  if (rows) most = max(most, (size_t)rows + (size_t)B * rows_pad(slots) / 8 + 256 + window_prompt_drafts_workspace(B, seq_rows, H, keys));
   return most;
 }
 
@@ -708,6 +755,20 @@ int window_mla_decode_launch(const void* q, const void* cache, int record_bytes,
   a.scale_log2e = scale * 1.4426950408889634f;
   a.status = status;
   a.seq_rows = tokens_per_seq * H;
+  const int64_t slots = min((int64_t)max_ctx, (int64_t)window + first + tokens_per_seq), rows = rows_bytes(B, a.seq_rows, slots);
+  if (rows && workspace) {
+    a.pad = rows_pad(slots);
+    const size_t valid = ((size_t)B * a.pad / 8 + 255) / 256 * 256;
+    if (workspace_bytes >= rows + valid) {
+      a.valid = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + rows);
+      const unsigned grid = (unsigned)(((int64_t)B * (a.pad / kRowsSlots) + 7) / 8);
+      auto kern = record_bytes == kLatent4Bytes ? window_rows_kernel<kSrc4> : window_rows_kernel<kSrcFp8>;
+      kern<<<grid, 256, 0, stream>>>(a, a.kv, static_cast<uint4*>(workspace), B);
+      a.kv = static_cast<const uint8_t*>(workspace);
+      a.S = B * a.pad;
+      return window_prompt_drafts(a, static_cast<uint8_t*>(workspace) + rows + valid, workspace_bytes - rows - valid, stream);
+    }
+  }
   a.unit_rows = decode_unit_rows(B, a.seq_rows);
   a.seq_units = (a.seq_rows - 1) / a.unit_rows + 1;
   const int64_t units = (int64_t)B * a.seq_units, keys = window_keys(H, window, first, tokens_per_seq, max_ctx);

@@ -30,6 +30,9 @@ struct WinArgs {
   float* part_o;                  // [parts, 128, 512] fp32 normalised partial outputs
   float* part_lse;                // [parts, 2, 128] their log2-sum-exp as each CTA of the pair has it (-inf: nothing seen)
   int tma_out;                    // the output tensor map is valid: full units leave through TMA stores
+  // drafts over rows that were made bf16 first: kv is [B * pad] rows, slot j of sequence b row b * pad + j, with a bit for each that has a page
+  int pad;
+  uint32_t* valid;
 };
 
 // What a row sees: two stretches of positions, a1 <= b0, and single ones behind `at`.
@@ -136,6 +139,33 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 // which of the 32 keys from k0 on are in [lo, hi)
 __device__ __forceinline__ uint32_t range_bits(int lo, int hi, int k0) { return low_bits(hi - k0) & ~low_bits(lo - k0); }
 
+// which of the 32 keys from k0 on have their bit set, bit j at `at` + j
+__device__ __forceinline__ uint32_t draft_bits(uint64_t bits, int at, int k0) {
+  const int sh = k0 - at;
+  return sh >= 64 || sh <= -32 ? 0u : sh >= 0 ? static_cast<uint32_t>(bits >> sh) : static_cast<uint32_t>(bits) << -sh;
+}
+
+// The keys of tokens tok0 .. tok1 of a sequence by slots: the first tokens' [0, head) and behind them the windows' [shift + head, ...); slot j is
+// position j, from head on j + shift.  Slots [full0, full1) are seen by all of these tokens.
+struct Slots {
+  int head, shift, n, full0, full1;
+};
+__device__ __forceinline__ Slots slots_of(const WinArgs& a, const Drafts& dr, int tok0, int tok1) {
+  Slots s{};
+  if (tok0 >= dr.m) return s;
+  const bool tree = a.drafts.tree != nullptr;
+  const int P = dr.ctx - dr.m, hi = P + min(tok1, dr.m - 1) + 1, near = P + 1 + (tree ? 0 : tok0), lo = max(0, near - a.window);
+  const int least = tree ? P : near;                   // positions up to here are seen by every row
+  s.head = min(a.first, hi);
+  if (lo <= s.head) s.head = 0;
+  else s.shift = lo - s.head;
+  s.n = hi - s.shift;
+  s.full0 = max(min(a.first, hi), hi - a.window);      // (of a tree: its path may be shorter)
+  s.full0 = s.full0 <= min(a.first, least) ? 0 : s.full0 - s.shift;
+  s.full1 = least - s.shift;
+  return s;
+}
+
 // Units run in rounds of one to a pair of SMs.  The keys of a partly filled last round's units are cut into parts, as many as there are pairs for.
 constexpr int kWinMaxParts = 16;
 constexpr int kWinPartBlocks = 2;                      // blocks of a part at least
@@ -174,6 +204,9 @@ inline void window_plan(WinArgs& a, int64_t units, int64_t keys, void* workspace
     a.part_lse = a.part_o + (size_t)rest * ns * 128 * kMlaDv;
   }
 }
+// Drafts of sequences over rows that were made bf16 first (window_prompt.cu); a.kv and what goes with it is set.
+int window_prompt_drafts(WinArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+size_t window_prompt_drafts_workspace(int B, int64_t seq_rows, int H, int64_t keys);
 // The kernel that merges the parts of units n_full .. of `units` (window_mla.cu).
 void window_combine(const WinArgs& a, int64_t units, cudaStream_t stream);
 int make_tmap_2d_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t inner_bytes, uint64_t row_pitch, uint32_t box_bytes, uint32_t box_rows);

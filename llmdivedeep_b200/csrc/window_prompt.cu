@@ -26,8 +26,9 @@ struct PromptPlan {
   int blocks, blk_lo;                                  // blocks of the job (-1: there are no more jobs), and which is its first
   int full0, full1;                                    // keys that every row sees which sees any (one sequence in the unit)
   int row0, rows, part, tok0;                          // first query row, rows, part (-1: a whole unit), token of the first row
-  int job, pad[3];
+  int job, at, holes, pad;                             // drafts: key of the first draft; a key without a page
   int4 sees[kWpTokens];                                // of the unit's tokens: {a0, a1, b0, b1}
+  uint64_t more[kWpTokens];                            // drafts: which of them each sees
   int4 segs[kWpSegs + 1];                              // {first key, end, blocks before, tokens of the unit that it is for}
 };
 constexpr int kWpPlans = 4;                            // jobs that are planned ahead of the one whose output is on its way
@@ -36,7 +37,7 @@ constexpr int kWpOffPm = kWpOffBars + 640;
 constexpr int kWpOffSums = kWpOffPm + kMlaPairBytes;   // [4][128] (m, l)
 constexpr int kWpOffPlans = kWpOffSums + 4 * 128 * 8;
 constexpr int kWpOffRedo = kWpOffPlans + kWpPlans * (int)sizeof(PromptPlan);
-constexpr int kWpRedo = 48;                            // quadrants of jobs that a warp has on its list of rows to be done key by key
+constexpr int kWpRedo = 12;                            // quadrants of jobs that a warp has on its list of rows to be done key by key
 constexpr int kWpSmem = kWpOffRedo + 4 * kWpRedo * 8;
 static_assert(kWpSmem <= 232448 && sizeof(PromptPlan) % 16 == 0, "shared memory budget of one CTA");
 
@@ -45,8 +46,36 @@ __device__ __forceinline__ float dot_bf16x2(uint32_t x, uint32_t y, float d) {
   return fmaf(__uint_as_float(x & 0xffff0000u), __uint_as_float(y & 0xffff0000u), d);
 }
 
+// The keys of a unit of drafts, all of one sequence: one stretch of its slots' rows.
+__device__ __forceinline__ int draft_segs(const WinArgs& a, int n_tok, PromptPlan& p) {
+  const int lane = threadIdx.x & 31, seq = p.tok0 / a.drafts.per_seq, i0 = p.tok0 - seq * a.drafts.per_seq, base = seq * a.pad;
+  const Drafts dr = drafts_of(a.drafts, seq);
+  if (i0 >= dr.m) return 0;
+  const Slots all = slots_of(a, dr, 0, a.drafts.per_seq - 1), mine = slots_of(a, dr, i0, i0 + n_tok - 1);
+  const int n = mine.n + mine.shift - all.shift;       // up to the last of its tokens, by the sequence's slots
+  for (int t = lane; t < n_tok; t += 32) {
+    const Sees s = sees_draft(a, dr, seq, i0 + t);
+    p.sees[t] = i0 + t < dr.m ? make_int4(base, base + (all.shift ? min(s.a1, all.head) : s.a1), base + s.b0 - all.shift, base + s.b1 - all.shift) : make_int4(0, 0, 0, 0);
+    p.more[t] = s.bits;
+  }
+  bool holes = false;
+  for (int w = lane; w < (n + 31) / 32; w += 32) holes |= (a.valid[base / 32 + w] & low_bits(n - 32 * w)) != low_bits(n - 32 * w);
+  holes = __any_sync(0xffffffffu, holes);
+  if (lane == 0) {
+    p.at = base + dr.ctx - dr.m - all.shift;
+    p.holes = holes;
+    p.segs[0] = make_int4(base, base + n, 0, (n_tok - 1) << 16);
+    p.segs[1] = make_int4(0, 0, 0x7fffffff, 0);
+    p.full0 = holes ? 0x7fffffff : base + mine.full0 + mine.shift - all.shift;
+    p.full1 = base + mine.full1 + mine.shift - all.shift;
+  }
+  return (n + kMlaBlk - 1) / kMlaBlk;
+}
+
 // The keys of a unit, by one warp.  Neighbouring rows of a sequence whose windows touch share two stretches: its first keys and those of their windows.
+template <bool DRAFTS>
 __device__ __forceinline__ int build_segs(const WinArgs& a, int n_tok, PromptPlan& p) {
+  if constexpr (DRAFTS) return draft_segs(a, n_tok, p);
   const int lane = threadIdx.x & 31;
   int n = 0, blocks = 0, runs = 0;
   int rk = 0, ra = 0, rlo = 0, rhi = 0, r0 = 0, r1 = -1;             // the run that is open (r1 >= r0)
@@ -98,16 +127,20 @@ __device__ __forceinline__ int build_segs(const WinArgs& a, int n_tok, PromptPla
 struct JobRows {
   int part, n_split, split, row0, rows;                // part < 0: a whole unit
 };
+template <bool DRAFTS>
 __device__ __forceinline__ JobRows job_rows(const WinArgs& a, int job) {
   JobRows j;
   j.part = job < a.n_full ? -1 : job - a.n_full;
   j.n_split = j.part < 0 ? 1 : a.n_split;
   j.split = j.part < 0 ? 0 : j.part % j.n_split;
-  j.row0 = (j.part < 0 ? job : a.n_full + j.part / j.n_split) * a.unit_rows;
-  j.rows = min(a.unit_rows, a.seq_rows - j.row0);
+  const int unit = j.part < 0 ? job : a.n_full + j.part / j.n_split, seq = DRAFTS ? unit / a.seq_units : 0, row = (unit - seq * a.seq_units) * a.unit_rows;
+  j.row0 = seq * a.seq_rows + row;
+  j.rows = min(a.unit_rows, a.seq_rows - row);
   return j;
 }
 
+// DRAFTS: units of the drafts of one sequence, over the rows of its slots.
+template <bool DRAFTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWpThreads, 1)
 window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ CUtensorMap tmap_lat,
                      const __grid_constant__ CUtensorMap tmap_rope, const WinArgs a, const int jobs) {
@@ -247,8 +280,13 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             if (tok < kWpTokens) {
               const int4 v = p.sees[tok];
               if (tok >= (s.w & 0xffff) && tok <= (s.w >> 16))
-                seen = (range_bits(v.x, v.y, k0 + 32 * hf) | range_bits(v.z, v.w, k0 + 32 * hf)) & low_bits(s.y - k0 - 32 * hf);
-              if (v.y > v.x || v.w > v.z) {
+                seen = range_bits(v.x, v.y, k0 + 32 * hf) | range_bits(v.z, v.w, k0 + 32 * hf);
+              if constexpr (DRAFTS) {
+                seen |= draft_bits(p.more[tok], p.at, k0 + 32 * hf);
+                if (p.holes) seen &= a.valid[(k0 >> 5) + hf];
+              }
+              seen &= low_bits(s.y - k0 - 32 * hf);
+              if (v.y > v.x || v.w > v.z || (DRAFTS && p.more[tok] != 0)) {
                 float z = 0.f;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) z = fmaf((seen >> i) & 1u ? 0.f : __uint_as_float(sv[i]), 0.f, z);
@@ -360,8 +398,9 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     auto drain = [&](uint32_t k, uint32_t e) {         // the output of job k, staged in entry e
       const PromptPlan& p = plans[k % kWpPlans];
       const int row0 = p.row0, rows = p.rows, part = p.part;
-      const int4 v = row < rows ? p.sees[(row0 + row) / a.H - p.tok0] : make_int4(0, 0, 0, 0);
-      const bool any = v.y > v.x || v.w > v.z;         // the row sees something
+      const int tok = row < rows ? (row0 + row) / a.H - p.tok0 : 0;
+      const int4 v = row < rows ? p.sees[tok] : make_int4(0, 0, 0, 0);
+      const bool any = v.y > v.x || v.w > v.z || (DRAFTS && row < rows && p.more[tok] != 0);      // the row sees something
       ok = wait(sums_full, k) && wait(o_final, k) && wait(&ring_full[e % NB], e / NB);
       if (!ok) return;
       tc_fence_after();
@@ -507,12 +546,12 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const int job = redos > kWpRedo ? pair + x * n_pairs : (int)redo_s[x].x;
       uint32_t mask = redos > kWpRedo ? 0xffffffffu : redo_s[x].y;
       PromptPlan& p = plans[qd];                       // each warp its own; of the jobs' plans nobody needs more than `blocks`
-      const JobRows j = job_rows(a, job);
+      const JobRows j = job_rows<DRAFTS>(a, job);
       if (j.rows < qd * 32 + 32) mask &= low_bits(j.rows - qd * 32);
       __syncwarp();
       if (lane == 0) p.tok0 = j.row0 / a.H;
       __syncwarp();
-      const int blocks = build_segs(a, (j.row0 + j.rows - 1) / a.H - j.row0 / a.H + 1, p);
+      const int blocks = build_segs<DRAFTS>(a, (j.row0 + j.rows - 1) / a.H - j.row0 / a.H + 1, p);
       __syncwarp();
       const int per = (blocks + j.n_split - 1) / j.n_split, blk_lo = min(blocks, j.split * per), n_blk = min(blocks, blk_lo + per) - blk_lo;
 #pragma unroll 1
@@ -530,7 +569,9 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           const int blk = blk_lo + (n >> 1);
           const int4 s = seg_of(p, at, blk);
           const int k0 = s.x + (blk - s.z) * kMlaBlk + 32 * (n & 1);
-          uint32_t todo = (range_bits(sees.x, sees.y, k0) | range_bits(sees.z, sees.w, k0)) & low_bits(s.y - k0);
+          uint32_t todo = range_bits(sees.x, sees.y, k0) | range_bits(sees.z, sees.w, k0);
+          if constexpr (DRAFTS) todo = (todo | draft_bits(p.more[tok], p.at, k0)) & a.valid[k0 >> 5];
+          todo &= low_bits(s.y - k0);
           if (tok < (s.w & 0xffff) || tok > (s.w >> 16)) todo = 0;
 #pragma unroll 1
           for (; todo; todo &= todo - 1) {
@@ -754,12 +795,12 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           }
           break;
         }
-        const JobRows j = job_rows(a, job);
+        const JobRows j = job_rows<DRAFTS>(a, job);
         const int row0 = j.row0, rows = j.rows, part = j.part, tok0 = row0 / a.H;
         __syncwarp();
         if (lane == 0) p.tok0 = tok0;
         __syncwarp();
-        const int blocks = build_segs(a, (row0 + rows - 1) / a.H - tok0 + 1, p);
+        const int blocks = build_segs<DRAFTS>(a, (row0 + rows - 1) / a.H - tok0 + 1, p);
         const int per = (blocks + j.n_split - 1) / j.n_split, blk_lo = min(blocks, j.split * per), n = min(blocks, blk_lo + per) - blk_lo;
         if (n == 0) {                                    // nothing seen: zeros (a part: weight zero when they are merged)
           if (part < 0) {
@@ -807,6 +848,32 @@ size_t window_mla_prefill_workspace(int T, int H, int window, int first) {
   return window_workspace(prompt_units(T, H), window_keys(H, window, first, T, 0x7fffffff));
 }
 
+template <bool DRAFTS>
+static int launch_prompt(WinArgs a, int64_t units, int64_t keys, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  window_plan(a, units, keys, workspace, workspace_bytes);
+  const int64_t rows = (int64_t)a.T * a.H;
+  CUtensorMap tq, to, tl, tr;
+  int rc = make_tmap_2d_bytes(&tq, a.q, rows, kMlaDqk * 2, kMlaDqk * 2, 128, 128);
+  if (!rc) rc = make_tmap_2d_bytes(&to, a.out, rows, kMlaDv * 2, kMlaDv * 2, 128, 32);
+  if (rc) return rc;
+  tl = tr = tq;
+  if (a.S > 0) {
+    rc = make_tmap_2d_bytes(&tl, a.kv, a.S, kMlaDqk * 2, kMlaDqk * 2, 128, kMlaBlk);
+    if (!rc) rc = make_tmap_2d_bytes(&tr, a.kv, a.S, kMlaDqk * 2, kMlaDqk * 2, 64, kMlaBlk);
+    if (rc) return rc;
+  }
+  auto kern = window_prompt_kernel<DRAFTS>;
+  static uint64_t allowed = 0;
+  if (!allow_smem(reinterpret_cast<const void*>(kern), kWpSmem, &allowed))
+    return set_error(DSA_ERR_CUDA, "window_mla: cannot raise dynamic shared memory to %d", kWpSmem);
+  const int64_t jobs = a.n_full + (units - a.n_full) * a.n_split;
+  if (jobs > 0x7ffffff0) return set_error(DSA_ERR_SHAPE, "window_mla: too many work units");
+  const int pairs = (int)min(jobs, (int64_t)max(1, sm_count() / 2));
+  kern<<<2 * pairs, kWpThreads, kWpSmem, stream>>>(tq, to, tl, tr, a, (int)jobs);
+  if (a.n_split > 1) window_combine(a, units, stream);
+  return check_launch("window_mla");
+}
+
 int window_mla_prefill_launch(const void* q, const void* kv, const int32_t* ks, const int32_t* ke, void* out, int T, int H, int S, int window, int first,
                               float scale, void* workspace, size_t workspace_bytes, int32_t* status, cudaStream_t stream) {
   WinArgs a{};
@@ -820,29 +887,18 @@ int window_mla_prefill_launch(const void* q, const void* kv, const int32_t* ks, 
   a.status = status;
   a.unit_rows = prompt_unit_rows(H);
   a.seq_rows = T * H;
-  const int64_t units = prompt_units(T, H);
-  a.seq_units = (int)units;
-  window_plan(a, units, window_keys(H, window, first, T, S), workspace, workspace_bytes);
-  const int64_t rows = (int64_t)T * H;
-  CUtensorMap tq, to, tl, tr;
-  int rc = make_tmap_2d_bytes(&tq, q, rows, kMlaDqk * 2, kMlaDqk * 2, 128, 128);
-  if (!rc) rc = make_tmap_2d_bytes(&to, out, rows, kMlaDv * 2, kMlaDv * 2, 128, 32);
-  if (rc) return rc;
-  tl = tr = tq;
-  if (S > 0) {
-    rc = make_tmap_2d_bytes(&tl, kv, S, kMlaDqk * 2, kMlaDqk * 2, 128, kMlaBlk);
-    if (!rc) rc = make_tmap_2d_bytes(&tr, kv, S, kMlaDqk * 2, kMlaDqk * 2, 64, kMlaBlk);
-    if (rc) return rc;
-  }
-  static uint64_t allowed = 0;
-  if (!allow_smem(reinterpret_cast<const void*>(window_prompt_kernel), kWpSmem, &allowed))
-    return set_error(DSA_ERR_CUDA, "window_mla: cannot raise dynamic shared memory to %d", kWpSmem);
-  const int64_t jobs = a.n_full + (units - a.n_full) * a.n_split;
-  if (jobs > 0x7ffffff0) return set_error(DSA_ERR_SHAPE, "window_mla: too many work units");
-  const int pairs = (int)min(jobs, (int64_t)max(1, sm_count() / 2));
-  window_prompt_kernel<<<2 * pairs, kWpThreads, kWpSmem, stream>>>(tq, to, tl, tr, a, (int)jobs);
-  if (a.n_split > 1) window_combine(a, units, stream);
-  return check_launch("window_mla");
+  a.seq_units = (int)prompt_units(T, H);
+  return launch_prompt<false>(a, a.seq_units, window_keys(H, window, first, T, S), workspace, workspace_bytes, stream);
+}
+
+size_t window_prompt_drafts_workspace(int B, int64_t seq_rows, int H, int64_t keys) {
+  return window_workspace(B * ((seq_rows + prompt_unit_rows(H) - 1) / prompt_unit_rows(H)), keys);
+}
+int window_prompt_drafts(WinArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  a.unit_rows = prompt_unit_rows(a.H);
+  a.seq_units = (a.seq_rows + a.unit_rows - 1) / a.unit_rows;
+  const int64_t units = (int64_t)(a.T / a.drafts.per_seq) * a.seq_units;
+  return launch_prompt<true>(a, units, window_keys(a.H, a.window, a.first, a.drafts.per_seq, a.drafts.max_ctx), workspace, workspace_bytes, stream);
 }
 
 }  // namespace dsa

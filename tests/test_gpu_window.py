@@ -267,6 +267,49 @@ def test_trees(record, H, per, window, first):
     assert bool((out.view(5, per, -1)[3] == 0).all()) and bool((out.view(5, per, -1)[4, 1:] == 0).all())
 
 
+@pytest.mark.parametrize("record", [656, 416])
+@pytest.mark.parametrize("H,per,window,first", [(128, 13, 100, 0), (128, 5, 70, 40), (64, 9, 1, 0), (200, 4, 300, 3), (16, 64, 33, 0), (5, 100, 40, 2), (2, 300, 64, 1), (40, 30, 1 << 30, 0)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_many_rows_a_sequence(record, H, per, window, first, tree):
+    """Sequences of several units, with room for their records as rows and without; lengths of drafts alone, pages that are none."""
+    if tree and per > 64:
+        pytest.skip("a tree has at most 64 drafts")
+    ctx, n_new = [700, per, 0, 333], [per, per, 0, max(1, per - 2)]
+    ctx[3] = max(333, per)
+    c = Case(4, per, H, ctx, record, seed=per + H, n_new=n_new, tree=tree)
+    want = c.want(window, first)
+    args = c.args()
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    for ws in (None, none):
+        check(ops.window_mla_decode_paged(**args, window=window, first=first, scale=SCALE, workspace=ws), want)
+    ops.check_status("cuda")
+    hole = int((ctx[0] - per) // 64)                                      # the page of the first draft, and of tokens before
+    args["block_table"][0, hole] = -1
+    sees = c.sees(window, first)
+    sees[:per, hole * 64:hole * 64 + 64] = False
+    want = D.attend(c.q, c.kv.repeat_interleave(per, 0), sees, SCALE)
+    for ws in (None, none):
+        check(ops.window_mla_decode_paged(**args, window=window, first=first, scale=SCALE, workspace=ws), want)
+        with pytest.raises(ops.DsaError, match="out of range"):
+            ops.check_status("cuda")
+
+
+@pytest.mark.parametrize("record", [656, 416])
+def test_many_rows_a_sequence_and_records_that_are_no_numbers(record):
+    c = Case(2, 11, 64, [400, 90], record, seed=7, tree=True)
+    sees, clean = c.sees(100, 2), c.want(100, 2)
+    for b, pos in ((0, 389), (0, 395), (0, 399), (1, 1), (1, 85)):
+        dirty = c.args()
+        dirty["cache"] = c.rec.clone()
+        dirty["cache"][int(c.table[b, pos // 64]) * 64 + pos % 64] = 255
+        out = ops.window_mla_decode_paged(**dirty, window=100, first=2, scale=SCALE)
+        ops.check_status("cuda")
+        touched = torch.zeros(22, dtype=torch.bool)
+        touched[b * 11:(b + 1) * 11] = sees[b * 11:(b + 1) * 11, pos]
+        assert bool(out[touched.cuda()].isnan().flatten(1).any(1).all())
+        check(out[~touched.cuda()], clean[~touched.cuda()])
+
+
 def test_masks_are_held_to_the_drafts_before():
     c = Case(2, 6, 16, [90, 64], 416, seed=4, n_new=[6, 4], tree=True)
     a = ops.window_mla_decode_paged(**c.args(), window=40, first=2, scale=SCALE)
