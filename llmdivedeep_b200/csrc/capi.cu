@@ -101,7 +101,7 @@ int topk_select_drafts_launch(const float* logits, int64_t ld, const int32_t* ct
 int window_mla_prefill_launch(const void* q, const void* kv, const int32_t* ks, const int32_t* ke, void* out, int T, int H, int S, int window, int first,
                               float scale, void* workspace, size_t workspace_bytes, int32_t* status, cudaStream_t stream);
 size_t window_mla_prefill_workspace(int T, int H, int window, int first);
-size_t window_mla_decode_workspace(int B, int tokens_per_seq, int H, int window, int first, int max_ctx);
+size_t window_mla_decode_workspace(int record_bytes, int B, int tokens_per_seq, int H, int window, int first, int max_ctx);
 int window_mla_decode_launch(const void* q, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride, const int32_t* ctx_len,
                              const int32_t* n_new, const int64_t* tree, int tokens_per_seq, void* out, int B, int H, int window, int first, int num_pages,
                              int max_ctx, float scale, void* workspace, size_t workspace_bytes, int32_t* status, cudaStream_t stream);
@@ -527,7 +527,7 @@ int dsa_window_mla_prefill(const void* q_bf16, const void* kv_bf16, const int32_
 }
 
 size_t dsa_window_mla_decode_workspace_bytes(int record_bytes, int B, int tokens_per_seq, int H, int window, int first, int max_ctx) {
-  return B <= 0 || tokens_per_seq < 1 || H <= 0 || window < 1 || first < 0 || max_ctx <= 0 ? 0 : window_mla_decode_workspace(B, tokens_per_seq, H, window, first, max_ctx);
+  return B <= 0 || tokens_per_seq < 1 || H <= 0 || window < 1 || first < 0 || max_ctx <= 0 ? 0 : window_mla_decode_workspace(record_bytes, B, tokens_per_seq, H, window, first, max_ctx);
 }
 
 int dsa_window_mla_decode_paged(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table, int64_t table_stride,

@@ -664,6 +664,13 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const WinArgs a, const
   const Drafts dr = drafts_of(a.drafts, b);
   if (dr.bad && j0 == 0 && lane == 0 && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
   const Slots sl = slots_of(a, dr, 0, a.drafts.per_seq - 1);
+  if (a.live) {                                        // rows of units without a draft
+    const int row0 = (dr.m * a.H + a.unit_rows - 1) / a.unit_rows * a.unit_rows;
+    for (int r = row0 + j0 / kRowsSlots; r < a.seq_rows; r += per) {
+      uint4* o = reinterpret_cast<uint4*>(a.out + ((int64_t)b * a.seq_rows + r) * kMlaDv);
+      o[lane] = o[32 + lane] = make_uint4(0, 0, 0, 0);
+    }
+  }
   if (j0 >= sl.n) return;
   int id = -1;
   if (lane < kRowsSlots && j0 + lane < sl.n) {
@@ -705,13 +712,15 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const WinArgs a, const
     reinterpret_cast<uint32_t*>(out + j * (kMlaDqk / 8) + 64)[lane] = rope;
   }
 }
-constexpr int kRowsUnits = 4;                          // units of 128 rows from which on a sequence's records are made rows first
 constexpr int64_t kRowsMost = 512ll << 20;             // bytes of rows at most
 static int rows_pad(int64_t keys) { return (int)((keys + 63) / 64 * 64); }
-// Bytes of the rows, 0: not this way.
-static int64_t rows_bytes(int B, int64_t seq_rows, int64_t keys) {
-  const int64_t bytes = (int64_t)B * rows_pad(keys) * (kMlaDqk * 2);
-  return seq_rows > (kRowsUnits - 1) * 128 && bytes <= kRowsMost ? bytes : 0;
+// Bytes of the rows, 0: not this way.  Made rows once, a sequence's records cost its units 0.93 us a block of 64 in place of 1.3 (FP8) and 1.2 (4 bits), and 64 rows
+// 0.02 us of the whole GPU.  us with records and with rows, 128 heads, FP8: 32 sequences of 3 drafts, window 512, 47.5 / 47.4, of 4 48.6 / 45.5, of 5 70 / 59, of 13
+// 145 / 104; 4 bits of 4 43.3 / 44.4, of 5 61 / 57, of 13 128 / 101.  Calls that leave pairs idle cut keys into parts instead, unless there are many: 4
+// sequences of 13, window 512, 25.5 / 28.5, window 2048 60 / 51.
+static int64_t rows_bytes(int record_bytes, int B, int64_t seq_rows, int64_t keys) {
+  const int64_t bytes = (int64_t)B * rows_pad(keys) * (kMlaDqk * 2), units = (seq_rows + 127) / 128;
+  return units >= (record_bytes == kLatent4Bytes ? 5 : 4) && (B * units >= sm_count() / 2 || keys >= 1024) && bytes <= kRowsMost ? bytes : 0;
 }
 
 // Rows of a unit.  Calls that leave most pairs idle have fewer: a block's exchange and softmax take less time, and there are more units to share its keys.
@@ -726,7 +735,7 @@ static int64_t decode_units(int B, int64_t seq_rows) {
   return B * ((seq_rows + rows - 1) / rows);
 }
 // Of every call of up to B sequences.
-size_t window_mla_decode_workspace(int B, int tokens_per_seq, int H, int window, int first, int max_ctx) {
+size_t window_mla_decode_workspace(int record_bytes, int B, int tokens_per_seq, int H, int window, int first, int max_ctx) {
   const int64_t seq_rows = (int64_t)tokens_per_seq * H, keys = window_keys(H, window, first, tokens_per_seq, max_ctx);
   size_t most = window_workspace(B * ((seq_rows + 127) / 128), keys);
   for (int b = 1; b <= min(B, 16); ++b) {              // more have units of 128 rows
@@ -734,7 +743,7 @@ size_t window_mla_decode_workspace(int B, int tokens_per_seq, int H, int window,
     const int parts = window_parts(units, keys);
     if (parts > 1) most = max(most, (size_t)(units % max(1, sm_count() / 2)) * parts * kWinPartBytes);
   }
-  const int64_t slots = min((int64_t)max_ctx, (int64_t)window + first + tokens_per_seq), rows = rows_bytes(B, seq_rows, slots);
+  const int64_t slots = min((int64_t)max_ctx, (int64_t)window + first + tokens_per_seq), rows = rows_bytes(record_bytes, B, seq_rows, slots);
   if (rows) most = max(most, (size_t)rows + (size_t)B * rows_pad(slots) / 8 + 256 + window_prompt_drafts_workspace(B, seq_rows, H, keys));
   return most;
 }
@@ -755,12 +764,13 @@ int window_mla_decode_launch(const void* q, const void* cache, int record_bytes,
   a.scale_log2e = scale * 1.4426950408889634f;
   a.status = status;
   a.seq_rows = tokens_per_seq * H;
-  const int64_t slots = min((int64_t)max_ctx, (int64_t)window + first + tokens_per_seq), rows = rows_bytes(B, a.seq_rows, slots);
+  const int64_t slots = min((int64_t)max_ctx, (int64_t)window + first + tokens_per_seq), rows = rows_bytes(record_bytes, B, a.seq_rows, slots);
   if (rows && workspace) {
     a.pad = rows_pad(slots);
     const size_t valid = ((size_t)B * a.pad / 8 + 255) / 256 * 256;
     if (workspace_bytes >= rows + valid) {
       a.valid = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + rows);
+      window_prompt_units(a);
       const unsigned grid = (unsigned)(((int64_t)B * (a.pad / kRowsSlots) + 7) / 8);
       auto kern = record_bytes == kLatent4Bytes ? window_rows_kernel<kSrc4> : window_rows_kernel<kSrcFp8>;
       kern<<<grid, 256, 0, stream>>>(a, a.kv, static_cast<uint4*>(workspace), B);

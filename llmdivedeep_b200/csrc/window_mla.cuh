@@ -33,6 +33,7 @@ struct WinArgs {
   // drafts over rows that were made bf16 first: kv is [B * pad] rows, slot j of sequence b row b * pad + j, with a bit for each that has a page
   int pad;
   uint32_t* valid;
+  int live;                       // only units with drafts in them are jobs; the other rows' zeros come with the rows of the keys
 };
 
 // What a row sees: two stretches of positions, a1 <= b0, and single ones behind `at`.
@@ -205,7 +206,8 @@ inline void window_plan(WinArgs& a, int64_t units, int64_t keys, void* workspace
   }
 }
 // Drafts of sequences over rows that were made bf16 first (window_prompt.cu); a.kv and what goes with it is set.
-int window_prompt_drafts(WinArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+int window_prompt_drafts(const WinArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+void window_prompt_units(WinArgs& a);                  // sets unit_rows, seq_units and live
 size_t window_prompt_drafts_workspace(int B, int64_t seq_rows, int H, int64_t keys);
 // The kernel that merges the parts of units n_full .. of `units` (window_mla.cu).
 void window_combine(const WinArgs& a, int64_t units, cudaStream_t stream);

@@ -139,6 +139,29 @@ __device__ __forceinline__ JobRows job_rows(const WinArgs& a, int job) {
   return j;
 }
 
+// The J-th unit that has a draft in it, for ascending J; -1: there are fewer.  By a warp.
+struct LiveUnits {
+  int s0 = -32, before = 0, total = 0, upto = 0, own = 0;      // 32 sequences: their first, units before them, of them, of a lane's up to its own, its own
+  __device__ __forceinline__ int find(const WinArgs& a, int J) {
+    const int lane = threadIdx.x & 31, B = a.T / a.drafts.per_seq;
+    while (J >= before + total) {
+      before += total;
+      s0 += 32;
+      if (s0 >= B) return -1;
+      own = s0 + lane < B ? (drafts_of(a.drafts, s0 + lane).m * a.H + a.unit_rows - 1) / a.unit_rows : 0;
+      upto = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      total = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    const int l = __ffs(__ballot_sync(0xffffffffu, upto > J - before)) - 1;
+    return (s0 + l) * a.seq_units + J - before - __shfl_sync(0xffffffffu, upto - own, l);
+  }
+};
+
 // DRAFTS: units of the drafts of one sequence, over the rows of its slots.
 template <bool DRAFTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWpThreads, 1)
@@ -541,9 +564,11 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     // Rare: rows key by key over what they see of their job's blocks, this CTA's half of the output from whole scores.  Nobody waits for this warp now (but at the
     // barrier that the pair leaves through, which has no limit).  With more on the list than it holds: every row of the pair's jobs.
     const int redo_jobs = redos > kWpRedo ? (jobs - pair + n_pairs - 1) / n_pairs : redos;
+    LiveUnits found;
 #pragma unroll 1
     for (int x = 0; ok && x < redo_jobs; ++x) {
-      const int job = redos > kWpRedo ? pair + x * n_pairs : (int)redo_s[x].x;
+      int job = redos > kWpRedo ? pair + x * n_pairs : (int)redo_s[x].x;
+      if (DRAFTS && a.live && redos > kWpRedo && (job = found.find(a, job)) < 0) break;
       uint32_t mask = redos > kWpRedo ? 0xffffffffu : redo_s[x].y;
       PromptPlan& p = plans[qd];                       // each warp its own; of the jobs' plans nobody needs more than `blocks`
       const JobRows j = job_rows<DRAFTS>(a, job);
@@ -782,10 +807,12 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       // ------------------------------- plans -------------------------------
       uint32_t k = 0;
       bool ok = true, mine = false;                      // the buffer of plan k is this warp's
-      for (int job = pair; ok && !aborted_warp(abort_flag); job += n_pairs) {
+      LiveUnits found;
+    for (int next = pair; ok && !aborted_warp(abort_flag); next += n_pairs) {
+      const int job = DRAFTS && a.live ? found.find(a, next) : next < jobs ? next : -1;
         if (!mine) ok = wait(&plan_free[k % kWpPlans], (k / kWpPlans) + 1);
         mine = true;
-        const bool more = job < jobs;
+        const bool more = job >= 0;
         PromptPlan& p = plans[k % kWpPlans];
         if (!ok) break;
         if (!more) {
@@ -894,11 +921,14 @@ int window_mla_prefill_launch(const void* q, const void* kv, const int32_t* ks, 
 size_t window_prompt_drafts_workspace(int B, int64_t seq_rows, int H, int64_t keys) {
   return window_workspace(B * ((seq_rows + prompt_unit_rows(H) - 1) / prompt_unit_rows(H)), keys);
 }
-int window_prompt_drafts(WinArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+void window_prompt_units(WinArgs& a) {
   a.unit_rows = prompt_unit_rows(a.H);
   a.seq_units = (a.seq_rows + a.unit_rows - 1) / a.unit_rows;
+  a.live = (int64_t)(a.T / a.drafts.per_seq) * a.seq_units >= sm_count() / 2;      // fewer are cut into parts
+}
+int window_prompt_drafts(const WinArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   const int64_t units = (int64_t)(a.T / a.drafts.per_seq) * a.seq_units;
-  return launch_prompt<true>(a, units, window_keys(a.H, a.window, a.first, a.drafts.per_seq, a.drafts.max_ctx), workspace, workspace_bytes, stream);
+  return launch_prompt<true>(a, units, window_keys(a.H, a.window, a.first, a.drafts.per_seq, a.drafts.max_ctx), workspace, a.live ? 0 : workspace_bytes, stream);
 }
 
 }  // namespace dsa
