@@ -582,7 +582,7 @@ int dsa_topk_select_drafts(const float* logits, int64_t ld_logits, const int32_t
   if (rc) return rc;
   if (k < 0) return set_error(DSA_ERR_SHAPE, "%s: negative size", who);
   if (B == 0 || k == 0) return DSA_OK;
-  if (!logits || !ctx_len || !out_idx) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
+  if ((max_ctx > 0 && !logits) || !ctx_len || !out_idx) return set_error(DSA_ERR_ARG, "%s: NULL pointer argument", who);
   if (ld_logits < max_ctx) return set_error(DSA_ERR_SHAPE, "%s: ld_logits < max_ctx", who);
   if (k > 65535) return set_error(DSA_ERR_SHAPE, "%s: k (%d) exceeds 65535", who, k);
   const size_t need = dsa_topk_select_drafts_workspace_bytes(B, tokens_per_seq);

@@ -151,6 +151,95 @@ def test_selection(k, tree):
     assert ops.topk_select_drafts(logits, 0, **lens).shape == (35, 0)
 
 
+@pytest.mark.parametrize("k", [4, 150])
+def test_scores_that_are_no_numbers_select_nothing_unseen(k):
+    """Most scores of a row -inf or NaN of either sign: what its draft does not see is not in its list all the same."""
+    per, ctx = 5, 200
+    c = Case(3, per, 64, [ctx] * 3, seed=k, tree=True)
+    c.tree = torch.tensor([1, 0, 1, 4, 8], dtype=torch.int64).expand(3, per).contiguous()
+    logits = c.logits()
+    logits[:per, 2:ctx - per] = -float("inf")
+    logits[per:2 * per, 2:ctx - per] = float("nan")
+    logits[2 * per:, 2:ctx - per] = -torch.full((), float("nan"), device="cuda")
+    idx = ops.topk_select_drafts(logits, k, **c.lens()).cpu()
+    sees = c.sees().cpu()
+    for r in range(3 * per):
+        got = [x for x in idx[r].tolist() if x >= 0]
+        assert all(bool(sees[r, x]) for x in got) and len(set(got)) == len(got)
+
+
+def test_keys_that_are_no_numbers_where_a_draft_does_not_see():
+    """Another draft's key, and what lies behind the sequence in its last page: values, and a scale, that are none."""
+    per, ctx = 4, [300, 70]
+    c = Case(2, per, 64, ctx, seed=5, tree=True)
+    c.tree = torch.tensor([[1, 0, 1, 2]] * 2, dtype=torch.int64)
+    clean = c.logits()
+    k8, ksc = c.k8.view(torch.uint8).clone(), c.ksc.clone().view(-1)
+    for b in range(2):
+        row = lambda s: int(c.table[b, s // 64]) * 64 + s % 64
+        k8[row(ctx[b] - per)] = 0x7f                      # draft 0, which 2 descends from and 1 and 3 do not
+        ksc[row(ctx[b] - per + 2)] = float("inf")         # draft 2, which nobody else sees
+        for s in range(ctx[b], -(-ctx[b] // 64) * 64):
+            k8[row(s)], ksc[row(s)] = 0xff, float("nan")
+    c.k8, c.ksc = k8.view(ops.FP8), ksc.view_as(c.ksc)
+    got = c.logits()
+    for r in (1, 3, 5, 7):
+        end = min(c.max_ctx, -(-ctx[r // per] // 128) * 128)
+        assert torch.equal(got[r, :end], clean[r, :end])
+    for r in (0, 2, 4, 6):
+        P = ctx[r // per] - per
+        assert torch.equal(got[r, :P], clean[r, :P])
+
+
+def test_logits_in_two_graphs_and_on_two_streams():
+    """One set of inputs, outputs of their own: replays in either order, and two calls at once, give what a call gave."""
+    a, b = Case(3, 4, 64, [700, 90, 333], seed=1, tree=True), Case(2, 2, 32, [1200, 64], seed=2)
+    want = [x.logits().clone() for x in (a, b)]
+    idx = [ops.topk_select_drafts(w, 64, **x.lens()).clone() for w, x in zip(want, (a, b))]
+    lens = [x.lens() for x in (a, b)]
+    outs, sel, graphs = [], [], []
+    for x, ln in zip((a, b), lens):
+        o, s, gr = torch.empty(x.B * x.per, x.max_ctx, device="cuda"), torch.empty(x.B * x.per, 64, dtype=torch.int32, device="cuda"), torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(gr, stream=side):
+            ops.fp8_paged_mqa_logits(x.q8, x.w, x.k8, x.ksc, x.table, max_ctx=x.max_ctx, out=o, **ln)
+            ops.topk_select_drafts(o, 64, out=s, **ln)
+        outs.append(o), sel.append(s), graphs.append(gr)
+    pick = lambda x, o: torch.cat([o[r, :-(-x.ctx[r // x.per] // 128) * 128] for r in range(x.B * x.per)])
+    seen = [pick(x, w) for x, w in zip((a, b), want)]
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for o, s in zip(outs, sel):
+            o.fill_(3.0), s.fill_(-7)
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for x, o, s, w, k in zip((a, b), outs, sel, seen, idx):
+            assert torch.equal(pick(x, o), w) and torch.equal(s.sort(1)[0], k.sort(1)[0])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(4):
+        for i, (x, ln, st) in enumerate(zip((a, b), lens, streams)):
+            with torch.cuda.stream(st):
+                got[i] = ops.fp8_paged_mqa_logits(x.q8, x.w, x.k8, x.ksc, x.table, max_ctx=x.max_ctx, **ln)
+    torch.cuda.synchronize()
+    for x, o, w in zip((a, b), got, seen):
+        assert torch.equal(pick(x, o), w)
+
+
+def test_no_context_at_all():
+    """Tables without a page: scores of no columns, lists of no positions."""
+    q8, _ = quantised(torch.randn(6, 64, 128, device="cuda"))
+    k8, ksc = quantised(torch.randn(64, 128, device="cuda"))
+    table, lens = torch.empty(2, 0, dtype=torch.int32, device="cuda"), dict(ctx_len=i32([0, 0]), tokens_per_seq=3)
+    logits = ops.fp8_paged_mqa_logits(q8, torch.ones(6, 64, device="cuda"), k8, ksc, table, max_ctx=0, **lens)
+    assert logits.shape == (6, 0)
+    idx = ops.topk_select_drafts(logits, 5, **lens)
+    ops.check_status("cuda")
+    assert bool((idx == -1).all()) and idx.shape == (6, 5)
+
+
 @pytest.mark.parametrize("record", [656, 416])
 @pytest.mark.parametrize("per,k", [(4, 64), (6, 512)])
 def test_a_step_of_drafts_is_a_step_of_each(record, per, k):
