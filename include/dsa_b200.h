@@ -322,7 +322,9 @@ int dsa_window_mla_prefill(const void* q_bf16, const void* kv_bf16, const int32_
 
 /* The window attention over records of record_bytes = 656 or 416 of a paged latent cache: q_bf16
  * [B*tokens_per_seq, H, 576], out_bf16 [B*tokens_per_seq, H, 512]; rows without a token give
- * zeros.  Positions are those along a draft's path. */
+ * zeros.  Positions are those along a draft's path.  A record's values are rounded to bf16
+ * before they are multiplied (as for dsa_sparse_mla_decode_paged).  Where sequences have many
+ * query rows the workspace holds their records as bf16 rows, made once a call. */
 size_t dsa_window_mla_decode_workspace_bytes(int record_bytes, int B, int tokens_per_seq, int H, int window, int first, int max_ctx);
 int dsa_window_mla_decode_paged(const void* q_bf16, const void* cache, int record_bytes, const int32_t* block_table,
                                 int64_t table_stride, const int32_t* ctx_len, const int32_t* n_new, const int64_t* tree,

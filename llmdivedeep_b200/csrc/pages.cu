@@ -555,7 +555,8 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
 // ---- acceptance of drafts ----------------------------------------------------------------------------------------------
 // Row rows[i] keeps the drafts path[i, 0 .. n_keep[i]) of its last n_new[i] tokens: draft path[k] moves to place k behind the P tokens before
 // them, in every cache; what lies behind goes.  path[k] >= k, so a place that is written is read by no later move, and a thread that takes
-// the same 16 bytes of every token in order needs no barrier.
+// the same 16 bytes of every token in order needs no barrier.  One CTA a row and 128 columns of 16 bytes; what bounds it is latency: list, table, then eight
+// records under way at a time, and the pages in a second kernel, which starts under the first (8 rows x 2 layers 10.3 us, 200 x 16 14.4).
 template <int N>
 struct AcceptCaches {                                  // of a launch; eight hold most models' in a tenth of the parameters
   CacheEntry cache[N];

@@ -3,6 +3,13 @@
 //   o[r, :] = sum_s softmax_s(scale * q[r, :] . kv[s, :]) * kv[s, :512],   s < first or p - window < s <= p,
 // here over the records of the paged latent caches: decode, one or several query tokens a sequence, a chain or a tree of drafts (drafts.cuh).  Prompts:
 // window_prompt.cu.
+//
+// A unit is up to 128 query rows (token, head) of one sequence, and its keys are the union of what they see, as slots: the first tokens, then the window's,
+// then the drafts.  Rows of one sequence share the fetch and the conversion of their records, which is why a unit has several tokens where heads are few.  A pair
+// of CTAs has a unit, each half of the latent dims (sparse_mla.cu): whole, O of 128 rows and 512 dims and S, P and Q of 576 do not fit one SM's tensor memory.
+// What bounds it: a block of 64 slots takes a pair 1.33 to 1.46 us from FP8 records and 1.10 to 1.23 from 4 bits, the chain of conversion, exchange, softmax and
+// P.V with the issue slots 63 % used (74 sequences x 128 heads, window 2048: 65.9 us, tensor pipe 32 %, DRAM 21 %).  64 sequences x 128 heads at
+// 128K, window 4096: 100 to 110 us for 29 us of bytes and 45 of operations; 160 x 4 drafts x 16 heads, 4 bits, window 1024: 76 us.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
