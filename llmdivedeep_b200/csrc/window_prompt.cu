@@ -5,8 +5,9 @@
 // cross over in fp16, each side runs the softmax, P.V accumulates in tensor memory.  What differs:
 //   * a block is 64 rows of a stretch of keys, fetched by five TMA boxes; rows of one sequence that follow one another share the blocks, and what
 //     each of them sees of a block is a 32-bit mask to a thread, from two ranges;
-//   * blocks, query panels and the output's staging go through one ring of five buffers, in the order Q(u) Q(u) Q(u) K(u, 0) O(u - 1) K(u, 1) ..., so that
-//     the next unit's queries and keys are on their way while the last blocks of this one are worked on;
+//   * blocks, query panels and the output's staging go through one ring of five buffers, in the order Q(u) Q(u) Q(u)+O(u - 1) K(u, 0) K(u, 1) ..., so that
+//     the next unit's queries and keys are on their way while the last blocks of this one are worked on.  (The third entry has one query panel; the
+//     output before is staged behind it.)  An entry of the ring costs a unit about as much as a block does;
 //   * four more warps move Q into tensor memory and O out of it, so that the softmax goes from unit to unit without a pause.
 // Roles: warps 0-15 exchange + softmax, 16 MMA issuer, 17 loads, 18 zeros in the rows behind the end of a stretch, 19 plans the next unit, 20-23 Q and O.
 // Every wait is bounded (dsa_common.cuh); the two CTAs leave together through a cluster barrier.
@@ -457,7 +458,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (part >= 0)                                   // what this CTA's half of the columns is weighted with
         a.part_lse[((int64_t)part * 2 + cta) * 128 + row] = l > 0.f ? mt + log2f(l) : l == 0.f ? -CUDART_INF_F : l;
       {
-        uint8_t* const stage0 = smem + (e % NB) * kMlaKBytes + qd * 8192 + lane * 128;      // two panels of 32 rows to a warp
+        uint8_t* const stage0 = smem + (e % NB) * kMlaKBytes + kMlaQPanelBytes + qd * 4096 + lane * 64;      // two pieces of 32 rows x 32 columns to a warp
         __nv_bfloat16* const orow = a.out + (int64_t)(row0 + row) * kMlaDv + cta * kMlaDvHalf;
         const uint64_t inv2 = pack_f32x2(inv, inv);
         const bool blind = __any_sync(0xffffffffu, !any);
@@ -487,19 +488,19 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             uint32_t (&now)[16] = ov[(c >> 4) & 1];
             tmem_wait_ld();
             if (c + 16 < kMlaDvHalf) tmem_ld16(t_row + kColO + c + 16, ov[((c >> 4) & 1) ^ 1]);
-            if (c >= 128 && (c & 63) == 0) {           // the store of two panels before has read its own
+            if (c >= 64 && (c & 31) == 0) {            // the store of two pieces before has read its own
               if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
               __syncwarp();
             }
             scaled(now);
-            uint8_t* stage = stage0 + ((c >> 6) & 1) * 4096;
-            *reinterpret_cast<uint4*>(stage + (((((c & 63) >> 3) + 0) ^ (lane & 7)) << 4)) = eight(now, 0);
-            *reinterpret_cast<uint4*>(stage + (((((c & 63) >> 3) + 1) ^ (lane & 7)) << 4)) = eight(now, 8);
-            if ((c & 63) == 48) {
-              fence_async_smem();                      // the store reads the panel through the async proxy
+            uint8_t* stage = stage0 + ((c >> 5) & 1) * 2048;
+            *reinterpret_cast<uint4*>(stage + (((((c & 31) >> 3) + 0) ^ (lane >> 1 & 3)) << 4)) = eight(now, 0);
+            *reinterpret_cast<uint4*>(stage + (((((c & 31) >> 3) + 1) ^ (lane >> 1 & 3)) << 4)) = eight(now, 8);
+            if ((c & 31) == 16) {
+              fence_async_smem();                      // the store reads the piece through the async proxy
               __syncwarp();
               if (lane == 0) {
-                tma_store_2d(&tmap_o, stage, (cta * 4 + (c >> 6)) * 32, row0 + qd * 32);      // x in 4-byte units: 32 per 64-column panel
+                tma_store_2d(&tmap_o, stage, (cta * 8 + (c >> 5)) * 16, row0 + qd * 32);      // x in 4-byte units: 16 per 32 columns
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
               }
             }
@@ -550,17 +551,16 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           }
           tmem_st16(t_row + kColQ + (4 * j + hp) * 16, qv);
         }
-        give_back(e);
+        if (j < 2 || k == 0) give_back(e);
       }
       if (!ok) break;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
-      // the output of the unit before is staged in the entry behind this unit's first block
-      if (k > 0) drain(k - 1, e + 1);
+      if (k > 0) drain(k - 1, e - 1);                  // the output of the unit before is staged behind the last query panel
       if (!ok) break;
-      e += n + (k > 0);
+      e += n;
     }
     if (ok && k > 0) drain(k - 1, e);
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -683,7 +683,6 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (n_last > 0) {
           if (n_last == 2 && k > 1 && !(ok = wait(o_free, k - 2))) break;
           issue_pv(n_last > 1 ? gp : gp ^ 1, n_last <= 2, n_last == 1);
-          if (k > 1 && n_last == 2) vbuf = vbuf == NB - 1 ? 0 : vbuf + 1;      // (the output's buffer between its two blocks)
         }
         if (n < 0) {
           if (n_last > 1 && (ok = wait(p_full, gp ^ 1))) issue_pv(gp ^ 1, false, true);
@@ -718,11 +717,10 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             if (ok && i == 2 && k > 0) ok = wait(o_free, k - 1);       // the first P.V of the unit: the output before has been read
             if (!ok) break;
             issue_pv(parity, i == 2, i == 0);
-            if (i == 2 && k > 0) vbuf = vbuf == NB - 1 ? 0 : vbuf + 1;      // the output's buffer
           }
           if (i == 0) vbuf = vfirst;
           gp ^= 1;
-          skip(i == 0 && k > 0 ? 2 : 1);                 // and the entry of the output before
+          skip(1);
         }
         n_last = n;
       }
@@ -768,10 +766,6 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           else if (lane == 4) tma_load_2d(dst + kMlaRopeOff, &tmap_rope, kMlaDv / 2 + cta * 16, key0, full);
           __syncwarp();
           ++e;
-          if (i == 0 && k > 0) {
-            claim(ring_full, 0);
-            ++e;
-          }
         }
         plan_done(k);
       }
@@ -803,7 +797,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(&ring_full[buf]);
           }
-          e += i == 0 && k > 0 ? 2 : 1;
+          ++e;
         }
         plan_done(k);
       }
@@ -885,7 +879,7 @@ static int launch_prompt(WinArgs a, int64_t units, int64_t keys, void* workspace
   const int64_t rows = (int64_t)a.T * a.H;
   CUtensorMap tq, to, tl, tr;
   int rc = make_tmap_2d_bytes(&tq, a.q, rows, kMlaDqk * 2, kMlaDqk * 2, 128, 128);
-  if (!rc) rc = make_tmap_2d_bytes(&to, a.out, rows, kMlaDv * 2, kMlaDv * 2, 128, 32);
+  if (!rc) rc = make_tmap_2d_bytes(&to, a.out, rows, kMlaDv * 2, kMlaDv * 2, 64, 32);
   if (rc) return rc;
   tl = tr = tq;
   if (a.S > 0) {
