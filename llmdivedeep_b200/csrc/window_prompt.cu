@@ -33,9 +33,12 @@ struct PromptPlan {
   int row0, rows, part, tok0;                          // first query row, rows, part (-1: a whole unit), token of the first row
   int job, at, holes, pad;                             // drafts: key of the first draft; a key without a page
   int4 sees[kWpTokens];                                // of the unit's tokens: {a0, a1, b0, b1}
-  uint64_t more[kWpTokens];                            // drafts: which of them each sees
+  // Drafts: which of them each sees.  Prompts, of the first token of a stretch: the last keys of the stretch may be the sequence's first ones, behind its own,
+  // and are known by their places in the tokens' `sees`; which is the first of those | how many << 32.
+  uint64_t more[kWpTokens];
   int4 segs[kWpSegs + 1];                              // {first key, end, blocks before, tokens of the unit that it is for}
 };
+constexpr int kWpHead = 16;                            // first keys that come behind a stretch at most
 constexpr int kWpPlans = 4;                            // jobs that are planned ahead of the one whose output is on its way
 constexpr int kWpOffBars = kMlaBufs * kMlaKBytes + 2 * kMlaXBytes;
 constexpr int kWpOffPm = kWpOffBars + 640;
@@ -49,6 +52,14 @@ static_assert(kWpSmem <= 232448 && sizeof(PromptPlan) % 16 == 0, "shared memory 
 __device__ __forceinline__ float dot_bf16x2(uint32_t x, uint32_t y, float d) {
   d = fmaf(__uint_as_float(x << 16), __uint_as_float(y << 16), d);
   return fmaf(__uint_as_float(x & 0xffff0000u), __uint_as_float(y & 0xffff0000u), d);
+}
+
+// The first keys behind a stretch: which is the first, and how many.
+template <bool DRAFTS>
+__device__ __forceinline__ int2 head_of(const PromptPlan& p, const int4& seg) {
+  if (DRAFTS) return make_int2(0, 0);
+  const uint64_t x = p.more[seg.w & 0xffff];
+  return make_int2((int)(uint32_t)x, (int)(x >> 32));
 }
 
 // The keys of a unit of drafts, all of one sequence: one stretch of its slots' rows.
@@ -77,7 +88,8 @@ __device__ __forceinline__ int draft_segs(const WinArgs& a, int n_tok, PromptPla
   return (n + kMlaBlk - 1) / kMlaBlk;
 }
 
-// The keys of a unit, by one warp.  Neighbouring rows of a sequence whose windows touch share two stretches: its first keys and those of their windows.
+// The keys of a unit, by one warp.  Neighbouring rows of a sequence whose windows touch share two stretches: its first keys and those of their windows.  Where
+// the first keys fit into the last block of the other stretch they are no block of their own, which costs a unit 1.1 to 1.7 us.
 template <bool DRAFTS>
 __device__ __forceinline__ int build_segs(const WinArgs& a, int n_tok, PromptPlan& p) {
   if constexpr (DRAFTS) return draft_segs(a, n_tok, p);
@@ -85,17 +97,28 @@ __device__ __forceinline__ int build_segs(const WinArgs& a, int n_tok, PromptPla
   int n = 0, blocks = 0, runs = 0;
   int rk = 0, ra = 0, rlo = 0, rhi = 0, r0 = 0, r1 = -1;             // the run that is open (r1 >= r0)
   int full0 = 0, full1 = 0x7fffffff, heads = 0x7fffffff;
-  auto put = [&](int lo, int hi) {
+  auto put = [&](int lo, int hi, int head) {
     if (lo >= hi) return;
-    if (lane == 0) p.segs[n] = make_int4(lo, hi, blocks, r0 | r1 << 16);
+    if (lane == 0) {
+      p.segs[n] = make_int4(lo, hi, blocks, r0 | r1 << 16);
+      p.more[r0] = (uint32_t)rk | (uint64_t)head << 32;
+    }
     ++n;
     blocks += (hi - lo + kMlaBlk - 1) / kMlaBlk;
   };
   auto close = [&]() {
     if (r1 < r0) return;
     ++runs;
-    put(rk, rlo <= ra ? rhi : ra);
-    if (rlo > ra) put(rlo, rhi);
+    // (with a gap between the stretches every row sees all of the first keys)
+    const int head = ra - rk, tail = (rhi - rlo) % kMlaBlk;
+    if (rlo <= ra || head > kWpHead || tail == 0 || tail + head > kMlaBlk) {
+      put(rk, rlo <= ra ? rhi : ra, 0);
+      if (rlo > ra) put(rlo, rhi, 0);
+    } else {
+      put(rlo, rhi + head, head);
+      for (int t = r0 + (lane - r0 & 31); t <= r1; t += 32)
+        if (p.sees[t].y > p.sees[t].x) p.sees[t].x = rhi, p.sees[t].y = rhi + head;
+    }
   };
   for (int base = 0; base < n_tok; base += 32) {
     const Sees mine = base + lane < n_tok ? sees_prompt(a, p.tok0 + base + lane) : Sees{};
@@ -604,7 +627,10 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           if (tok < (s.w & 0xffff) || tok > (s.w >> 16)) todo = 0;
 #pragma unroll 1
           for (; todo; todo &= todo - 1) {
-            const uint4* kp = reinterpret_cast<const uint4*>(a.kv + (int64_t)(k0 + __ffs(todo) - 1) * (kMlaDqk * 2));
+            int key = k0 + __ffs(todo) - 1;
+            const int2 head = head_of<DRAFTS>(p, s);
+            if (key >= s.y - head.y) key += head.x - (s.y - head.y);
+            const uint4* kp = reinterpret_cast<const uint4*>(a.kv + (int64_t)key * (kMlaDqk * 2));
             const uint4 v0 = __ldg(kp + lane), v1 = __ldg(kp + 32 + lane);
             float d = dot_bf16x2(qr, __ldg(reinterpret_cast<const uint32_t*>(kp + 64) + lane), 0.f);
             d = dot_bf16x2(q0.x, v0.x, d); d = dot_bf16x2(q0.y, v0.y, d); d = dot_bf16x2(q0.z, v0.z, d); d = dot_bf16x2(q0.w, v0.w, d);
@@ -757,7 +783,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         for (int i = 0; i < n && ok; ++i) {
           const int4 s = seg_of(p, at, blk_lo + i);
           const int key0 = s.x + (blk_lo + i - s.z) * kMlaBlk;
-          uint64_t* full = s.y - key0 < kMlaBlk ? part_full : ring_full;
+          uint64_t* full = s.y - head_of<DRAFTS>(p, s).y - key0 < kMlaBlk ? part_full : ring_full;
           claim(full, kMlaKBytes);
           if (!ok) break;
           full += e % NB;
@@ -770,8 +796,8 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         plan_done(k);
       }
     } else if (warp == kWpFixWarp) {
-      // ---- blocks that are not whole: their rows behind the end of the stretch become zeros, whatever they are (P is 0 there, and 0 x NaN is none).  No buffer is
-      // loaded again before what this warp does with it is done and used, so it is never two of a barrier's phases behind ----
+      // ---- blocks that are not whole: the rows behind the end of the stretch become the sequence's first keys, where they come there, and zeros, whatever they are
+      // (P is 0 there, and 0 x NaN is none).  No buffer is loaded again before what this warp does with it is done and used, so it is never two of a barrier's phases behind ----
       uint32_t e = 0, used = 0;                          // parity of each buffer's part_full
       bool ok = true;
       for (uint32_t k = 0; ok; ++k) {
@@ -783,13 +809,35 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         int at = 0;
         for (int i = 0; i < n && ok; ++i) {
           const int4 s = seg_of(p, at, blk_lo + i);
-          const int rows = s.y - s.x - (blk_lo + i - s.z) * kMlaBlk;
+          const int2 head = head_of<DRAFTS>(p, s);
+          const int rows = s.y - head.y - s.x - (blk_lo + i - s.z) * kMlaBlk;
           if (rows < kMlaBlk) {
             const uint32_t buf = e % NB;
+            uint8_t* dst = smem + buf * kMlaKBytes;
+            // a lane has 16 bytes of each of their latent halves, and of every eighth row's rope values; the first loads are under way before the block has landed
+            const uint8_t* src = a.kv + (int64_t)head.x * (kMlaDqk * 2);
+            uint4 v[4], x;
+            auto load = [&](int r0) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (r0 + j < head.y) v[j] = __ldg(reinterpret_cast<const uint4*>(src + (r0 + j) * (kMlaDqk * 2) + cta * kMlaDvHalf * 2) + lane);
+              if (r0 + (lane >> 2) < min(head.y, r0 + 4)) x = __ldg(reinterpret_cast<const uint4*>(src + (r0 + (lane >> 2)) * (kMlaDqk * 2) + kMlaDv * 2 + cta * 64) + (lane & 3));
+            };
+            load(0);
             if (!(ok = wait(&part_full[buf], used >> buf))) break;
             used ^= 1u << buf;
-            uint8_t* dst = smem + buf * kMlaKBytes;
-            for (int r = rows; r < kMlaBlk; ++r) {
+#pragma unroll 1
+            for (int r0 = 0; r0 < head.y; r0 += 4) {
+              if (r0 > 0) load(r0);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int r = rows + r0 + j;
+                if (r0 + j < head.y) *reinterpret_cast<uint4*>(dst + (lane >> 3) * kMlaKPanelBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = v[j];
+              }
+              const int r = rows + r0 + (lane >> 2);
+              if (r0 + (lane >> 2) < min(head.y, r0 + 4)) *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4)) = x;
+            }
+            for (int r = rows + head.y; r < kMlaBlk; ++r) {
               *reinterpret_cast<uint4*>(dst + (lane >> 3) * kMlaKPanelBytes + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
               if (lane < 4) *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + lane * 16) = make_uint4(0, 0, 0, 0);
             }

@@ -65,6 +65,31 @@ def test_packed_prompts_and_rows_that_see_nothing(H, window, first):
 
 
 @pytest.mark.parametrize("H", [128, 16, 5])
+@pytest.mark.parametrize("first", [1, 4, 8, 9, 16, 17])
+def test_first_tokens_and_windows_that_end_anywhere_in_a_block(H, first):
+    """Windows whose last block has room for the first tokens, just not, or none of its own; two sequences of them side by side, rows between that see nothing."""
+    n, S, at = 24, 900, 400                               # a sequence of 400 tokens and one of 500
+    g = torch.Generator().manual_seed(first)
+    for window in (33, 64 - first, 65 - first, 64, 65, 129, 150):
+        last = torch.cat((torch.arange(370, 370 + n), at + torch.arange(200, 200 + n)))
+        ks = torch.cat((torch.zeros(n), torch.full((n,), at))).long()
+        ke = last + 1
+        none = torch.randperm(2 * n, generator=g)[:5]
+        ke[none] = ks[none]
+        q, kv = rows(2 * n, H, seed=window), rows(S, seed=first)
+        sees = D.prompt_sees(2 * n, S, window, first, ks, ke)
+        check(ops.window_mla_prefill(q, kv, i32(ks), i32(ke), window, first, SCALE), D.attend(q, kv, sees, SCALE))
+        for bad in (0, at + first - 1, at + first, 372 - window, 394, 600 - window):      # keys that are no numbers: first tokens, one behind them, ends of windows
+            dirty = kv.clone()
+            dirty[bad, 300], dirty[bad, 30] = float("nan"), float("inf")
+            out = ops.window_mla_prefill(q, dirty, i32(ks), i32(ke), window, first, SCALE)
+            touched = sees[:, bad].cuda()
+            assert bool((~out[touched].isfinite()).flatten(1).any(1).all())
+            check(out[~touched], D.attend(q, kv, sees, SCALE).cuda()[~touched])
+        ops.check_status("cuda")
+
+
+@pytest.mark.parametrize("H", [128, 16, 5])
 def test_rows_in_any_order(H):
     """Rows of a rank that has every other stretch of a sequence, and rows in no order at all."""
     S, window, first = 700, 90, 4
