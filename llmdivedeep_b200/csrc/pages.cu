@@ -556,7 +556,9 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
 // Row rows[i] keeps the drafts path[i, 0 .. n_keep[i]) of its last n_new[i] tokens: draft path[k] moves to place k behind the P tokens before
 // them, in every cache; what lies behind goes.  path[k] >= k, so a place that is written is read by no later move, and a thread that takes
 // the same 16 bytes of every token in order needs no barrier.  One CTA a row and 128 columns of 16 bytes; what bounds it is latency: list, table, then eight
-// records under way at a time, and the pages in a second kernel, which starts under the first (8 rows x 2 layers 10.3 us, 200 x 16 14.4).
+// records under way at a time, and the pages in a second kernel, which starts under the first (200 rows x 16 layers 14.4 us).  Calls of up to eight rows whose columns
+// are a CTA's threads are one cluster, and one launch: 8 rows x 2 layers 15.4 -> 13.8 us on the host, which the GPU's 8 wait for.
+constexpr int kAcceptAlone = 8, kAcceptThreads = 1024;
 template <int N>
 struct AcceptCaches {                                  // of a launch; eight hold most models' in a tenth of the parameters
   CacheEntry cache[N];
@@ -611,19 +613,33 @@ __device__ __forceinline__ void accept_column(const AcceptArgs& a, const CacheEn
       if (from[j] > k0 + j) *at(P + k0 + j) = v[j];
   }
 }
-template <int N>
-__global__ void __launch_bounds__(kCopyThreads) accept_kernel(const AcceptArgs a, const __grid_constant__ AcceptCaches<N> cs, int lead) {
-  launch_dependents();
+// The length and the pages of entry i, when all contents have moved; every thread of the CTA has read the length.
+__device__ __forceinline__ void accept_pages(const AcceptArgs& a, int row, int c, int now) {
+  if (threadIdx.x == 0) a.ctx[row] = now;
+  for (int p = pages_of(now) + threadIdx.x; p < pages_of(c); p += blockDim.x) {
+    int32_t* entry = a.table + (int64_t)row * a.stride + p;
+    const int page = *entry;
+    *entry = -1;
+    if (atomicSub(&a.refs[page], 1) > 0) continue;
+    atomicAdd(&a.refs[page], 1);                       // was free already: the state is not what it says
+    if (a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
+  }
+}
+// ALONE: the whole call is one cluster, a CTA a row, and the pages go here: every row has been looked at before one changes.
+template <int N, bool ALONE>
+__global__ void __launch_bounds__(ALONE ? kAcceptThreads : kCopyThreads) accept_kernel(const AcceptArgs a, const __grid_constant__ AcceptCaches<N> cs, int lead) {
+  if (!ALONE) launch_dependents();
   const int i = blockIdx.x, cols = cs.first[cs.n_caches];
   const bool ok = accept_valid(a, i);
-  if (lead && blockIdx.y == 0 && threadIdx.x == 0) a.accepted[i] = ok;
+  if (ALONE) pool_sync();
+  else if (lead && blockIdx.y == 0 && threadIdx.x == 0) a.accepted[i] = ok;
   if (!ok) {
     if (threadIdx.x == 0 && a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
     return;
   }
-  const int row = a.rows[i], P = a.ctx[row] - a.n_new[i], keep = a.n_keep[i];
+  const int row = a.rows[i], ctx = a.ctx[row], P = ctx - a.n_new[i], keep = a.n_keep[i];
   const int32_t *trow = a.table + (int64_t)row * a.stride, *path = a.path + (int64_t)i * a.path_stride;
-  for (int c = blockIdx.y * kCopyThreads + threadIdx.x; c < cols; c += gridDim.y * kCopyThreads) {
+  for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < cols; c += gridDim.y * blockDim.x) {
     int e = 0;
     for (int hi = cs.n_caches; hi - e > 1;) {          // the cache that column c belongs to
       const int mid = (e + hi) / 2;
@@ -635,22 +651,17 @@ __global__ void __launch_bounds__(kCopyThreads) accept_kernel(const AcceptArgs a
     if (wide == 16) accept_column<uint4>(a, ce, base, trow, path, P, keep);
     else accept_column<uint32_t>(a, ce, base, trow, path, P, keep);
   }
+  if (ALONE) {
+    __syncthreads();
+    accept_pages(a, row, ctx, P + keep);
+  }
 }
-// Lengths and pages, when all contents have moved.
 __global__ void __launch_bounds__(kCopyThreads) accept_pages_kernel(const AcceptArgs a) {
   const int i = blockIdx.x;
   if (!grid_wait(a.accepted)[i]) return;
-  const int row = a.rows[i], c = a.ctx[row], now = c - a.n_new[i] + a.n_keep[i];
-  __syncthreads();                                     // every thread has read the length
-  if (threadIdx.x == 0) a.ctx[row] = now;
-  for (int p = pages_of(now) + threadIdx.x; p < pages_of(c); p += kCopyThreads) {
-    int32_t* entry = a.table + (int64_t)row * a.stride + p;
-    const int page = *entry;
-    *entry = -1;
-    if (atomicSub(&a.refs[page], 1) > 0) continue;
-    atomicAdd(&a.refs[page], 1);                       // was free already: the state is not what it says
-    if (a.status) atomicCAS(a.status, kStatusOk, kStatusBadIndex);
-  }
+  const int row = a.rows[i], c = a.ctx[row];
+  __syncthreads();
+  accept_pages(a, row, c, c - a.n_new[i] + a.n_keep[i]);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------
@@ -786,8 +797,9 @@ int compact_pages_launch(const int32_t* table, int64_t stride, int32_t* new_tabl
   return launch_copies<kCopyCompact>(c, PoolArgs{}, m, caches, n_caches, num_pages / 2, ((int64_t)B * P + 31) / 32, stream);
 }
 
+// Whether the pages have gone too.
 template <int N>
-static void launch_accept(const AcceptArgs& a, const dsa_page_cache* caches, int n_caches, int lead, cudaStream_t stream) {
+static bool launch_accept(const AcceptArgs& a, const dsa_page_cache* caches, int n_caches, int lead, cudaStream_t stream) {
   AcceptCaches<N> cs;
   cs.n_caches = n_caches;
   cs.first[0] = 0;
@@ -797,7 +809,24 @@ static void launch_accept(const AcceptArgs& a, const dsa_page_cache* caches, int
     cs.first[c + 1] = cs.first[c] + h.layers * (h.token_bytes / (h.token_bytes % 16 == 0 ? 16 : 4));
   }
   const int split = min(max(1, (cs.first[n_caches] + kCopyThreads - 1) / kCopyThreads), 65535);
-  accept_kernel<N><<<dim3(a.n, split), kCopyThreads, 0, stream>>>(a, cs, lead);
+  if constexpr (N == 8) {
+    if (a.n <= kAcceptAlone && split * kCopyThreads <= kAcceptThreads) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = a.n;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(a.n);
+      cfg.blockDim = dim3(split * kCopyThreads);
+      cfg.stream = stream;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      cudaLaunchKernelEx(&cfg, accept_kernel<8, true>, a, cs, lead);      // its error is the launch check's
+      return true;
+    }
+  }
+  accept_kernel<N, false><<<dim3(a.n, split), kCopyThreads, 0, stream>>>(a, cs, lead);
+  return false;
 }
 
 int accept_drafts_launch(int32_t* table, int64_t stride, int P, int B, int32_t* ctx, int32_t* refs, int num_pages, const int32_t* rows, const int32_t* n_new,
@@ -809,12 +838,13 @@ int accept_drafts_launch(int32_t* table, int64_t stride, int P, int B, int32_t* 
   a.rows = rows; a.n_new = n_new; a.path = path; a.path_stride = path_stride; a.n_keep = n_keep;
   a.accepted = workspace;
   a.status = status;
+  bool done = false;
   if (n_caches <= 8) {
-    launch_accept<8>(a, caches, n_caches, 1, stream);
+    done = launch_accept<8>(a, caches, n_caches, 1, stream);
   } else {
     for (int c0 = 0; c0 < n_caches; c0 += kCopyCaches) launch_accept<kCopyCaches>(a, caches + c0, min(n_caches - c0, kCopyCaches), c0 == 0, stream);
   }
-  launch_after(1, accept_pages_kernel, dim3(n), kCopyThreads, 0, stream, a);
+  if (!done) launch_after(1, accept_pages_kernel, dim3(n), kCopyThreads, 0, stream, a);
   return check_launch("accept_drafts");
 }
 

@@ -335,6 +335,24 @@ def test_pages_that_another_sequence_holds_are_not_written():
     p.extend([0, 1], [3, 3], 4)
 
 
+@pytest.mark.parametrize("others", [0, 7])
+def test_rows_are_judged_before_any_changes(others):
+    """A row that drops a page and one that keeps drafts in it, in one call of few rows and of more: the second is refused, in either order."""
+    for order in ((0, 1), (1, 0)):
+        p = Drafting(2 + others, 4, 60)
+        p.extend(range(2 + others), [128] + [0] + [20] * others, 128)
+        p.fork([0], [1])                                   # both pages are full, and shared
+        rows = list(order) + list(range(2, 2 + others))
+        p.accept(rows, [64, 64] + [3] * others, [[0, 1] if r > 1 else [3, 0] for r in rows], [2 if r > 1 else 0 if r == 0 else 1 for r in rows], status=2)
+
+
+def test_few_rows_that_make_no_sense_stay_as_they_are():
+    p = Drafting(8, 3, 30, 2)
+    p.extend(range(8), [10, 70, 100, 40, 50, 60, 64, 128], 192)
+    p.accept([0, 1, 3, 4, 8, 0], [4, 71, 5, 5, 1, 2], [[0, 3], [0, 1], [3, 2], [0, 5], [0, 1], [0, 1]], [2, 2, 2, 2, 1, 1], status=2)
+    p.accept([7], [100], [[99]], [1])
+
+
 def test_accept_refused():
     p = Drafting(2, 2, 9)
     args = dict(block_table=p.table, ctx_len=p.ctx, refs=p.refs, rows=ints([0]), n_new=ints([1]), path=ints([[0]]), n_keep=ints([1]), caches=p.caches)
