@@ -11,10 +11,11 @@
 //   * four more warps move Q into tensor memory and O out of it, so that the softmax goes from unit to unit without a pause.
 // Roles: warps 0-15 exchange + softmax, 16 MMA issuer, 17 loads, 18 zeros in the rows behind the end of a stretch, 19 plans the next unit, 20-23 Q and O.
 // Every wait is bounded (dsa_common.cuh); the two CTAs leave together through a cluster barrier.
-// What bounds it: 0.93 us a block, of which the tensor pipe works 0.58 and the softmax warps' chain the rest, and what a unit costs besides.  us a unit of 128 heads
-// by window: 64 5.9, 128 7.3, 256 8.2, 512 11.4, 1024 19.0, 2048 34.6 (one CTA pair a unit, not persistent: 10.3 with one block); of 8 tokens x 16
-// heads 8.6, 9.1, 10.7, 13.8, 21, 36.  8192 tokens x 128 heads at 128K, window 4096: 7600 to 8000 us = 1175 to 1235 TFLOP/s at the power cap, 8660 by the kernel of
-// one unit a pair; packed prompts of 16 heads 190 us for 64 us of operations: their units have few blocks, and the last round of them is a part of one.
+// What bounds it: 0.93 us a block, of which the tensor pipe works 0.58 and the softmax warps' chain the rest -- a buffer is held for 4.6 us, load, exchange, softmax
+// and P.V -- and the entries of the ring that a unit needs besides.  us a unit, four first tokens, by window: 128 heads 64 7.6, 512 13.4, 2048 36.3; 8 tokens x
+// 16 heads 64 8.1, 512 12.9, 1024 20.4 (a unit of one block 6.2; by a pair that takes one unit only, 10.3).  8192 tokens x 128 heads at 128K, window 4096:
+// 7600 to 8000 us = 1175 to 1235 TFLOP/s at the power cap, 8660 by pairs of one unit; packed prompts of 16 heads, window 512, 184 us for 64 us of operations:
+// their units have few blocks, and the last round of units is a part of one.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
