@@ -251,6 +251,21 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     tmem_alloc(tmem_slot, kMlaTmemCols);
     tmem_relinquish();
   }
+  // The first job's plan while the others set up.
+  LiveUnits found;
+  int job0 = -1, blocks0 = 0;
+  auto job_at = [&](int nth) { return DRAFTS && a.live ? found.find(a, nth) : nth < jobs ? nth : -1; };
+  auto keys_of = [&](const JobRows& j, PromptPlan& p) {
+    const int tok0 = j.row0 / a.H;
+    __syncwarp();
+    if (lane == 0) p.tok0 = tok0;
+    __syncwarp();
+    return build_segs<DRAFTS>(a, (j.row0 + j.rows - 1) / a.H - tok0 + 1, p);
+  };
+  if (warp == kWpPlanWarp) {
+    job0 = job_at(pair);
+    if (job0 >= 0) blocks0 = keys_of(job_rows<DRAFTS>(a, job0), plans[0]);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -587,16 +602,18 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       e += n;
     }
     if (ok && k > 0) drain(k - 1, e);
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-    __syncwarp();
+    if (redos > 0) {                                   // what is written again has been written
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      __syncwarp();
+    }
     // Rare: rows key by key over what they see of their job's blocks, this CTA's half of the output from whole scores.  Nobody waits for this warp now (but at the
     // barrier that the pair leaves through, which has no limit).  With more on the list than it holds: every row of the pair's jobs.
     const int redo_jobs = redos > kWpRedo ? (jobs - pair + n_pairs - 1) / n_pairs : redos;
-    LiveUnits found;
+    LiveUnits units;
 #pragma unroll 1
     for (int x = 0; ok && x < redo_jobs; ++x) {
       int job = redos > kWpRedo ? pair + x * n_pairs : (int)redo_s[x].x;
-      if (DRAFTS && a.live && redos > kWpRedo && (job = found.find(a, job)) < 0) break;
+      if (DRAFTS && a.live && redos > kWpRedo && (job = units.find(a, job)) < 0) break;
       uint32_t mask = redos > kWpRedo ? 0xffffffffu : redo_s[x].y;
       PromptPlan& p = plans[qd];                       // each warp its own; of the jobs' plans nobody needs more than `blocks`
       const JobRows j = job_rows<DRAFTS>(a, job);
@@ -854,9 +871,8 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       // ------------------------------- plans -------------------------------
       uint32_t k = 0;
       bool ok = true, mine = false;                      // the buffer of plan k is this warp's
-      LiveUnits found;
-    for (int next = pair; ok && !aborted_warp(abort_flag); next += n_pairs) {
-      const int job = DRAFTS && a.live ? found.find(a, next) : next < jobs ? next : -1;
+      for (int next = pair; ok && !aborted_warp(abort_flag); next += n_pairs) {
+        const int job = next == pair ? job0 : job_at(next);
         if (!mine) ok = wait(&plan_free[k % kWpPlans], (k / kWpPlans) + 1);
         mine = true;
         const bool more = job >= 0;
@@ -870,11 +886,8 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           break;
         }
         const JobRows j = job_rows<DRAFTS>(a, job);
-        const int row0 = j.row0, rows = j.rows, part = j.part, tok0 = row0 / a.H;
-        __syncwarp();
-        if (lane == 0) p.tok0 = tok0;
-        __syncwarp();
-        const int blocks = build_segs<DRAFTS>(a, (row0 + rows - 1) / a.H - tok0 + 1, p);
+        const int row0 = j.row0, rows = j.rows, part = j.part;
+        const int blocks = next == pair ? blocks0 : keys_of(j, p);
         const int per = (blocks + j.n_split - 1) / j.n_split, blk_lo = min(blocks, j.split * per), n = min(blocks, blk_lo + per) - blk_lo;
         if (n == 0) {                                    // nothing seen: zeros (a part: weight zero when they are merged)
           if (part < 0) {
