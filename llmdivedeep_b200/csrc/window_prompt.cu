@@ -32,7 +32,8 @@ struct PromptPlan {
   int blocks, blk_lo;                                  // blocks of the job (-1: there are no more jobs), and which is its first
   int full0, full1;                                    // keys that every row sees which sees any (one sequence in the unit)
   int row0, rows, part, tok0;                          // first query row, rows, part (-1: a whole unit), token of the first row
-  int job, at, holes, pad;                             // drafts: key of the first draft; a key without a page
+  int job, at, holes;                                  // drafts: key of the first draft; a key without a page
+  int ready;                                           // of the first plan: written before the CTA's first barrier
   int4 sees[kWpTokens];                                // of the unit's tokens: {a0, a1, b0, b1}
   // Drafts: which of them each sees.  Prompts, of the first token of a stretch: the last keys of the stretch may be the sequence's first ones, behind its own,
   // and are known by their places in the tokens' `sees`; which is the first of those | how many << 32.
@@ -251,20 +252,27 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     tmem_alloc(tmem_slot, kMlaTmemCols);
     tmem_relinquish();
   }
-  // The first job's plan while the others set up.
+  // The plan of a job, by a warp: its blocks (0: nothing is seen), all else in p.
   LiveUnits found;
-  int job0 = -1, blocks0 = 0;
   auto job_at = [&](int nth) { return DRAFTS && a.live ? found.find(a, nth) : nth < jobs ? nth : -1; };
-  auto keys_of = [&](const JobRows& j, PromptPlan& p) {
+  auto make_plan = [&](int job, const JobRows& j, PromptPlan& p) {
     const int tok0 = j.row0 / a.H;
     __syncwarp();
     if (lane == 0) p.tok0 = tok0;
     __syncwarp();
-    return build_segs<DRAFTS>(a, (j.row0 + j.rows - 1) / a.H - tok0 + 1, p);
+    const int blocks = build_segs<DRAFTS>(a, (j.row0 + j.rows - 1) / a.H - tok0 + 1, p);
+    const int per = j.n_split == 1 ? blocks : (blocks + j.n_split - 1) / j.n_split, blk_lo = min(blocks, j.split * per), n = min(blocks, blk_lo + per) - blk_lo;
+    if (lane == 0) {
+      p.blocks = n; p.blk_lo = blk_lo;
+      p.row0 = j.row0; p.rows = j.rows; p.part = j.part; p.job = job;
+    }
+    return n;
   };
-  if (warp == kWpPlanWarp) {
+  int job0 = -1, n0 = 0;
+  if (warp == kWpPlanWarp) {                                   // the first one while the others set up
     job0 = job_at(pair);
-    if (job0 >= 0) blocks0 = keys_of(job_rows<DRAFTS>(a, job0), plans[0]);
+    if (job0 >= 0) n0 = make_plan(job0, job_rows<DRAFTS>(a, job0), plans[0]);
+    if (lane == 0) plans[0].ready = n0 > 0;
   }
   tc_fence_before();
   __syncthreads();
@@ -275,7 +283,8 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 
   auto wait = [&](uint64_t* bar, uint32_t phase) { return mla_wait(bar, phase & 1, abort_flag, a.status); };
   // the plan of this CTA's k-th job; false: give up
-  auto plan_of = [&](uint32_t k) { return wait(&plan_full[k % kWpPlans], k / kWpPlans); };
+  const bool ready = plans[0].ready != 0;
+  auto plan_of = [&](uint32_t k) { return (k == 0 && ready) || wait(&plan_full[k % kWpPlans], k / kWpPlans); };
   auto plan_done = [&](uint32_t k) {
     __syncwarp();
     if (lane == 0) mbar_arrive(&plan_free[k % kWpPlans]);
@@ -462,7 +471,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       named_bar_sync(1, 128);
       if (warp == kWpOutWarp && lane == 0) mbar_arrive(&ring_free[e % NB]);
     };
-    auto drain = [&](uint32_t k, uint32_t e) {         // the output of job k, staged in entry e
+    auto drain = [&](uint32_t k, uint32_t e, bool last) {      // the output of job k, staged in entry e, of the last job one of its own
       const PromptPlan& p = plans[k % kWpPlans];
       const int row0 = p.row0, rows = p.rows, part = p.part;
       const int tok = row < rows ? (row0 + row) / a.H - p.tok0 : 0;
@@ -497,7 +506,9 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (part >= 0)                                   // what this CTA's half of the columns is weighted with
         a.part_lse[((int64_t)part * 2 + cta) * 128 + row] = l > 0.f ? mt + log2f(l) : l == 0.f ? -CUDART_INF_F : l;
       {
-        uint8_t* const stage0 = smem + (e % NB) * kMlaKBytes + kMlaQPanelBytes + qd * 4096 + lane * 64;      // two pieces of 32 rows x 32 columns to a warp
+        // pieces of 32 rows x 32 columns, two to a warp, of the last job four
+        uint8_t* const stage0 = smem + (e % NB) * kMlaKBytes + (last ? qd * 8192 : kMlaQPanelBytes + qd * 4096) + lane * 64;
+        const uint32_t wrap = last ? 3 * 2048 : 2048;
         __nv_bfloat16* const orow = a.out + (int64_t)(row0 + row) * kMlaDv + cta * kMlaDvHalf;
         const uint64_t inv2 = pack_f32x2(inv, inv);
         const bool blind = __any_sync(0xffffffffu, !any);
@@ -527,12 +538,15 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             uint32_t (&now)[16] = ov[(c >> 4) & 1];
             tmem_wait_ld();
             if (c + 16 < kMlaDvHalf) tmem_ld16(t_row + kColO + c + 16, ov[((c >> 4) & 1) ^ 1]);
-            if (c >= 64 && (c & 31) == 0) {            // the store of two pieces before has read its own
-              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            if (c >= 64 && (c & 31) == 0 && (!last || c >= 128)) {      // the store of two, or four, pieces before has read its own
+              if (lane == 0) {
+                if (last) asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory");
+                else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+              }
               __syncwarp();
             }
             scaled(now);
-            uint8_t* stage = stage0 + ((c >> 5) & 1) * 2048;
+            uint8_t* stage = stage0 + (((c >> 5) * 2048) & wrap);
             *reinterpret_cast<uint4*>(stage + (((((c & 31) >> 3) + 0) ^ (lane >> 1 & 3)) << 4)) = eight(now, 0);
             *reinterpret_cast<uint4*>(stage + (((((c & 31) >> 3) + 1) ^ (lane >> 1 & 3)) << 4)) = eight(now, 8);
             if ((c & 31) == 16) {
@@ -597,11 +611,16 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
-      if (k > 0) drain(k - 1, e - 1);                  // the output of the unit before is staged behind the last query panel
+      if (k == 0) {                                    // nothing remote is ever left to do for this warp
+        cluster_wait();
+        cluster_arrive();
+        left = true;
+      }
+      if (k > 0) drain(k - 1, e - 1, false);           // the output of the unit before is staged behind the last query panel
       if (!ok) break;
       e += n;
     }
-    if (ok && k > 0) drain(k - 1, e);
+    if (ok && k > 0) drain(k - 1, e, true);
     if (redos > 0) {                                   // what is written again has been written
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       __syncwarp();
@@ -678,6 +697,12 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     }
   } else {
     regs_dec<kWpRegsRoles>();
+    auto load_keys = [&](uint32_t buf, int key0, uint64_t* full) {
+      uint8_t* dst = smem + buf * kMlaKBytes;
+      if (lane < 4) tma_load_2d(dst + lane * kMlaKPanelBytes, &tmap_lat, (cta * 4 + lane) * 32, key0, full);      // x in 4-byte units
+      else if (lane == 4) tma_load_2d(dst + kMlaRopeOff, &tmap_rope, kMlaDv / 2 + cta * 16, key0, full);
+      __syncwarp();
+    };
     if (warp == kWpMmaWarp) {
       // ------------------------------- MMA issuer -------------------------------
       // Of a unit the scores of a block, then P.V two blocks behind; across units P.V of the last but one, the next unit's first scores, P.V of the last.
@@ -790,6 +815,10 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           break;
         }
         for (int j = 0; j < 3 && ok; ++j) {              // Q: panels 2 j and 2 j + 1
+          if (k == 0 && j == 2) {
+            ++e;
+            break;
+          }
           claim(ring_full, j < 2 ? 2 * kMlaQPanelBytes : kMlaQPanelBytes);
           const int lp = 2 * j + lane;                   // x in 4-byte units: 32 per panel
           if (ok && lane < 2 && lp < kMlaPanels)
@@ -802,13 +831,11 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           const int4 s = seg_of(p, at, blk_lo + i);
           const int key0 = s.x + (blk_lo + i - s.z) * kMlaBlk;
           uint64_t* full = s.y - head_of<DRAFTS>(p, s).y - key0 < kMlaBlk ? part_full : ring_full;
-          claim(full, kMlaKBytes);
-          if (!ok) break;
-          full += e % NB;
-          uint8_t* dst = smem + (e % NB) * kMlaKBytes;
-          if (lane < 4) tma_load_2d(dst + lane * kMlaKPanelBytes, &tmap_lat, (cta * 4 + lane) * 32, key0, full);      // x in 4-byte units
-          else if (lane == 4) tma_load_2d(dst + kMlaRopeOff, &tmap_rope, kMlaDv / 2 + cta * 16, key0, full);
-          __syncwarp();
+          if (k > 0 || i > 0) {
+            claim(full, kMlaKBytes);
+            if (!ok) break;
+            load_keys(e % NB, key0, full + e % NB);
+          }
           ++e;
         }
         plan_done(k);
@@ -829,8 +856,14 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           const int4 s = seg_of(p, at, blk_lo + i);
           const int2 head = head_of<DRAFTS>(p, s);
           const int rows = s.y - head.y - s.x - (blk_lo + i - s.z) * kMlaBlk;
+          const uint32_t buf = e % NB;
+          if (k == 0 && i == 0) {                        // (the first block's loads: while others see to the queries')
+            uint64_t* full = (rows < kMlaBlk ? part_full : ring_full) + buf;
+            if (lane == 0) mbar_expect_tx(full, kMlaKBytes);
+            __syncwarp();
+            load_keys(buf, s.y - head.y - rows, full);
+          }
           if (rows < kMlaBlk) {
-            const uint32_t buf = e % NB;
             uint8_t* dst = smem + buf * kMlaKBytes;
             // a lane has 16 bytes of each of their latent halves, and of every eighth row's rope values; the first loads are under way before the block has landed
             const uint8_t* src = a.kv + (int64_t)head.x * (kMlaDqk * 2);
@@ -855,10 +888,10 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
               const int r = rows + r0 + (lane >> 2);
               if (r0 + (lane >> 2) < min(head.y, r0 + 4)) *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4)) = x;
             }
-            for (int r = rows + head.y; r < kMlaBlk; ++r) {
-              *reinterpret_cast<uint4*>(dst + (lane >> 3) * kMlaKPanelBytes + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-              if (lane < 4) *reinterpret_cast<uint4*>(dst + kMlaRopeOff + r * 64 + lane * 16) = make_uint4(0, 0, 0, 0);
-            }
+            uint8_t* zero = dst + (lane >> 3) * kMlaKPanelBytes + (lane & 7) * 16;
+#pragma unroll 4
+            for (int r = rows + head.y; r < kMlaBlk; ++r) *reinterpret_cast<uint4*>(zero + r * 128) = make_uint4(0, 0, 0, 0);
+            for (int c = 4 * (rows + head.y) + lane; c < 4 * kMlaBlk; c += 32) *reinterpret_cast<uint4*>(dst + kMlaRopeOff + c * 16) = make_uint4(0, 0, 0, 0);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ring_full[buf]);
@@ -870,15 +903,14 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     } else if (warp == kWpPlanWarp) {
       // ------------------------------- plans -------------------------------
       uint32_t k = 0;
-      bool ok = true, mine = false;                      // the buffer of plan k is this warp's
+      bool ok = true, mine = true;                       // the buffer of plan k is this warp's: the first one from the start
       for (int next = pair; ok && !aborted_warp(abort_flag); next += n_pairs) {
         const int job = next == pair ? job0 : job_at(next);
         if (!mine) ok = wait(&plan_free[k % kWpPlans], (k / kWpPlans) + 1);
         mine = true;
-        const bool more = job >= 0;
         PromptPlan& p = plans[k % kWpPlans];
         if (!ok) break;
-        if (!more) {
+        if (job < 0) {
           if (lane == 0) {
             p.blocks = -1;
             mbar_arrive(&plan_full[k % kWpPlans]);
@@ -886,24 +918,23 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           break;
         }
         const JobRows j = job_rows<DRAFTS>(a, job);
-        const int row0 = j.row0, rows = j.rows, part = j.part;
-        const int blocks = next == pair ? blocks0 : keys_of(j, p);
-        const int per = (blocks + j.n_split - 1) / j.n_split, blk_lo = min(blocks, j.split * per), n = min(blocks, blk_lo + per) - blk_lo;
+        const int n = next == pair ? n0 : make_plan(job, j, p);
         if (n == 0) {                                    // nothing seen: zeros (a part: weight zero when they are merged)
-          if (part < 0) {
-            for (int r = 0; r < rows; ++r)
-              reinterpret_cast<uint4*>(a.out + (int64_t)(row0 + r) * kMlaDv + cta * kMlaDvHalf)[lane] = make_uint4(0, 0, 0, 0);
+          if (j.part < 0) {
+            for (int r = 0; r < j.rows; ++r)
+              reinterpret_cast<uint4*>(a.out + (int64_t)(j.row0 + r) * kMlaDv + cta * kMlaDvHalf)[lane] = make_uint4(0, 0, 0, 0);
           } else {
-            for (int r = lane; r < 128; r += 32) a.part_lse[((int64_t)part * 2 + cta) * 128 + r] = -CUDART_INF_F;
+            for (int r = lane; r < 128; r += 32) a.part_lse[((int64_t)j.part * 2 + cta) * 128 + r] = -CUDART_INF_F;
           }
           continue;
         }
-        if (lane == 0) {
-          p.blocks = n; p.blk_lo = blk_lo;
-          p.row0 = row0; p.rows = rows; p.part = part; p.job = job;
-        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&plan_full[k % kWpPlans]);
+        if (k == 0 && lane == 0) {                       // the third entry of the first job: three warps share what it waits for
+          mbar_expect_tx(ring_full + 2, kMlaQPanelBytes);
+          tma_load_2d(smem + 2 * kMlaKBytes, &tmap_q, 8 * 32, j.row0, ring_full + 2);
+        }
+        __syncwarp();
         ++k;
         mine = false;
       }
@@ -911,7 +942,8 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   }
 
   __syncwarp();
-  if (warp >= 16) cluster_wait();                    // the wait that pairs with the arrive above (softmax: before its first remote access)
+  if (warp >= 16 && !left) cluster_wait();           // the wait that pairs with the arrive above (softmax: before its first remote access)
+  if (!left) cluster_arrive();                       // remote accesses, if any, are behind this warp: the others need not wait for the output
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
@@ -920,7 +952,6 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       for (int w = 0; w < 64; ++w) __nanosleep(1000);
     __syncthreads();
   }
-  if (!left) cluster_arrive();
   cluster_wait();                 // neither CTA leaves while the other may still copy into it or arrive on its barriers
   if (warp == kWpMmaWarp) {
     tc_fence_after();
