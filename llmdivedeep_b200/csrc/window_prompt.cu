@@ -13,9 +13,10 @@
 // Every wait is bounded (dsa_common.cuh); the two CTAs leave together through a cluster barrier.
 // What bounds it: 0.93 us a block, of which the tensor pipe works 0.58 and the softmax warps' chain the rest -- a buffer is held for 4.6 us, load, exchange, softmax
 // and P.V -- and the entries of the ring that a unit needs besides.  us a unit, four first tokens, by window: 128 heads 64 7.6, 512 13.4, 2048 36.3; 8 tokens x
-// 16 heads 64 8.1, 512 12.9, 1024 20.4 (a unit of one block 6.2; by a pair that takes one unit only, 10.3).  8192 tokens x 128 heads at 128K, window 4096:
-// 7600 to 8000 us = 1175 to 1235 TFLOP/s at the power cap, 8660 by pairs of one unit; packed prompts of 16 heads, window 512, 184 us for 64 us of operations:
-// their units have few blocks, and the last round of units is a part of one.
+// 16 heads 64 8.4, 512 12.7, 1024 20.1 (a unit of one block 6.3; by a pair that takes one unit only, 10.3).  8192 tokens x 128 heads at 128K, window 4096:
+// 7600 to 8000 us = 1175 to 1235 TFLOP/s at the power cap, 8660 by pairs of one unit; packed prompts of 16 heads, window 512, 181 us for 64 us of operations:
+// their units have few blocks, and the last round of units is a part of one.  40 tokens x 128 heads: 10.4 to 10.9 us, a chain of set-up and plan 1.2, loads 1.6 to 2,
+// scores 0.9, exchange and softmax 1.8, P.V 0.6, output 2.2.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
