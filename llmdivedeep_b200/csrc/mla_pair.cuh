@@ -23,10 +23,10 @@ constexpr int kMlaKBytes = kMlaRopeOff + kMlaBlk * 64;        // 36864 per buffe
 constexpr int kMlaXBytes = 128 * kMlaBlk * 2;      // one partial score tile, fp16: 16384
 constexpr int kMlaXWarp = kMlaXBytes / 8;          // ... a warp's part of it
 constexpr int kMlaValidRing = 8;                   // validity bytes (64 per block) for the softmax: >= blocks in flight
-// The registers of the launch (896 threads x 72) are dealt out again: setmaxnreg moves what the issuing and gathering
-// warps do not need to the softmax.
 // Where the rows come from: bf16 rows (prefill), records of the paged FP8 latent cache, records of the paged 4-bit one (latent4.cuh).
 enum MlaSrc : int { kSrcRows = 0, kSrcFp8 = 1, kSrc4 = 2 };
+// The registers of the launch (896 threads x 72) are dealt out again: setmaxnreg moves what the issuing and gathering
+// warps do not need to the softmax.
 template <bool PAGED>
 struct MlaRegs {                                   // decode's gather converts in registers
   static constexpr int kSoftmax = PAGED ? 88 : 96, kOther = PAGED ? 48 : 40;
