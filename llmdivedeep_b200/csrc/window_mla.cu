@@ -55,14 +55,14 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   const int cta = blockIdx.x & 1, peer = cta ^ 1;              // rank in the cluster = V half = contraction part
   const int job = blockIdx.x >> 1;
   const int part = job < a.n_full ? -1 : job - a.n_full;       // >= 0: a part of a unit's keys
-  const int n_split = part < 0 ? 1 : a.n_split, unit = part < 0 ? job : a.n_full + part / n_split, split = part < 0 ? 0 : part % n_split;
+  const int n_split = part < 0 ? 1 : a.n_split, nth = part < 0 ? 0 : part / n_split, unit = part < 0 ? job : a.n_full + nth, split = part < 0 ? 0 : part - nth * n_split;
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int seq = unit / a.seq_units;
+  const int seq = a.seq_units == 1 ? unit : unit / a.seq_units;      // (divisions stand before the first load)
   const int row0 = (unit - seq * a.seq_units) * a.unit_rows;   // of the sequence's query rows
   const int rows_here = min(a.unit_rows, a.seq_rows - row0);
   const int64_t g0 = (int64_t)seq * a.seq_rows + row0;
   const int n_quad = (rows_here + 31) / 32;                    // quadrants of tensor memory with rows in them: the others' warps stand by
-  const int tok0 = row0 / a.H, tok1 = (row0 + rows_here - 1) / a.H;
+  const int tok0 = row0 == 0 ? 0 : row0 / a.H, tok1 = a.seq_units == 1 ? a.drafts.per_seq - 1 : (row0 + rows_here - 1) / a.H;
   // the five Q panels wait at the end of the KV buffers (from buffer kQBuf0 on) for their move into tensor memory
   constexpr int kQStage = NB * kMlaKBytes - kMlaPanels * kMlaQPanelBytes, kQBuf0 = kQStage / kMlaKBytes;
   static_assert(kQStage >= 0 && kQStage % 1024 == 0, "Q staging");
@@ -575,6 +575,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 
   __syncwarp();
   if (warp >= kMlaSoftmaxWarps) cluster_wait();      // the wait that pairs with the arrive above
+  if (!left) cluster_arrive();                       // nothing remote is left to do for this warp either
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
@@ -583,7 +584,6 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       for (int w = 0; w < 64; ++w) __nanosleep(1000);
     __syncthreads();
   }
-  if (!left) cluster_arrive();
   cluster_wait();                 // neither CTA leaves while the other may still copy into it or arrive on its barriers
   if (warp == kMlaMmaWarp) {
     tc_fence_after();
