@@ -9,7 +9,8 @@
 // of CTAs has a unit, each half of the latent dims (sparse_mla.cu): whole, O of 128 rows and 512 dims and S, P and Q of 576 do not fit one SM's tensor memory.
 // What bounds it: a block of 64 slots takes a pair 1.33 to 1.46 us from FP8 records and 1.10 to 1.23 from 4 bits, the chain of conversion, exchange, softmax and
 // P.V with the issue slots 63 % used (74 sequences x 128 heads, window 2048: 65.9 us, tensor pipe 32 %, DRAM 21 %).  64 sequences x 128 heads at
-// 128K, window 4096: 100 to 110 us for 29 us of bytes and 45 of operations; 160 x 4 drafts x 16 heads, 4 bits, window 1024: 76 us.
+// 128K, window 4096: 100 to 110 us for 29 us of bytes and 45 of operations; 160 x 4 drafts x 16 heads, 4 bits, window 1024: 74 to 77 us,
+// of which a unit's start, a chain of lengths, pages, records and its first scores, takes 6 and its end 2 in each of three rounds.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
