@@ -293,8 +293,8 @@ int dsa_compact_pages(const int32_t* block_table, int64_t table_stride, int32_t*
  *   out[r,h,:] = sum_s softmax_s(scale * q[r,h,:576] . kv[s,:576]) * kv[s,:512];
  * a row that sees nothing gives zeros, and what a row does not see -- infinities and NaN
  * too -- leaves it as it is.  window >= 1 (as large as the sequence: all of it), first >= 0,
- * any H >= 1.  The two halves of a score are exchanged between two SMs in fp16 (as for
- * dsa_sparse_mla_decode_records).
+ * any H >= 1.  The two halves of a score come from two SMs and are added in fp32; weights are
+ * rounded to bf16 before they are multiplied.  A row whose scores are all -inf gives zeros.
  * Calls that would leave SMs idle cut their rows' keys into parts that a second kernel
  * merges in fp32: `workspace` (16-byte aligned) of ..._workspace_bytes bytes holds
  * those; with a smaller one, or NULL, the call works with fewer parts or none. */

@@ -22,7 +22,7 @@ namespace dsa {
 template <int SRC>
 struct WinCfg {
   static constexpr int kBufs = kMlaBufs - 1;           // the fifth one's space holds raw rows
-  static constexpr int kOffBars = kMlaBufs * kMlaKBytes + 2 * kMlaXBytes;
+  static constexpr int kOffBars = kMlaBufs * kMlaKBytes + kWinXBytes;
   static constexpr int kOffValid = kOffBars + 640;
   static constexpr int kOffPm = kOffValid + kMlaValidRing * kMlaBlk;
   static constexpr int kOffSees = kOffPm + kMlaPairBytes;             // int4 a row
@@ -40,8 +40,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   extern __shared__ __align__(1024) uint8_t smem[];            // the swizzled panels need 1024-byte alignment
   launch_dependents();                                         // (the kernel that merges the parts)
   uint8_t* kv_s = smem;                                        // five buffers: four panels [64 keys x 128 B] and 64 x 64 B
-  uint8_t* send_s = kv_s + kMlaBufs * kMlaKBytes;              // this CTA's partial score tile on its way out
-  uint8_t* recv_s = send_s + kMlaXBytes;                       // the peer's
+  uint8_t* recv_s = kv_s + kMlaBufs * kMlaKBytes;              // the peer's partial score tile
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBars);      // as in sparse_mla.cu
   uint64_t *q_full = bars + 0, *q_moved = bars + 1, *o_final = bars + 2, *s_free = bars + 3, *p_full = bars + 4, *s_full = bars + 5, *pv_done = bars + 7,
            *pm_full = bars + 9, *recv_full = bars + 17, *xchg_free = bars + 33, *kv_full = bars + 49, *kv_free = bars + 54;
@@ -321,9 +320,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     named_bar_sync(3 + qd, 128);
     cluster_wait();
-    const int xw = hf * 4 + qd;                        // this warp's part of the set's partial tile: 32 rows x 32 keys, 2 KB
-    uint8_t* send = send_s + xw * kMlaXWarp;
-    const uint8_t* recv = recv_s + xw * kMlaXWarp;
+    const uint8_t* recv = recv_s + (hf * 4 + qd) * kWinXWarp + lane * 16;      // this thread's part of the set's partial tile
     const uint32_t peer_recv = mapa_u32(smem_u32(recv), peer);
     auto pm_of = [&](int blk) -> uint16_t* { return pm_s + (blk & 3) * 256 + row; };      // [key half][row]
     auto raise = [&](float m_old, float bmax) { return bmax - m_old > kMaxRaise ? bmax : m_old; };   // -inf - -inf: stays
@@ -336,7 +333,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const int k0 = g * kMlaBlk + 32 * half;
       return (range_bits(0, v.x, k0) | range_bits(v.y, v.z, k0) | draft_bits(more_s[r], v.w, k0)) & low_bits(n_slots - k0);
     };
-    if (qd < n_quad && set < nblk && lane == 0) mbar_expect_tx(&recv_full[warp], kMlaXWarp);
+    if (qd < n_quad && set < nblk && lane == 0) mbar_expect_tx(&recv_full[warp], kWinXWarp);
     for (int n = qd < n_quad ? set : nblk; n < nblk && ok; n += 2) {
       const uint32_t ph = (n >> 1) & 1;
       uint32_t sv[32];                                 // this CTA's partial scores
@@ -348,19 +345,11 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);              // the next block's scores may overwrite S now
-      if (n > 0) {                                     // the peer has read block n-1: both stages are free
+      if (n > 0) {                                     // the peer has read block n-1
         ok = mla_wait(&xchg_free[warp ^ 8], ((n - 1) >> 1) & 1, abort_flag, a.status);
         if (!ok) break;
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        auto h2 = [&](int k) { return pack_f16x2(__uint_as_float(sv[8 * c + 2 * k]), __uint_as_float(sv[8 * c + 2 * k + 1])); };
-        *reinterpret_cast<uint4*>(send + xchg_off(lane, c)) = make_uint4(h2(0), h2(1), h2(2), h2(3));
-      }
-      fence_async_smem();                              // the bulk copy reads the tile through the async proxy
-      __syncwarp();
-      if (elect_one()) bulk_copy_to_peer(peer_recv, send, kMlaXWarp, peer_recv_full);
-      __syncwarp();
+      send_scores(peer_recv, peer_recv_full, sv);
       uint32_t seen = 0xffffffffu;
       const int k0 = (blk_lo + n) * kMlaBlk;
       const bool whole = k0 >= full0 && k0 + kMlaBlk <= full1;
@@ -382,14 +371,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       ok = mla_wait(&recv_full[warp], ph, abort_flag, a.status);
       if (!ok) break;
       float s[32];                                     // raw scores; the (positive) scale is folded into the exponent's FMA
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint4 theirs = *reinterpret_cast<const uint4*>(recv + xchg_off(lane, c));
-        const uint32_t tw[4] = {theirs.x, theirs.y, theirs.z, theirs.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          add_f16x2(tw[k], __uint_as_float(sv[8 * c + 2 * k]), __uint_as_float(sv[8 * c + 2 * k + 1]), s[8 * c + 2 * k], s[8 * c + 2 * k + 1]);
-      }
+      add_scores(recv, sv, s);
       seen &= __ballot_sync(0xffffffffu, valid_s[(n % kMlaValidRing) * kMlaBlk + 32 * hf + lane]);
       auto largest = [&]() {
         float bm[4] = {s[0], s[1], s[2], s[3]};        // four independent chains
@@ -408,7 +390,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(&pm_full[set * 4 + qd]);
       mbar_arrive_remote_after(peer_xchg_free, top, lane == 0);      // the peer may send into this stage again
-      if (lane == 0 && n + 2 < nblk) mbar_expect_tx(&recv_full[warp], kMlaXWarp);
+      if (lane == 0 && n + 2 < nblk) mbar_expect_tx(&recv_full[warp], kWinXWarp);
       ok = mla_wait(&pm_full[set * 4 + qd], ph, abort_flag, a.status);
       if (!ok) break;
       m = raise(m_prev, pair_max(pm_of(n)));

@@ -10,6 +10,34 @@
 
 namespace dsa {
 
+// A block's partial scores cross between the pair as they are, in fp32: both sides add the same two numbers, so that one softmax weights all of a row's columns.  It
+// is 32 KB a block and direction, and that costs: 2048 tokens x 128 heads, window 4096, 2236 us, 1.23 a block, where half of the bits took 1821 (24 of them
+// 2068), 64 sequences of decode, FP8, 128 for 103.  But a half rounded to fp16 is off by 2^-11 of itself, which the sum of two that cancel need not be large
+// against (an output 7 % off with halves of 4000), and it is lost beyond 65504.  A shared form with 16 bits for numbers that a rounding to 2^-10 does not hurt and
+// 32 for others took 2016 and 112, few blocks more time than this (160 sequences of drafts 78 for 72), and its time went by the data.
+// Every thread has its counterpart's row and keys: it stores its 32 numbers straight into the peer's shared memory, a warp's 16-byte pieces side by side, with no copy
+// of its own in between.
+constexpr int kWinXWarp = 32 * 32 * 4;                 // a warp's part of a tile: 32 rows x 32 keys
+constexpr int kWinXBytes = 8 * kWinXWarp;
+static_assert(kWinXBytes == 2 * kMlaXBytes, "in the place of a tile on its way out and one that comes in");
+__device__ __forceinline__ void send_scores(uint32_t dst_cluster, uint32_t bar_cluster, const uint32_t (&sv)[32]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                 ::"r"(dst_cluster + c * 512), "r"(sv[4 * c]), "r"(sv[4 * c + 1]), "r"(sv[4 * c + 2]), "r"(sv[4 * c + 3]), "r"(bar_cluster) : "memory");
+}
+// s = this side's scores + the peer's
+__device__ __forceinline__ void add_scores(const uint8_t* recv, const uint32_t (&sv)[32], float (&s)[32]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const float4 x = *reinterpret_cast<const float4*>(recv + c * 512);
+    s[4 * c + 0] = __uint_as_float(sv[4 * c + 0]) + x.x;
+    s[4 * c + 1] = __uint_as_float(sv[4 * c + 1]) + x.y;
+    s[4 * c + 2] = __uint_as_float(sv[4 * c + 2]) + x.z;
+    s[4 * c + 3] = __uint_as_float(sv[4 * c + 3]) + x.w;
+  }
+}
+
 struct WinArgs {
   const __nv_bfloat16* q;         // [T, H, 576]
   const uint8_t* kv;              // prompts: [S, 576] bf16 rows; decode: [num_phys_rows] records

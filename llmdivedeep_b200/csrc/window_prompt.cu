@@ -2,7 +2,7 @@
 //
 // A persistent cluster of two CTAs takes units of 128 query rows (token, head) one after the other.  Within a unit it is the kernel of
 // sparse_mla.cu: CTA c has half of the latent dims (its half of V and of the scores' contraction), the partial scores of a block of 64 keys
-// cross over in fp16, each side runs the softmax, P.V accumulates in tensor memory.  What differs:
+// cross over in fp32, each side runs the softmax, P.V accumulates in tensor memory.  What differs:
 //   * a block is 64 rows of a stretch of keys, fetched by five TMA boxes; rows of one sequence that follow one another share the blocks, and what
 //     each of them sees of a block is a 32-bit mask to a thread, from two ranges;
 //   * blocks, query panels and the output's staging go through one ring of five buffers, in the order Q(u) Q(u) Q(u)+O(u - 1) K(u, 0) K(u, 1) ..., so that
@@ -43,7 +43,7 @@ struct PromptPlan {
 };
 constexpr int kWpHead = 16;                            // first keys that come behind a stretch at most
 constexpr int kWpPlans = 4;                            // jobs that are planned ahead of the one whose output is on its way
-constexpr int kWpOffBars = kMlaBufs * kMlaKBytes + 2 * kMlaXBytes;
+constexpr int kWpOffBars = kMlaBufs * kMlaKBytes + kWinXBytes;
 constexpr int kWpOffPm = kWpOffBars + 640;
 constexpr int kWpOffSums = kWpOffPm + kMlaPairBytes;   // [4][128] (m, l)
 constexpr int kWpOffPlans = kWpOffSums + 4 * 128 * 8;
@@ -200,8 +200,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                      const __grid_constant__ CUtensorMap tmap_rope, const WinArgs a, const int jobs) {
   constexpr int NB = kMlaBufs;
   extern __shared__ __align__(1024) uint8_t smem[];            // the swizzled panels need 1024-byte alignment
-  uint8_t* send_s = smem + NB * kMlaKBytes;                    // this CTA's partial score tile on its way out
-  uint8_t* recv_s = send_s + kMlaXBytes;                       // the peer's
+  uint8_t* recv_s = smem + NB * kMlaKBytes;                    // the peer's partial score tile
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWpOffBars);
   uint64_t* q_ready = bars + 0;                      // Q of a unit is in tensor memory
   uint64_t* qk_done = bars + 1;                      // the unit's scores have all been computed: Q's columns are free
@@ -304,16 +303,14 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const uint32_t t_row = tmem + (uint32_t(qd * 32) << 16);
     const uint32_t peer_xchg_free = mapa_u32(smem_u32(xchg_free + warp), peer);
     const uint32_t peer_recv_full = mapa_u32(smem_u32(recv_full + warp), peer);
-    const int xw = hf * 4 + qd;                        // this warp's part of the set's partial tile: 32 rows x 32 keys, 2 KB
-    uint8_t* send = send_s + xw * kMlaXWarp;
-    const uint8_t* recv = recv_s + xw * kMlaXWarp;
+    const uint8_t* recv = recv_s + (hf * 4 + qd) * kWinXWarp + lane * 16;      // this thread's part of the set's partial tile
     const uint32_t peer_recv = mapa_u32(smem_u32(recv), peer);
     auto pm_of = [&](uint32_t blk) -> uint16_t* { return pm_s + (blk & 3) * 256 + row; };      // [key half][row]
     auto raise = [&](float m_old, float bmax) { return bmax - m_old > kMaxRaise ? bmax : m_old; };   // -inf - -inf: stays
     auto pair_max = [&](const uint16_t* pm) {
       return fmaxf(__uint_as_float(uint32_t(pm[0]) << 16), __uint_as_float(uint32_t(pm[128]) << 16));
     };
-    if (lane == 0) mbar_expect_tx(&recv_full[warp], kMlaXWarp);
+    if (lane == 0) mbar_expect_tx(&recv_full[warp], kWinXWarp);
     cluster_wait();
     bool ok = true;
     uint32_t n = set, base = 0;                        // this set's next block, the first block of the unit, both of all blocks
@@ -337,16 +334,8 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);            // the next block's scores may overwrite S now
-        if (n > 0 && !(ok = wait(&xchg_free[warp ^ 8], (n - 1) >> 1))) break;      // the peer has read block n-1: both stages are free
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          auto h2 = [&](int j) { return pack_f16x2(__uint_as_float(sv[8 * c + 2 * j]), __uint_as_float(sv[8 * c + 2 * j + 1])); };
-          *reinterpret_cast<uint4*>(send + xchg_off(lane, c)) = make_uint4(h2(0), h2(1), h2(2), h2(3));
-        }
-        fence_async_smem();                            // the bulk copy reads the tile through the async proxy
-        __syncwarp();
-        if (elect_one()) bulk_copy_to_peer(peer_recv, send, kMlaXWarp, peer_recv_full);
-        __syncwarp();
+        if (n > 0 && !(ok = wait(&xchg_free[warp ^ 8], (n - 1) >> 1))) break;      // the peer has read block n-1
+        send_scores(peer_recv, peer_recv_full, sv);
         uint32_t seen = 0xffffffffu;                   // which of this thread's keys its row sees
         {
           const int blk = p.blk_lo + (int)(n - base);
@@ -379,14 +368,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         const float m_prev = m;
         if (!(ok = wait(&recv_full[warp], ph))) break;
         float s[32];                                   // raw scores; the (positive) scale is folded into the exponent's FMA
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint4 theirs = *reinterpret_cast<const uint4*>(recv + xchg_off(lane, c));
-          const uint32_t tw[4] = {theirs.x, theirs.y, theirs.z, theirs.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            add_f16x2(tw[j], __uint_as_float(sv[8 * c + 2 * j]), __uint_as_float(sv[8 * c + 2 * j + 1]), s[8 * c + 2 * j], s[8 * c + 2 * j + 1]);
-        }
+        add_scores(recv, sv, s);
         auto largest = [&]() {
           float bm[4] = {s[0], s[1], s[2], s[3]};      // four independent chains
 #pragma unroll
@@ -404,7 +386,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(&pm_full[set * 4 + qd]);
         mbar_arrive_remote_after(peer_xchg_free, top, lane == 0);      // the peer may send into this stage again
-        if (lane == 0) mbar_expect_tx(&recv_full[warp], kMlaXWarp);
+        if (lane == 0) mbar_expect_tx(&recv_full[warp], kWinXWarp);
         if (!(ok = wait(&pm_full[set * 4 + qd], ph))) break;
         m = raise(m_prev, pair_max(pm_of(n)));
         if (m != m_own && m_own != -CUDART_INF_F) l *= fast_exp2(m_own - m);      // (without a reference l is 0, or NaN, and stays so)
