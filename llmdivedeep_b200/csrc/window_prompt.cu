@@ -604,6 +604,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       e += n;
     }
     if (ok && k > 0) drain(k - 1, e, true);
+    if (redos > 0 && ok) ok = wait(&plan_free[(k - 1) % kWpPlans], (k - 1) / kWpPlans);      // nobody reads the last job's plan, nor one before it
     if (redos > 0) {                                   // what is written again has been written
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       __syncwarp();
@@ -617,7 +618,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       int job = redos > kWpRedo ? pair + x * n_pairs : (int)redo_s[x].x;
       if (DRAFTS && a.live && redos > kWpRedo && (job = units.find(a, job)) < 0) break;
       uint32_t mask = redos > kWpRedo ? 0xffffffffu : redo_s[x].y;
-      PromptPlan& p = plans[qd];                       // each warp its own; of the jobs' plans nobody needs more than `blocks`
+      PromptPlan& p = plans[qd];                       // each warp its own; of the jobs' plans nobody needs more than `blocks` now
       const JobRows j = job_rows<DRAFTS>(a, job);
       if (j.rows < qd * 32 + 32) mask &= low_bits(j.rows - qd * 32);
       __syncwarp();
