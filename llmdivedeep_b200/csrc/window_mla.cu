@@ -47,6 +47,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 64);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint32_t* odd_s = tmem_slot + 2;                             // [4 quadrants] rows with a key that they do not see and that is no number
+  volatile uint32_t* lost_s = odd_s + 4;                       // [4 quadrants] a warp of it has given up
   uint8_t* valid_s = smem + C::kOffValid;                      // decode: [kMlaValidRing][64] 1 = the slot of the block has a page
   uint16_t* pm_s = reinterpret_cast<uint16_t*>(smem + C::kOffPm);        // block maxima, rounded up to bf16
   int4* sees_s = reinterpret_cast<int4*>(smem + C::kOffSees);
@@ -79,7 +80,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       mbar_init(bars + i, count);
     }
     mbar_fence_init();
-    if (lane < 5) const_cast<int*>(abort_flag)[lane] = 0;      // and odd_s
+    if (lane < 9) const_cast<int*>(abort_flag)[lane] = 0;      // and odd_s, lost_s
     __syncwarp();
     if (lane == 0) mbar_expect_tx(q_full, kMlaPanels * kMlaQPanelBytes);
     __syncwarp();
@@ -451,7 +452,9 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     if (ok) sum_s[quarter * 128 + row] = make_float2(m, l);
     const uint32_t odds = __ballot_sync(0xffffffffu, odd && any && row < rows_here);
     if (odds && lane == 0) atomicOr(odd_s + qd, odds);
+    if (!ok && lane == 0) lost_s[qd] = 1;
     named_bar_sync(3 + qd, 128);
+    ok = lost_s[qd] == 0;                              // the same for the quadrant's four warps: there are barriers behind, and sums of all four
     uint32_t again = 0;                                // rows of the quadrant that have to be done again
     __nv_bfloat16* const orow = a.out + (g0 + row) * kMlaDv + cta * kMlaDvHalf;
     const int64_t prow = (int64_t)part * 128 + row;

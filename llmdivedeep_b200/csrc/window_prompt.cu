@@ -216,7 +216,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   uint64_t* xchg_free = bars + 34;                   // [16] the peer has read what this CTA's warp sent
   uint64_t* ring_full = bars + 50;                   // [5] a buffer is ready to be read (the output's: to be written)
   uint64_t* part_full = bars + 55;                   // [5] a block that is no whole one has landed: it is ready when its other rows are zeros
-  uint64_t* ring_free = bars + 60;                   // [5]
+  uint64_t* ring_free = bars + 60;                   // [5] the four warps of Q and O, or P.V of a block and three arrivals with it
   uint64_t* plan_full = bars + 65;                   // [4]
   uint64_t* plan_free = bars + 69;                   // [4]
   uint64_t* sums_full = bars + 73;                   // the row sums of a unit, and whether a row must be done key by key
@@ -234,7 +234,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const int warp = warp_index(), lane = threadIdx.x & 31;
   if (warp == 0) {
     for (int i = lane; i < 75; i += 32) {
-      const uint32_t count = (i == 0 || i == 3 || i == 74) ? 4u                      // q_ready, o_free, sums_free: the warps of Q and O
+      const uint32_t count = (i == 0 || i == 3 || i == 74 || (i >= 60 && i <= 64)) ? 4u      // q_ready, o_free, sums_free, ring_free: the warps of Q and O
                              : (i == 4 || i == 5) ? 8u                               // s_free, p_full: lane 0 of a set's warps
                              : (i >= 10 && i <= 17) ? 2u                             // pm_full: the two warps of a quadrant
                              : (i >= 69 && i <= 72) ? 23u                            // plan_free: all that read it
@@ -450,9 +450,10 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     bool ok = true;
     uint2* redo_s = reinterpret_cast<uint2*>(smem + kWpOffRedo) + qd * kWpRedo;
     int redos = 0;
-    auto give_back = [&](uint32_t e) {                 // the four warps are done with a buffer
-      named_bar_sync(1, 128);
-      if (warp == kWpOutWarp && lane == 0) mbar_arrive(&ring_free[e % NB]);
+    // A buffer goes back when all four warps have said that they are done with it.  (They do not meet at a barrier: one may have given up, and a barrier has no limit.)
+    auto give_back = [&](uint32_t e) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring_free[e % NB]);
     };
     auto drain = [&](uint32_t k, uint32_t e, bool last) {      // the output of job k, staged in entry e, of the last job one of its own
       const PromptPlan& p = plans[k % kWpPlans];
@@ -717,6 +718,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll
           for (int ks = 0; ks < kMlaBlk / 16; ++ks)      // 16 keys per step: 16 rows x 128 B further into each panel
             umma_f16_ts(tmem + kColO, tmem + kColP + 8 * ks, vd + ks * (2048 >> 4), idesc_pv, !first || ks != 0);
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 3;" ::"r"(smem_u32(&ring_free[vbuf])) : "memory");
           umma_commit(&ring_free[vbuf]);
           umma_commit(&pv_done[parity]);
           if (last) umma_commit(o_final);
