@@ -340,7 +340,8 @@ int dsa_indexer_logits_drafts(const void* q_fp8, const void* w, int w_dtype, con
                               const int64_t* tree, int tokens_per_seq, float* logits, int64_t ld_logits, int B, int H, int D,
                               int num_pages, int max_ctx, int32_t* status, void* stream);
 /* dsa_topk_select of such logits: of every row the k largest of the positions that its draft sees, -1 in the slots
- * that are left (anywhere in the list); rows without a token: -1. */
+ * that are left (anywhere in the list); rows without a token: -1.  A score of -inf is that of a position that is not
+ * seen (its page is none). */
 size_t dsa_topk_select_drafts_workspace_bytes(int B, int tokens_per_seq);
 int dsa_topk_select_drafts(const float* logits, int64_t ld_logits, const int32_t* ctx_len, const int32_t* n_new,
                            const int64_t* tree, int tokens_per_seq, int B, int max_ctx, int k, int32_t* out_idx,

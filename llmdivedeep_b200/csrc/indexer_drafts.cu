@@ -426,18 +426,29 @@ __global__ void __launch_bounds__(256) draft_ends_kernel(const DraftArgs d, int 
   ends[r] = i < dr.m ? dr.ctx - dr.m + i + 1 : 0;
 }
 // What a row does not see has the lowest score there is, and is selected where too few others are higher: where the row sees fewer positions than it has slots, or has
-// scores that are no numbers.  Those become empty slots.
-__global__ void __launch_bounds__(256) draft_unsee_kernel(const DraftArgs d, int k, int32_t* idx) {
+// scores that are no numbers.  Those become empty slots: drafts by the row's mask, whatever their scores are, and positions of pages that are none by theirs, which only the
+// scores tell of.  It starts under the selection's end, and a thread has eight slots' scores under way (256 rows of 2048 slots at 128K: 4 us behind the selection's 39).
+__global__ void __launch_bounds__(256) draft_unsee_kernel(const float* __restrict__ logits, int64_t ld, const DraftArgs d, int k, int32_t* idx) {
+  constexpr int kAhead = 8;
   const int r = blockIdx.x, b = r / d.per_seq, i = r - b * d.per_seq;
   const Drafts dr = drafts_of(d, b);
   const int P = dr.ctx - dr.m;
+  const uint64_t bits = d.tree ? draft_mask(d, b, i) : 0;
+  const float* scores = logits + (int64_t)r * ld;
+  int32_t* row = grid_wait(idx) + (int64_t)r * k;      // (no block goes before: what comes next waits for this kernel)
   if (i >= dr.m) return;
-  const uint64_t bits = draft_mask(d, b, i);
-  if (__popcll(bits) == i + 1) return;
-  int32_t* row = idx + (int64_t)r * k;
-  for (int j = threadIdx.x; j < k; j += 256) {
-    const int at = row[j] - P;
-    if (at >= 0 && !(bits >> at & 1)) row[j] = -1;     // at <= i < 64
+  for (int j0 = threadIdx.x; j0 < k; j0 += 256 * kAhead) {
+    int at[kAhead];
+    float score[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) at[u] = j0 + 256 * u < k ? row[j0 + 256 * u] : -1;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) score[u] = at[u] >= 0 ? __ldg(scores + at[u]) : 0.f;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const bool other = d.tree && at[u] >= P && !(bits >> (at[u] - P) & 1);     // at - P <= i < 64
+      if (at[u] >= 0 && (other || score[u] == -CUDART_INF_F)) row[j0 + 256 * u] = -1;
+    }
   }
 }
 
@@ -455,8 +466,8 @@ int topk_select_drafts_launch(const float* logits, int64_t ld, const int32_t* ct
   draft_ends_kernel<<<(T + 255) / 256, 256, 0, stream>>>(d, T, ends);
   int rc = check_launch("topk_select_drafts");
   if (!rc) rc = topk_select_launch(logits, ld, nullptr, ends, T, max_ctx, k, out, /*sample=*/1, /*overlapped=*/0, stream);
-  if (rc || !tree || k == 0) return rc;
-  draft_unsee_kernel<<<T, 256, 0, stream>>>(d, k, out);
+  if (rc || k == 0) return rc;
+  launch_after(1, draft_unsee_kernel, dim3(T), 256, 0, stream, logits, ld, d, k, out);
   return check_launch("topk_select_drafts");
 }
 

@@ -524,7 +524,8 @@ def _draft_logits(q_fp8, weights, kcache, kscale, block_table, ctx_len, max_ctx,
 def topk_select_drafts(logits, k: int, ctx_len, tokens_per_seq: int = 1, n_new: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """topk_select of what fp8_paged_mqa_logits gives for drafts (arguments as there): of every row the k largest of the positions that its draft
-    sees, int32 [B*tokens_per_seq, k], unsorted, -1 in the slots that are left, wherever they are in the list."""
+    sees, int32 [B*tokens_per_seq, k], unsorted, -1 in the slots that are left, wherever they are in the list.  A score of -inf is that of a position that
+    is not seen: its page is none."""
     i = _index_with(logits, ctx_len, n_new, tree, out)
     if logits.dtype is not torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise DsaError("logits must be fp32 [T, S] with unit column stride")
