@@ -509,6 +509,12 @@ class PagedCache:
     def _rows(self, rows) -> torch.Tensor:
         return rows if isinstance(rows, torch.Tensor) else torch.tensor(rows, dtype=torch.int32, device=self.device)
 
+    @staticmethod
+    def _sequences(q, tokens_per_seq: int) -> int:
+        if tokens_per_seq < 1 or q.shape[0] % tokens_per_seq:
+            raise ops.DsaError(f"{q.shape[0]} query rows are no {tokens_per_seq} a sequence")
+        return q.shape[0] // tokens_per_seq
+
     @property
     def caches(self) -> tuple:
         return self.k8, self.k_scale, self.latent
@@ -534,14 +540,14 @@ class PagedCache:
 
     def decode_drafts(self, layer: int, q8, w, q, softmax_scale: float, ws: DecodeWorkspace, tokens_per_seq: int, n_new=None, tree=None):
         """dsa_draft_step of the first q.shape[0] / tokens_per_seq rows: the last n_new[b] tokens of a row (None: tokens_per_seq) are drafts."""
-        B = q.shape[0] // tokens_per_seq
+        B = self._sequences(q, tokens_per_seq)
         return dsa_draft_step(q8, w, self.k8[layer], self.k_scale[layer], self.table[:B], self.ctx[:B], q, self.latent[layer], softmax_scale, ws,
                               tokens_per_seq, n_new, tree)
 
     def window(self, layer: int, q, window: int, first: int, softmax_scale: float, tokens_per_seq: int = 1, n_new=None, tree=None,
                out: Optional[torch.Tensor] = None):
         """Attention of the newest tokens, or of drafts, over a sliding window and the first tokens of this layer's latents."""
-        B = q.shape[0] // tokens_per_seq
+        B = self._sequences(q, tokens_per_seq)
         return ops.window_mla_decode_paged(q, self.latent[layer], self.table[:B], self.ctx[:B], window, first, softmax_scale, tokens_per_seq, n_new, tree,
                                            out=out)
 
