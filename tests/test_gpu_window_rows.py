@@ -177,3 +177,34 @@ def test_in_a_graph_with_lengths_that_change():
         graph.replay()
         ops.check_status("cuda")
         check(out, c.want(c.seen()))
+
+
+@pytest.mark.parametrize("record", [656, 416])
+@pytest.mark.parametrize("shape", [WHOLE[0], WHOLE[5], PARTS[0], PARTS[3]])
+@pytest.mark.parametrize("idle", ["tokens", "drafts"])
+def test_nobody_has_a_draft(record, shape, idle):
+    """Sequences without a token, and sequences without a draft: zeros in every row."""
+    c = Rows(shape, record, False)
+    none = torch.zeros(c.B, dtype=torch.int32, device="cuda")
+    out = torch.full((c.B * c.per, c.q.shape[1], 512), 9.0, dtype=torch.bfloat16, device="cuda")
+    changes = dict(n_new=none, ctx_len=none) if idle == "tokens" else dict(n_new=none)
+    ops.window_mla_decode_paged(**{**c.args(), **changes}, window=c.window, first=c.first, scale=SCALE, out=out)
+    ops.check_status("cuda")
+    assert bool((out == 0).all())
+
+
+def test_two_calls_at_once():
+    """On streams of their own, each with its own workspace, whole units beside parts: what each gives alone."""
+    cases = [Rows(WHOLE[0], 656, True), Rows(PARTS[0], 416, True), Rows(WHOLE[5], 416, False)]
+    call = lambda c, a: ops.window_mla_decode_paged(**a, window=c.window, first=c.first, scale=SCALE)
+    args = [c.args() for c in cases]
+    want = [call(c, a) for c, a in zip(cases, args)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[] for _ in cases]
+    for _ in range(10):
+        for s, c, a, g in zip(streams, cases, args, got):
+            with torch.cuda.stream(s):
+                g.append(call(c, a))
+    torch.cuda.synchronize()
+    ops.check_status("cuda")
+    assert all(torch.equal(o, w) for g, w in zip(got, want) for o in g)
