@@ -7,9 +7,9 @@
 // A unit is up to 128 query rows (token, head) of one sequence, and its keys are the union of what they see, as slots: the first tokens, then the window's,
 // then the drafts.  Rows of one sequence share the fetch and the conversion of their records, which is why a unit has several tokens where heads are few.  A pair
 // of CTAs has a unit, each half of the latent dims (sparse_mla.cu): whole, O of 128 rows and 512 dims and S, P and Q of 576 do not fit one SM's tensor memory.
-// What bounds it: a block of 64 slots takes a pair 1.33 to 1.46 us from FP8 records and 1.10 to 1.23 from 4 bits, the chain of conversion, exchange, softmax and
-// P.V with the issue slots 63 % used (74 sequences x 128 heads, window 2048: 65.9 us, tensor pipe 32 %, DRAM 21 %).  64 sequences x 128 heads at
-// 128K, window 4096: 100 to 110 us for 29 us of bytes and 45 of operations; 160 x 4 drafts x 16 heads, 4 bits, window 1024: 74 to 77 us,
+// What bounds it: a block of 64 slots takes a pair 1.8 us from FP8 records and 1.5 from 4 bits, the chain of conversion, exchange (32 KB either way), softmax and
+// P.V with half of the issue slots used (74 sequences x 128 heads, FP8, window 2048: 80 us under the profiler, issue slots 47 %, tensor pipe 26 %, DRAM 18 %).  64
+// sequences x 128 heads at 128K, window 4096: 136 to 139 us for 29 us of bytes and 45 of operations; 160 x 4 drafts x 16 heads, 4 bits, window 1024: 75 to 78 us,
 // of which a unit's start, a chain of lengths, pages, records and its first scores, takes 6 and its end 2 in each of three rounds.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -707,10 +707,10 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const WinArgs a, const
 }
 constexpr int64_t kRowsMost = 512ll << 20;             // bytes of rows at most
 static int rows_pad(int64_t keys) { return (int)((keys + 63) / 64 * 64); }
-// Bytes of the rows, 0: not this way.  Made rows once, a sequence's records cost its units 0.93 us a block of 64 in place of 1.3 (FP8) and 1.2 (4 bits), and 64 rows
-// 0.02 us of the whole GPU.  us with records and with rows, 128 heads, FP8: 32 sequences of 3 drafts, window 512, 47.5 / 47.4, of 4 48.6 / 45.5, of 5 70 / 59, of 13
-// 145 / 104; 4 bits of 4 43.3 / 44.4, of 5 61 / 57, of 13 128 / 101.  Calls that leave pairs idle cut keys into parts instead, unless there are many: 4
-// sequences of 13, window 512, 25.5 / 28.5, window 2048 60 / 51.
+// Bytes of the rows, 0: not this way.  Made rows once, a sequence's records cost its units 1.17 us a block of 64 in place of 1.8 (FP8) and 1.5 (4 bits), and 64 rows
+// 0.02 us of the whole GPU.  us with records and with rows, 128 heads, FP8: 32 sequences of 3 drafts, window 512, 51.5 / 50.0, of 4 55.0 / 50.7, of 5 77 / 65, of 13
+// 162 / 111; 4 bits of 4 47.9 / 49.0, of 5 69 / 63, of 13 141 / 108.  Calls that leave pairs idle cut keys into parts instead, unless there are many: 4
+// sequences of 13, window 512, 28.1 / 28.7 (4 bits 24.7 / 28.2), window 2048 71 / 59.
 static int64_t rows_bytes(int record_bytes, int B, int64_t seq_rows, int64_t keys) {
   const int64_t bytes = (int64_t)B * rows_pad(keys) * (kMlaDqk * 2), units = (seq_rows + 127) / 128;
   return units >= (record_bytes == kLatent4Bytes ? 5 : 4) && (B * units >= sm_count() / 2 || keys >= 1024) && bytes <= kRowsMost ? bytes : 0;

@@ -13,8 +13,8 @@ namespace dsa {
 // A block's partial scores cross between the pair as they are, in fp32: both sides add the same two numbers, so that one softmax weights all of a row's columns.  It
 // is 32 KB a block and direction, and that costs: 2048 tokens x 128 heads, window 4096, 2236 us, 1.23 a block, where half of the bits took 1821 (24 of them
 // 2068), 64 sequences of decode, FP8, 128 for 103.  But a half rounded to fp16 is off by 2^-11 of itself, which the sum of two that cancel need not be large
-// against (an output 7 % off with halves of 4000), and it is lost beyond 65504.  A shared form with 16 bits for numbers that a rounding to 2^-10 does not hurt and
-// 32 for others took 2016 and 112, few blocks more time than this (160 sequences of drafts 78 for 72), and its time went by the data.
+// against (an output 7 % off with halves of 4000), and it is lost beyond 65504.  A form with 16 bits for numbers that a rounding to 2^-10 does not hurt and
+// 32 for others took 2016 and 112, but few blocks more time than this (160 sequences of drafts 78 for 73), and its time went by the data; two messages of half a part 2530.
 // Every thread has its counterpart's row and keys: it stores its 32 numbers straight into the peer's shared memory, a warp's 16-byte pieces side by side, with no copy
 // of its own in between.
 constexpr int kWinXWarp = 32 * 32 * 4;                 // a warp's part of a tile: 32 rows x 32 keys

@@ -11,10 +11,10 @@
 //   * four more warps move Q into tensor memory and O out of it, so that the softmax goes from unit to unit without a pause.
 // Roles: warps 0-15 exchange + softmax, 16 MMA issuer, 17 loads, 18 zeros in the rows behind the end of a stretch, 19 plans the next unit, 20-23 Q and O.
 // Every wait is bounded (dsa_common.cuh); the two CTAs leave together through a cluster barrier.
-// What bounds it: 0.93 us a block, of which the tensor pipe works 0.58 and the softmax warps' chain the rest -- a buffer is held for 4.6 us, load, exchange, softmax
-// and P.V -- and the entries of the ring that a unit needs besides.  us a unit, four first tokens, by window: 128 heads 64 7.6, 512 13.4, 2048 36.3; 8 tokens x
-// 16 heads 64 8.4, 512 12.7, 1024 20.1 (a unit of one block 6.3; by a pair that takes one unit only, 10.3).  8192 tokens x 128 heads at 128K, window 4096:
-// 7600 to 8000 us = 1175 to 1235 TFLOP/s at the power cap, 8660 by pairs of one unit; packed prompts of 16 heads, window 512, 181 us for 64 us of operations:
+// What bounds it: 1.17 us a block, of which the tensor pipe works 0.58: the softmax warps' chain, in which 32 KB of scores cross to the other SM and as many come back (with
+// half of the bits it was 0.93; window_mla.cuh) -- a buffer is held for 5.8 us, load, exchange, softmax and P.V -- and the entries of the ring that a unit needs
+// besides.  us a unit, four first tokens, by window: 128 heads 64 7.6, 512 15.3, 2048 43.3; 8 tokens x 16 heads 64 8.6, 512 14.9, 1024 24.2 (a unit of one block 6.8).
+// 8192 tokens x 128 heads at 128K, window 4096: 10.3 to 10.5 ms = 890 to 910 TFLOP/s; packed prompts of 16 heads, window 512, 220 us for 64 us of operations:
 // their units have few blocks, and the last round of units is a part of one.  40 tokens x 128 heads: 10.4 to 10.9 us, a chain of set-up and plan 1.2, loads 1.6 to 2,
 // scores 0.9, exchange and softmax 1.8, P.V 0.6, output 2.2.
 #include <cuda.h>
@@ -92,7 +92,8 @@ __device__ __forceinline__ int draft_segs(const WinArgs& a, int n_tok, PromptPla
 }
 
 // The keys of a unit, by one warp.  Neighbouring rows of a sequence whose windows touch share two stretches: its first keys and those of their windows.  Where
-// the first keys fit into the last block of the other stretch they are no block of their own, which costs a unit 1.1 to 1.7 us.
+// the first keys fit into the last block of the other stretch they are no block of their own (16 heads, window 512, 14.9 us a unit, 16.4 to 18 without; 64
+// heads, window 1024, 24.2 and 26.3 to 28).
 template <bool DRAFTS>
 __device__ __forceinline__ int build_segs(const WinArgs& a, int n_tok, PromptPlan& p) {
   if constexpr (DRAFTS) return draft_segs(a, n_tok, p);
@@ -697,7 +698,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const uint64_t vdesc0 = umma_smem_desc(smem_u32(smem), kMlaKPanelBytes, 1024, kSwz128);
       const uint64_t rdesc0 = umma_smem_desc(smem_u32(smem + kMlaRopeOff), 16, 512, kSwz64);
       const uint32_t rope_ks = 2 * cta;                  // this CTA's two K-steps of the rope panel
-      // What this warp does beside issuing is on the path from block to block (of 1650 cycles 930 are the issue itself), so it counts in steps and walks
+      // What this warp does beside issuing is on the path from block to block (930 cycles of a block are the issue itself), so it counts in steps and walks
       // one loop: three waits, the scores of block i, P.V of block i - 2 -- in a unit's first turn of the last block before it.
       uint32_t gp = 0;                                   // parity of the next block, counted over all units
       uint32_t buf = 0, ring = 0;                        // the next entry's buffer, and the parity of its use
