@@ -65,9 +65,19 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// CLUSTER: what another CTA of the cluster has stored is waited for.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
+  if constexpr (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+  else asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
@@ -79,12 +89,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 
 // Wait for `parity` on `bar`, giving up after `limit` polls.  Returns false (after
 // flagging) when the wait expired or another role already aborted.
-template <int UNROLL = 1>
+template <int UNROLL = 1, bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait_limit(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                                 int* status, uint32_t limit) {
 #pragma unroll UNROLL
   for (uint32_t i = 0; i < limit; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait<CLUSTER>(bar, parity)) return true;
     if (i > kFastSpins) {
       if (*abort_flag) return false;
       __nanosleep(40);
@@ -103,10 +113,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 // that a wait which finds its phase complete costs a poll, a vote and a branch and leaves nothing to test behind it; with the
 // loop alone (which the compiler unrolls by four at every place) the indexer took 2379 us for 4096 x 65536 instead of 2204,
 // block-sparse attention 247 instead of 244.
-template <int UNROLL = 1>
+template <int UNROLL = 1, bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  return __all_sync(0xffffffffu, mbar_wait_limit<UNROLL>(bar, parity, abort_flag, status, kSpinLimit));
+  if (__all_sync(0xffffffffu, mbar_try_wait<CLUSTER>(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_limit<UNROLL, CLUSTER>(bar, parity, abort_flag, status, kSpinLimit));
 }
 
 // Whether another role has given up, for a warp whose lanes all come here: one answer for all of them (the flag may be raised

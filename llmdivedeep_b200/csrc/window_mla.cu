@@ -369,7 +369,7 @@ window_mla_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const float m_own = m;                           // what l is relative to
       if (n > 0) m = raise(m, pair_max(pm_of(n - 1)));
       const float m_prev = m;
-      ok = mla_wait(&recv_full[warp], ph, abort_flag, a.status);
+      ok = wait_scores(&recv_full[warp], ph, abort_flag, a.status);
       if (!ok) break;
       float s[32];                                     // raw scores; the (positive) scale is folded into the exponent's FMA
       add_scores(recv, sv, s);

@@ -26,6 +26,10 @@ __device__ __forceinline__ void send_scores(uint32_t dst_cluster, uint32_t bar_c
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
                  ::"r"(dst_cluster + c * 512), "r"(sv[4 * c]), "r"(sv[4 * c + 1]), "r"(sv[4 * c + 2]), "r"(sv[4 * c + 3]), "r"(bar_cluster) : "memory");
 }
+// The peer's numbers have come.  (The stores belong to the cluster's scope, and so does this wait.)
+__device__ __forceinline__ bool wait_scores(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
+  return mbar_wait_warp<4, true>(bar, parity, abort_flag, status);
+}
 // s = this side's scores + the peer's
 __device__ __forceinline__ void add_scores(const uint8_t* recv, const uint32_t (&sv)[32], float (&s)[32]) {
 #pragma unroll

@@ -367,7 +367,7 @@ window_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         const float m_own = m;                         // what l is relative to
         if (begun) m = raise(m, pair_max(pm_of(n - 1)));
         const float m_prev = m;
-        if (!(ok = wait(&recv_full[warp], ph))) break;
+        if (!(ok = wait_scores(&recv_full[warp], ph & 1, abort_flag, a.status))) break;
         float s[32];                                   // raw scores; the (positive) scale is folded into the exponent's FMA
         add_scores(recv, sv, s);
         auto largest = [&]() {

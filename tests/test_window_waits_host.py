@@ -29,3 +29,10 @@ def test_barriers_behind_a_condition_are_reached_by_all_of_a_quadrant():
     # from the last softmax block to that barrier nothing leaves
     tail = said[said.index("if (ok) ok = mla_wait(o_final"):]
     assert not re.search(r"\b(return|break|continue)\b", tail)
+
+
+def test_what_the_other_sm_stores_is_waited_for_at_the_clusters_scope():
+    for name in ("window_prompt.cu", "window_mla.cu"):
+        text = source(name)
+        assert "wait_scores(&recv_full[warp]" in text and not re.search(r"\b(mla_)?wait\(&recv_full", text)
+    assert "mbar_wait_warp<4, true>" in source("window_mla.cuh") and "try_wait.parity.acquire.cluster" in source("dsa_common.cuh")
